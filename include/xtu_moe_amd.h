@@ -594,6 +594,27 @@ hipError_t xtu_i8_row_fallback(int gate_up, const void* x, const int32_t* sorted
                                const int32_t* tile_hi, int max_tiles, int bm, void* out,
                                float limit, float alpha, float beta, hipStream_t stream);
 
+/* ------------------------------------------------ dense product with epilogue
+ * y[m][n] = residual[m][n] + row_scale[m] * act(sum_k x[m][k] w[n][k] + bias[n])
+ * for what surrounds the experts: the router product (fp32 logits), an
+ * unquantised shared expert's gate/up (act 6) and down (row_scale = its gate,
+ * residual = the routed experts' sum), plain projections.  x [M][K], w [N][K]
+ * bf16, rows ldx / ldw elements apart (any alignment; 0 repeats one row);
+ * bias [N], residual [M][N] and out [M][N] bf16 (flag 1) or fp32, rows ldr /
+ * ldo apart; row_scale fp32 [M], elements scale_stride apart; bias, row_scale
+ * and residual may be NULL.  act: 0 none, 1 relu, 2 silu, 3 gelu (erf), 4 gelu
+ * (tanh), 5 sigmoid, 6 swiglu: w and bias hold 2N rows, gate rows [0, N) then
+ * up rows, act = the experts' clamped gated SiLU (limit, alpha, beta; the
+ * others ignore them).  fp32 sums and epilogue, one rounding to out's type.
+ * out may be residual itself (same rows), else it overlaps no input.  M = 0
+ * returns at once.  The reference leaves these products to its host
+ * (vllm_xiaotu_moe/hybrid_model.py:1752 _shared_out, :1877 the router). */
+hipError_t xtu_linear(const void* x, long ldx, const void* w, long ldw, int M, int N, int K,
+                      int act, const void* bias, int bias_bf16, const float* row_scale,
+                      long scale_stride, const void* residual, int residual_bf16, long ldr,
+                      void* out, int out_bf16, long ldo, float limit, float alpha, float beta,
+                      hipStream_t stream);
+
 /* ------------------------------------------------ expert staging (ring / pool)
  * dst[i*dst_stride, +bytes) <- src[experts[i]*src_stride, +bytes), i < n, as
  * one hipMemcpyAsync per expert on `stream` (experts: host array; src/dst:
