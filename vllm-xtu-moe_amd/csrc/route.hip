@@ -142,6 +142,13 @@ __device__ void route_token(const float* __restrict__ l, const float* __restrict
     s.ce[c] = 0x7fffffff;
   }
   team_sync<TEAM>();
+  // NaN scores leave slots that no candidate takes: those hold expert k, a
+  // valid id, with what its score gives (K <= E)
+  if (tid < K) {
+    s.sel_e[tid] = tid;
+    s.sel_ws[tid] = valid ? s.ws[tid] : 0.f;
+    s.sel_sc[tid] = valid ? s.sc[tid] : 0.f;
+  }
   // rank inside the group / chunk; the K best of each become candidates
   if (valid) {
     for (int e = tid; e < E; e += TEAM) {
