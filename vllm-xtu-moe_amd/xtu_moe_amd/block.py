@@ -1,0 +1,129 @@
+"""The MoE block from hidden states: router product, selection, routed and
+shared experts.
+
+    logits = x Wg^T;  (ids, weights) = selection(logits)
+    y = sum_k weights_k E_{ids_k}(x) + sum_s g_s S_s(x),   g_s = sigmoid(x . v_s) or 1
+
+The layer entries of this package begin at router logits or at ids, as the
+reference's hook does (vllm_xiaotu_moe/mixed_experts.py:1919-2123); the block
+begins where a model's MoE layer does, at the hidden states, with the
+reference host's router (hybrid_model.py:1877) and shared expert (:1752)
+inside.
+"""
+from __future__ import annotations
+
+import torch
+
+from .layer import ExpertWeights, _same_device, moe_forward, route
+from .linear import _overlap, linear, on_stream
+
+MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 16, 64   # the routers' limits
+
+
+class MoeBlock:
+    """One layer's MoE block over resident experts.
+
+    gate_weight: bf16 [E, H], the router's rows.  weights: ExpertWeights (E
+    routed, then n_shared shared experts).  scoring "softmax" or "sigmoid"
+    (grouped, selection by score + bias), with the arguments of ``route``.
+    shared_gate: bf16 [n_shared, H]; shared expert s is scaled by
+    sigmoid(x . shared_gate[s]) (without it by 1).  swiglu_*: the clamped gated
+    SiLU of every expert.
+    """
+
+    def __init__(self, gate_weight, weights: ExpertWeights, *, top_k, scoring="softmax",
+                 renormalize=True, bias=None, n_group=1, topk_group=1, routed_scaling_factor=1.0,
+                 shared_gate=None, swiglu_limit=0.0, swiglu_alpha=1.0, swiglu_beta=0.0):
+        W = weights
+        self.check(gate_weight, W, top_k=top_k, scoring=scoring, bias=bias, n_group=n_group,
+                   topk_group=topk_group, shared_gate=shared_gate)
+        if not W.w13.is_cuda:
+            raise ValueError("the block needs device-resident expert weights")
+        _same_device(W.device, gate_weight=gate_weight, bias=bias, shared_gate=shared_gate)
+        self.W, self.gate_weight, self.shared_gate = W, gate_weight, shared_gate
+        self.top_k, self.scoring, self.renormalize = int(top_k), scoring, bool(renormalize)
+        self.bias = None if bias is None else bias.to(torch.float32).contiguous()
+        self.n_group, self.topk_group = int(n_group), int(topk_group)
+        self.routed_scaling_factor = float(routed_scaling_factor)
+        self.limit = float(swiglu_limit or 0.0)
+        self.alpha, self.beta = float(swiglu_alpha), float(swiglu_beta)
+        # the shared experts as further routed ones: their weight is then the
+        # gate's (the same planes)
+        self._W_all = None
+        if shared_gate is not None:
+            self._W_all = ExpertWeights(W.fmt, W.H, W.I, W.n_experts, 0, W.w13, W.s13, W.w2, W.s2,
+                                        W.gs13, W.gs2, mutable=W.mutable,
+                                        fp8_scales_ok=W.slot_fp8_scales_ok)
+
+    @staticmethod
+    def check(gate_weight, W, *, top_k, scoring="softmax", bias=None, n_group=1, topk_group=1,
+              shared_gate=None):
+        """Raises ValueError for a router or shared gate that does not fit W."""
+        if gate_weight is None:
+            raise ValueError("gate_weight is missing")
+        if shared_gate is not None and W.n_shared == 0:
+            raise ValueError("shared_gate without shared experts")
+        for name, t, n in (("gate_weight", gate_weight, W.E),
+                           ("shared_gate", shared_gate, W.n_shared)):
+            if t is not None and (tuple(t.shape) != (n, W.H) or t.dtype != torch.bfloat16
+                                  or not t.is_contiguous()):
+                raise ValueError(f"{name} must be contiguous bf16 [{n}, {W.H}], got "
+                                 f"{tuple(t.shape)} {t.dtype}")
+        if scoring not in ("softmax", "sigmoid"):
+            raise ValueError(f"unsupported scoring function {scoring!r}")
+        if bias is not None and (tuple(bias.shape) != (W.E,) or scoring != "sigmoid"):
+            raise ValueError(f"bias must be [{W.E}] and goes with sigmoid scoring")
+        top_k, n_group, topk_group = int(top_k), int(n_group), int(topk_group)
+        if not 1 <= top_k <= min(W.E, MAX_TOP_K):
+            raise ValueError(f"top_k {top_k} is not in 1 .. min(E, {MAX_TOP_K})")
+        if W.E > MAX_EXPERTS:
+            raise ValueError(f"{W.E} routed experts, at most {MAX_EXPERTS}")
+        if scoring == "sigmoid" and (not 1 <= n_group <= MAX_GROUPS or W.E % n_group
+                                     or not 1 <= topk_group <= n_group
+                                     or top_k > topk_group * (W.E // n_group)):
+            raise ValueError(f"{n_group} groups with {topk_group} kept do not fit {W.E} experts, "
+                             f"top {top_k}")
+
+    def __call__(self, x, *, out=None, out_dtype=None, return_routing=False, stream=None):
+        """x bf16 [T, H] -> [T, H] bf16 (or out_dtype fp32, or into out); with
+        return_routing (out, topk_weights fp32 [T, K], topk_ids int32 [T, K])."""
+        W = self.W
+        if x.dim() != 2 or x.dtype != torch.bfloat16 or not x.is_contiguous() \
+                or x.shape[1] != W.H:
+            raise ValueError(f"x must be contiguous bf16 [T, {W.H}], got {tuple(x.shape)} {x.dtype}")
+        odt = out.dtype if out is not None else out_dtype or torch.bfloat16
+        if odt not in (torch.bfloat16, torch.float32) or (out_dtype or odt) != odt:
+            raise ValueError(f"output type {odt} (out_dtype {out_dtype}): bf16 or fp32")
+        if out is not None and (tuple(out.shape) != tuple(x.shape) or not out.is_contiguous()):
+            raise ValueError(f"out must be contiguous {tuple(x.shape)}, got {tuple(out.shape)}")
+        _same_device(W.device, x=x, out=out)
+        if stream is not None or W.device.index != torch.cuda.current_device():
+            with on_stream(stream, W.device):
+                return self(x, out=out, out_dtype=out_dtype, return_routing=return_routing)
+        if out is not None and _overlap(out, x):
+            raise ValueError("out overlaps x")
+        if out is None:
+            out = torch.empty(x.shape, dtype=odt, device=x.device)
+        T = x.shape[0]
+        ids = torch.empty((T, self.top_k), dtype=torch.int32, device=x.device)
+        wts = torch.empty((T, self.top_k), dtype=torch.float32, device=x.device)
+        if T:
+            self._composed(x, out, ids, wts)
+        return (out, wts, ids) if return_routing else out
+
+    def _composed(self, x, out, ids, wts):
+        """Any number of tokens: the products and the layer one after the other."""
+        logits = linear(x, self.gate_weight, out_dtype=torch.float32)
+        kw = dict(scoring=self.scoring, bias=self.bias, n_group=self.n_group,
+                  topk_group=self.topk_group, routed_scaling_factor=self.routed_scaling_factor,
+                  renormalize=self.renormalize)
+        act = dict(swiglu_limit=self.limit, swiglu_alpha=self.alpha, swiglu_beta=self.beta,
+                   out=out)
+        if self.shared_gate is None:
+            moe_forward(x, ids, wts, self.W, router=dict(logits=logits, **kw), **act)
+            return
+        route(logits, top_k=self.top_k, ids_out=ids, wts_out=wts, **kw)
+        gates = linear(x, self.shared_gate, activation="sigmoid", out_dtype=torch.float32)
+        shared = torch.arange(self.W.E, self.W.n_experts, dtype=torch.int32, device=x.device)
+        moe_forward(x, torch.cat([ids, shared.expand(x.shape[0], -1)], 1),
+                    torch.cat([wts, gates], 1), self._W_all, **act)
