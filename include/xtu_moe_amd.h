@@ -607,13 +607,17 @@ hipError_t xtu_i8_row_fallback(int gate_up, const void* x, const int32_t* sorted
  * up rows, act = the experts' clamped gated SiLU (limit, alpha, beta; the
  * others ignore them).  fp32 sums and epilogue, one rounding to out's type.
  * out may be residual itself (same rows), else it overlaps no input.  M = 0
- * returns at once.  The reference leaves these products to its host
+ * returns at once.  workspace (16-byte aligned, may be NULL):
+ * xtu_linear_workspace_bytes() lets a product of few tiles split K, and one
+ * whose operands are not aligned (rows of x and w on 16 bytes, K % 8 == 0) copy
+ * them first; with less the call takes another way, slower.  The reference leaves these products to its host
  * (vllm_xiaotu_moe/hybrid_model.py:1752 _shared_out, :1877 the router). */
 hipError_t xtu_linear(const void* x, long ldx, const void* w, long ldw, int M, int N, int K,
                       int act, const void* bias, int bias_bf16, const float* row_scale,
                       long scale_stride, const void* residual, int residual_bf16, long ldr,
                       void* out, int out_bf16, long ldo, float limit, float alpha, float beta,
-                      hipStream_t stream);
+                      void* workspace, size_t workspace_bytes, hipStream_t stream);
+size_t xtu_linear_workspace_bytes(int M, int N, int K, int act, int aligned);
 
 /* ------------------------------------------------ expert staging (ring / pool)
  * dst[i*dst_stride, +bytes) <- src[experts[i]*src_stride, +bytes), i < n, as

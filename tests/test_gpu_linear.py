@@ -100,6 +100,18 @@ def test_swiglu_sizes(M, N, K):
     _check(out, x, w, "swiglu", b, limit=0.75, alpha=1.7, beta=1.0)
 
 
+@pytest.mark.parametrize("M,N,K", [(2100, 4096, 192), (4096, 2052, 1000), (3000, 3001, 129),
+                                   (257, 20000, 64), (20000, 300, 72), (2304, 256, 4096)])
+@pytest.mark.parametrize("act", ["none", "swiglu", "gelu"])
+def test_large_tiles(M, N, K, act):
+    rows = 2 * N if act == "swiglu" else N
+    x, w = _rand((M, K), 60), _rand((rows, K), 61, 0.05)
+    b, r = _rand((rows,), 62, 0.5, F32), _rand((M, N), 63)
+    for odt in (BF, F32):
+        _check(linear(x, w, bias=b, activation=act, residual=r, out_dtype=odt), x, w, act, b,
+               residual=r)
+
+
 @pytest.mark.parametrize("act", sorted(ACTIVATIONS))
 @pytest.mark.parametrize("M,N,K", [(4, 96, 256), (70, 200, 136), (300, 512, 1024)])
 @pytest.mark.parametrize("bias_dtype,res_dtype,scale", [(BF, F32, True), (F32, BF, False),

@@ -1,4 +1,6 @@
-// The dense product with its epilogue: dispatch and the kernel for any shape.
+// The dense product with its epilogue: dispatch, the join of K splits, and what
+// rows that do not start on 16 bytes need: a copy that makes them (linear_pack_kernel),
+// or, without a workspace for it, the kernel for any operands (linear_any_kernel).
 #include "linear.hpp"
 
 namespace xtu {
@@ -74,16 +76,106 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a) {
     for (int t = 0; t < 4; ++t) {
       if (GATED) {
         const int n = n0 + 16 * wn + 4 * q + t;
-        if (n < a.N) finish_one(a, m, n, acc[0][j][t], acc[1][j][t]);
+        if (n < a.N) finish_one<kActSwiglu>(a, m, n, acc[0][j][t], acc[1][j][t]);
       } else {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int n = n0 + 32 * wn + 16 * i + 4 * q + t;
-          if (n < a.N) finish_one(a, m, n, acc[i][j][t], 0.f);
+          if (n < a.N) finish_one<kActOther>(a, m, n, acc[i][j][t], 0.f);
         }
       }
     }
   }
+}
+
+// Adds the partial sums of the K splits, in their order, and finishes the
+// elements; one thread per V (4 or 1) columns of a row.
+template <int AK, int V>
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int split,
+                                                          const float* part) {
+  constexpr bool GATED = AK == kActSwiglu;
+  const int gn = a.N / V;
+  const long t = (long)blockIdx.x * 256 + threadIdx.x;
+  if (t >= (long)a.M * gn) return;
+  const int m = (int)(t / gn), n = (int)(t % gn) * V;
+  const long plane = part_plane(a);
+  const float* p = part + (long)m * a.N * (GATED ? 2 : 1) + n;
+  if constexpr (V == 4) {
+    f32x4_t z = {0.f, 0.f, 0.f, 0.f}, u = z;
+    for (int k = 0; k < split; ++k, p += plane) {
+      z += *reinterpret_cast<const f32x4_t*>(p);
+      if constexpr (GATED) u += *reinterpret_cast<const f32x4_t*>(p + a.N);
+    }
+    finish4<AK>(a, m, n, z, u);
+  } else {
+    float z = 0.f, u = 0.f;
+    for (int k = 0; k < split; ++k, p += plane) {
+      z += p[0];
+      if constexpr (GATED) u += p[a.N];
+    }
+    finish_one<AK>(a, m, n, z, u);
+  }
+}
+
+// x and w as rows of K8 = K rounded up to 8, zeros behind K: what the tile
+// kernels read.  1013 x 1187 by 771 rows of it: the two launches take 14 us where
+// linear_any_kernel takes 24.
+__global__ __launch_bounds__(256) void linear_pack_kernel(const uint16_t* x, long ldx, int M,
+                                                          const uint16_t* w, long ldw, int rows,
+                                                          int K, uint16_t* out) {
+  const int per = (K + 7) / 8;
+  const long p = (long)blockIdx.x * 256 + threadIdx.x;
+  if (p >= (long)(M + rows) * per) return;
+  const long r = p / per;
+  const int k = (int)(p - r * per) * 8;
+  const uint16_t* row = r < M ? x + r * ldx : w + (r - M) * ldw;
+  *reinterpret_cast<u32x4_t*>(out + p * 8) = load8(row, k, K);
+}
+
+}  // namespace
+
+hipError_t launch_join(const LinearArgs& a, int split, const float* part, hipStream_t stream) {
+  const long n = (long)a.M * (a.vec ? a.N / 4 : a.N);
+  void (*k)(LinearArgs, int, const float*);
+  if (a.act == kSwiglu) k = a.vec ? linear_join_kernel<kActSwiglu, 4> : linear_join_kernel<kActSwiglu, 1>;
+  else if (a.act == kNone) k = a.vec ? linear_join_kernel<kActNone, 4> : linear_join_kernel<kActNone, 1>;
+  else k = a.vec ? linear_join_kernel<kActOther, 4> : linear_join_kernel<kActOther, 1>;
+  k<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(a, split, part);
+  return hipPeekAtLastError();
+}
+
+hipError_t launch_any(const LinearArgs& a, hipStream_t stream) {
+  const int nb = a.act == kSwiglu ? kAnyN / 2 : kAnyN;
+  const long gm = (a.M + (long)kAnyM - 1) / kAnyM, gn = ((long)a.N + nb - 1) / nb;
+  const unsigned grid = (unsigned)(gm * gn);
+  if (a.act == kSwiglu) linear_any_kernel<true><<<grid, 256, 0, stream>>>(a);
+  else linear_any_kernel<false><<<grid, 256, 0, stream>>>(a);
+  return hipPeekAtLastError();
+}
+
+}  // namespace lin
+}  // namespace xtu
+
+namespace xtu {
+namespace lin {
+namespace {
+
+size_t pack_bytes(int M, long rows, int K) { return (size_t)(M + rows) * ((K + 7) / 8) * 16; }
+
+size_t split_bytes(const TilePlan& p, int M, long rows) {
+  return p.split > 1 ? (size_t)p.split * M * rows * 4 : 0;
+}
+
+hipError_t launch_pack(LinearArgs& a, long rows, void* ws, hipStream_t stream) {
+  const long K8 = (a.K + 7) / 8 * 8, pieces = (a.M + rows) * (K8 / 8);
+  uint16_t* out = reinterpret_cast<uint16_t*>(ws);
+  linear_pack_kernel<<<(unsigned)((pieces + 255) / 256), 256, 0, stream>>>(
+      a.x, a.ldx, a.M, a.w, a.ldw, (int)rows, a.K, out);
+  a.x = out;
+  a.w = out + a.M * K8;
+  a.ldx = a.ldw = K8;
+  a.K = (int)K8;
+  return hipPeekAtLastError();
 }
 
 }  // namespace
@@ -95,27 +187,63 @@ using namespace xtu::lin;
 
 extern "C" {
 
+size_t xtu_linear_workspace_bytes(int M, int N, int K, int act, int aligned) {
+  if (M <= 0 || N <= 0 || K <= 0 || N > (1 << 28) || K > (1 << 28)) return 0;
+  LinearArgs a{};
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.act = act;
+  if (skinny_fits(a)) return 0;
+  const long rows = (long)N * (act == kSwiglu ? 2 : 1);
+  const size_t pack = aligned ? 0 : pack_bytes(M, rows, K);
+  return pack + split_bytes(plan_tile(M, N, K, act == kSwiglu, true), M, rows);
+}
+
 hipError_t xtu_linear(const void* x, long ldx, const void* w, long ldw, int M, int N, int K,
                       int act, const void* bias, int bias_bf16, const float* row_scale,
                       long scale_stride, const void* residual, int residual_bf16, long ldr,
                       void* out, int out_bf16, long ldo, float limit, float alpha, float beta,
-                      hipStream_t stream) {
+                      void* workspace, size_t workspace_bytes, hipStream_t stream) {
   XTU_CHECK_ARG(M >= 0 && N >= 1 && K >= 1 && act >= kNone && act <= kSwiglu);
   XTU_CHECK_ARG(N <= (1 << 28) && K <= (1 << 28));
   if (M == 0) return hipSuccess;
   XTU_CHECK_ARG(x && w && out && ldx >= 0 && ldw >= 0 && ldr >= 0 && scale_stride >= 0);
   XTU_CHECK_ARG(M == 1 || ldo >= N);
-  const int nb = act == kSwiglu ? kAnyN / 2 : kAnyN;
-  const long gm = (M + (long)kAnyM - 1) / kAnyM, gn = ((long)N + nb - 1) / nb;
-  XTU_CHECK_ARG(gm * gn < (1L << 31));
-  (void)hipGetLastError();
+  XTU_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0);
+  const bool gated = act == kSwiglu;
+  const long gm = (M + (long)kAnyM - 1) / kAnyM, gn = ((long)N + kAnyN / 2 - 1) / (kAnyN / 2);
+  XTU_CHECK_ARG(gm * gn < (1L << 31) && (long)M * N < (1L << 38));   // grids
+  const auto al = [](const void* p, long bytes) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0;
+  };
+  // vectors of four elements in the epilogue
+  const int rb = residual_bf16 ? 8 : 16, ob = out_bf16 ? 8 : 16, bb = bias_bf16 ? 8 : 16;
+  const int vec = N % 4 == 0 && al(out, ob) && (M == 1 || ldo % 4 == 0) &&
+                  (!residual || (al(residual, rb) && (M == 1 || ldr % 4 == 0))) &&
+                  (!bias || al(bias, bb));
   LinearArgs a{(const uint16_t*)x, (const uint16_t*)w, ldx, ldw, M, N, K, act, bias, bias_bf16,
                row_scale, scale_stride, residual, residual_bf16, ldr, out, out_bf16, ldo, limit,
-               alpha, beta};
-  const unsigned grid = (unsigned)(gm * gn);
-  if (act == kSwiglu) linear_any_kernel<true><<<grid, 256, 0, stream>>>(a);
-  else linear_any_kernel<false><<<grid, 256, 0, stream>>>(a);
-  return hipPeekAtLastError();
+               alpha, beta, vec};
+  (void)hipGetLastError();
+  if (skinny_fits(a)) return launch_skinny(a, stream);
+  const long rows = (long)N * (gated ? 2 : 1);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  size_t left = ws ? workspace_bytes : 0;
+  if (!tile_fits(a)) {
+    const size_t need = pack_bytes(M, rows, K);
+    const long K8 = (K + 7) / 8 * 8;
+    if (left < need || 256 * K8 * 2 + K8 * 2 >= (1L << 31) ||
+        (M + rows) * (K8 / 8) >= (1L << 38))
+      return launch_any(a, stream);
+    const hipError_t e = launch_pack(a, rows, ws, stream);
+    if (e != hipSuccess) return e;
+    ws += need;
+    left -= need;
+  }
+  TilePlan p = plan_tile(M, N, a.K, gated, true);
+  if (split_bytes(p, M, rows) > left) p = plan_tile(M, N, a.K, gated, false);
+  return launch_tile_kind(p.kind, a, p.split, reinterpret_cast<float*>(ws), stream);
 }
 
 }  // extern "C"

@@ -30,7 +30,13 @@ struct LinearArgs {
   int out_bf16;
   long ldo;
   float limit, alpha, beta;
+  int vec;                // bias, residual and out take vectors of 4 elements
 };
+
+// Split K: the partial sums of one split, [M][rows of w] fp32.
+__host__ __device__ __forceinline__ long part_plane(const LinearArgs& a) {
+  return (long)a.M * a.N * (a.act == kSwiglu ? 2 : 1);
+}
 
 // NaN stays NaN in every activation (relu: the comparison is false for it).
 __device__ __forceinline__ float activate(int act, float z) {
@@ -50,13 +56,28 @@ __device__ __forceinline__ float load_bias(const LinearArgs& a, int n) {
                      : reinterpret_cast<const float*>(a.bias)[n];
 }
 
+// What a kernel's epilogue is compiled for: no activation, swiglu, or any of
+// the others (chosen at run time).  An epilogue's code is run through once per
+// tile, so its size counts: instructions fetched for the first time cost more
+// than they take to run (a 256 x 256 tile's epilogue took 24 us with every
+// activation inlined at each of its four row blocks).
+enum ActKind : int { kActNone = 0, kActSwiglu, kActOther };
+
+template <int AK>
+__device__ __forceinline__ float act_of(const LinearArgs& a, float z, float u) {
+  if constexpr (AK == kActNone) return z;
+  else if constexpr (AK == kActSwiglu) return silu_gate(z, u, a.limit, a.alpha, a.beta);
+  else return activate(a.act, z);
+}
+
 // One output element from its product(s): z, and for swiglu the up product u.
+template <int AK>
 __device__ __forceinline__ void finish_one(const LinearArgs& a, int m, int n, float z, float u) {
   if (a.bias) {
     z += load_bias(a, n);
-    if (a.act == kSwiglu) u += load_bias(a, a.N + n);
+    if constexpr (AK == kActSwiglu) u += load_bias(a, a.N + n);
   }
-  float y = a.act == kSwiglu ? silu_gate(z, u, a.limit, a.alpha, a.beta) : activate(a.act, z);
+  float y = act_of<AK>(a, z, u);
   if (a.scale) y *= a.scale[(long)m * a.sstride];
   if (a.res) {
     const long o = (long)m * a.ldr + n;
@@ -66,6 +87,44 @@ __device__ __forceinline__ void finish_one(const LinearArgs& a, int m, int n, fl
   const long o = (long)m * a.ldo + n;
   if (a.out_bf16) reinterpret_cast<uint16_t*>(a.out)[o] = f32_to_bf16(y);
   else reinterpret_cast<float*>(a.out)[o] = y;
+}
+
+__device__ __forceinline__ f32x4_t load4(const void* p, long o, int is_bf16) {
+  if (!is_bf16) return *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(p) + o);
+  const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + o);
+  return f32x4_t{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u),
+                 __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
+}
+
+// Columns n .. n + 3 of row m, all of them there (a.vec: N % 4 == 0).
+template <int AK>
+__device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, f32x4_t z, f32x4_t u) {
+  if (a.bias) {
+    z += load4(a.bias, n, a.bias_bf16);
+    if constexpr (AK == kActSwiglu) u += load4(a.bias, a.N + n, a.bias_bf16);
+  }
+  f32x4_t y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = act_of<AK>(a, z[e], u[e]);
+  if (a.scale) y *= a.scale[(long)m * a.sstride];
+  if (a.res) y += load4(a.res, (long)m * a.ldr + n, a.res_bf16);
+  const long o = (long)m * a.ldo + n;
+  if (a.out_bf16) {
+    uint2 v;
+    v.x = f32_to_bf16(y[0]) | (uint32_t)f32_to_bf16(y[1]) << 16;
+    v.y = f32_to_bf16(y[2]) | (uint32_t)f32_to_bf16(y[3]) << 16;
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + o) = v;
+  } else {
+    *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(a.out) + o) = y;
+  }
+}
+
+// Order this wave's LDS writes before its later LDS reads by other lanes: a
+// wave's LDS instructions execute in issue order, so only the compiler must
+// not move them.
+__device__ __forceinline__ void lds_order() {
+  __builtin_amdgcn_wave_barrier();
+  __asm__ __volatile__("" ::: "memory");
 }
 
 // Eight consecutive k of one row from k on, zeros past K.  Rows need not start
@@ -81,6 +140,23 @@ __device__ __forceinline__ u32x4_t load8(const uint16_t* row, int k, int K) {
   }
   return v;
 }
+
+struct TilePlan {
+  int kind, split;
+};
+TilePlan plan_tile(int M, int N, int K, bool gated, bool may_split);
+// Whether the tile kernels take the operands (16-byte rows, K % 8 == 0).
+bool tile_fits(const LinearArgs& a);
+// `split` K ranges; part: split * part_plane(a) floats when split > 1.
+hipError_t launch_tile_kind(int kind, const LinearArgs& a, int split, float* part,
+                            hipStream_t stream);
+// At most 16 rows of x, all of x in LDS; any alignment.
+constexpr int kSkinnyM = 16;
+constexpr size_t kSkinnyLds = 120 * 1024;
+bool skinny_fits(const LinearArgs& a);
+hipError_t launch_skinny(const LinearArgs& a, hipStream_t stream);
+hipError_t launch_any(const LinearArgs& a, hipStream_t stream);
+hipError_t launch_join(const LinearArgs& a, int split, const float* part, hipStream_t stream);
 
 }  // namespace lin
 }  // namespace xtu

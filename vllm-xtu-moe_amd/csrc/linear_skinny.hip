@@ -1,0 +1,177 @@
+// The dense product for at most 16 rows of x (linear.hpp has the formula): a
+// stream of w.  One workgroup of sixteen waves per panel of up to 16 output
+// columns (further panels in steps of the grid); the waves split K (swiglu:
+// eight on the gate rows, eight on the matching up rows) and their sums are
+// added through LDS in a fixed order.  All of x sits in LDS.  A wave keeps U MFMA
+// steps of 32 k of w in flight: a lane loads 16 bytes of its w row straight
+// into the operand registers, and each slot is loaded again, for what comes U
+// steps later, over panel ends too, as soon as it is used.  Rows past M or N
+// repeat the last one; what they give is not written.
+//
+// Few columns: a CU takes in about 25 GB/s whatever its waves ask for, so a
+// product of 256 columns by 7168 k in panels of 16 waits 14 us for 16 CUs; panels
+// of as few columns as give each CU one (the MFMA's other rows repeat the
+// panel's last row, at no further traffic) take 6.6 us.  512 gated columns by
+// 2048 k 7.8 -> 5.1 us.  Cached loads of w beat non-temporal ones here (28672
+// columns by 7168 k 73 us = 5.65 TB/s against 91).
+#include "linear.hpp"
+
+namespace xtu {
+namespace lin {
+namespace {
+
+constexpr int kSkW = 16;           // waves per workgroup
+constexpr int kSkinnyGrid = 256;   // one workgroup per CU
+
+// 16 bytes at a wave-uniform base plus a lane's 32-bit offset.
+template <bool ALIGNED>
+__device__ __forceinline__ u32x4_t load_w(const uint16_t* base, uint32_t off) {
+  const uint8_t* p = reinterpret_cast<const uint8_t*>(base) + off;
+  if constexpr (ALIGNED) {
+    return *reinterpret_cast<const u32x4_t*>(p);
+  } else {
+    u32x4_t v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+  }
+}
+
+template <bool GATED, bool ALIGNED, int U>
+__global__ __launch_bounds__(64 * kSkW) void linear_skinny_kernel(LinearArgs a, int rp) {
+  constexpr int KW = GATED ? kSkW / 2 : kSkW;   // waves along K
+  extern __shared__ __attribute__((aligned(16))) uint16_t xs[];   // [M][K32 + 8]
+  __shared__ f32x4_t red[2][kSkW][64];
+  const int tid = threadIdx.x, lane = tid % 64;
+  const int w = __builtin_amdgcn_readfirstlane(tid / 64);
+  const int kw = GATED ? w % KW : w;
+  const long up = GATED && w >= KW ? a.N : 0;   // first row of the wave's half
+  const int q = lane / 16, c = lane % 16;
+  const int npan = (a.N + rp - 1) / rp;
+  // whole steps of 32 k, dealt to the waves; the partial last one, if any,
+  // goes to the last wave along K
+  const int nst = a.K / 32;
+  const int s0 = kw * nst / KW, s1 = (kw + 1) * nst / KW;
+  const int nch = max((s1 - s0 + U - 1) / U, 1);
+  auto wbase = [&](int pan) { return a.w + (up + (long)rp * pan) * a.ldw; };
+  auto woffs = [&](int pan) {
+    return (uint32_t)(min(min(c, rp - 1), a.N - 1 - rp * pan) * a.ldw + 8 * q) * 2u;
+  };
+  // loads are unconditional (past the wave's range: its last step again, or
+  // for a wave without steps the row's start, not used), so that every wait
+  // is for exactly the slot about to be used
+  u32x4_t wv[U];
+  const int k_last = max(s1 - 1, s0 > 0 ? s0 - 1 : 0);
+  auto issue = [&](int i, const uint16_t* wb, uint32_t wo, int s) {
+    wv[i] = load_w<ALIGNED>(wb + 32L * min(s, k_last), wo);
+  };
+  int pan = blockIdx.x;
+  const uint16_t* wb = wbase(pan);
+  uint32_t wo = woffs(pan);
+  const bool any = nst > 0;   // K < 32: the partial step alone
+  if (any) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) issue(i, wb, wo, s0 + i);
+  }
+  __builtin_amdgcn_sched_barrier(0);   // x after the first loads of w
+  // x to LDS, zeros behind K up to a whole step
+  const int k32 = (a.K + 31) / 32 * 32, ldx = k32 + 8, per_row = k32 / 8;
+  for (int p = tid; p < a.M * per_row; p += 64 * kSkW) {
+    const int r = p / per_row, k = (p - r * per_row) * 8;
+    *reinterpret_cast<u32x4_t*>(xs + r * ldx + k) = load8(a.x + (long)r * a.ldx, k, a.K);
+  }
+  __syncthreads();
+  const uint16_t* xl = xs + min(c, a.M - 1) * ldx + 8 * q;
+
+  for (int it = 0; pan < npan; pan += gridDim.x, ++it) {
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    auto use = [&](int i, int s) {
+      if (s < s1) {
+        const u32x4_t xv = *reinterpret_cast<const u32x4_t*>(xl + 32 * s);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(wv[i]), as_bf16x8(xv), acc, 0, 0,
+                                                      0);
+      }
+    };
+    const int next = pan + (int)gridDim.x;
+    const uint16_t* nb = wbase(next < npan ? next : pan);
+    const uint32_t no = woffs(next < npan ? next : pan);
+    if (any) {
+      for (int ch = 0; ch + 1 < nch; ++ch) {
+        const int s = s0 + ch * U;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          use(i, s + i);
+          issue(i, wb, wo, s + U + i);
+        }
+      }
+      const int s = s0 + (nch - 1) * U;
+      if (next < npan) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          use(i, s + i);
+          issue(i, nb, no, s0 + i);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < U; ++i) use(i, s + i);
+      }
+    }
+    if (a.K % 32 && kw == KW - 1) {
+      const u32x4_t tw =
+          load8(wb + min(min(c, rp - 1), a.N - 1 - rp * pan) * a.ldw, 32 * nst + 8 * q, a.K);
+      const u32x4_t tx = *reinterpret_cast<const u32x4_t*>(xl + 32 * nst);
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(tw), as_bf16x8(tx), acc, 0, 0, 0);
+    }
+    red[it & 1][w][lane] = acc;
+    __syncthreads();   // the other half of red is written before the next barrier
+    if (tid < 256) {
+      const int e = tid / 64, nl = 4 * q + e, n = rp * pan + nl;
+      float z = 0.f, u = 0.f;
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        z += red[it & 1][k][lane][e];
+        if constexpr (GATED) u += red[it & 1][KW + k][lane][e];
+      }
+      if (c < a.M && nl < rp && n < a.N) finish_one<GATED ? kActSwiglu : kActOther>(a, c, n, z, u);
+    }
+    wb = nb;
+    wo = no;
+  }
+}
+
+size_t skinny_lds(const LinearArgs& a) { return (size_t)a.M * ((a.K + 31) / 32 * 32 + 8) * 2; }
+
+template <bool GATED, bool ALIGNED>
+hipError_t launch(const LinearArgs& a, hipStream_t stream) {
+  int rp = 2;   // columns of a panel: about one panel per CU, 16 at most
+  while (rp < 16 && (a.N + rp - 1) / rp > kSkinnyGrid) rp *= 2;
+  const int npan = (a.N + rp - 1) / rp;
+  const int grid = npan < kSkinnyGrid ? npan : kSkinnyGrid;
+  const size_t lds = skinny_lds(a);
+  // steps of a wave: U of them in flight
+  const bool few = a.K / 32 <= 4 * (GATED ? kSkW / 2 : kSkW);
+  auto k = few ? linear_skinny_kernel<GATED, ALIGNED, 4> : linear_skinny_kernel<GATED, ALIGNED, 8>;
+  if (lds > 32 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  k<<<grid, 64 * kSkW, lds, stream>>>(a, rp);
+  return hipPeekAtLastError();
+}
+
+}  // namespace
+
+bool skinny_fits(const LinearArgs& a) {
+  return a.M <= kSkinnyM && a.K <= (1 << 20) && skinny_lds(a) <= kSkinnyLds &&
+         16 * a.ldw * 2 < (1L << 31);
+}
+
+hipError_t launch_skinny(const LinearArgs& a, hipStream_t stream) {
+  const auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  const bool aligned = al(a.w) && a.ldw % 8 == 0;
+  if (a.act == kSwiglu) return aligned ? launch<true, true>(a, stream) : launch<true, false>(a, stream);
+  return aligned ? launch<false, true>(a, stream) : launch<false, false>(a, stream);
+}
+
+}  // namespace lin
+}  // namespace xtu

@@ -1,0 +1,434 @@
+// The dense product on matrix tiles staged through LDS (linear.hpp has the
+// formula).  A workgroup computes BM rows of x times BN rows of w, K in steps
+// of BK; the loads go from global memory straight to LDS, STAGES - 1 steps
+// ahead of the MFMAs.
+//
+// LDS: a stage holds BM + BN rows of BK k, x rows first.  The
+// 16-byte piece p of row r sits at slot p ^ (r & 7) (64-byte rows: p ^ (r / 2
+// & 3)), so that the eight lanes that a 16-byte LDS read serves together
+// (consecutive rows, one piece) touch all 32 banks; the loads write LDS linearly, so the swizzle is in the global
+// address of each lane.  Pieces past K are loaded out of the buffer's range,
+// which gives zeros; rows past M or N repeat the last row and are not written.
+//
+// The MFMA takes w as its A operand and x as B: a lane then holds four
+// consecutive output columns of one row, which the epilogue reads and writes
+// as vectors.  swiglu: the w rows of a tile alternate between gate and up in
+// blocks of 32 (16 on the 16-row blocks), so both products of an element sit
+// in one lane.
+#include "linear.hpp"
+
+namespace xtu {
+namespace lin {
+namespace {
+
+// 16 bytes per lane to LDS at dst + 16 * lane, from the buffer's base + off +
+// soff (zeros out of range).
+__device__ __forceinline__ void buf_to_lds(u32x4_t rsrc, uint32_t off, uint32_t soff,
+                                           const uint8_t* dst) {
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+               :: "v"(off), "s"(rsrc), "s"(soff), "{m0}"((uint32_t)(uintptr_t)dst)
+               : "memory");
+}
+
+// Raw buffer over [base, base + bytes), wave-uniform.
+__device__ __forceinline__ u32x4_t raw_buffer(const void* base, uint32_t bytes) {
+  const uint64_t p = reinterpret_cast<uint64_t>(base);
+  u32x4_t r = {(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, bytes, 0x00020000u};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
+  return r;
+}
+
+// s_waitcnt immediates: vmcnt(n), and vmcnt(n) with lgkmcnt(0)
+constexpr int wait_vm(int n) { return 0x0f70 | (n & 15) | ((n >> 4) << 14); }
+constexpr int wait_vm_lgkm0(int n) { return 0x0070 | (n & 15) | ((n >> 4) << 14); }
+
+// Slot of piece p of row r in an LDS row of PCS pieces.
+template <int PCS>
+__device__ __forceinline__ int slot_of(int p, int r) {
+  return p ^ (PCS == 4 ? (r >> 1) & 3 : r & 7);
+}
+
+// LDS row of the epilogue's sums, in floats (16 bytes of padding: eight
+// lanes' 16-byte writes to consecutive rows touch all banks).
+template <int WN>
+__host__ __device__ constexpr int epi_ld() { return WN + 4; }
+
+template <int MB>
+struct AccOf { typedef f32x16_t type; };
+template <>
+struct AccOf<16> { typedef f32x4_t type; };
+
+// WM x WN of x rows x w rows per wave, in MB x MB blocks (MB 32: the 32x32x16
+// MFMA, 16: 16x16x32).  SPLIT: the K range of blockIdx.y only, fp32 sums to
+// a plane of the workspace [split][M][w rows] (finished by linear_join_kernel).
+template <int BM, int BN, int WM, int WN, int MB, int BK, int STAGES, bool PIPE, int AK,
+          bool SPLIT, int OCC>
+__global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_kernel(
+    LinearArgs a, int kstep_per, float* part) {
+  constexpr bool GATED = AK == kActSwiglu;
+  constexpr int WAVES = BM / WM * (BN / WN), NT = WAVES * 64;
+  constexpr int PCS = BK / 8, LROW = BK * 2;   // 16-byte pieces and bytes of an LDS row
+  constexpr int ROWS = BM + BN, STAGE = ROWS * LROW;
+  constexpr int LOADS = ROWS * PCS / NT;       // per thread and step
+  constexpr int LEAD = STAGES - 1;
+  constexpr int NI = WN / MB, NJ = WM / MB;   // blocks of a wave
+  constexpr int KK = MB == 32 ? 16 : 32;      // k of an MFMA
+  constexpr int NB = GATED ? BN / 2 : BN;     // output columns of the tile
+  static_assert(ROWS * PCS % NT == 0 && BM * PCS % 64 == 0, "whole waves of loads");
+  static_assert(!PIPE || (BK / KK) % 2 == 0, "two sets of fragments in turn");
+  static_assert((STAGES - 1) * LOADS <= 63, "vmcnt");
+  static_assert(!GATED || NI % 2 == 0, "gate and up blocks pair up in a wave");
+  static_assert(MB % (64 / PCS) == 0, "a load stays within a block of rows");
+  typedef typename AccOf<MB>::type acc_t;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid % 64;
+  const int w = __builtin_amdgcn_readfirstlane(tid / 64);
+  const int wn = w % (BN / WN), wm = w / (BN / WN);
+
+  // tile: contiguous ranges of tiles per XCD (workgroup b runs on XCD b % 8),
+  // eight m tiles side by side so that concurrent workgroups share rows of both
+  const int gm = (a.M + BM - 1) / BM, gn = (a.N + NB - 1) / NB, total = gm * gn;
+  int t = blockIdx.x;
+  {
+    const int per = total / 8, rem = total % 8, x = t % 8;
+    t = x * per + min(x, rem) + t / 8;
+  }
+  const int grp = t / (8 * gn), rows_g = min(8, gm - 8 * grp), in_g = t - grp * 8 * gn;
+  const int m0 = (grp * 8 + in_g % rows_g) * BM, n0 = in_g / rows_g * NB;
+
+  // k steps of this workgroup
+  const int nk = (a.K + BK - 1) / BK;
+  const int s0 = SPLIT ? (int)blockIdx.y * kstep_per : 0;
+  const int s1 = SPLIT ? min(nk, s0 + kstep_per) : nk;
+
+  const int mrows = min(BM, a.M - m0);
+  const u32x4_t xr = raw_buffer(a.x + (long)m0 * a.ldx,
+                                (uint32_t)(((long)(mrows - 1) * a.ldx + a.K) * 2));
+  // w rows of the tile: from its first row, swiglu the same of the up half too
+  const int ncols = min(NB, a.N - n0);
+  const uint32_t wbytes = (uint32_t)(((long)(ncols - 1) * a.ldw + a.K) * 2);
+  const u32x4_t wr = raw_buffer(a.w + (long)n0 * a.ldw, wbytes);
+  const u32x4_t ur = GATED ? raw_buffer(a.w + (long)(a.N + n0) * a.ldw, wbytes) : wr;
+
+  // this thread's pieces of a step: piece c = (w * LOADS + j) * 64 + lane
+  uint32_t off[LOADS];
+  int kof[LOADS];
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) {
+    const int c = (w * LOADS + j) * 64 + lane;
+    const int r = c / PCS, p = slot_of<PCS>(c % PCS, r);
+    kof[j] = 8 * p;
+    if (r < BM) {
+      off[j] = (uint32_t)min(r, mrows - 1) * (uint32_t)(a.ldx * 2) + 16 * p;
+    } else {
+      const int rr = r - BM;
+      const int col = GATED ? rr / (2 * MB) * MB + rr % MB : rr;
+      off[j] = (uint32_t)min(col, ncols - 1) * (uint32_t)(a.ldw * 2) + 16 * p;
+    }
+  }
+  // the 64 / PCS rows of a wave's load are all x's, or all gate or up rows
+  u32x4_t rsrc[LOADS];
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) {
+    const int row = (w * LOADS + j) * (64 / PCS);
+    const bool isx = row < BM, isu = GATED && (row - BM) / MB % 2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      rsrc[j][i] = __builtin_amdgcn_readfirstlane(isx ? xr[i] : isu ? ur[i] : wr[i]);
+  }
+  auto issue_one = [&](int s, int st, int j) {
+    const bool tail = BK * s + BK > a.K;
+    const uint32_t o = tail && BK * s + kof[j] >= a.K ? 0x80000000u : off[j];
+    buf_to_lds(rsrc[j], o, (uint32_t)s * (uint32_t)LROW,
+               lds + st * STAGE + (w * LOADS + j) * 1024);
+  };
+  auto issue = [&](int s, int st) {
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) issue_one(s, st, j);
+  };
+
+  acc_t acc[NI][NJ];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int k = 0; k < (MB == 32 ? 16 : 4); ++k) acc[i][j][k] = 0.f;
+
+  const int rl = lane % MB, h = lane / MB;   // row of a block, k group of 8
+  const uint8_t* xb = lds + (WM * wm + rl) * LROW;
+  const uint8_t* wb = lds + (BM + WN * wn + rl) * LROW;
+  struct Frags {
+    u32x4_t w[NI], x[NJ];
+  };
+  // fragment f of k group kk: w block f, then x block f - NI
+  auto read_one = [&](Frags& fr, int st, int kk, int f) {
+    const int o = st * STAGE + slot_of<PCS>(kk * (KK / 8) + h, rl) * 16;
+    if (f < NI) fr.w[f] = *reinterpret_cast<const u32x4_t*>(wb + o + f * MB * LROW);
+    else fr.x[f - NI] = *reinterpret_cast<const u32x4_t*>(xb + o + (f - NI) * MB * LROW);
+  };
+  auto mma_one = [&](const Frags& fr, int n) {
+    const int i = n / NJ, j = n % NJ;
+    if constexpr (MB == 32)
+      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(fr.w[i]), as_bf16x8(fr.x[j]),
+                                                          acc[i][j], 0, 0, 0);
+    else
+      acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(fr.w[i]), as_bf16x8(fr.x[j]),
+                                                          acc[i][j], 0, 0, 0);
+  };
+
+  if constexpr (!PIPE) {
+    // Step s: wait for its loads (the later LEAD - 1 steps' may be in
+    // flight), meet the barrier (every wave is done with step s - 1, whose
+    // stage the loads of step s + LEAD take), issue them, multiply.
+#pragma unroll
+    for (int p = 0; p < LEAD; ++p)
+      if (s0 + p < s1) issue(s0 + p, p);
+    int st = 0, sl = LEAD % STAGES;
+    for (int s = s0; s < s1; ++s) {
+      if (s + LEAD <= s1) __builtin_amdgcn_s_waitcnt(wait_vm((LEAD - 1) * LOADS));
+      else __builtin_amdgcn_s_waitcnt(wait_vm(0));
+      __syncthreads();
+      if (s + LEAD < s1) issue(s + LEAD, sl);
+#pragma unroll
+      for (int kk = 0; kk < BK / KK; ++kk) {
+        Frags fr;
+#pragma unroll
+        for (int f = 0; f < NI + NJ; ++f) read_one(fr, st, kk, f);
+#pragma unroll
+        for (int n = 0; n < NI * NJ; ++n) mma_one(fr, n);
+      }
+      st = st + 1 == STAGES ? 0 : st + 1;
+      sl = sl + 1 == STAGES ? 0 : sl + 1;
+    }
+  } else {
+    // The barrier sits before a step's last k group: by then the fragments of
+    // all its groups are read (each group's between the MFMAs of the one
+    // before), so behind it the loads of step s + STAGES may take its stage;
+    // step s + 1 has landed, and its group 0 is read between the last group's
+    // MFMAs, as are the loads issued.  The MFMAs wait for nothing but the
+    // barrier itself.
+    constexpr int M = NI * NJ, R = NI + NJ, KG = BK / KK;
+#pragma unroll
+    for (int p = 0; p < STAGES; ++p)
+      if (s0 + p < s1) issue(s0 + p, p);
+    if (s0 + STAGES <= s1) __builtin_amdgcn_s_waitcnt(wait_vm((STAGES - 1) * LOADS));
+    else __builtin_amdgcn_s_waitcnt(wait_vm(0));
+    __syncthreads();
+    Frags f[2];
+#pragma unroll
+    for (int k = 0; k < R; ++k) read_one(f[0], 0, 0, k);
+    int st = 0;
+    for (int s = s0; s < s1; ++s) {
+#pragma unroll
+      for (int g = 0; g + 1 < KG; ++g)
+#pragma unroll
+        for (int n = 0; n < M; ++n) {
+          mma_one(f[g & 1], n);
+#pragma unroll
+          for (int k = n * R / M; k < (n + 1) * R / M; ++k)
+            read_one(f[(g + 1) & 1], st, g + 1, k);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      // step s + 1 landed (the STAGES - 2 after it may be in flight), the reads done
+      if (s + STAGES <= s1) __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((STAGES - 2) * LOADS));
+      else __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+      const bool ahead = s + STAGES < s1;
+      const int nst = st + 1 == STAGES ? 0 : st + 1;
+#pragma unroll
+      for (int n = 0; n < M; ++n) {
+        mma_one(f[(KG - 1) & 1], n);
+        // (the last step reads what lies in the next stage; not used)
+#pragma unroll
+        for (int k = n * R / M; k < (n + 1) * R / M; ++k) read_one(f[0], nst, 0, k);
+        if (ahead) {
+#pragma unroll
+          for (int d = n * LOADS / M; d < (n + 1) * LOADS / M; ++d) issue_one(s + STAGES, st, d);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      st = nst;
+    }
+  }
+
+  // Epilogue, MB rows of x at a time: the wave lays its sums out as rows in
+  // its own part of LDS, then takes them with consecutive lanes along a row
+  // (whole lines to memory).  The loops stay rolled (ActKind).
+  constexpr int LD = epi_ld<WN>();
+  constexpr int W = GATED ? WN / 2 : WN;   // output columns of the wave
+  __syncthreads();   // every wave is done with the stages
+  float* eb = reinterpret_cast<float*>(lds) + w * (MB * LD);
+  const int nw = n0 + W * wn;
+  float* plane = SPLIT ? part + (long)blockIdx.y * part_plane(a) : nullptr;
+#pragma unroll 1
+  for (int j = 0; j < NJ; ++j) {
+    lds_order();
+#pragma unroll
+    for (int jj = 0; jj < NJ; ++jj) {
+      if (jj != j) continue;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int g = 0; g < (MB == 32 ? 4 : 1); ++g) {
+          const f32x4_t v = {acc[i][jj][4 * g], acc[i][jj][4 * g + 1], acc[i][jj][4 * g + 2],
+                             acc[i][jj][4 * g + 3]};
+          *reinterpret_cast<f32x4_t*>(eb + rl * LD + MB * i + (MB == 32 ? 8 * g : 0) + 4 * h) = v;
+        }
+    }
+    lds_order();
+    const int mb = m0 + WM * wm + MB * j;
+    // column col of the wave: its gate (or only) sum's place in the row
+    auto place = [&](int col) { return GATED ? col / MB * 2 * MB + col % MB : col; };
+    if (a.vec) {
+#pragma unroll 1
+      for (int c = lane; c < MB * W / 4; c += 64) {
+        const int r = c / (W / 4), col = c % (W / 4) * 4;
+        const int m = mb + r, n = nw + col;
+        if (m >= a.M || n >= a.N) continue;
+        const float* row = eb + r * LD + place(col);
+        const f32x4_t z = *reinterpret_cast<const f32x4_t*>(row);
+        f32x4_t u = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (GATED) u = *reinterpret_cast<const f32x4_t*>(row + MB);
+        if constexpr (SPLIT) {
+          float* pr = plane + (long)m * a.N * (GATED ? 2 : 1) + n;
+          *reinterpret_cast<f32x4_t*>(pr) = z;
+          if constexpr (GATED) *reinterpret_cast<f32x4_t*>(pr + a.N) = u;
+        } else {
+          finish4<AK>(a, m, n, z, u);
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int c = lane; c < MB * W; c += 64) {
+        const int r = c / W, col = c % W;
+        const int m = mb + r, n = nw + col;
+        if (m >= a.M || n >= a.N) continue;
+        const float* row = eb + r * LD + place(col);
+        const float z = row[0], u = GATED ? row[MB] : 0.f;
+        if constexpr (SPLIT) {
+          float* pr = plane + (long)m * a.N * (GATED ? 2 : 1) + n;
+          pr[0] = z;
+          if constexpr (GATED) pr[a.N] = u;
+        } else {
+          finish_one<AK>(a, m, n, z, u);
+        }
+      }
+    }
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int MB, int BK, int STAGES, bool PIPE, int OCC>
+hipError_t launch_tile(const LinearArgs& a, int split, float* part, hipStream_t stream) {
+  const bool gated = a.act == kSwiglu;
+  const int nb = gated ? BN / 2 : BN;
+  const long gm = ((long)a.M + BM - 1) / BM, gn = ((long)a.N + nb - 1) / nb;
+  const int nk = (a.K + BK - 1) / BK;
+  const int per = (nk + split - 1) / split;
+  split = (nk + per - 1) / per;   // no empty range
+  constexpr int WAVES = BM / WM * (BN / WN), NT = WAVES * 64;
+  constexpr size_t kStages = (size_t)STAGES * (BM + BN) * BK * 2;
+  constexpr size_t kEpi = (size_t)WAVES * MB * epi_ld<WN>() * 4;
+  constexpr size_t lds = kStages > kEpi ? kStages : kEpi;
+  static_assert(lds <= 160 * 1024, "LDS of a CU");
+  const dim3 grid((unsigned)(gm * gn), (unsigned)split);
+  void (*k)(LinearArgs, int, float*) = nullptr;
+  if (split > 1)
+    k = gated ? linear_tile_kernel<BM, BN, WM, WN, MB, BK, STAGES, PIPE, kActSwiglu, true, OCC>
+              : linear_tile_kernel<BM, BN, WM, WN, MB, BK, STAGES, PIPE, kActNone, true, OCC>;
+  else if (gated)
+    k = linear_tile_kernel<BM, BN, WM, WN, MB, BK, STAGES, PIPE, kActSwiglu, false, OCC>;
+  else if (a.act == kNone)
+    k = linear_tile_kernel<BM, BN, WM, WN, MB, BK, STAGES, PIPE, kActNone, false, OCC>;
+  else
+    k = linear_tile_kernel<BM, BN, WM, WN, MB, BK, STAGES, PIPE, kActOther, false, OCC>;
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  k<<<grid, NT, lds, stream>>>(a, per, part);
+  hipError_t e = hipPeekAtLastError();
+  if (e == hipSuccess && split > 1) e = launch_join(a, split, part, stream);
+  return e;
+}
+
+}  // namespace
+
+bool tile_fits(const LinearArgs& a) {
+  const auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  if (!al(a.x) || !al(a.w) || a.K % 8) return false;
+  if ((a.M > 1 && a.ldx % 8) || a.ldw % 8) return false;
+  // 32-bit offsets inside a tile
+  return (256 * a.ldx + a.K) * 2 < (1L << 31) && (256 * a.ldw + a.K) * 2 < (1L << 31);
+}
+
+namespace {
+
+// The variants: tile, k of a step, workgroups that share a CU, and what they
+// cost on MI355X, in us: t[i] a step, o[i] a round beside its steps, with i + 1
+// workgroups on a CU.  Fitted to products that fill the chip one to three times
+// over at K = 256, 1024 and 4096 (64 x 64: one per CU 4.6 / 8.5 / 22.5, two
+// 6.3 / 11.2 / 30.6, three 8.8 / 16.4 / 51.4; 256 x 256: 22.5 / 41.6 / 127).
+struct TileKind {
+  int m, n, k, occ;
+  float t[2], o[2];
+};
+constexpr TileKind kTileKinds[] = {
+    {64, 32, 128, 1, {0.42f, 0.42f}, {1.2f, 1.2f}},
+    {64, 64, 64, 2, {0.295f, 0.40f}, {1.2f, 1.9f}},
+    {128, 64, 64, 2, {0.42f, 0.69f}, {3.2f, 3.6f}},
+    {128, 128, 64, 2, {0.78f, 1.12f}, {3.5f, 5.5f}},
+    {256, 256, 64, 1, {1.72f, 1.72f}, {12.0f, 12.0f}},
+};
+constexpr float kLaunch = 2.3f;
+constexpr int kCus = 256;
+
+}  // namespace
+
+// The variant and K split with the least estimated time.  A split costs the
+// second launch that adds the partial sums, and their way through memory.
+TilePlan plan_tile(int M, int N, int K, bool gated, bool may_split) {
+  TilePlan best{0, 1};
+  float best_t = 1e30f;
+  for (int kind = 0; kind < (int)(sizeof(kTileKinds) / sizeof(kTileKinds[0])); ++kind) {
+    const TileKind& v = kTileKinds[kind];
+    const int nb = gated ? v.n / 2 : v.n;
+    const long tiles1 = (((long)M + v.m - 1) / v.m) * (((long)N + nb - 1) / nb);
+    const int nk = (K + v.k - 1) / v.k;
+    for (int split : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      if (split > 1 && (!may_split || nk < 2 * split || tiles1 >= 2 * kCus)) break;
+      const int steps = (nk + split - 1) / split;
+      const long tiles = tiles1 * ((nk + steps - 1) / steps);
+      const long full = tiles / (kCus * v.occ), rem = tiles % (kCus * v.occ);
+      float t = kLaunch + full * (v.t[v.occ - 1] * steps + v.o[v.occ - 1]);
+      if (rem) {
+        const int i = (int)((rem + kCus - 1) / kCus) - 1;
+        t += v.t[i] * steps + v.o[i];
+      }
+      if (split > 1) t += 3.0f + 2.0f * split * M * (float)N * (gated ? 2 : 1) * 4.0f / 5e6f;
+      if (t < best_t) {
+        best_t = t;
+        best = TilePlan{kind, split};
+      }
+    }
+  }
+  return best;
+}
+
+hipError_t launch_tile_kind(int kind, const LinearArgs& a, int split, float* part,
+                            hipStream_t stream) {
+  switch (kind) {
+    case 0: return launch_tile<64, 32, 16, 32, 16, 128, 4, false, 1>(a, split, part, stream);
+    case 1: return launch_tile<64, 64, 16, 32, 16, 64, 4, false, 4>(a, split, part, stream);
+    case 2: return launch_tile<128, 64, 64, 32, 16, 64, 3, false, 2>(a, split, part, stream);
+    case 3: return launch_tile<128, 128, 32, 64, 32, 64, 2, true, 4>(a, split, part, stream);
+    case 4: return launch_tile<256, 256, 128, 64, 32, 64, 2, true, 2>(a, split, part, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace lin
+}  // namespace xtu

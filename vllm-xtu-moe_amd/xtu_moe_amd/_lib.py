@@ -108,7 +108,8 @@ SIGNATURES = {
     "xtu_gemm_pair_down": (_i, [_i, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _l, _l, _vp, _vp, _vp,
                                 _vp, _vp, _vp, _vp, _i, _vp, _vp]),
     "xtu_linear": (_i, [_vp, _l, _vp, _l, _i, _i, _i, _i, _vp, _i, _vp, _l, _vp, _i, _l, _vp, _i,
-                        _l, _f, _f, _f, _vp]),
+                        _l, _f, _f, _f, _vp, _sz, _vp]),
+    "xtu_linear_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "xtu_copy_experts": (_i, [_i, _vp, _vp, _l, _vp, _l, _l, _vp]),
     "xtu_copy_2d": (_i, [_vp, _sz, _vp, _sz, _sz, _sz, _vp]),
     "xtu_i8_weight_bytes": (_sz, [_i, _i]),
@@ -154,7 +155,7 @@ _NOT_STATUS = {"xtu_version", "xtu_error_string", "xtu_segment_workspace_bytes",
                "xtu_decode_down_combine_ok", "xtu_decode_route_shared_ok",
                "xtu_decode_route_gate_up_ok", "xtu_decode_layer_ok",
                "xtu_decode_layer_barrier_words",
-               "xtu_i8_weight_bytes"}
+               "xtu_i8_weight_bytes", "xtu_linear_workspace_bytes"}
 
 _LIB = None
 

@@ -20,6 +20,8 @@ from .layer import _p, _same_device, _stream
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "sigmoid": 5,
                "swiglu": 6}
+# workspace bytes per (M, N, K, swiglu, aligned)
+_WS_BYTES: dict = {}
 _TYPES = (torch.bfloat16, torch.float32)
 
 
@@ -132,9 +134,18 @@ def linear(x, w, *, bias=None, activation="none", row_scale=None, residual=None,
         out = torch.empty((M, N), dtype=odt, device=dev)
     if M == 0:
         return out
-    _lib.call("xtu_linear", _p(x), ldx, _p(w), ldw, M, N, K, act, _p(bias),
-            int(bias is not None and bias.dtype == torch.bfloat16), _p(row_scale), sst,
-            _p(residual), int(residual is not None and residual.dtype == torch.bfloat16), ldr,
-            _p(out), int(out.dtype == torch.bfloat16), ldo, float(swiglu_limit or 0.0),
-              float(swiglu_alpha), float(swiglu_beta), _stream())
+    xp, wp = x.data_ptr(), w.data_ptr()
+    aligned = not ((ldx if M > 1 else 0) | ldw | K) & 7 and not (xp | wp) & 15
+    key = (M, N, K, act == 6, aligned)
+    nws = _WS_BYTES.get(key)
+    if nws is None:
+        nws = _WS_BYTES[key] = int(_lib.call("xtu_linear_workspace_bytes", M, N, K, act,
+                                             int(aligned)))
+    # allocated per call: calls on other streams, and graphs, have their own
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    _lib.call("xtu_linear", xp, ldx, wp, ldw, M, N, K, act, _p(bias),
+              int(bias is not None and bias.dtype == torch.bfloat16), _p(row_scale), sst,
+              _p(residual), int(residual is not None and residual.dtype == torch.bfloat16), ldr,
+              out.data_ptr(), int(odt == torch.bfloat16), ldo, float(swiglu_limit or 0.0),
+              float(swiglu_alpha), float(swiglu_beta), _p(ws), nws, _stream())
     return out
