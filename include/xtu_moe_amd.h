@@ -612,12 +612,60 @@ hipError_t xtu_i8_row_fallback(int gate_up, const void* x, const int32_t* sorted
  * whose operands are not aligned (rows of x and w on 16 bytes, K % 8 == 0) copy
  * them first; with less the call takes another way, slower.  The reference leaves these products to its host
  * (vllm_xiaotu_moe/hybrid_model.py:1752 _shared_out, :1877 the router). */
-hipError_t xtu_linear(const void* x, long ldx, const void* w, long ldw, int M, int N, int K,
-                      int act, const void* bias, int bias_bf16, const float* row_scale,
-                      long scale_stride, const void* residual, int residual_bf16, long ldr,
-                      void* out, int out_bf16, long ldo, float limit, float alpha, float beta,
-                      void* workspace, size_t workspace_bytes, hipStream_t stream);
+typedef struct xtu_linear_args {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const float* row_scale;
+  const void* residual;
+  void* out;
+  void* workspace;
+  long ldx, ldw, ldr, ldo, scale_stride;
+  size_t workspace_bytes;
+  int M, N, K, act;
+  int bias_bf16, residual_bf16, out_bf16;
+  float limit, alpha, beta;
+} xtu_linear_args;
+hipError_t xtu_linear(const xtu_linear_args* args, hipStream_t stream);
 size_t xtu_linear_workspace_bytes(int M, int N, int K, int act, int aligned);
+
+/* ------------------------------------------------ MoE block of a few tokens
+ * From hidden states x bf16 [T][H] to the layer's output, in two launches:
+ * router product with gate bf16 [E][H], selection (mode 0 softmax, 1 grouped
+ * sigmoid + bias, as xtu_route_*), routed experts, shared experts (slots E ..
+ * E + n_shared of the planes, scaled by sigmoid(x . shared_gate[s]) with
+ * shared_gate bf16 [n_shared][H], else 1), weighted sum.  out bf16 or fp32
+ * [T][H]; ids int32 / weights fp32 [T][K] get the selection.  Planes in the
+ * device layout, dense (no expert strides); pointers on 16 bytes.
+ * xtu_few_workspace_bytes: 0 where the shape does not fit (T <= 16, T K <= 256,
+ * E <= 1024, n_shared <= 4, H % 256 == 0, I % 128 == 0, the x rows in a CU's LDS;
+ * xtu_few_block then refuses).  The workspace carries nothing from call to
+ * call; calls that may overlap each need their own.  Replaces, for decode, the
+ * host's router and shared expert (vllm_xiaotu_moe/hybrid_model.py:1877, :1752)
+ * with _build_segmentation (gpu_prefill.py:849-887) and moe4_smallm_gu2 / dn2
+ * (moe4_smallm.cu:395-430). */
+typedef struct xtu_few_args {
+  const void* x;
+  const void* gate;
+  const void* shared_gate;
+  const float* bias;
+  const void* w13;
+  const void* s13;
+  const float* gs13;
+  const void* w2;
+  const void* s2;
+  const float* gs2;
+  void* out;
+  int32_t* ids;
+  float* weights;
+  void* workspace;
+  size_t workspace_bytes;
+  int fmt, T, H, I, E, n_shared, K;
+  int mode, renormalize, n_group, topk_group, out_bf16;
+  float routed_scaling, limit, alpha, beta;
+} xtu_few_args;
+size_t xtu_few_workspace_bytes(int T, int E, int K, int n_shared, int H, int I);
+hipError_t xtu_few_block(const xtu_few_args* args, hipStream_t stream);
 
 /* ------------------------------------------------ expert staging (ring / pool)
  * dst[i*dst_stride, +bytes) <- src[experts[i]*src_stride, +bytes), i < n, as

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from xtu_moe_amd import _lib
-from xtu_moe_amd.linear import ACTIVATIONS, linear
+from xtu_moe_amd.linear import ACTIVATIONS, ARGS, linear
 
 BF = torch.bfloat16
 
@@ -75,13 +75,13 @@ def test_outputs_refused():
 def test_entry_refuses_on_the_host():
     call = _lib.load().xtu_linear
 
-    def rc(x=16, ldx=8, w=16, ldw=8, M=1, N=1, K=1, act=0, out=16, ldo=8, ldr=0, sst=0,
-           ws=None):
-        return call(x, ldx, w, ldw, M, N, K, act, None, 0, None, sst, None, 0, ldr, out, 1, ldo,
-                    0.0, 1.0, 0.0, ws, 0, None)
+    def rc(x=16, ldx=8, w=16, ldw=8, M=1, N=1, K=1, act=0, out=16, ldo=8, ldr=0, sst=0, ws=0):
+        return call(ARGS.pack(x, w, 0, 0, 0, out, ws, ldx, ldw, ldr, ldo, sst, 0, M, N, K, act, 0,
+                              0, 1, 0.0, 1.0, 0.0), None)
 
+    assert call(None, None) == 1
     assert rc(M=0) == 0                       # nothing to do, nothing launched
-    for bad in (dict(x=None), dict(w=None), dict(out=None), dict(M=-1), dict(N=0), dict(K=0),
+    for bad in (dict(x=0), dict(w=0), dict(out=0), dict(M=-1), dict(N=0), dict(K=0),
                 dict(act=7), dict(act=-1), dict(ldx=-1), dict(ldw=-1), dict(ldr=-1),
                 dict(sst=-1), dict(ws=8), dict(M=2, N=9), dict(N=1 << 29), dict(K=1 << 29),
                 dict(M=1 << 30, N=1 << 20, ldo=1 << 20)):

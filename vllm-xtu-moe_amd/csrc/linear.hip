@@ -3,6 +3,8 @@
 // or, without a workspace for it, the kernel for any operands (linear_any_kernel).
 #include "linear.hpp"
 
+#include "../../include/xtu_moe_amd.h"
+
 namespace xtu {
 namespace lin {
 namespace {
@@ -200,17 +202,17 @@ size_t xtu_linear_workspace_bytes(int M, int N, int K, int act, int aligned) {
   return pack + split_bytes(plan_tile(M, N, K, act == kSwiglu, true), M, rows);
 }
 
-hipError_t xtu_linear(const void* x, long ldx, const void* w, long ldw, int M, int N, int K,
-                      int act, const void* bias, int bias_bf16, const float* row_scale,
-                      long scale_stride, const void* residual, int residual_bf16, long ldr,
-                      void* out, int out_bf16, long ldo, float limit, float alpha, float beta,
-                      void* workspace, size_t workspace_bytes, hipStream_t stream) {
+hipError_t xtu_linear(const xtu_linear_args* args, hipStream_t stream) {
+  XTU_CHECK_ARG(args);
+  const xtu_linear_args& t = *args;
+  const int M = t.M, N = t.N, K = t.K, act = t.act;
   XTU_CHECK_ARG(M >= 0 && N >= 1 && K >= 1 && act >= kNone && act <= kSwiglu);
   XTU_CHECK_ARG(N <= (1 << 28) && K <= (1 << 28));
   if (M == 0) return hipSuccess;
-  XTU_CHECK_ARG(x && w && out && ldx >= 0 && ldw >= 0 && ldr >= 0 && scale_stride >= 0);
-  XTU_CHECK_ARG(M == 1 || ldo >= N);
-  XTU_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0);
+  XTU_CHECK_ARG(t.x && t.w && t.out && t.ldx >= 0 && t.ldw >= 0 && t.ldr >= 0 &&
+                t.scale_stride >= 0);
+  XTU_CHECK_ARG(M == 1 || t.ldo >= N);
+  XTU_CHECK_ARG(reinterpret_cast<uintptr_t>(t.workspace) % 16 == 0);
   const bool gated = act == kSwiglu;
   const long gm = (M + (long)kAnyM - 1) / kAnyM, gn = ((long)N + kAnyN / 2 - 1) / (kAnyN / 2);
   XTU_CHECK_ARG(gm * gn < (1L << 31) && (long)M * N < (1L << 38));   // grids
@@ -218,18 +220,18 @@ hipError_t xtu_linear(const void* x, long ldx, const void* w, long ldw, int M, i
     return reinterpret_cast<uintptr_t>(p) % bytes == 0;
   };
   // vectors of four elements in the epilogue
-  const int rb = residual_bf16 ? 8 : 16, ob = out_bf16 ? 8 : 16, bb = bias_bf16 ? 8 : 16;
-  const int vec = N % 4 == 0 && al(out, ob) && (M == 1 || ldo % 4 == 0) &&
-                  (!residual || (al(residual, rb) && (M == 1 || ldr % 4 == 0))) &&
-                  (!bias || al(bias, bb));
-  LinearArgs a{(const uint16_t*)x, (const uint16_t*)w, ldx, ldw, M, N, K, act, bias, bias_bf16,
-               row_scale, scale_stride, residual, residual_bf16, ldr, out, out_bf16, ldo, limit,
-               alpha, beta, vec};
+  const int vec = N % 4 == 0 && al(t.out, t.out_bf16 ? 8 : 16) && (M == 1 || t.ldo % 4 == 0) &&
+                  (!t.residual || (al(t.residual, t.residual_bf16 ? 8 : 16) &&
+                                   (M == 1 || t.ldr % 4 == 0))) &&
+                  (!t.bias || al(t.bias, t.bias_bf16 ? 8 : 16));
+  LinearArgs a{(const uint16_t*)t.x, (const uint16_t*)t.w, t.ldx, t.ldw, M, N, K, act, t.bias,
+               t.bias_bf16, t.row_scale, t.scale_stride, t.residual, t.residual_bf16, t.ldr,
+               t.out, t.out_bf16, t.ldo, t.limit, t.alpha, t.beta, vec};
   (void)hipGetLastError();
   if (skinny_fits(a)) return launch_skinny(a, stream);
   const long rows = (long)N * (gated ? 2 : 1);
-  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-  size_t left = ws ? workspace_bytes : 0;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(t.workspace);
+  size_t left = ws ? t.workspace_bytes : 0;
   if (!tile_fits(a)) {
     const size_t need = pack_bytes(M, rows, K);
     const long K8 = (K + 7) / 8 * 8;

@@ -150,11 +150,6 @@ hipError_t launch(const LinearArgs& a, hipStream_t stream) {
   // steps of a wave: U of them in flight
   const bool few = a.K / 32 <= 4 * (GATED ? kSkW / 2 : kSkW);
   auto k = few ? linear_skinny_kernel<GATED, ALIGNED, 4> : linear_skinny_kernel<GATED, ALIGNED, 8>;
-  if (lds > 32 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
-  }
   k<<<grid, 64 * kSkW, lds, stream>>>(a, rp);
   return hipPeekAtLastError();
 }

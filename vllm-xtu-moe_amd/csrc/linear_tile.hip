@@ -344,11 +344,6 @@ hipError_t launch_tile(const LinearArgs& a, int split, float* part, hipStream_t 
     k = linear_tile_kernel<BM, BN, WM, WN, MB, BK, STAGES, PIPE, kActNone, false, OCC>;
   else
     k = linear_tile_kernel<BM, BN, WM, WN, MB, BK, STAGES, PIPE, kActOther, false, OCC>;
-  if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
-  }
   k<<<grid, NT, lds, stream>>>(a, per, part);
   hipError_t e = hipPeekAtLastError();
   if (e == hipSuccess && split > 1) e = launch_join(a, split, part, stream);

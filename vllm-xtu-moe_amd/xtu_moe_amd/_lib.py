@@ -107,8 +107,9 @@ SIGNATURES = {
                                    _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _f, _f, _f, _vp]),
     "xtu_gemm_pair_down": (_i, [_i, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _l, _l, _vp, _vp, _vp,
                                 _vp, _vp, _vp, _vp, _i, _vp, _vp]),
-    "xtu_linear": (_i, [_vp, _l, _vp, _l, _i, _i, _i, _i, _vp, _i, _vp, _l, _vp, _i, _l, _vp, _i,
-                        _l, _f, _f, _f, _vp, _sz, _vp]),
+    "xtu_few_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "xtu_few_block": (_i, [_vp, _vp]),
+    "xtu_linear": (_i, [_vp, _vp]),
     "xtu_linear_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "xtu_copy_experts": (_i, [_i, _vp, _vp, _l, _vp, _l, _l, _vp]),
     "xtu_copy_2d": (_i, [_vp, _sz, _vp, _sz, _sz, _sz, _vp]),
@@ -155,7 +156,8 @@ _NOT_STATUS = {"xtu_version", "xtu_error_string", "xtu_segment_workspace_bytes",
                "xtu_decode_down_combine_ok", "xtu_decode_route_shared_ok",
                "xtu_decode_route_gate_up_ok", "xtu_decode_layer_ok",
                "xtu_decode_layer_barrier_words",
-               "xtu_i8_weight_bytes", "xtu_linear_workspace_bytes"}
+               "xtu_i8_weight_bytes", "xtu_few_workspace_bytes",
+               "xtu_linear_workspace_bytes"}
 
 _LIB = None
 
@@ -183,13 +185,19 @@ def exported_symbols() -> list[str]:
     return sorted(SIGNATURES)
 
 
+def check(name: str, rc: int):
+    """Raise on a non-zero hipError_t that entry point `name` returned."""
+    if rc != 0:
+        msg = load().xtu_error_string(int(rc))
+        raise RuntimeError(f"{name} failed: hipError {rc} ({msg.decode() if msg else '?'})")
+
+
 def call(name: str, *args):
     """Call an entry point; raise on a non-zero hipError_t."""
     fn = getattr(load(), name)
     rc = fn(*args)
-    if name not in _NOT_STATUS and rc != 0:
-        msg = load().xtu_error_string(int(rc))
-        raise RuntimeError(f"{name} failed: hipError {rc} ({msg.decode() if msg else '?'})")
+    if name not in _NOT_STATUS:
+        check(name, rc)
     return rc
 
 

@@ -12,11 +12,19 @@ inside.
 """
 from __future__ import annotations
 
+import struct
+
 import torch
 
+from . import _lib
+from .formats import FMT_BF16, FMT_FP8, FMT_MXFP4, FMT_NVFP4
 from .layer import ExpertWeights, _same_device, moe_forward, route
-from .linear import _overlap, linear, on_stream
+from .linear import _current_device, _overlap, linear, on_stream, raw_stream
 
+# xtu_few_args: x, gate, shared_gate, bias, six planes, out, ids, weights,
+# workspace; its bytes; fmt, T, H, I, E, n_shared, K, mode, renormalize, n_group,
+# topk_group, out_bf16; routed_scaling, limit, alpha, beta
+ARGS = struct.Struct("@14PN12i4f")
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 16, 64   # the routers' limits
 
 
@@ -39,6 +47,8 @@ class MoeBlock:
                    topk_group=topk_group, shared_gate=shared_gate)
         if not W.w13.is_cuda:
             raise ValueError("the block needs device-resident expert weights")
+        if W.fmt not in (FMT_BF16, FMT_FP8, FMT_MXFP4, FMT_NVFP4) or W.n_slots != W.n_experts:
+            raise ValueError("the block needs BF16, FP8, MXFP4 or NVFP4 planes of every expert")
         _same_device(W.device, gate_weight=gate_weight, bias=bias, shared_gate=shared_gate)
         self.W, self.gate_weight, self.shared_gate = W, gate_weight, shared_gate
         self.top_k, self.scoring, self.renormalize = int(top_k), scoring, bool(renormalize)
@@ -47,6 +57,18 @@ class MoeBlock:
         self.routed_scaling_factor = float(routed_scaling_factor)
         self.limit = float(swiglu_limit or 0.0)
         self.alpha, self.beta = float(swiglu_alpha), float(swiglu_beta)
+        # what xtu_few_block takes of the layer, in its order
+        ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+        if any(ptr(t) & 15 for t in (gate_weight, shared_gate)):
+            raise ValueError("gate_weight and shared_gate must start on 16 bytes")
+        self._planes = tuple(ptr(t) for t in (gate_weight, shared_gate, self.bias, W.w13, W.s13,
+                                              W.gs13, W.w2, W.s2, W.gs2))
+        self._keep = (W.w13, W.s13, W.gs13, W.w2, W.s2, W.gs2)
+        self._shape = (W.H, W.I, W.E, W.n_shared, self.top_k, int(scoring == "sigmoid"),
+                       self.renormalize, self.n_group, self.topk_group)
+        self._floats = (self.routed_scaling_factor, self.limit, self.alpha, self.beta)
+        self._few_bytes = {}   # workspace by token count (0: composed)
+        self._entry = _lib.load().xtu_few_block
         # the shared experts as further routed ones: their weight is then the
         # gate's (the same planes)
         self._W_all = None
@@ -97,7 +119,7 @@ class MoeBlock:
         if out is not None and (tuple(out.shape) != tuple(x.shape) or not out.is_contiguous()):
             raise ValueError(f"out must be contiguous {tuple(x.shape)}, got {tuple(out.shape)}")
         _same_device(W.device, x=x, out=out)
-        if stream is not None or W.device.index != torch.cuda.current_device():
+        if stream is not None or W.device.index != _current_device():
             with on_stream(stream, W.device):
                 return self(x, out=out, out_dtype=out_dtype, return_routing=return_routing)
         if out is not None and _overlap(out, x):
@@ -105,11 +127,30 @@ class MoeBlock:
         if out is None:
             out = torch.empty(x.shape, dtype=odt, device=x.device)
         T = x.shape[0]
-        ids = torch.empty((T, self.top_k), dtype=torch.int32, device=x.device)
-        wts = torch.empty((T, self.top_k), dtype=torch.float32, device=x.device)
-        if T:
+        need = self._few_bytes.get(T)
+        if need is None:
+            need = self._few_bytes[T] = int(_lib.call(
+                "xtu_few_workspace_bytes", T, W.E, self.top_k, W.n_shared, W.H, W.I)) if T else 0
+        ids = x.new_empty((T, self.top_k), dtype=torch.int32)
+        wts = x.new_empty((T, self.top_k), dtype=torch.float32)
+        if need:
+            self._few(x, out, ids, wts, need)
+        elif T:
             self._composed(x, out, ids, wts)
         return (out, wts, ids) if return_routing else out
+
+    def _few(self, x, out, ids, wts, need):
+        """A few tokens, in two launches."""
+        if x.data_ptr() & 15:
+            x = x.clone()
+        # per call: calls on other streams, and graphs, have their own
+        ws = x.new_empty(need, dtype=torch.uint8)
+        rc = self._entry(ARGS.pack(x.data_ptr(), *self._planes, out.data_ptr(), ids.data_ptr(),
+                                   wts.data_ptr(), ws.data_ptr(), need, self.W.fmt, x.shape[0],
+                                   *self._shape, out.dtype == torch.bfloat16, *self._floats),
+                         raw_stream(x.device.index))
+        if rc:
+            _lib.check("xtu_few_block", rc)
 
     def _composed(self, x, out, ids, wts):
         """Any number of tokens: the products and the layer one after the other."""

@@ -12,17 +12,23 @@ the routed experts' sum), or any projection.
 from __future__ import annotations
 
 import contextlib
+import struct
 
 import torch
 
 from . import _lib
-from .layer import _p, _same_device, _stream
+from .layer import _same_device, _stream
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "sigmoid": 5,
                "swiglu": 6}
+# xtu_linear_args: x, w, bias, row_scale, residual, out, workspace; ldx, ldw, ldr,
+# ldo, scale_stride, workspace_bytes; M, N, K, act, three bf16 flags; limit, alpha, beta
+ARGS = struct.Struct("@7P5lN7i3f")
 # workspace bytes per (M, N, K, swiglu, aligned)
 _WS_BYTES: dict = {}
 _TYPES = (torch.bfloat16, torch.float32)
+_OPERAND = (torch.bfloat16,)
+_ENTRY = None
 
 
 def _extent(t):
@@ -40,14 +46,31 @@ def _overlap(a, b) -> bool:
 
 def _rows(name, t, dtypes, cols=None):
     """A matrix whose rows are contiguous; returns its row stride."""
-    if t.dim() != 2 or t.dtype not in dtypes:
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or t.dtype not in dtypes:
         raise ValueError(f"{name} must be a 2-D {' or '.join(str(d) for d in dtypes)} tensor, got "
-                         f"{tuple(t.shape)} {t.dtype}")
-    if cols is not None and t.shape[1] != cols:
-        raise ValueError(f"{name} has {t.shape[1]} columns, expected {cols}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name}'s rows must be contiguous (column stride {t.stride(1)})")
-    return t.stride(0)
+                         f"{tuple(shape)} {t.dtype}")
+    if cols is not None and shape[1] != cols:
+        raise ValueError(f"{name} has {shape[1]} columns, expected {cols}")
+    if strides[1] != 1 and shape[1] > 1:
+        raise ValueError(f"{name}'s rows must be contiguous (column stride {strides[1]})")
+    return strides[0]
+
+
+def _entry():
+    global _ENTRY
+    if _ENTRY is None:
+        _ENTRY = _lib.load().xtu_linear
+    return _ENTRY
+
+
+def raw_stream(index: int) -> int:
+    """Handle of the current stream of device `index`."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()
 
 
 @contextlib.contextmanager
@@ -80,29 +103,36 @@ def linear(x, w, *, bias=None, activation="none", row_scale=None, residual=None,
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"unknown activation {activation!r} (one of {', '.join(ACTIVATIONS)})")
-    ldx = _rows("x", x, (torch.bfloat16,))
+    ldx = _rows("x", x, _OPERAND)
     M, K = x.shape
-    ldw = _rows("w", w, (torch.bfloat16,), K)
+    ldw = _rows("w", w, _OPERAND, K)
     rows = w.shape[0]
     if rows == 0 or K == 0 or (act == 6 and rows % 2):
         raise ValueError(f"w of shape {tuple(w.shape)} does not fit activation {activation!r} "
                          "(at least one row and column; an even number of rows for swiglu)")
     N = rows // 2 if act == 6 else rows
-    if bias is not None and (tuple(bias.shape) != (rows,) or bias.dtype not in _TYPES
-                             or not bias.is_contiguous()):
-        raise ValueError(f"bias must be a contiguous bf16 or fp32 [{rows}], got "
-                         f"{tuple(bias.shape)} {bias.dtype}")
-    sst = 0
+    dev = x.device
+    same = w.device == dev
+    bp = sp = rp = sst = ldr = 0
+    b16 = r16 = False
+    if bias is not None:
+        if bias.shape != (rows,) or bias.dtype not in _TYPES or not bias.is_contiguous():
+            raise ValueError(f"bias must be a contiguous bf16 or fp32 [{rows}], got "
+                             f"{tuple(bias.shape)} {bias.dtype}")
+        bp, b16 = bias.data_ptr(), bias.dtype == torch.bfloat16
+        same = same and bias.device == dev
     if row_scale is not None:
-        if row_scale.dtype != torch.float32 or tuple(row_scale.shape) not in ((M,), (M, 1)):
+        if row_scale.dtype != torch.float32 or row_scale.shape not in ((M,), (M, 1)):
             raise ValueError(f"row_scale must be fp32 [{M}] or [{M}, 1], got "
                              f"{tuple(row_scale.shape)} {row_scale.dtype}")
-        sst = row_scale.stride(0)
-    ldr = 0
+        sp, sst = row_scale.data_ptr(), row_scale.stride(0)
+        same = same and row_scale.device == dev
     if residual is not None:
         ldr = _rows("residual", residual, _TYPES, N)
         if residual.shape[0] != M:
             raise ValueError(f"residual has {residual.shape[0]} rows, expected {M}")
+        rp, r16 = residual.data_ptr(), residual.dtype == torch.bfloat16
+        same = same and residual.device == dev
     odt = out.dtype if out is not None else out_dtype or torch.bfloat16
     if odt not in _TYPES or (out_dtype or odt) != odt:
         raise ValueError(f"output type {odt} (out_dtype {out_dtype}): bf16 or fp32")
@@ -120,32 +150,33 @@ def linear(x, w, *, bias=None, activation="none", row_scale=None, residual=None,
                     and (ldr == ldo or M == 1):
                 continue   # in place: every element is read before it is written
             raise ValueError(f"out overlaps {name}")
-    dev = x.device
+        same = same and out.device == dev
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor")
-    _same_device(dev, w=w, bias=bias, row_scale=row_scale, residual=residual, out=out)
-    if stream is not None or dev.index != torch.cuda.current_device():
+    if not same:
+        _same_device(dev, w=w, bias=bias, row_scale=row_scale, residual=residual, out=out)
+    if stream is not None or dev.index != _current_device():
         with on_stream(stream, dev):   # outputs belong to the stream that writes them
             return linear(x, w, bias=bias, activation=activation, row_scale=row_scale,
                           residual=residual, out=out, out_dtype=out_dtype,
                           swiglu_limit=swiglu_limit, swiglu_alpha=swiglu_alpha,
                           swiglu_beta=swiglu_beta)
     if out is None:
-        out = torch.empty((M, N), dtype=odt, device=dev)
+        out = x.new_empty((M, N), dtype=odt)
     if M == 0:
         return out
     xp, wp = x.data_ptr(), w.data_ptr()
     aligned = not ((ldx if M > 1 else 0) | ldw | K) & 7 and not (xp | wp) & 15
-    key = (M, N, K, act == 6, aligned)
-    nws = _WS_BYTES.get(key)
+    nws = _WS_BYTES.get((M, N, K, act == 6, aligned))
     if nws is None:
-        nws = _WS_BYTES[key] = int(_lib.call("xtu_linear_workspace_bytes", M, N, K, act,
-                                             int(aligned)))
+        nws = int(_lib.call("xtu_linear_workspace_bytes", M, N, K, act, int(aligned)))
+        _WS_BYTES[M, N, K, act == 6, aligned] = nws
     # allocated per call: calls on other streams, and graphs, have their own
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-    _lib.call("xtu_linear", xp, ldx, wp, ldw, M, N, K, act, _p(bias),
-              int(bias is not None and bias.dtype == torch.bfloat16), _p(row_scale), sst,
-              _p(residual), int(residual is not None and residual.dtype == torch.bfloat16), ldr,
-              out.data_ptr(), int(odt == torch.bfloat16), ldo, float(swiglu_limit or 0.0),
-              float(swiglu_alpha), float(swiglu_beta), _p(ws), nws, _stream())
+    ws = x.new_empty(nws, dtype=torch.uint8) if nws else None
+    rc = _entry()(ARGS.pack(xp, wp, bp, sp, rp, out.data_ptr(), ws.data_ptr() if nws else 0, ldx,
+                            ldw, ldr, ldo, sst, nws, M, N, K, act, b16, r16,
+                            odt == torch.bfloat16, swiglu_limit or 0.0, swiglu_alpha, swiglu_beta),
+                  raw_stream(dev.index))
+    if rc:
+        _lib.check("xtu_linear", rc)
     return out
