@@ -247,7 +247,9 @@ def test_nan_stays_in_its_token(layer):
         x2[0, 3] = float("nan")
         out, wts, ids = blk(x2, return_routing=True)
         assert torch.equal(ids[1:], ref[2][1:]) and torch.equal(wts[1:], ref[1][1:])
-        assert torch.equal(out[1:], ref[0][1:])
+        # (the order of a token's fp32 sums goes by the batch's active experts,
+        # so its outputs are held to their bounds, not to the other batch's bits)
+        _check(blk, dense, x[1:], (out[1:], wts[1:], ids[1:]), sg, kw)
         assert bool(((ids >= 0) & (ids < layer[0])).all())
 
 

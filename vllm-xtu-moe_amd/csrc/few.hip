@@ -9,6 +9,11 @@ namespace {
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
+// bits of a weight with its scales
+float format_bits(int fmt) {
+  return fmt == kBF16 ? 16.0f : fmt == kFP8 ? 8.0f : fmt == kMXFP4 ? 4.25f : 4.5f;
+}
+
 struct Layout {
   int ldl, ctl_words;
   size_t logits, act, part, ctl, total;   // byte offsets
@@ -35,9 +40,12 @@ using namespace xtu::few;
 
 extern "C" {
 
-size_t xtu_few_workspace_bytes(int T, int E, int K, int n_shared, int H, int I) {
+size_t xtu_few_workspace_bytes(int fmt, int T, int E, int K, int n_shared, int n_group, int H,
+                               int I) {
   Plan p;
-  if (!make_plan(T, E, K, n_shared, H, I, p)) return 0;
+  if (fmt < 0 || fmt > 3 ||
+      !make_plan(T, E, K, n_shared, H, I, format_bits(fmt), n_group > 1, p))
+    return 0;
   return layout_of(p, T, E, K, n_shared, H, I).total;
 }
 
@@ -45,8 +53,9 @@ hipError_t xtu_few_block(const xtu_few_args* args, hipStream_t stream) {
   XTU_CHECK_ARG(args);
   const xtu_few_args& t = *args;
   Plan p;
-  XTU_CHECK_ARG(make_plan(t.T, t.E, t.K, t.n_shared, t.H, t.I, p));
   XTU_CHECK_ARG(t.fmt >= 0 && t.fmt <= 3 && (t.mode == 0 || t.mode == 1));
+  XTU_CHECK_ARG(make_plan(t.T, t.E, t.K, t.n_shared, t.H, t.I, format_bits(t.fmt),
+                          t.n_group > 1, p));
   XTU_CHECK_ARG(t.x && t.gate && t.w13 && t.w2 && t.out && t.ids && t.weights && t.workspace);
   XTU_CHECK_ARG(t.fmt == kBF16 || (t.s13 && t.s2));
   XTU_CHECK_ARG(!t.shared_gate || t.n_shared > 0);

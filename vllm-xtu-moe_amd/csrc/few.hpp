@@ -12,12 +12,17 @@
 //
 // Launch 2 (few_experts_kernel) is persistent: every workgroup selects the
 // batch's experts in LDS for itself (same code, same logits: all agree), then
-// takes work items off one counter: first the routed gate/up panels, expert by
-// expert, then the output panels (down projection and weighted sum).  A
-// workgroup that reaches the output panels waits until every gate/up panel is
-// done.  Items are handed out in order to workgroups that already run, so the
-// ones waited for are in the hands of running workgroups, whatever else shares
-// the device: the wait ends without the launch being resident as a whole.
+// draws work items: first the routed gate/up panels, expert by expert, then the
+// output panels (down projection and weighted sum).  Before its first output
+// panel a workgroup waits until every gate/up panel is done, and before that
+// wait it has seen every gate/up panel drawn: those waited for are in the hands
+// of workgroups that run and wait for nothing, so the wait ends whatever else
+// shares the device, also where part of this launch is not resident yet.
+//
+// Items are dealt into eight groups, item i to group i % 8, with a counter each
+// (one address takes about 100 atomics in a microsecond: all workgroups on one
+// counter spent 10 us on their first items); a workgroup draws from the group of
+// its XCD, and from the others' gate/up items when that is used up.
 //
 // Both phases are weight streams (the arithmetic is decode.hpp's): a wave's
 // loads for its next item are issued as the registers of the present one are
@@ -33,6 +38,8 @@
 // timing.
 #pragma once
 #include "decode.hpp"
+
+#include <cmath>
 
 namespace xtu {
 namespace few {
@@ -78,11 +85,35 @@ constexpr int kMaxT = 16, kMaxPairs = 256, kMaxShared = 4, kMaxE = 1024, kMaxGro
 constexpr int kThreads = 512, kWaves = 8, kKS = 4;   // waves along K per gate/up half
 constexpr int kLine = 64;                            // words of a counter's own 256 bytes
 
-// Counters (words): the ticket, eight partial counts of finished gate/up items,
-// a flag set if a wait ever ran out, then the chunks done per output panel.
-constexpr int kTicket = 0, kDone = kLine, kFlag = 9 * kLine, kPanels = 10 * kLine;
+// Counters (words): per group the gate/up items drawn, the output items drawn
+// and the gate/up items done; a flag set if a wait ever ran out; then the chunks
+// done per output panel.
+constexpr int kGroups = 8;
+constexpr int kTicket = 0, kTicket3 = 8 * kLine, kDone = 16 * kLine, kFlag = 24 * kLine,
+              kPanels = 25 * kLine;
 constexpr int kSpin = 1 << 20;
 
+
+// The x rows to LDS, 16 bytes of padding each; a thread's loads go out eight
+// at a time.
+__device__ __forceinline__ void stage_x(const FewArgs& f, uint16_t* xs) {
+  const int ldx = f.H + 8, per_row = f.H / 8, pieces = f.T * per_row;
+  constexpr int SB = 8;
+  for (int c0 = threadIdx.x; c0 < pieces; c0 += SB * kThreads) {
+    u32x4_t v[SB];
+#pragma unroll
+    for (int k = 0; k < SB; ++k)
+      v[k] = *reinterpret_cast<const u32x4_t*>(f.x + 8L * min(c0 + k * kThreads, pieces - 1));
+#pragma unroll
+    for (int k = 0; k < SB; ++k) {
+      const int p = c0 + k * kThreads;
+      if (p < pieces) {
+        const int r = p / per_row;
+        *reinterpret_cast<u32x4_t*>(xs + r * ldx + (p - r * per_row) * 8) = v[k];
+      }
+    }
+  }
+}
 
 // ---------------------------------------------------------------- launch 1
 template <int FMT, int NU>
@@ -94,16 +125,9 @@ __global__ __launch_bounds__(kThreads, 2) void few_router_kernel(FewArgs f) {
   const int w = wave_id();
   const uint32_t lane = tid % kWave;
   const int q = lane / 16, m = lane % 16;
-  const int ldx = f.H + 8, per_row = f.H / 8, pieces = f.T * per_row;
+  const int ldx = f.H + 8;
   if (blockIdx.x == gridDim.x - 1)
     for (int i = tid; i < f.ctl_words; i += kThreads) f.ctl[i] = 0u;
-  auto stage_x = [&]() {
-    for (int p = tid; p < pieces; p += kThreads) {
-      const int r = p / per_row, k = (p - r * per_row) * 8;
-      *reinterpret_cast<u32x4_t*>(xs + r * ldx + k) =
-          *reinterpret_cast<const u32x4_t*>(f.x + (long)r * f.H + k);
-    }
-  };
   const uint16_t* xrow = xs + min(m, f.T - 1) * ldx;
 
   if ((int)blockIdx.x < f.n_sh) {   // a shared expert's gate/up panel, all T rows
@@ -129,7 +153,7 @@ __global__ __launch_bounds__(kThreads, 2) void few_router_kernel(FewArgs f) {
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
     if (u0 < u1) issue_round<FMT, NU>(r, st, u0, u1, lane);
     __builtin_amdgcn_sched_barrier(0);
-    stage_x();
+    stage_x(f, xs);
     __syncthreads();
     const uint16_t* xa = xrow + q * F::kCK;
     if (u0 < u1) {
@@ -154,7 +178,7 @@ __global__ __launch_bounds__(kThreads, 2) void few_router_kernel(FewArgs f) {
   for (int i = 0; i < U; ++i)
     wv[i] = *reinterpret_cast<const u32x4_t*>(wr + 32 * (s0 + min(i, nst - 1)));
   __builtin_amdgcn_sched_barrier(0);
-  stage_x();
+  stage_x(f, xs);
   __syncthreads();
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
   auto use = [&](int i, int s) {
@@ -310,12 +334,28 @@ struct Sel {
   int last;
 };
 
+// One thread of a workgroup draws an item of group g: which = kTicket (gate/up)
+// or kTicket3 (output panels).
+__device__ __forceinline__ int draw(const FewArgs& f, int which, int g) {
+  return kGroups * (int)__hip_atomic_fetch_add(f.ctl + which + kLine * g, 1u, __ATOMIC_RELAXED,
+                                               __HIP_MEMORY_SCOPE_AGENT) + g;
+}
+
 // rowof / wof: [slot][16] activation row and weight of token t in that slot
 // (weight 0: the token does not use it).
-__device__ void build_selection(const FewArgs& f, Sel& g, uint16_t* rowof, float* wof,
-                                float* scr) {
-  const int tid = threadIdx.x, lane = tid % kWave, wv = tid / kWave;
+// stage gets the x rows; scr: E floats per wave for select_any's groups.
+// The workgroup's first two tickets are drawn on the way, the second once the
+// first is back: by then every workgroup has drawn its first, so work spreads
+// over all of them before anyone takes a second item.
+__device__ __forceinline__ void build_selection(const FewArgs& f, Sel& g, uint16_t* rowof,
+                                                float* wof, uint16_t* stage, float* scr) {
+  const int tid = threadIdx.x, lane = tid % kWave, wv = wave_id();
   const int T = f.T, K = f.K, A = T * K, NS = f.NS;
+  const bool drawer = tid == kThreads - kWave;
+  int t0 = 0;
+  const int grp = blockIdx.x % kGroups;
+  if (drawer) t0 = draw(f, kTicket, grp);
+  stage_x(f, stage);
   for (int t = wv; t < T; t += kWaves) {
     const float* l = f.logits + (long)t * f.ldl;
     int* ids = g.ids + t * K;
@@ -326,6 +366,11 @@ __device__ void build_selection(const FewArgs& f, Sel& g, uint16_t* rowof, float
       case 8: select_wave<8>(f, l, lane, ids, wts); break;
       default: select_any(f, l, lane, ids, wts, scr + wv * f.E); break;
     }
+  }
+  if (drawer) {
+    g.ticket[0] = t0;
+    __asm__ __volatile__("" ::"v"(t0) : "memory");   // the first ticket is back
+    g.ticket[1] = draw(f, kTicket, grp);
   }
   for (int i = tid; i < kMaxPairs; i += kThreads)
     if (i >= A) g.ids[i] = 0x7fffffff;
@@ -339,6 +384,7 @@ __device__ void build_selection(const FewArgs& f, Sel& g, uint16_t* rowof, float
   int r0 = 0, rank = 0, e = 0;
   if (tid < A) {   // thread p: pair p
     e = g.ids[tid];
+#pragma unroll 4
     for (int j = 0; j < A4; ++j) {
       const i32x4_t v = *reinterpret_cast<const i32x4_t*>(g.ids + 4 * j);
 #pragma unroll
@@ -355,6 +401,7 @@ __device__ void build_selection(const FewArgs& f, Sel& g, uint16_t* rowof, float
   __syncthreads();
   if (tid < A) {
     int slot = 0;   // experts below e
+#pragma unroll 4
     for (int j = 0; j < A4; ++j) {
       const i32x4_t v = *reinterpret_cast<const i32x4_t*>(g.first + 4 * j);
       slot += (v[0] < e) + (v[1] < e) + (v[2] < e) + (v[3] < e);
@@ -520,8 +567,9 @@ __host__ __device__ inline size_t table_bytes(int max_slots) {
   return (size_t)max_slots * kMaxT * 6;
 }
 
-template <int FMT, int NU, int NPER>
-__global__ __launch_bounds__(kThreads, 4) void few_experts_kernel(FewArgs f) {
+// OCC: workgroups that are to share a CU (128 or 256 VGPRs).
+template <int FMT, int NU, int NPER, int OCC>
+__global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs f) {
   using F = WFmt<FMT>;
   constexpr int D = ring_depth<FMT, NPER>();
   extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
@@ -536,33 +584,26 @@ __global__ __launch_bounds__(kThreads, 4) void few_experts_kernel(FewArgs f) {
   const int T = f.T, H = f.H, I = f.I;
   const int max_slots = min(f.E, T * f.K) + f.NS;
   uint16_t* rowof = reinterpret_cast<uint16_t*>(wof + max_slots * kMaxT);
-  auto claim = [&]() -> int {   // thread 0
-    return (int)__hip_atomic_fetch_add(f.ctl + kTicket, 1u, __ATOMIC_RELAXED,
-                                       __HIP_MEMORY_SCOPE_AGENT);
-  };
-  int t_new = 0;
-  if (tid == 0) t_new = claim();   // the first item; its latency is the selection's
-  build_selection(f, g, rowof, wof, reinterpret_cast<float*>(stage));
+  build_selection(f, g, rowof, wof, stage,
+                  reinterpret_cast<float*>(dyn + (size_t)T * (H + 8) * 2));
   if (blockIdx.x == 0) {
     for (int i = tid; i < T * f.K; i += kThreads) {
       f.ids[i] = g.ids[i];
       f.wts[i] = g.wts[i];
     }
   }
-  if (tid == 0) {
-    g.ticket[0] = t_new;
-    g.ticket[1] = claim();
-  }
-  __syncthreads();
   int cur = __builtin_amdgcn_readfirstlane(g.ticket[0]);
   int nxt = __builtin_amdgcn_readfirstlane(g.ticket[1]);
+  __syncthreads();   // the words are read before an item's draw takes one
   const int n_routed = __builtin_amdgcn_readfirstlane(g.n_routed);
   const int npan = I / 16, hpan = H / 16;
   const int n2 = n_routed * npan, n3 = f.chunks * hpan;
+  const int grp = blockIdx.x % kGroups;
+  int t_new = 0;
   int it = 0;   // items done: which half of red, which ticket word
 
   // ---- routed gate/up
-  if (cur < n2) {
+  {
     DecodeArgs a{};
     a.w = f.w13;
     a.s = f.s13;
@@ -585,53 +626,79 @@ __global__ __launch_bounds__(kThreads, 4) void few_experts_kernel(FewArgs f) {
       const int e = __builtin_amdgcn_readfirstlane(g.slot_e[slot]);
       return make_stream<FMT>(a, e, half ? npan + sub : sub, H, live);
     };
-    Stream<FMT> st = stream_of(cur);
-    Round<FMT, NU> r;
-    if (u0 < u1) issue_round<FMT, NU>(r, st, u0, u1, lane);
-    __builtin_amdgcn_sched_barrier(0);
-    const int ldx = H + 8, per_row = H / 8, pieces = T * per_row;
-    for (int p = tid; p < pieces; p += kThreads) {
-      const int rr = p / per_row, k = (p - rr * per_row) * 8;
-      *reinterpret_cast<u32x4_t*>(stage + rr * ldx + k) =
-          *reinterpret_cast<const u32x4_t*>(f.x + (long)rr * H + k);
-    }
-    __syncthreads();
+    const int ldx = H + 8;
     int count = 0;
+    Round<FMT, NU> r;
     while (true) {
-      if (tid == 0) t_new = claim();
-      const int slot = cur / npan, sub = cur - slot * npan;
-      const int r0 = g.slot_r0[slot], na = g.slot_r0[slot + 1] - r0;
-      const int ws = g.slot_e[slot];
-      const int tok = g.row_tok[r0 + min(m, na - 1)];
-      const uint16_t* xa = stage + tok * ldx + q * F::kCK;
-      f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-      for (int rd = 0; rd + 1 < rounds; ++rd) {
-        const int ub = u0 + rd * NU;
-        roll_round<FMT, NU>(r, acc, ub, u1, xa, st, ub + NU, u1, lane);
+      if (cur >= n2) {
+        // the own group is used up: an item of another one, if any is left
+        nxt = n2;
+        if (w == 0) {
+          int got = n2;
+          while (true) {
+            const int left = (int)lane < kGroups
+                                 ? (int)__hip_atomic_load(f.ctl + kTicket + kLine * lane,
+                                                          __ATOMIC_RELAXED,
+                                                          __HIP_MEMORY_SCOPE_AGENT) * kGroups +
+                                       (int)lane
+                                 : n2;
+            const unsigned long long some = __ballot(left < n2);
+            if (!some) break;
+            int t = 0;
+            if (lane == 0) t = draw(f, kTicket, __builtin_ctzll(some));
+            got = __builtin_amdgcn_readfirstlane(t);
+            if (got < n2) break;   // (else someone was quicker: look again)
+          }
+          if (lane == 0) g.ticket[it & 1] = got;
+        }
+        __syncthreads();
+        cur = __builtin_amdgcn_readfirstlane(g.ticket[it & 1]);
+        __syncthreads();
+        if (cur >= n2) break;
       }
-      const Stream<FMT> sn = stream_of(nxt);
-      roll_round<FMT, NU>(r, acc, u0 + (rounds - 1) * NU, u1, xa, sn, u0, u1, lane);
-      st = sn;
-      if (tid == 0) g.ticket[it & 1] = t_new;
-      // (ends with every wave past a barrier: the ticket is visible)
-      gate_up_epilogue<FMT, true>(a, red[it & 1], acc, w, lane, r0, na, ws, sub);
-      ++count;
-      cur = nxt;
-      nxt = __builtin_amdgcn_readfirstlane(g.ticket[it & 1]);
-      ++it;
-      if (cur >= n2) break;
+      Stream<FMT> st = stream_of(cur);
+      if (u0 < u1) issue_round<FMT, NU>(r, st, u0, u1, lane);
+      __builtin_amdgcn_sched_barrier(0);
+      while (true) {   // cur is loaded; nxt rolls in behind it
+        if (tid == 0) t_new = nxt < n2 ? draw(f, kTicket, grp) : n2;
+        const int slot = cur / npan, sub = cur - slot * npan;
+        const int r0 = g.slot_r0[slot], na = g.slot_r0[slot + 1] - r0;
+        const int ws = g.slot_e[slot];
+        const int tok = g.row_tok[r0 + min(m, na - 1)];
+        const uint16_t* xa = stage + tok * ldx + q * F::kCK;
+        f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+        for (int rd = 0; rd + 1 < rounds; ++rd) {
+          const int ub = u0 + rd * NU;
+          roll_round<FMT, NU>(r, acc, ub, u1, xa, st, ub + NU, u1, lane);
+        }
+        const Stream<FMT> sn = stream_of(nxt);
+        roll_round<FMT, NU>(r, acc, u0 + (rounds - 1) * NU, u1, xa, sn, u0, u1, lane);
+        st = sn;
+        if (tid == 0) g.ticket[it & 1] = t_new;
+        // (ends with every wave past a barrier: the ticket is visible)
+        gate_up_epilogue<FMT, true>(a, red[it & 1], acc, w, lane, r0, na, ws, sub);
+        ++count;
+        cur = nxt;
+        nxt = __builtin_amdgcn_readfirstlane(g.ticket[it & 1]);
+        ++it;
+        if (cur >= n2) break;
+      }
     }
-    // this workgroup's rows are written: count its items
+    // this workgroup's rows are written: count its items; and draw its first
+    // output panel
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (tid == 0)
-      __hip_atomic_fetch_add(f.ctl + kDone + kLine * (blockIdx.x % 8), (unsigned)count,
-                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) {
+      if (count)
+        __hip_atomic_fetch_add(f.ctl + kDone + kLine * grp, (unsigned)count, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+      g.ticket[0] = draw(f, kTicket3, grp);
+    }
+    __syncthreads();
   }
 
   // ---- output panels
-  cur -= n2;
-  nxt -= n2;
+  cur = __builtin_amdgcn_readfirstlane(g.ticket[0]);
   if (cur >= n3) return;   // whole workgroup
   const int nu = I / 128, nseg = (nu + NPER - 1) / NPER;   // segments of an expert
   const int n_slots = n_routed + f.NS;
@@ -660,7 +727,7 @@ __global__ __launch_bounds__(kThreads, 4) void few_experts_kernel(FewArgs f) {
   for (int d = 0; d < D; ++d) issue_item(d, d, j0, j1, p, true);
   __builtin_amdgcn_sched_barrier(0);
 
-  // wait for every gate/up item (see the top: their workgroups run)
+  // wait for every gate/up item: all are drawn (see the top)
   if (w == 0) {
     for (int n = 0;; ++n) {
       unsigned v = 0u;
@@ -678,8 +745,12 @@ __global__ __launch_bounds__(kThreads, 4) void few_experts_kernel(FewArgs f) {
       }
       __builtin_amdgcn_s_sleep(2);
     }
+    // the second panel, drawn when every workgroup has come this far
+    if (lane == 0) g.ticket[1] = draw(f, kTicket3, grp);
   }
   __syncthreads();
+  nxt = __builtin_amdgcn_readfirstlane(g.ticket[1]);
+  __syncthreads();   // read before an item's draw takes the word
 
   const int lda = I + 8, per_row = I / 8;
   const __amdgpu_buffer_rsrc_t ract = __builtin_amdgcn_make_buffer_rsrc(
@@ -711,7 +782,7 @@ __global__ __launch_bounds__(kThreads, 4) void few_experts_kernel(FewArgs f) {
       }
       __syncthreads();
     }
-    if (tid == 0) t_new = claim();
+    if (tid == 0) t_new = draw(f, kTicket3, grp);
     // next item
     const bool more = nxt < n3;
     const int cn = more ? nxt / hpan : c, pn = more ? nxt - cn * hpan : p;
@@ -797,37 +868,52 @@ __global__ __launch_bounds__(kThreads, 4) void few_experts_kernel(FewArgs f) {
     p = pn;
     j0 = jn0;
     j1 = jn1;
-    nxt = nn - n2;
+    nxt = nn;
   }
 }
 
 // ---------------------------------------------------------------- host
 
-inline bool make_plan(int T, int E, int K, int NS, int H, int I, Plan& p) {
+// bits: of a weight, with its scales.  More chunks than the LDS asks for give
+// the output panels more items: where there are fewer panels than CUs, or their
+// last round leaves CUs idle.  Times in us: a CU streams about 25 GB/s, an item
+// costs 0.7 beside its stream, the joining of chunks 2.
+inline bool make_plan(int T, int E, int K, int NS, int H, int I, float bits, bool groups,
+                      Plan& p) {
   if (T < 1 || T > kMaxT || K < 1 || K > 16 || K > E || E > kMaxE || T * K > kMaxPairs ||
       NS < 0 || NS > kMaxShared || H < 256 || H % 256 || H > 16384 || I < 128 || I % 128 ||
       I > 16384)
     return false;
-  const size_t fixed = (size_t)2 * kWaves * kWave * 16 + sel_bytes() +
-                       table_bytes(std::min(E, T * K) + NS) + 256;
-  const size_t xb = (size_t)T * (H + 8) * 2, row = (size_t)(I + 8) * 2;
-  const size_t scr = (size_t)kWaves * E * 4;   // select_any's scores
-  const int R = T * (K + NS);
-  const size_t want = std::max({xb, R * row, scr});
+  const int slots = std::min(E, T * K) + NS, R = T * (K + NS);
+  const size_t fixed = (size_t)2 * kWaves * kWave * 16 + sel_bytes() + table_bytes(slots) + 256;
   const size_t half = 80 * 1024, full = 160 * 1024;
-  p.occ = fixed + want <= half ? 2 : 1;
-  if (fixed + std::max(xb, scr) > full) return false;
-  p.stage = std::min(want, full - fixed) / 16 * 16;
-  const int cap = (int)(p.stage / row);
-  p.chunks = 1;
-  p.rows_per_chunk = R;
+  // x rows, and behind them select_any's scores
+  const size_t xb = (size_t)T * (H + 8) * 2 + (groups ? (size_t)kWaves * E * 4 : 0);
+  const size_t row = (size_t)(I + 8) * 2;
+  if (fixed + xb > full) return false;
+  const int cap = (int)((full - fixed) / row);
+  int least = 1;
   if (cap < R) {   // a chunk's last slot may begin on its last row
     const int rpc = cap - (T - 1);
     if (rpc < 1) return false;
-    p.chunks = (R + rpc - 1) / rpc;
-    p.rows_per_chunk = (R + p.chunks - 1) / p.chunks;
+    least = (R + rpc - 1) / rpc;
   }
-  p.lds = p.stage + sel_bytes() + table_bytes(std::min(E, T * K) + NS);
+  const double active = E * (1.0 - std::pow(1.0 - (double)K / E, T)) + NS;
+  const double panel_us = active * I * 16 * bits / 8 / 25e3;
+  const int hpan = H / 16, cus = cu_count();
+  double best = 1e30;
+  for (int c = least; c <= std::min(least + 7, R); ++c) {
+    const double t = (c * hpan + cus - 1) / cus * (panel_us / c + 0.7) + (c > 1 ? 2.0 : 0.0);
+    if (t < best - 0.01) {
+      best = t;
+      p.chunks = c;
+    }
+  }
+  p.rows_per_chunk = (R + p.chunks - 1) / p.chunks;
+  const int rows = p.chunks == 1 ? R : p.rows_per_chunk + T - 1;
+  p.stage = (std::max(xb, rows * row) + 15) / 16 * 16;
+  p.occ = fixed + p.stage <= half ? 2 : 1;
+  p.lds = p.stage + sel_bytes() + table_bytes(slots);
   return true;
 }
 
@@ -843,7 +929,8 @@ void launch_experts(const FewArgs& f, const Plan& p, hipStream_t stream) {
   const long items = std::max<long>((long)std::min(f.E, f.T * f.K) * (f.I / 16),
                                     (long)p.chunks * (f.H / 16));
   const int grid = (int)std::min<long>((long)p.occ * cu_count(), items);
-  few_experts_kernel<FMT, NU, NPER><<<grid, kThreads, p.lds, stream>>>(f);
+  if (p.occ == 2) few_experts_kernel<FMT, NU, NPER, 2><<<grid, kThreads, p.lds, stream>>>(f);
+  else few_experts_kernel<FMT, NU, NPER, 1><<<grid, kThreads, p.lds, stream>>>(f);
 }
 
 template <int FMT, int NU>
