@@ -664,8 +664,7 @@ typedef struct xtu_few_args {
   int mode, renormalize, n_group, topk_group, out_bf16;
   float routed_scaling, limit, alpha, beta;
 } xtu_few_args;
-size_t xtu_few_workspace_bytes(int fmt, int T, int E, int K, int n_shared, int n_group, int H,
-                               int I);
+size_t xtu_few_workspace_bytes(int fmt, int T, int E, int K, int n_shared, int H, int I);
 hipError_t xtu_few_block(const xtu_few_args* args, hipStream_t stream);
 
 /* ------------------------------------------------ expert staging (ring / pool)

@@ -40,11 +40,10 @@ using namespace xtu::few;
 
 extern "C" {
 
-size_t xtu_few_workspace_bytes(int fmt, int T, int E, int K, int n_shared, int n_group, int H,
-                               int I) {
+size_t xtu_few_workspace_bytes(int fmt, int T, int E, int K, int n_shared, int H, int I) {
   Plan p;
   if (fmt < 0 || fmt > 3 ||
-      !make_plan(T, E, K, n_shared, H, I, format_bits(fmt), n_group > 1, p))
+      !make_plan(T, E, K, n_shared, H, I, format_bits(fmt), p))
     return 0;
   return layout_of(p, T, E, K, n_shared, H, I).total;
 }
@@ -54,8 +53,7 @@ hipError_t xtu_few_block(const xtu_few_args* args, hipStream_t stream) {
   const xtu_few_args& t = *args;
   Plan p;
   XTU_CHECK_ARG(t.fmt >= 0 && t.fmt <= 3 && (t.mode == 0 || t.mode == 1));
-  XTU_CHECK_ARG(make_plan(t.T, t.E, t.K, t.n_shared, t.H, t.I, format_bits(t.fmt),
-                          t.n_group > 1, p));
+  XTU_CHECK_ARG(make_plan(t.T, t.E, t.K, t.n_shared, t.H, t.I, format_bits(t.fmt), p));
   XTU_CHECK_ARG(t.x && t.gate && t.w13 && t.w2 && t.out && t.ids && t.weights && t.workspace);
   XTU_CHECK_ARG(t.fmt == kBF16 || (t.s13 && t.s2));
   XTU_CHECK_ARG(!t.shared_gate || t.n_shared > 0);
@@ -110,7 +108,7 @@ hipError_t xtu_few_block(const xtu_few_args* args, hipStream_t stream) {
   f.rp = 1;   // router rows per panel: a CU each, beside the shared panels
   while (f.rp < 16 && f.n_sh + (er + f.rp - 1) / f.rp > cu_count()) f.rp *= 2;
   f.epl = tiny::wave_epl(t.mode, t.E, f.n_group, t.renormalize, f.logits, f.bias);
-  f.rows_per_chunk = p.rows_per_chunk;
+  f.chunk_units = p.chunk_units;
   f.chunks = p.chunks;
   f.stage_bytes = p.stage;
   switch (t.fmt) {

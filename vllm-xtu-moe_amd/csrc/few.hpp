@@ -30,12 +30,16 @@
 // output panel is loaded while it waits.
 //
 // gate/up: an item is (expert, 16 gate and the 16 up rows); four waves split K
-// for each half.  Down: an item is 16 output columns over a chunk of the active
-// experts; the eight waves take (expert, up to 4 x 128 k) segments in turn and
-// multiply by the token's weight as they add up.  The chunk's activation rows sit
-// in LDS; with more than one chunk the chunks' sums go to memory and the last
-// one to finish a panel adds them in chunk order, so results do not depend on
-// timing.
+// for each half.  The MFMA's rows are the batch's tokens, the same x rows for
+// every expert; a row is written where its token uses the expert.  Down: an item
+// is 16 output columns over a range of K (a chunk) of all active experts; the
+// eight waves take (expert, up to 4 x 128 k) segments in turn and multiply by the
+// token's weight as they add up.  The chunk's part of the activation rows sits in
+// LDS, and a workgroup stays with its chunk while that has panels left; with more
+// than one chunk the chunks' sums go to memory and the last one to finish a panel
+// adds them in chunk order, so results do not depend on timing.
+// (They do depend on the batch, in the last bits: a token's experts are added in
+// the order in which the batch's tokens bring them up.)
 #pragma once
 #include "decode.hpp"
 
@@ -58,7 +62,7 @@ struct FewArgs {
   float limit, alpha, beta;
   float* logits;            // [T][ldl]: E router logits, then the shared gates'
   int ldl;
-  uint16_t* act;            // [T K + NS T][I]: routed rows by expert, then the shared experts'
+  uint16_t* act;            // [T K + NS T][I]: row t K + k, then T K + s T + t
   float* part;              // [chunks][T][H] (chunks > 1)
   unsigned* ctl;
   int ctl_words;
@@ -68,7 +72,7 @@ struct FewArgs {
   int out_bf16;
   int rp, n_sh;             // launch 1: router rows per panel; its shared gate/up items
   int epl;                  // experts per lane of the wave router (0: any E)
-  int rows_per_chunk, chunks;              // launch 2: activation rows in LDS
+  int chunk_units, chunks;  // launch 2: 128-k units of a chunk of the down projection
   size_t stage_bytes;
 };
 
@@ -76,7 +80,7 @@ struct FewArgs {
 // and all activation rows fit half its LDS; otherwise one takes what it needs.
 struct Plan {
   size_t stage, lds;
-  int rows_per_chunk, chunks, occ;
+  int nper, chunk_units, chunks, occ;
 };
 
 namespace {
@@ -85,12 +89,12 @@ constexpr int kMaxT = 16, kMaxPairs = 256, kMaxShared = 4, kMaxE = 1024, kMaxGro
 constexpr int kThreads = 512, kWaves = 8, kKS = 4;   // waves along K per gate/up half
 constexpr int kLine = 64;                            // words of a counter's own 256 bytes
 
-// Counters (words): per group the gate/up items drawn, the output items drawn
-// and the gate/up items done; a flag set if a wait ever ran out; then the chunks
-// done per output panel.
-constexpr int kGroups = 8;
-constexpr int kTicket = 0, kTicket3 = 8 * kLine, kDone = 16 * kLine, kFlag = 24 * kLine,
-              kPanels = 25 * kLine;
+// Counters (words): per group the gate/up items drawn and those done; a flag set
+// if a wait ever ran out; per chunk and group the output panels drawn; then the
+// chunks done per output panel.
+constexpr int kGroups = 8, kMaxChunks = 8;
+constexpr int kTicket = 0, kDone = kGroups * kLine, kFlag = 2 * kGroups * kLine,
+              kTicket3 = kFlag + kLine, kPanels = kTicket3 + kMaxChunks * kGroups * kLine;
 constexpr int kSpin = 1 << 20;
 
 
@@ -210,28 +214,19 @@ __global__ __launch_bounds__(kThreads, 2) void few_router_kernel(FewArgs f) {
 
 // ---------------------------------------------------------------- selection
 // One wave selects one token's experts for any E <= 1024 (lane l holds experts
-// l, l + 64, ..): K rounds of a wave-wide maximum of order-preserving keys,
-// equal ones to the lowest index.  Scores, group scores and weights are
-// route_token_wave's, in the same fp32 sequences (the sum over all experts,
-// where the weights are not renormalised, lane by lane).
-__device__ void select_any(const FewArgs& f, const float* l, int lane, int* ids_lds,
-                           float* wts_lds, float* scr) {
+// l, l + 64, .. as order-preserving keys in kb, E words of this wave's own): K
+// rounds of a wave-wide maximum, equal keys to the lowest index.  Scores, group
+// scores and weights are route_token_wave's, in the same fp32 sequences (the sum
+// over all experts, where the weights are not renormalised, lane by lane).
+__device__ __forceinline__ void select_any(const FewArgs& f, const float* l, int lane,
+                                           int* ids_lds, float* wts_lds, uint32_t* kb) {
 #pragma clang fp contract(off)
-  constexpr int N = kMaxE / kWave;
   const int E = f.E, K = f.K;
-  uint32_t key[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = lane + kWave * i;
-    key[i] = 0u;
-    if (e < E) {
-      float sc = l[e];
-      if (f.mode == 1) {
-        sc = xtu_sigmoid(sc) + (f.bias ? f.bias[e] : 0.0f);
-        if (f.n_group > 1) scr[e] = sc;   // E floats of this wave's own
-      }
-      key[i] = max(tiny::score_key(sc), 1u);   // 0: no expert, or taken
-    }
+#pragma unroll 1
+  for (int e = lane; e < E; e += kWave) {
+    float sc = l[e];
+    if (f.mode == 1) sc = xtu_sigmoid(sc) + (f.bias ? f.bias[e] : 0.0f);
+    kb[e] = max(tiny::score_key(sc), 1u);   // 0: taken, or not in a kept group
   }
   if (f.mode == 1 && f.n_group > 1) {
     // group score: the two best of the group, added; the topk_group best stay
@@ -239,49 +234,51 @@ __device__ void select_any(const FewArgs& f, const float* l, int lane, int* ids_
     const int gsz = E / f.n_group;
     float gs = 0.f;
     if (lane < f.n_group) {
-      float v1 = -__builtin_inff(), v2 = v1;
+      uint32_t k1 = 0u, k2 = 0u;
+#pragma unroll 1
       for (int j = 0; j < gsz; ++j) {
-        const float v = scr[lane * gsz + j];
-        if (v > v1) {
-          v2 = v1;
-          v1 = v;
-        } else if (v > v2) {
-          v2 = v;
-        }
+        const uint32_t k = kb[lane * gsz + j];
+        k2 = max(k2, min(k1, k));
+        k1 = max(k1, k);
       }
-      gs = gsz >= 2 ? v1 + v2 : v1;
+      const auto value = [](uint32_t k) {
+        return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+      };
+      gs = gsz >= 2 ? value(k1) + value(k2) : value(k1);
     }
     int r = 0;
+#pragma unroll 1
     for (int j = 0; j < f.n_group; ++j) {
       const float o = tiny::readlane_f(gs, j);
       r += (o > gs || (o == gs && j < lane)) ? 1 : 0;
     }
     const unsigned long long kept = __ballot(lane < f.n_group && r < f.topk_group);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = lane + kWave * i;
-      if (e < E && !((kept >> (e / gsz)) & 1ull)) key[i] = 0u;
-    }
+    tiny::lds_wave_order();
+#pragma unroll 1
+    for (int e = lane; e < E; e += kWave)
+      if (!((kept >> (e / gsz)) & 1ull)) kb[e] = 0u;
   }
   int my_e = 0;
+#pragma unroll 1
   for (int k = 0; k < K; ++k) {
+    tiny::lds_wave_order();
     uint32_t best = 0u;
-    int bi = 0;
-#pragma unroll
-    for (int i = N - 1; i >= 0; --i)
-      if (key[i] >= best) {   // equal keys: the lower i
-        best = key[i];
-        bi = i;
+    int be = 0;
+#pragma unroll 1
+    for (int e = lane; e < E; e += kWave) {
+      const uint32_t v = kb[e];
+      if (v > best) {   // equal keys: the lower index
+        best = v;
+        be = e;
       }
+    }
     const uint32_t top = tiny::wave_max_u32(best);
-    // lowest index among the lanes that hold the maximum (none left, which
-    // NaN groups can bring about: expert k)
-    const uint32_t e_inv = best == top ? (uint32_t)(kMaxE - (lane + kWave * bi)) : 0u;
-    const int e = top ? kMaxE - (int)tiny::wave_max_u32(e_inv) : k;
+    // the lowest index of the lanes that hold the maximum (none left, which NaN
+    // groups can bring about: expert k)
+    const uint32_t inv = top && best == top ? (uint32_t)(kMaxE - be) : 0u;
+    const int e = top ? kMaxE - (int)tiny::wave_max_u32(inv) : k;
     if (lane == k) my_e = e;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (lane + kWave * i == e) key[i] = 0u;
+    if (lane == 0) kb[e] = 0u;
   }
   const float my_l = lane < K ? l[my_e] : 0.f;
   float w = 0.f;
@@ -320,42 +317,45 @@ __device__ __forceinline__ void select_wave(const FewArgs& f, const float* l, in
 }
 
 // The batch's selection, as every workgroup of launch 2 holds it.  A slot is an
-// active expert: the routed ones ascending, then the shared ones.
+// active expert: the routed ones in the order of their first pairs, then the
+// shared ones.
 struct Sel {
-  int ids[kMaxPairs];
+  int ids[kMaxPairs];                        // of pair t K + k
   float wts[kMaxPairs];
-  int rank[kMaxPairs];                       // earlier pairs of the same expert
+  unsigned long long first[kMaxPairs / kWave];   // pairs that are their expert's first
   int slot_e[kMaxPairs + kMaxShared];
-  int slot_r0[kMaxPairs + kMaxShared + 1];   // first activation row
-  int row_tok[kMaxPairs + kMaxShared * kMaxT];
-  int first[kMaxPairs];
-  int n_routed;                              // slots of routed experts
   int ticket[2];
   int last;
 };
 
-// One thread of a workgroup draws an item of group g: which = kTicket (gate/up)
-// or kTicket3 (output panels).
+// One thread of a workgroup draws an item of group g: which = kTicket (gate/up),
+// or for the output panels of chunk c kTicket3 + c * kGroups * kLine.
 __device__ __forceinline__ int draw(const FewArgs& f, int which, int g) {
   return kGroups * (int)__hip_atomic_fetch_add(f.ctl + which + kLine * g, 1u, __ATOMIC_RELAXED,
                                                __HIP_MEMORY_SCOPE_AGENT) + g;
 }
 
 // rowof / wof: [slot][16] activation row and weight of token t in that slot
-// (weight 0: the token does not use it).
-// stage gets the x rows; scr: E floats per wave for select_any's groups.
-// The workgroup's first two tickets are drawn on the way, the second once the
-// first is back: by then every workgroup has drawn its first, so work spreads
-// over all of them before anyone takes a second item.
-__device__ __forceinline__ void build_selection(const FewArgs& f, Sel& g, uint16_t* rowof,
-                                                float* wof, uint16_t* stage, float* scr) {
+// (weight 0: the token does not use it).  stage gets the x rows; scr: E words
+// per wave for select_any.  Returns the routed slots.  The workgroup's
+// first two items are drawn on the way, the second once the first is back: by
+// then every workgroup has drawn its first, so work spreads over all of them
+// before anyone takes a second item.
+__device__ __forceinline__ int build_selection(const FewArgs& f, Sel& g, uint16_t* rowof,
+                                               float* wof, uint16_t* stage, uint32_t* scr) {
   const int tid = threadIdx.x, lane = tid % kWave, wv = wave_id();
   const int T = f.T, K = f.K, A = T * K, NS = f.NS;
   const bool drawer = tid == kThreads - kWave;
-  int t0 = 0;
   const int grp = blockIdx.x % kGroups;
+  int t0 = 0;
   if (drawer) t0 = draw(f, kTicket, grp);
   stage_x(f, stage);
+  const int max_slots = min(f.E, A) + NS;
+  for (int i = tid; i < max_slots * kMaxT; i += kThreads) {
+    rowof[i] = 0;
+    wof[i] = 0.f;
+  }
+  if (tid < kMaxPairs && tid >= A) g.ids[tid] = -1;
   for (int t = wv; t < T; t += kWaves) {
     const float* l = f.logits + (long)t * f.ldl;
     int* ids = g.ids + t * K;
@@ -364,77 +364,58 @@ __device__ __forceinline__ void build_selection(const FewArgs& f, Sel& g, uint16
       case 2: select_wave<2>(f, l, lane, ids, wts); break;
       case 4: select_wave<4>(f, l, lane, ids, wts); break;
       case 8: select_wave<8>(f, l, lane, ids, wts); break;
-      default: select_any(f, l, lane, ids, wts, scr + wv * f.E); break;
+      default:
+        select_any(f, l, lane, ids, wts, scr + wv * f.E);
     }
   }
   if (drawer) {
     g.ticket[0] = t0;
-    __asm__ __volatile__("" ::"v"(t0) : "memory");   // the first ticket is back
+    __asm__ __volatile__("" ::"v"(t0) : "memory");   // the first item is back
     g.ticket[1] = draw(f, kTicket, grp);
   }
-  for (int i = tid; i < kMaxPairs; i += kThreads)
-    if (i >= A) g.ids[i] = 0x7fffffff;
-  const int max_slots = min(f.E, A) + NS;
-  for (int i = tid; i < max_slots * kMaxT; i += kThreads) {
-    rowof[i] = 0;
-    wof[i] = 0.f;
-  }
   __syncthreads();
-  const int A4 = (A + 3) / 4;
-  int r0 = 0, rank = 0, e = 0;
-  if (tid < A) {   // thread p: pair p
+  // thread p: pair p; its expert's first pair
+  int fp = tid, e = 0;
+  if (tid < A) {
     e = g.ids[tid];
+    const int q1 = (tid + 3) / 4;
 #pragma unroll 4
-    for (int j = 0; j < A4; ++j) {
+    for (int j = q1 - 1; j >= 0; --j) {
       const i32x4_t v = *reinterpret_cast<const i32x4_t*>(g.ids + 4 * j);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        r0 += v[i] < e ? 1 : 0;
-        rank += v[i] == e && 4 * j + i < tid ? 1 : 0;
-      }
+      for (int i = 3; i >= 0; --i)
+        if (v[i] == e) fp = min(fp, 4 * j + i);
     }
-    g.rank[tid] = rank;
-    g.first[tid] = rank == 0 ? e : 0x7fffffff;   // an expert's first pair
-  } else if (tid < kMaxPairs) {
-    g.first[tid] = 0x7fffffff;
   }
+  const unsigned long long mine = __ballot(tid < A && fp == tid);
+  if (lane == 0 && wv < kMaxPairs / kWave) g.first[wv] = mine;
   __syncthreads();
+  int n = 0, slot = 0;   // slots in all; slots before pair fp's
+#pragma unroll
+  for (int i = 0; i < kMaxPairs / kWave; ++i) {
+    const unsigned long long mk = g.first[i];
+    const int c = __popcll(mk);
+    n += c;
+    slot += fp >= kWave * (i + 1) ? c
+            : fp > kWave * i      ? __popcll(mk & ((1ull << (fp - kWave * i)) - 1))
+                                  : 0;
+  }
   if (tid < A) {
-    int slot = 0;   // experts below e
-#pragma unroll 4
-    for (int j = 0; j < A4; ++j) {
-      const i32x4_t v = *reinterpret_cast<const i32x4_t*>(g.first + 4 * j);
-      slot += (v[0] < e) + (v[1] < e) + (v[2] < e) + (v[3] < e);
-    }
-    const int t = tid / K, row = r0 + rank;
-    g.row_tok[row] = t;
-    rowof[slot * kMaxT + t] = (uint16_t)row;
+    const int t = tid / K;
+    rowof[slot * kMaxT + t] = (uint16_t)tid;
     wof[slot * kMaxT + t] = g.wts[tid];
-    if (rank == 0) {
-      g.slot_e[slot] = e;
-      g.slot_r0[slot] = r0;
-    }
-  }
-  if (wv == kWaves - 1) {   // the shared experts' slots, behind the routed ones
-    int n = 0;
-    for (int i = 0; i < kMaxPairs; i += kWave)
-      n += __popcll(__ballot(g.first[i + lane] != 0x7fffffff));
-    if (lane == 0) {
-      g.n_routed = n;
-      g.slot_r0[n + NS] = A + NS * T;
-    }
-    if (lane < NS) {
-      g.slot_e[n + lane] = f.E + lane;
-      g.slot_r0[n + lane] = A + lane * T;
-    }
-    for (int i = lane; i < NS * T; i += kWave) {
-      const int s = i / T, t = i - s * T;
-      rowof[(n + s) * kMaxT + t] = (uint16_t)(A + i);
-      wof[(n + s) * kMaxT + t] =
-          f.sgate ? xtu_sigmoid(f.logits[(long)t * f.ldl + f.E + s]) : 1.0f;
-    }
+    if (fp == tid) g.slot_e[slot] = e;
+  } else if (wv == kWaves - 1) {   // the shared experts' slots, behind the routed ones
+    if (lane < NS) g.slot_e[n + lane] = f.E + lane;
+    for (int s = 0; s < NS; ++s)
+      if (lane < T) {
+        rowof[(n + s) * kMaxT + lane] = (uint16_t)(A + s * T + lane);
+        wof[(n + s) * kMaxT + lane] =
+            f.sgate ? xtu_sigmoid(f.logits[(long)lane * f.ldl + f.E + s]) : 1.0f;
+      }
   }
   __syncthreads();
+  return __builtin_amdgcn_readfirstlane(n);
 }
 
 // ---------------------------------------------------------------- launch 2
@@ -514,7 +495,7 @@ __device__ __forceinline__ void issue_seg(Seg<FMT, NPER>& r, const FewArgs& f, i
         (void*)(sx + (long)panel * gbytes), 0, live ? (int)gbytes : 0, kRawBufferFlags);
     const int off = (u0 % F::kUG) * F::kSBY;   // the units' bytes sit in one aligned word of 8
     const auto v = __builtin_amdgcn_raw_buffer_load_b64(
-        sr, (int)lane * 16 + (off & 8), (u0 / F::kUG) * 1024, kAuxNontemporal);
+        sr, (int)lane * 16 + (off & 8), (u0 / F::kUG) * 1024, 0);   // cached: chunks share lines
     const uint64_t b = ((uint64_t)v[1] << 32 | v[0]) >> (8 * (off & 7));
     r.sc0 = (uint32_t)b;
     r.sc1 = (uint32_t)(b >> 32);
@@ -556,7 +537,10 @@ __device__ __forceinline__ f32x4_t use_seg(const Seg<FMT, NPER>& r, int u0, int 
 // Segments in flight per wave: as many as keep the kernel at 128 VGPRs.
 template <int FMT, int NPER>
 constexpr int ring_depth() {
-  return FMT == kBF16 ? 2 : FMT == kFP8 ? (NPER == 4 ? 2 : 4) : (NPER == 4 ? 4 : 6);
+  return FMT == kBF16   ? 2
+         : FMT == kFP8  ? (NPER == 4 ? 2 : 4)
+         : FMT == kNVFP4 ? (NPER == 4 ? 2 : 4)
+                         : (NPER == 4 ? 4 : 6);
 }
 
 constexpr int kAuxDev = 16;   // buffer access at device scope (sc1)
@@ -584,8 +568,8 @@ __global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs 
   const int T = f.T, H = f.H, I = f.I;
   const int max_slots = min(f.E, T * f.K) + f.NS;
   uint16_t* rowof = reinterpret_cast<uint16_t*>(wof + max_slots * kMaxT);
-  build_selection(f, g, rowof, wof, stage,
-                  reinterpret_cast<float*>(dyn + (size_t)T * (H + 8) * 2));
+  const int n_routed = build_selection(
+      f, g, rowof, wof, stage, reinterpret_cast<uint32_t*>(dyn + (size_t)T * (H + 8) * 2));
   if (blockIdx.x == 0) {
     for (int i = tid; i < T * f.K; i += kThreads) {
       f.ids[i] = g.ids[i];
@@ -595,10 +579,10 @@ __global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs 
   int cur = __builtin_amdgcn_readfirstlane(g.ticket[0]);
   int nxt = __builtin_amdgcn_readfirstlane(g.ticket[1]);
   __syncthreads();   // the words are read before an item's draw takes one
-  const int n_routed = __builtin_amdgcn_readfirstlane(g.n_routed);
   const int npan = I / 16, hpan = H / 16;
-  const int n2 = n_routed * npan, n3 = f.chunks * hpan;
+  const int n2 = n_routed * npan;
   const int grp = blockIdx.x % kGroups;
+  int chunk = blockIdx.x / kGroups % f.chunks;   // of the down projection
   int t_new = 0;
   int it = 0;   // items done: which half of red, which ticket word
 
@@ -607,16 +591,8 @@ __global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs 
     DecodeArgs a{};
     a.w = f.w13;
     a.s = f.s13;
-    a.gs = f.gs13;
-    a.out = f.act;
-    a.H = H;
-    a.I = I;
     a.w_estride = f.w13_es;
     a.s_estride = f.s13_es;
-    a.limit = f.limit;
-    a.alpha = f.alpha;
-    a.beta = f.beta;
-    a.ksplit = kKS;
     const int half = w / kKS, ks = w % kKS, nunits = H / 128;
     const int u0 = ks * nunits / kKS, u1 = (ks + 1) * nunits / kKS;
     const int rounds = max((u1 - u0 + NU - 1) / NU, 1);
@@ -626,7 +602,7 @@ __global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs 
       const int e = __builtin_amdgcn_readfirstlane(g.slot_e[slot]);
       return make_stream<FMT>(a, e, half ? npan + sub : sub, H, live);
     };
-    const int ldx = H + 8;
+    const uint16_t* xa = stage + min(m, T - 1) * (H + 8) + q * F::kCK;
     int count = 0;
     Round<FMT, NU> r;
     while (true) {
@@ -662,21 +638,44 @@ __global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs 
       while (true) {   // cur is loaded; nxt rolls in behind it
         if (tid == 0) t_new = nxt < n2 ? draw(f, kTicket, grp) : n2;
         const int slot = cur / npan, sub = cur - slot * npan;
-        const int r0 = g.slot_r0[slot], na = g.slot_r0[slot + 1] - r0;
-        const int ws = g.slot_e[slot];
-        const int tok = g.row_tok[r0 + min(m, na - 1)];
-        const uint16_t* xa = stage + tok * ldx + q * F::kCK;
         f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-        for (int rd = 0; rd + 1 < rounds; ++rd) {
+        // (one copy of the round's code: what is run through once costs more to
+        // fetch than to run)
+#pragma unroll 1
+        for (int rd = 0; rd < rounds; ++rd) {
           const int ub = u0 + rd * NU;
-          roll_round<FMT, NU>(r, acc, ub, u1, xa, st, ub + NU, u1, lane);
+          const bool last = rd + 1 == rounds;
+          if (last) st = stream_of(nxt);
+          roll_round<FMT, NU>(r, acc, ub, u1, xa, st, last ? u0 : ub + NU, u1, lane);
         }
-        const Stream<FMT> sn = stream_of(nxt);
-        roll_round<FMT, NU>(r, acc, u0 + (rounds - 1) * NU, u1, xa, sn, u0, u1, lane);
-        st = sn;
         if (tid == 0) g.ticket[it & 1] = t_new;
-        // (ends with every wave past a barrier: the ticket is visible)
-        gate_up_epilogue<FMT, true>(a, red[it & 1], acc, w, lane, r0, na, ws, sub);
+        // the K splits in their order; the rows of the tokens that use the
+        // expert, bf16, read by other workgroups in this launch
+        f32x4_t(*rd_)[kWave] = red[it & 1];
+        rd_[w][lane] = acc;
+        __syncthreads();
+        if (tid < 256) {
+          const int t = tid / 16, n = tid % 16;
+          if (t < T && wof[slot * kMaxT + t] != 0.f) {
+            const int l = (t / 4) * 16 + n, i = t % 4;
+            float gv = 0.f, uv = 0.f;
+#pragma unroll
+            for (int k = 0; k < kKS; ++k) {
+              gv += rd_[k][l][i];
+              uv += rd_[kKS + k][l][i];
+            }
+            if constexpr (FMT == kNVFP4) {
+              if (f.gs13) {
+                const int e = g.slot_e[slot];
+                gv *= f.gs13[2 * e];
+                uv *= f.gs13[2 * e + 1];
+              }
+            }
+            __hip_atomic_store(f.act + (long)rowof[slot * kMaxT + t] * I + 16 * sub + n,
+                               f32_to_bf16(silu_gate(gv, uv, f.limit, f.alpha, f.beta)),
+                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          }
+        }
         ++count;
         cur = nxt;
         nxt = __builtin_amdgcn_readfirstlane(g.ticket[it & 1]);
@@ -692,227 +691,212 @@ __global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs 
       if (count)
         __hip_atomic_fetch_add(f.ctl + kDone + kLine * grp, (unsigned)count, __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_AGENT);
-      g.ticket[0] = draw(f, kTicket3, grp);
+      g.ticket[0] = draw(f, kTicket3 + chunk * kGroups * kLine, grp);
     }
     __syncthreads();
   }
 
   // ---- output panels
-  cur = __builtin_amdgcn_readfirstlane(g.ticket[0]);
-  if (cur >= n3) return;   // whole workgroup
-  const int nu = I / 128, nseg = (nu + NPER - 1) / NPER;   // segments of an expert
-  const int n_slots = n_routed + f.NS;
-  // first slot of chunk c: rows of a slot belong to the chunk of its first row
-  auto chunk_slot = [&](int c) {
-    int lo = 0, hi = n_slots;
-    const int row = c * f.rows_per_chunk;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (g.slot_r0[mid] < row) lo = mid + 1;
-      else hi = mid;
-    }
-    return __builtin_amdgcn_readfirstlane(lo);
-  };
-  Seg<FMT, NPER> ring[D];
-  // segment i of this wave in an item over slots [j0, j1), panel p
-  auto issue_item = [&](int d, int i, int j0, int j1, int p, bool live) {
-    const int fl = w + kWaves * i, j = j0 + fl / nseg;
-    const bool ok = live && j < j1;
-    const int e = __builtin_amdgcn_readfirstlane(g.slot_e[ok ? j : 0]);
-    issue_seg<FMT, NPER>(ring[d], f, e, ok, p, (fl % nseg) * NPER, lane);
-  };
-  int c = cur / hpan, p = cur - c * hpan;
-  int j0 = chunk_slot(c), j1 = chunk_slot(c + 1);
-#pragma unroll
-  for (int d = 0; d < D; ++d) issue_item(d, d, j0, j1, p, true);
-  __builtin_amdgcn_sched_barrier(0);
-
-  // wait for every gate/up item: all are drawn (see the top)
-  if (w == 0) {
-    for (int n = 0;; ++n) {
-      unsigned v = 0u;
-      if (lane < 8)
-        v = __hip_atomic_load(f.ctl + kDone + kLine * lane, __ATOMIC_RELAXED,
-                              __HIP_MEMORY_SCOPE_AGENT);
-      v += __shfl_xor(v, 1, kWave);
-      v += __shfl_xor(v, 2, kWave);
-      v += __shfl_xor(v, 4, kWave);
-      if (__builtin_amdgcn_readfirstlane(v) == (unsigned)n2) break;
-      if (n == kSpin) {
-        if (lane == 0)
-          __hip_atomic_store(f.ctl + kFlag, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        break;
-      }
-      __builtin_amdgcn_s_sleep(2);
-    }
-    // the second panel, drawn when every workgroup has come this far
-    if (lane == 0) g.ticket[1] = draw(f, kTicket3, grp);
-  }
-  __syncthreads();
-  nxt = __builtin_amdgcn_readfirstlane(g.ticket[1]);
-  __syncthreads();   // read before an item's draw takes the word
-
-  const int lda = I + 8, per_row = I / 8;
+  const int nu = I / 128, n_slots = n_routed + f.NS, cun = f.chunk_units;
+  const int rows = T * f.K + f.NS * T, lda = cun * 128 + 8;
   const __amdgpu_buffer_rsrc_t ract = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)f.act, 0, (T * f.K + f.NS * T) * I * 2, kRawBufferFlags);
-  int staged = -1, row0 = 0;
-  while (true) {
-    if (c != staged) {   // the chunk's activation rows, read at device scope
-      if (staged >= 0) __syncthreads();   // the old chunk's are used
-      staged = c;
-      row0 = g.slot_r0[j0];
-      const int pieces = (g.slot_r0[j1] - row0) * per_row;
+      (void*)f.act, 0, rows * I * 2, kRawBufferFlags);
+  Seg<FMT, NPER> ring[D];
+  bool waited = false;
+  // the own chunk first, then what the others have left
+  for (int tries = 0; tries < f.chunks; ++tries, chunk = (chunk + 1) % f.chunks) {
+    const int which = kTicket3 + chunk * kGroups * kLine;
+    if (tries) {
+      __syncthreads();
+      if (tid == 0) g.ticket[0] = draw(f, which, grp);
+      __syncthreads();
+    }
+    int p = __builtin_amdgcn_readfirstlane(g.ticket[0]);
+    if (p >= hpan) continue;
+    // segment i of this wave in a panel: all slots, nseg each
+    const int units = min(cun, nu - chunk * cun), nseg = (units + NPER - 1) / NPER;
+    const int total = n_slots * nseg;
+    const int rounds = ((total + kWaves - 1) / kWaves + D - 1) / D;
+    auto issue_item = [&](int d, int i, int pn, bool live) {
+      const int fl = w + kWaves * i, j = fl / nseg;
+      const bool ok = live && j < n_slots;
+      const int e = __builtin_amdgcn_readfirstlane(g.slot_e[ok ? j : 0]);
+      issue_seg<FMT, NPER>(ring[d], f, e, ok, pn, chunk * cun + (fl - j * nseg) * NPER, lane);
+    };
+#pragma unroll
+    for (int d = 0; d < D; ++d) issue_item(d, d, p, true);
+    __builtin_amdgcn_sched_barrier(0);
+    if (!waited) {
+      // wait for every gate/up item: all are drawn (see the top)
+      if (w == 0) {
+        for (int n = 0;; ++n) {
+          unsigned v = 0u;
+          if (lane < 8)
+            v = __hip_atomic_load(f.ctl + kDone + kLine * lane, __ATOMIC_RELAXED,
+                                  __HIP_MEMORY_SCOPE_AGENT);
+          v += __shfl_xor(v, 1, kWave);
+          v += __shfl_xor(v, 2, kWave);
+          v += __shfl_xor(v, 4, kWave);
+          if (__builtin_amdgcn_readfirstlane(v) == (unsigned)n2) break;
+          if (n == kSpin) {
+            if (lane == 0)
+              __hip_atomic_store(f.ctl + kFlag, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            break;
+          }
+          __builtin_amdgcn_s_sleep(2);
+        }
+      }
+
+      waited = true;
+    }
+    // the second panel: drawn when every workgroup has come this far
+    if (tid == 0) g.ticket[1] = draw(f, which, grp);
+    __syncthreads();   // the wait is over for all; the old chunk's rows are used
+    {   // the rows' part of the chunk, read at device scope
+      const int per_row = units * 16, pieces = rows * per_row;
       constexpr int SB = 8;
       for (int c0 = tid; c0 < pieces; c0 += SB * kThreads) {
         u32x4_t v[SB];
-#pragma unroll
-        for (int k = 0; k < SB; ++k)
-          v[k] = __builtin_bit_cast(
-              u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                           ract, (row0 * per_row + min(c0 + k * kThreads, pieces - 1)) * 16, 0,
-                           kAuxDev));
+        int at[SB];
 #pragma unroll
         for (int k = 0; k < SB; ++k) {
-          const int pc = c0 + k * kThreads;
-          if (pc < pieces) {
-            const int rr = pc / per_row;
-            *reinterpret_cast<u32x4_t*>(stage + rr * lda + (pc - rr * per_row) * 8) = v[k];
+          const int pc = min(c0 + k * kThreads, pieces - 1);
+          const int rr = pc / per_row, kk = (pc - rr * per_row) * 8;
+          at[k] = rr * lda + kk;
+          v[k] = __builtin_bit_cast(
+              u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                           ract, (rr * I + chunk * cun * 128 + kk) * 2, 0, kAuxDev));
+        }
+#pragma unroll
+        for (int k = 0; k < SB; ++k)
+          if (c0 + k * kThreads < pieces) *reinterpret_cast<u32x4_t*>(stage + at[k]) = v[k];
+      }
+    }
+    int next = __builtin_amdgcn_readfirstlane(g.ticket[1]);
+    __syncthreads();
+    while (true) {
+      if (tid == 0) t_new = next < hpan ? draw(f, which, grp) : hpan;
+      const bool more = next < hpan;
+      f32x4_t tacc = {0.f, 0.f, 0.f, 0.f};   // tokens 4q + i, column m of the panel
+      auto use_item = [&](int d, int i) {
+        const int fl = w + kWaves * i;
+        if (fl < total) {
+          const int j = fl / nseg, u0 = (fl - j * nseg) * NPER;   // within the chunk
+          const uint16_t* xa = stage + (int)rowof[j * kMaxT + m] * lda + q * F::kCK;
+          f32x4_t pe = use_seg<FMT, NPER>(ring[d], u0, units, xa);
+          if constexpr (FMT == kNVFP4) {
+            if (f.gs2) pe = pe * f.gs2[__builtin_amdgcn_readfirstlane(g.slot_e[j])];
+          }
+          const f32x4_t wv = *reinterpret_cast<const f32x4_t*>(wof + j * kMaxT + 4 * q);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tacc[k] = wv[k] != 0.f ? __builtin_fmaf(wv[k], pe[k], tacc[k]) : tacc[k];
+        }
+      };
+#pragma unroll 1
+      for (int rd = 0; rd < rounds; ++rd) {
+        const bool last = rd + 1 == rounds;
+        const int pn = last && more ? next : p, base = last ? 0 : (rd + 1) * D;
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+          use_item(d, rd * D + d);
+          issue_item(d, base + d, pn, !last || more);
+        }
+      }
+      // the waves' sums, in their order
+      f32x4_t(*rd_)[kWave] = red[it & 1];
+      rd_[w][lane] = tacc;
+      if (tid == 0) g.ticket[it & 1] = t_new;
+      __syncthreads();
+      if (tid < 256) {
+        const int tok = tid / 16, n = tid % 16;
+        if (tok < T) {
+          const int l = (tok / 4) * 16 + n, k = tok % 4;
+          float v = 0.f;
+#pragma unroll
+          for (int i = 0; i < kWaves; ++i) v += rd_[i][l][k];
+          const long o = (long)tok * H + 16 * p + n;
+          if (f.chunks > 1)
+            __hip_atomic_store(f.part + (long)chunk * T * H + o, v, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+          else if (f.out_bf16)
+            reinterpret_cast<uint16_t*>(f.out)[o] = f32_to_bf16(v);
+          else
+            reinterpret_cast<float*>(f.out)[o] = v;
+        }
+      }
+      const int after = __builtin_amdgcn_readfirstlane(g.ticket[it & 1]);
+      ++it;
+      if (f.chunks > 1) {
+        // the last chunk of a panel to get here adds them all up, in order
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (tid == 0)
+          g.last = __hip_atomic_fetch_add(f.ctl + kPanels + p, 1u, __ATOMIC_RELAXED,
+                                          __HIP_MEMORY_SCOPE_AGENT) == (unsigned)f.chunks - 1;
+        __syncthreads();
+        if (g.last && tid < 256) {
+          const int tok = tid / 16, n = tid % 16;
+          if (tok < T) {
+            const long o = (long)tok * H + 16 * p + n;
+            float v = 0.f;
+            for (int i = 0; i < f.chunks; ++i)
+              v += __hip_atomic_load(f.part + (long)i * T * H + o, __ATOMIC_RELAXED,
+                                     __HIP_MEMORY_SCOPE_AGENT);
+            if (f.out_bf16) reinterpret_cast<uint16_t*>(f.out)[o] = f32_to_bf16(v);
+            else reinterpret_cast<float*>(f.out)[o] = v;
           }
         }
       }
-      __syncthreads();
+      if (!more) break;
+      p = next;
+      next = after;
     }
-    if (tid == 0) t_new = draw(f, kTicket3, grp);
-    // next item
-    const bool more = nxt < n3;
-    const int cn = more ? nxt / hpan : c, pn = more ? nxt - cn * hpan : p;
-    const int jn0 = cn == c ? j0 : chunk_slot(cn), jn1 = cn == c ? j1 : chunk_slot(cn + 1);
-    const int total = (j1 - j0) * nseg;
-    const int rounds = ((total + kWaves - 1) / kWaves + D - 1) / D;
-    f32x4_t tacc = {0.f, 0.f, 0.f, 0.f};   // tokens 4q + i, column m of the panel
-    auto use_item = [&](int d, int i) {
-      const int fl = w + kWaves * i;
-      if (fl < total) {
-        const int j = j0 + fl / nseg, sg = fl % nseg;
-        const uint16_t* xa =
-            stage + max((int)rowof[j * kMaxT + m] - row0, 0) * lda + q * F::kCK;
-        f32x4_t pe = use_seg<FMT, NPER>(ring[d], sg * NPER, nu, xa);
-        if constexpr (FMT == kNVFP4) {
-          if (f.gs2) pe = pe * f.gs2[__builtin_amdgcn_readfirstlane(g.slot_e[j])];
-        }
-        const f32x4_t wv = *reinterpret_cast<const f32x4_t*>(wof + j * kMaxT + 4 * q);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          tacc[k] = wv[k] != 0.f ? __builtin_fmaf(wv[k], pe[k], tacc[k]) : tacc[k];
-      }
-    };
-    for (int rd = 0; rd + 1 < rounds; ++rd) {
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        use_item(d, rd * D + d);
-        issue_item(d, (rd + 1) * D + d, j0, j1, p, true);
-      }
-    }
-#pragma unroll
-    for (int d = 0; d < D; ++d) {
-      if (rounds > 0) use_item(d, (rounds - 1) * D + d);
-      issue_item(d, d, jn0, jn1, pn, more);
-    }
-    // the waves' sums, in their order
-    f32x4_t(*rd_)[kWave] = red[it & 1];
-    rd_[w][lane] = tacc;
-    if (tid == 0) g.ticket[it & 1] = t_new;
-    __syncthreads();
-    if (tid < 256) {
-      const int tok = tid / 16, n = tid % 16;
-      if (tok < T) {
-        const int l = (tok / 4) * 16 + n, k = tok % 4;
-        float v = 0.f;
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) v += rd_[i][l][k];
-        const long o = (long)tok * H + 16 * p + n;
-        if (f.chunks > 1)
-          __hip_atomic_store(f.part + (long)c * T * H + o, v, __ATOMIC_RELAXED,
-                             __HIP_MEMORY_SCOPE_AGENT);
-        else if (f.out_bf16)
-          reinterpret_cast<uint16_t*>(f.out)[o] = f32_to_bf16(v);
-        else
-          reinterpret_cast<float*>(f.out)[o] = v;
-      }
-    }
-    const int nn = __builtin_amdgcn_readfirstlane(g.ticket[it & 1]);
-    ++it;
-    if (f.chunks > 1) {
-      // the last chunk of a panel to get here adds them all up, in order
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
-      if (tid == 0)
-        g.last = __hip_atomic_fetch_add(f.ctl + kPanels + p, 1u, __ATOMIC_RELAXED,
-                                        __HIP_MEMORY_SCOPE_AGENT) == (unsigned)f.chunks - 1;
-      __syncthreads();
-      if (g.last && tid < 256) {
-        const int tok = tid / 16, n = tid % 16;
-        if (tok < T) {
-          const long o = (long)tok * H + 16 * p + n;
-          float v = 0.f;
-          for (int i = 0; i < f.chunks; ++i)
-            v += __hip_atomic_load(f.part + (long)i * T * H + o, __ATOMIC_RELAXED,
-                                   __HIP_MEMORY_SCOPE_AGENT);
-          if (f.out_bf16) reinterpret_cast<uint16_t*>(f.out)[o] = f32_to_bf16(v);
-          else reinterpret_cast<float*>(f.out)[o] = v;
-        }
-      }
-    }
-    if (!more) break;
-    c = cn;
-    p = pn;
-    j0 = jn0;
-    j1 = jn1;
-    nxt = nn;
   }
 }
 
+
 // ---------------------------------------------------------------- host
 
-// bits: of a weight, with its scales.  More chunks than the LDS asks for give
-// the output panels more items: where there are fewer panels than CUs, or their
-// last round leaves CUs idle.  Times in us: a CU streams about 25 GB/s, an item
-// costs 0.7 beside its stream, the joining of chunks 2.
-inline bool make_plan(int T, int E, int K, int NS, int H, int I, float bits, bool groups,
-                      Plan& p) {
+// bits: of a weight, with its scales.  A segment is four units where the LDS
+// holds all rows of four units and their number divides (BF16: two, by its
+// registers).  More chunks than the LDS asks for give the output panels more
+// items: where there are fewer panels than CUs, or their last round leaves CUs
+// idle.  Times in us: a CU streams about 25 GB/s, an item costs 0.7 beside its
+// stream, the joining of chunks 2.
+__host__ inline bool make_plan(int T, int E, int K, int NS, int H, int I, float bits, Plan& p) {
   if (T < 1 || T > kMaxT || K < 1 || K > 16 || K > E || E > kMaxE || T * K > kMaxPairs ||
       NS < 0 || NS > kMaxShared || H < 256 || H % 256 || H > 16384 || I < 128 || I % 128 ||
       I > 16384)
     return false;
-  const int slots = std::min(E, T * K) + NS, R = T * (K + NS);
+  const int slots = std::min(E, T * K) + NS, R = T * (K + NS), nu = I / 128;
   const size_t fixed = (size_t)2 * kWaves * kWave * 16 + sel_bytes() + table_bytes(slots) + 256;
   const size_t half = 80 * 1024, full = 160 * 1024;
-  // x rows, and behind them select_any's scores
-  const size_t xb = (size_t)T * (H + 8) * 2 + (groups ? (size_t)kWaves * E * 4 : 0);
-  const size_t row = (size_t)(I + 8) * 2;
+  // x rows, and behind them select_any's keys
+  const size_t xb = (size_t)T * (H + 8) * 2 + (size_t)kWaves * E * 4;
   if (fixed + xb > full) return false;
-  const int cap = (int)((full - fixed) / row);
-  int least = 1;
-  if (cap < R) {   // a chunk's last slot may begin on its last row
-    const int rpc = cap - (T - 1);
-    if (rpc < 1) return false;
-    least = (R + rpc - 1) / rpc;
-  }
+  const auto stage_of = [&](int units) { return (size_t)R * (units * 128 + 8) * 2; };
+  p.nper = bits < 16.0f && nu % 4 == 0 && fixed + stage_of(4) <= full ? 4 : 2;
   const double active = E * (1.0 - std::pow(1.0 - (double)K / E, T)) + NS;
   const double panel_us = active * I * 16 * bits / 8 / 25e3;
   const int hpan = H / 16, cus = cu_count();
   double best = 1e30;
-  for (int c = least; c <= std::min(least + 7, R); ++c) {
+  for (int units = (nu + p.nper - 1) / p.nper * p.nper; units >= p.nper; units -= p.nper) {
+    if (fixed + stage_of(std::min(units, nu)) > full) continue;
+    const int c = (nu + units - 1) / units;
+    if (c > kMaxChunks) break;
     const double t = (c * hpan + cus - 1) / cus * (panel_us / c + 0.7) + (c > 1 ? 2.0 : 0.0);
     if (t < best - 0.01) {
       best = t;
       p.chunks = c;
+      p.chunk_units = std::min(units, nu);
     }
   }
-  p.rows_per_chunk = (R + p.chunks - 1) / p.chunks;
-  const int rows = p.chunks == 1 ? R : p.rows_per_chunk + T - 1;
-  p.stage = (std::max(xb, rows * row) + 15) / 16 * 16;
-  p.occ = fixed + p.stage <= half ? 2 : 1;
+  if (best > 1e29) return false;
+  p.stage = (std::max(xb, stage_of(p.chunk_units)) + 15) / 16 * 16;
+  // two workgroups on a CU where LDS allows and they have about an item each;
+  // with more, half as many workgroups end closer together
+  p.occ = fixed + p.stage <= half && (active - NS) * (I / 16) <= 2.0 * cus ? 2 : 1;
   p.lds = p.stage + sel_bytes() + table_bytes(slots);
   return true;
 }
@@ -939,7 +923,7 @@ hipError_t launch_nu(const FewArgs& f, const Plan& p, hipStream_t stream) {
   const hipError_t e = hipPeekAtLastError();
   if (e != hipSuccess) return e;
   if constexpr (FMT != kBF16) {
-    if (f.I / 128 % 4 == 0) {
+    if (p.nper == 4) {
       launch_experts<FMT, NU, 4>(f, p, stream);
       return hipPeekAtLastError();
     }

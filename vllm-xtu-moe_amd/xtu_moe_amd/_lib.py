@@ -107,7 +107,7 @@ SIGNATURES = {
                                    _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _f, _f, _f, _vp]),
     "xtu_gemm_pair_down": (_i, [_i, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _l, _l, _vp, _vp, _vp,
                                 _vp, _vp, _vp, _vp, _i, _vp, _vp]),
-    "xtu_few_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "xtu_few_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "xtu_few_block": (_i, [_vp, _vp]),
     "xtu_linear": (_i, [_vp, _vp]),
     "xtu_linear_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),

@@ -130,8 +130,8 @@ class MoeBlock:
         need = self._few_bytes.get(T)
         if need is None:
             need = self._few_bytes[T] = int(_lib.call(
-                "xtu_few_workspace_bytes", W.fmt, T, W.E, self.top_k, W.n_shared, self.n_group,
-                W.H, W.I)) if T else 0
+                "xtu_few_workspace_bytes", W.fmt, T, W.E, self.top_k, W.n_shared, W.H,
+                W.I)) if T else 0
         ids = x.new_empty((T, self.top_k), dtype=torch.int32)
         wts = x.new_empty((T, self.top_k), dtype=torch.float32)
         if need:
