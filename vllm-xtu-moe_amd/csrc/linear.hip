@@ -131,7 +131,7 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const uint16_t* x, lon
   const long r = p / per;
   const int k = (int)(p - r * per) * 8;
   const uint16_t* row = r < M ? x + r * ldx : w + (r - M) * ldw;
-  *reinterpret_cast<u32x4_t*>(out + p * 8) = load8(row, k, K);
+  *reinterpret_cast<u32x4_t*>(out + p * 8) = load8<true>(row, k, K);
 }
 
 }  // namespace

@@ -23,20 +23,18 @@ namespace {
 constexpr int kSkW = 16;           // waves per workgroup
 constexpr int kSkinnyGrid = 256;   // one workgroup per CU
 
-// 16 bytes at a wave-uniform base plus a lane's 32-bit offset.
-template <bool ALIGNED>
-__device__ __forceinline__ u32x4_t load_w(const uint16_t* base, uint32_t off) {
-  const uint8_t* p = reinterpret_cast<const uint8_t*>(base) + off;
-  if constexpr (ALIGNED) {
-    return *reinterpret_cast<const u32x4_t*>(p);
-  } else {
-    u32x4_t v;
-    __builtin_memcpy(&v, p, 16);
-    return v;
-  }
-}
+// A slot of the stream: 16 bytes of a row that starts on a word (WORDS), or the
+// five words around them.
+template <bool WORDS>
+struct Slot {
+  u32x4_t v;
+};
+template <>
+struct Slot<false> {
+  Words5 v;
+};
 
-template <bool GATED, bool ALIGNED, int U>
+template <bool GATED, bool WORDS, int U>
 __global__ __launch_bounds__(64 * kSkW) void linear_skinny_kernel(LinearArgs a, int rp) {
   constexpr int KW = GATED ? kSkW / 2 : kSkW;   // waves along K
   extern __shared__ __attribute__((aligned(16))) uint16_t xs[];   // [M][K32 + 8]
@@ -59,10 +57,12 @@ __global__ __launch_bounds__(64 * kSkW) void linear_skinny_kernel(LinearArgs a, 
   // loads are unconditional (past the wave's range: its last step again, or
   // for a wave without steps the row's start, not used), so that every wait
   // is for exactly the slot about to be used
-  u32x4_t wv[U];
+  Slot<WORDS> wv[U];
   const int k_last = max(s1 - 1, s0 > 0 ? s0 - 1 : 0);
   auto issue = [&](int i, const uint16_t* wb, uint32_t wo, int s) {
-    wv[i] = load_w<ALIGNED>(wb + 32L * min(s, k_last), wo);
+    const uint8_t* p = reinterpret_cast<const uint8_t*>(wb + 32L * min(s, k_last)) + wo;
+    if constexpr (WORDS) wv[i].v = *reinterpret_cast<const u32x4_w*>(p);
+    else wv[i].v = load_words(p, (uint32_t)reinterpret_cast<uintptr_t>(p) & 2u);
   };
   int pan = blockIdx.x;
   const uint16_t* wb = wbase(pan);
@@ -84,11 +84,15 @@ __global__ __launch_bounds__(64 * kSkW) void linear_skinny_kernel(LinearArgs a, 
 
   for (int it = 0; pan < npan; pan += gridDim.x, ++it) {
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    // of this lane's row of the panel (k steps are whole words)
+    const uint32_t wshift = ((uint32_t)reinterpret_cast<uintptr_t>(wb) + wo) & 2u;
     auto use = [&](int i, int s) {
       if (s < s1) {
         const u32x4_t xv = *reinterpret_cast<const u32x4_t*>(xl + 32 * s);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(wv[i]), as_bf16x8(xv), acc, 0, 0,
-                                                      0);
+        u32x4_t v;
+        if constexpr (WORDS) v = wv[i].v;
+        else v = shifted(wv[i].v, wshift);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(v), as_bf16x8(xv), acc, 0, 0, 0);
       }
     };
     const int next = pan + (int)gridDim.x;
@@ -140,7 +144,7 @@ __global__ __launch_bounds__(64 * kSkW) void linear_skinny_kernel(LinearArgs a, 
 
 size_t skinny_lds(const LinearArgs& a) { return (size_t)a.M * ((a.K + 31) / 32 * 32 + 8) * 2; }
 
-template <bool GATED, bool ALIGNED>
+template <bool GATED, bool WORDS>
 hipError_t launch(const LinearArgs& a, hipStream_t stream) {
   int rp = 2;   // columns of a panel: about one panel per CU, 16 at most
   while (rp < 16 && (a.N + rp - 1) / rp > kSkinnyGrid) rp *= 2;
@@ -149,7 +153,7 @@ hipError_t launch(const LinearArgs& a, hipStream_t stream) {
   const size_t lds = skinny_lds(a);
   // steps of a wave: U of them in flight
   const bool few = a.K / 32 <= 4 * (GATED ? kSkW / 2 : kSkW);
-  auto k = few ? linear_skinny_kernel<GATED, ALIGNED, 4> : linear_skinny_kernel<GATED, ALIGNED, 8>;
+  auto k = few ? linear_skinny_kernel<GATED, WORDS, 4> : linear_skinny_kernel<GATED, WORDS, 8>;
   k<<<grid, 64 * kSkW, lds, stream>>>(a, rp);
   return hipPeekAtLastError();
 }
@@ -162,10 +166,9 @@ bool skinny_fits(const LinearArgs& a) {
 }
 
 hipError_t launch_skinny(const LinearArgs& a, hipStream_t stream) {
-  const auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-  const bool aligned = al(a.w) && a.ldw % 8 == 0;
-  if (a.act == kSwiglu) return aligned ? launch<true, true>(a, stream) : launch<true, false>(a, stream);
-  return aligned ? launch<false, true>(a, stream) : launch<false, false>(a, stream);
+  const bool words = reinterpret_cast<uintptr_t>(a.w) % 4 == 0 && a.ldw % 2 == 0;
+  if (a.act == kSwiglu) return words ? launch<true, true>(a, stream) : launch<true, false>(a, stream);
+  return words ? launch<false, true>(a, stream) : launch<false, false>(a, stream);
 }
 
 }  // namespace lin
