@@ -280,9 +280,10 @@ def test_two_streams_at_once():
         assert torch.equal(o, refs[i])
 
 
-def test_graphs_captured_from_one_stream_replayed_at_once():
+@pytest.mark.parametrize("T", [3, 40])
+def test_graphs_captured_from_one_stream_replayed_at_once(T):
     blks = [_block(f, l)[0] for f, l in (("mxfp4", LAYERS[6]), ("nvfp4", LAYERS[7]))]
-    xs = [_x(3, b.W.H, 4) for b in blks]
+    xs = [_x(T, b.W.H, 4) for b in blks]
     outs, graphs = [], []
     for b, x in zip(blks, xs):
         b(x)

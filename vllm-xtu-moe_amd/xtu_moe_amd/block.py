@@ -12,13 +12,14 @@ inside.
 """
 from __future__ import annotations
 
+import contextlib
 import struct
 
 import torch
 
 from . import _lib
 from .formats import FMT_BF16, FMT_FP8, FMT_MXFP4, FMT_NVFP4
-from .layer import ExpertWeights, _same_device, moe_forward, route
+from .layer import ExpertWeights, _same_device, moe_forward, route, scratch_per_call
 from .linear import _current_device, _overlap, linear, on_stream, raw_stream
 
 # xtu_few_args: x, gate, shared_gate, bias, six planes, out, ids, weights,
@@ -67,7 +68,7 @@ class MoeBlock:
         self._shape = (W.H, W.I, W.E, W.n_shared, self.top_k, int(scoring == "sigmoid"),
                        self.renormalize, self.n_group, self.topk_group)
         self._floats = (self.routed_scaling_factor, self.limit, self.alpha, self.beta)
-        self._few_bytes = {}   # workspace by token count (0: composed)
+        self._few_bytes = {}   # workspace by token count, of the few
         self._entry = _lib.load().xtu_few_block
         # the shared experts as further routed ones: their weight is then the
         # gate's (the same planes)
@@ -129,15 +130,19 @@ class MoeBlock:
         T = x.shape[0]
         need = self._few_bytes.get(T)
         if need is None:
-            need = self._few_bytes[T] = int(_lib.call(
-                "xtu_few_workspace_bytes", W.fmt, T, W.E, self.top_k, W.n_shared, W.H,
-                W.I)) if T else 0
+            need = int(_lib.call("xtu_few_workspace_bytes", W.fmt, T, W.E, self.top_k, W.n_shared,
+                                 W.H, W.I)) if T else 0
+            if need:
+                self._few_bytes[T] = need
         ids = x.new_empty((T, self.top_k), dtype=torch.int32)
         wts = x.new_empty((T, self.top_k), dtype=torch.float32)
         if need:
             self._few(x, out, ids, wts, need)
         elif T:
-            self._composed(x, out, ids, wts)
+            # (eagerly the stream's scratch: calls on it run in order)
+            capturing = torch.cuda.is_current_stream_capturing()
+            with scratch_per_call() if capturing else contextlib.nullcontext():
+                self._composed(x, out, ids, wts)
         return (out, wts, ids) if return_routing else out
 
     def _few(self, x, out, ids, wts, need):

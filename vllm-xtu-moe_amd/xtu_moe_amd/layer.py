@@ -11,8 +11,10 @@ shape for the life of the process (as the reference does with its
 """
 from __future__ import annotations
 
+import contextlib
 import math
 import os
+import threading
 
 import torch
 
@@ -412,6 +414,26 @@ _BUF_CACHE: dict = {}
 # Buffers replaced by a larger one (kept for the same reason).  Growth is
 # geometric (power-of-two rows), so they total less than the live ones.
 _RETIRED: list = []
+_PER_CALL = threading.local()
+
+
+@contextlib.contextmanager
+def scratch_per_call():
+    """Calls inside allocate their scratch for themselves instead of sharing
+    the stream's: captured, it lies in the graph's own memory, so that graphs
+    captured on one stream may be replayed at once on several.  (For calls on
+    one stream; the one-launch decode layer, whose barrier words outlive the
+    call, is left out.)"""
+    before = per_call_scratch()
+    _PER_CALL.on = True
+    try:
+        yield
+    finally:
+        _PER_CALL.on = before
+
+
+def per_call_scratch() -> bool:
+    return getattr(_PER_CALL, "on", False)
 
 
 def segmentation(T, K, E, NS, bm, device, stream=None) -> _Segmentation:
@@ -419,6 +441,8 @@ def segmentation(T, K, E, NS, bm, device, stream=None) -> _Segmentation:
     device, stream): calls on one stream run in order and share them;
     another stream gets its own.  Capacity grows to the next power of two
     of T, so varying batch sizes allocate O(log T_max) times in total."""
+    if per_call_scratch():
+        return _Segmentation(_SegBuffers(T, K, E, NS, bm, device), T, K, E, NS, bm)
     st = _stream(stream)
     key = (K, E, NS, bm, str(device), st)
     b = _SEG_CACHE.get(key)
@@ -435,6 +459,8 @@ def _buf(name, shape, dtype, device, stream=None):
     first `rows` rows of a cached buffer whose row capacity is a power of two
     (stream-ordered reuse; concurrent streams get their own)."""
     rows, tail = int(shape[0]), tuple(int(s) for s in shape[1:])
+    if per_call_scratch():
+        return torch.empty((rows,) + tail, dtype=dtype, device=device)
     st = _stream(stream)
     key = (name, tail, dtype, str(device), st)
     t = _BUF_CACHE.get(key)
@@ -1070,7 +1096,8 @@ def moe_forward(x, topk_ids, topk_weights, W: ExpertWeights, *, swiglu_limit=0.0
     fused = (path == "decode" and T > 0 and seg.small
              and _route_gate_up_ok(fmt, rmode, T, E, K, router, H, I, NS,
                                    gu_bytes=min(seg.max_tiles, TINY_MAX_PAIRS) * _w13_bytes(W)))
-    layer_ok = fused and _layer_ok(fmt, rmode, T, E, K, router, H, I, NS)
+    layer_ok = (fused and not per_call_scratch()
+                and _layer_ok(fmt, rmode, T, E, K, router, H, I, NS))
     split = (path == "decode" and T > 0 and NS > 0 and seg.small
              and odt in (torch.bfloat16, torch.float32)
              and decode_fused_down_use(fmt, T, seg.A, H, I, max_active, E + NS, NS * T,
