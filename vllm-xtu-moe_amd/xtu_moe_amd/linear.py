@@ -170,6 +170,8 @@ def linear(x, w, *, bias=None, activation="none", row_scale=None, residual=None,
     nws = _WS_BYTES.get((M, N, K, act == 6, aligned))
     if nws is None:
         nws = int(_lib.call("xtu_linear_workspace_bytes", M, N, K, act, int(aligned)))
+        if len(_WS_BYTES) >= 4096:   # a server's prompt lengths
+            _WS_BYTES.clear()
         _WS_BYTES[M, N, K, act == 6, aligned] = nws
     # allocated per call: calls on other streams, and graphs, have their own
     ws = x.new_empty(nws, dtype=torch.uint8) if nws else None

@@ -7,7 +7,9 @@ checkpoint weights, scales, routing and SwiGLU attributes;
 given (topk_weights, topk_ids) (modular path) or routes from router_logits
 (monolithic path), maps global ids through expert_map (misses get weight
 0), and returns [T, H] in hidden_states.dtype, written into `output` when
-given; ``apply_router_weight_on_input`` raises.  Format subclasses fix the
+given; with neither routing nor logits it takes the router's product too, from
+the bf16 rows that the layer's ``gate`` holds (the reference leaves that to its
+host, hybrid_model.py:1877); ``apply_router_weight_on_input`` raises.  Format subclasses fix the
 scale attribute names and the scale groups (:3308-3476): BF16 1x1, MXFP4
 1x32, FP8 128x128, NVFP4 1x16 with per-expert second-level scales, and INT4
 (WNA16) 1xgroup with the GPTQ / compressed-tensors repack.
@@ -28,8 +30,10 @@ import enum
 import torch
 
 from . import formats as F
+from .block import MoeBlock
 from .host_layer import HostResidentLayer, layer_index, resident_decision
 from .layer import ExpertWeights, _buf as _scratch, int8_align_on, int8_dispatch, moe_forward, route
+from .linear import _overlap, linear
 
 _ROUTING_ATTRS = ("use_grouped_topk", "renormalize", "scoring_func", "custom_routing_function",
                   "num_expert_group", "topk_group", "e_score_correction_bias",
@@ -167,7 +171,8 @@ class XiaotuExperts:
                                                 self.renormalize)
             return w.to(torch.float32), i.to(torch.int32)
         if router_logits is None:
-            raise ValueError("no topk_ids / topk_weights and no router_logits")
+            raise ValueError("no topk_ids / topk_weights and no router_logits (and no gate in the "
+                             "layer with bf16 rows for these hidden states)")
         if self.use_grouped_topk or str(self.scoring_func) == "sigmoid":
             bias = self.e_score_correction_bias
             if bias is not None:
@@ -224,7 +229,24 @@ class XiaotuExperts:
                   swiglu_alpha=float(self.swiglu_alpha if self.swiglu_alpha is not None else 1.0),
                   swiglu_beta=float(self.swiglu_beta or 0.0),
                   out=output if direct else None, out_dtype=odt)
-        if topk_weights is not None and topk_ids is not None:
+        routed = topk_weights is not None and topk_ids is not None
+        gate, gate_bias = None, None
+        if not routed and router_logits is None and self.custom_routing_function is None:
+            gate, gate_bias = self._gate(x)
+        if gate is not None and (gate_bias is not None or gate.data_ptr() % 16 or expert_map is not None
+                                 or not self._monolithic or self._weights is None or self._int8(T)):
+            router_logits = linear(x, gate, bias=gate_bias, out_dtype=torch.float32)
+            gate = None
+        if gate is not None:
+            if direct and _overlap(output, x):   # in place: the block reads x to its end
+                direct, kw["out"] = False, None
+            out, odt = kw.pop("out"), kw.pop("out_dtype")
+            sel = self._selection_args(x.device)
+            if sel["scoring"] == "softmax":   # its selection takes no bias
+                sel["bias"] = None
+            res = MoeBlock(gate, self._weights, top_k=int(self.top_k), **sel, **kw)(
+                x, out=out, out_dtype=odt)
+        elif routed:
             res = self._experts(x, topk_ids.to(torch.int32).contiguous(),
                                 topk_weights.to(torch.float32).contiguous(), kw)
         elif (self._monolithic and self._weights is not None and expert_map is None
@@ -271,20 +293,37 @@ class XiaotuExperts:
             return out
         return res.to(kw.get("out_dtype", torch.float32))
 
-    def _router_args(self, router_logits) -> dict:
-        lg = router_logits
-        if lg.dtype != torch.float32 or not lg.is_contiguous():
-            lg = lg.float().contiguous()
+    def _gate(self, x):
+        """(rows [experts, H], logit bias or None) of the layer's router, or
+        (None, None) without bf16 rows for x.  A gate's bias that is the
+        selection's e_score_correction_bias is no term of the logits."""
+        gate = getattr(self._layer_ref, "gate", None)
+        w, b = getattr(gate, "weight", None), getattr(gate, "bias", None)
+        if not isinstance(w, torch.Tensor) or w.dtype != torch.bfloat16 or w.dim() != 2 \
+                or w.shape[1] != x.shape[1] or w.device != x.device or not w.is_contiguous():
+            return None, None
+        if not isinstance(b, torch.Tensor) or (b is self.e_score_correction_bias
+                                               and str(self.scoring_func) == "sigmoid"):
+            return w.detach(), None
+        return w.detach(), b.detach().to(device=x.device, dtype=torch.float32).contiguous()
+
+    def _selection_args(self, dev) -> dict:
         if self.use_grouped_topk or str(self.scoring_func) == "sigmoid":
             bias = self.e_score_correction_bias
             if bias is not None:
-                bias = bias.to(device=lg.device, dtype=torch.float32).contiguous()
-            return dict(logits=lg, scoring=str(self.scoring_func), bias=bias,
+                bias = bias.to(device=dev, dtype=torch.float32).contiguous()
+            return dict(scoring=str(self.scoring_func), bias=bias,
                         n_group=int(self.num_expert_group or 1),
                         topk_group=int(self.topk_group or 1),
                         routed_scaling_factor=float(self.routed_scaling_factor or 1.0),
                         renormalize=bool(self.renormalize))
-        return dict(logits=lg, scoring="softmax", renormalize=bool(self.renormalize))
+        return dict(scoring="softmax", renormalize=bool(self.renormalize))
+
+    def _router_args(self, router_logits) -> dict:
+        lg = router_logits
+        if lg.dtype != torch.float32 or not lg.is_contiguous():
+            lg = lg.float().contiguous()
+        return dict(logits=lg, **self._selection_args(lg.device))
 
 
 class XiaotuExpertsBF16(XiaotuExperts):
