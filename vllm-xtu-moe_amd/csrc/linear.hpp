@@ -96,18 +96,54 @@ __device__ __forceinline__ f32x4_t load4(const void* p, long o, int is_bf16) {
                  __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
 }
 
-// Columns n .. n + 3 of row m, all of them there (a.vec: N % 4 == 0).
+// Four columns' bias: of z, and for swiglu of u.
 template <int AK>
-__device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, f32x4_t z, f32x4_t u) {
-  if (a.bias) {
-    z += load4(a.bias, n, a.bias_bf16);
-    if constexpr (AK == kActSwiglu) u += load4(a.bias, a.N + n, a.bias_bf16);
-  }
-  f32x4_t y;
+__device__ __forceinline__ void load_bias4(const LinearArgs& a, int n, f32x4_t& bz, f32x4_t& bu) {
+  bz = bu = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  if (!a.bias) return;
+  bz = load4(a.bias, n, a.bias_bf16);
+  if constexpr (AK == kActSwiglu) bu = load4(a.bias, a.N + n, a.bias_bf16);
+}
+
+// What the epilogue of four columns of a row reads.
+struct Row4 {
+  f32x4_t res;
+  float scale;
+};
+
+__device__ __forceinline__ Row4 load_row4(const LinearArgs& a, int m, int n) {
+  Row4 r = {{0.f, 0.f, 0.f, 0.f}, 1.f};
+  if (a.res) r.res = load4(a.res, (long)m * a.ldr + n, a.res_bf16);
+  if (a.scale) r.scale = a.scale[(long)m * a.sstride];
+  return r;
+}
+
+// z[] = act(z[], u[]), the choice of an activation outside the loops.
+template <int AK, int C>
+__device__ __forceinline__ void act_all(const LinearArgs& a, f32x4_t (&z)[C], f32x4_t (&u)[C]) {
+  const auto each = [&](auto f) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = act_of<AK>(a, z[e], u[e]);
-  if (a.scale) y *= a.scale[(long)m * a.sstride];
-  if (a.res) y += load4(a.res, (long)m * a.ldr + n, a.res_bf16);
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[c][e] = f(z[c][e], u[c][e]);
+  };
+  if constexpr (AK == kActSwiglu) {
+    each([&](float g, float v) { return silu_gate(g, v, a.limit, a.alpha, a.beta); });
+  } else if constexpr (AK == kActOther) {
+    switch (a.act) {
+      case kRelu: each([](float g, float) { return activate(kRelu, g); }); break;
+      case kSilu: each([](float g, float) { return activate(kSilu, g); }); break;
+      case kGelu: each([](float g, float) { return activate(kGelu, g); }); break;
+      case kGeluTanh: each([](float g, float) { return activate(kGeluTanh, g); }); break;
+      case kSigmoid: each([](float g, float) { return activate(kSigmoid, g); }); break;
+    }
+  }
+}
+
+__device__ __forceinline__ void store_row4(const LinearArgs& a, int m, int n, f32x4_t y,
+                                           const Row4& r) {
+  if (a.scale) y *= r.scale;
+  if (a.res) y += r.res;
   const long o = (long)m * a.ldo + n;
   if (a.out_bf16) {
     uint2 v;
@@ -117,6 +153,17 @@ __device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, f32x4
   } else {
     *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(a.out) + o) = y;
   }
+}
+
+// Columns n .. n + 3 of row m, all of them there (a.vec: N % 4 == 0).
+template <int AK>
+__device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, f32x4_t z, f32x4_t u) {
+  f32x4_t bz, bu;
+  load_bias4<AK>(a, n, bz, bu);
+  const Row4 r = load_row4(a, m, n);
+  f32x4_t zz[1] = {z + bz}, uu[1] = {u + bu};
+  act_all<AK>(a, zz, uu);
+  store_row4(a, m, n, zz[0], r);
 }
 
 // Order this wave's LDS writes before its later LDS reads by other lanes: a

@@ -3,12 +3,15 @@
 // of BK; the loads go from global memory straight to LDS, STAGES - 1 steps
 // ahead of the MFMAs.
 //
-// LDS: a stage holds BM + BN rows of BK k, x rows first.  The
-// 16-byte piece p of row r sits at slot p ^ (r & 7) (64-byte rows: p ^ (r / 2
-// & 3)), so that the eight lanes that a 16-byte LDS read serves together
-// (consecutive rows, one piece) touch all 32 banks; the loads write LDS linearly, so the swizzle is in the global
-// address of each lane.  Pieces past K are loaded out of the buffer's range,
-// which gives zeros; rows past M or N repeat the last row and are not written.
+// LDS: a stage holds BM + BN rows of BK k, x rows first.  The 16-byte pieces of
+// a row are permuted by the row (slot_of).  A 16-byte LDS read serves 16 lanes
+// at once: lanes 0-3, 12-15 and 20-27, then 4-11, 16-19 and 28-31, and the same
+// of the upper half.  Lane l reads row l % MB of a block, piece l / MB, and with
+// these slots the 16 lanes touch all 64 banks once: 4.2 cycles a read instead of
+// 8.2 (p ^ (r & 7) with MB = 32).  The loads write LDS linearly, so the
+// permutation is in each lane's global address.  Pieces past K are loaded out of
+// the buffer's range, which gives zeros; rows past M or N repeat the last row and
+// are not written.
 //
 // The MFMA takes w as its A operand and x as B: a lane then holds four
 // consecutive output columns of one row, which the epilogue reads and writes
@@ -43,10 +46,12 @@ __device__ __forceinline__ u32x4_t raw_buffer(const void* base, uint32_t bytes) 
 constexpr int wait_vm(int n) { return 0x0f70 | (n & 15) | ((n >> 4) << 14); }
 constexpr int wait_vm_lgkm0(int n) { return 0x0070 | (n & 15) | ((n >> 4) << 14); }
 
-// Slot of piece p of row r in an LDS row of PCS pieces.
-template <int PCS>
+// Slot of piece p of row r in an LDS row of PCS pieces, for MB rows a read.
+template <int PCS, int MB>
 __device__ __forceinline__ int slot_of(int p, int r) {
-  return p ^ (PCS == 4 ? (r >> 1) & 3 : r & 7);
+  static_assert(PCS == 8 || (PCS == 16 && MB == 16), "rows of 128 or 256 bytes");
+  if (PCS == 16) return p ^ (r & 7) << 1;
+  return p ^ (r & 7) ^ (MB == 32 ? r >> 4 & 1 : 0);
 }
 
 // LDS row of the epilogue's sums, in floats (16 bytes of padding: eight
@@ -79,7 +84,6 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
   static_assert(!PIPE || (BK / KK) % 2 == 0, "two sets of fragments in turn");
   static_assert((STAGES - 1) * LOADS <= 63, "vmcnt");
   static_assert(!GATED || NI % 2 == 0, "gate and up blocks pair up in a wave");
-  static_assert(MB % (64 / PCS) == 0, "a load stays within a block of rows");
   typedef typename AccOf<MB>::type acc_t;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid % 64;
@@ -111,15 +115,19 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
   const u32x4_t wr = raw_buffer(a.w + (long)n0 * a.ldw, wbytes);
   const u32x4_t ur = GATED ? raw_buffer(a.w + (long)(a.N + n0) * a.ldw, wbytes) : wr;
 
-  // this thread's pieces of a step: piece c = (w * LOADS + j) * 64 + lane
+  // load j of a step takes rows RPJ j and on, RPW of them a wave, a piece a lane:
+  // all of x or all of w.  swiglu: gate or up goes by the wave, or by j
+  constexpr int RPW = 64 / PCS, RPJ = RPW * WAVES;
+  static_assert(BM % RPJ == 0 && BN % RPJ == 0, "a load is of x or of w");
+  static_assert(!GATED || RPJ % (2 * MB) == 0 || RPJ == MB, "a wave's load is of gate or of up");
   uint32_t off[LOADS];
   int kof[LOADS];
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) {
-    const int c = (w * LOADS + j) * 64 + lane;
-    const int r = c / PCS, p = slot_of<PCS>(c % PCS, r);
+    const int r = RPJ * j + RPW * w + lane / PCS;
+    const int p = slot_of<PCS, MB>(lane % PCS, RPJ * j % 32 + RPW * w + lane / PCS);
     kof[j] = 8 * p;
-    if (r < BM) {
+    if (RPJ * j < BM) {
       off[j] = (uint32_t)min(r, mrows - 1) * (uint32_t)(a.ldx * 2) + 16 * p;
     } else {
       const int rr = r - BM;
@@ -127,21 +135,15 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
       off[j] = (uint32_t)min(col, ncols - 1) * (uint32_t)(a.ldw * 2) + 16 * p;
     }
   }
-  // the 64 / PCS rows of a wave's load are all x's, or all gate or up rows
-  u32x4_t rsrc[LOADS];
-#pragma unroll
-  for (int j = 0; j < LOADS; ++j) {
-    const int row = (w * LOADS + j) * (64 / PCS);
-    const bool isx = row < BM, isu = GATED && (row - BM) / MB % 2;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      rsrc[j][i] = __builtin_amdgcn_readfirstlane(isx ? xr[i] : isu ? ur[i] : wr[i]);
-  }
+  const u32x4_t wave_wr = GATED && RPW * w / MB % 2 ? ur : wr;
+  const int kend = min(a.K, BK * s1);
   auto issue_one = [&](int s, int st, int j) {
-    const bool tail = BK * s + BK > a.K;
-    const uint32_t o = tail && BK * s + kof[j] >= a.K ? 0x80000000u : off[j];
-    buf_to_lds(rsrc[j], o, (uint32_t)s * (uint32_t)LROW,
-               lds + st * STAGE + (w * LOADS + j) * 1024);
+    const uint32_t o = kof[j] < kend - BK * s ? off[j] : 0x80000000u;
+    const uint8_t* to = lds + st * STAGE + (WAVES * j + w) * 1024;
+    const uint32_t k = (uint32_t)s * (uint32_t)LROW;
+    if (RPJ * j < BM) buf_to_lds(xr, o, k, to);
+    else if (GATED && RPJ == MB) buf_to_lds((RPJ * j - BM) / MB % 2 ? ur : wr, o, k, to);
+    else buf_to_lds(wave_wr, o, k, to);
   };
   auto issue = [&](int s, int st) {
 #pragma unroll
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
   };
   // fragment f of k group kk: w block f, then x block f - NI
   auto read_one = [&](Frags& fr, int st, int kk, int f) {
-    const int o = st * STAGE + slot_of<PCS>(kk * (KK / 8) + h, rl) * 16;
+    const int o = st * STAGE + slot_of<PCS, MB>(kk * (KK / 8) + h, rl) * 16;
     if (f < NI) fr.w[f] = *reinterpret_cast<const u32x4_t*>(wb + o + f * MB * LROW);
     else fr.x[f - NI] = *reinterpret_cast<const u32x4_t*>(xb + o + (f - NI) * MB * LROW);
   };
@@ -203,6 +205,9 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
       sl = sl + 1 == STAGES ? 0 : sl + 1;
     }
   } else {
+    // 16 x 16 blocks: 361 us at 8192 x 4096 x 7168, in 32 x 32 ones 378, though
+    // half the fragment registers are then enough; four waves of 128 x 128 with
+    // 32 x 32 blocks, which read LDS less, take 393.
     // The barrier sits before a step's last k group: by then the fragments of
     // all its groups are read (each group's between the MFMAs of the one
     // before), so behind it the loads of step s + STAGES may take its stage;
@@ -210,11 +215,16 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
     // MFMAs, as are the loads issued.  The MFMAs wait for nothing but the
     // barrier itself.
     constexpr int M = NI * NJ, R = NI + NJ, KG = BK / KK;
+    // reads of a group behind its n'th MFMA, in the order of their use: the
+    // last quarter of the MFMAs covers their latency
+    auto read_at = [&](Frags& fr, int stage, int g, int n) {
 #pragma unroll
-    for (int p = 0; p < STAGES; ++p)
-      if (s0 + p < s1) issue(s0 + p, p);
-    if (s0 + STAGES <= s1) __builtin_amdgcn_s_waitcnt(wait_vm((STAGES - 1) * LOADS));
-    else __builtin_amdgcn_s_waitcnt(wait_vm(0));
+      for (int k = n * R * 4 / (3 * M); k < min(R, (n + 1) * R * 4 / (3 * M)); ++k)
+        read_one(fr, stage, g, k == 0 ? 0 : k <= NJ ? NI + k - 1 : k - NJ);
+    };
+#pragma unroll
+    for (int p = 0; p < STAGES; ++p) issue(s0 + p, p);
+    __builtin_amdgcn_s_waitcnt(wait_vm((STAGES - 1) * LOADS));
     __syncthreads();
     Frags f[2];
 #pragma unroll
@@ -226,32 +236,29 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
 #pragma unroll
         for (int n = 0; n < M; ++n) {
           mma_one(f[g & 1], n);
-#pragma unroll
-          for (int k = n * R / M; k < (n + 1) * R / M; ++k)
-            read_one(f[(g + 1) & 1], st, g + 1, k);
+          read_at(f[(g + 1) & 1], st, g + 1, n);
           __builtin_amdgcn_sched_barrier(0);
         }
       // step s + 1 landed (the STAGES - 2 after it may be in flight), the reads done
-      if (s + STAGES <= s1) __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((STAGES - 2) * LOADS));
-      else __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+      __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((STAGES - 2) * LOADS));
       __syncthreads();
       __builtin_amdgcn_sched_barrier(0);
-      const bool ahead = s + STAGES < s1;
       const int nst = st + 1 == STAGES ? 0 : st + 1;
 #pragma unroll
       for (int n = 0; n < M; ++n) {
         mma_one(f[(KG - 1) & 1], n);
         // (the last step reads what lies in the next stage; not used)
+        read_at(f[0], nst, 0, n);
+        // (between the first quarter: spread over all of the group's MFMAs
+        // 361 us become 376 at 8192 x 4096 x 7168, over two groups 397)
 #pragma unroll
-        for (int k = n * R / M; k < (n + 1) * R / M; ++k) read_one(f[0], nst, 0, k);
-        if (ahead) {
-#pragma unroll
-          for (int d = n * LOADS / M; d < (n + 1) * LOADS / M; ++d) issue_one(s + STAGES, st, d);
-        }
+        for (int d = n * LOADS * 4 / M; d < min(LOADS, (n + 1) * LOADS * 4 / M); ++d)
+          issue_one(s + STAGES, st, d);
         __builtin_amdgcn_sched_barrier(0);
       }
       st = nst;
     }
+    __builtin_amdgcn_s_waitcnt(wait_vm(0));   // (loads past the end bring zeros)
   }
 
   // Epilogue, MB rows of x at a time: the wave lays its sums out as rows in
@@ -263,6 +270,12 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
   float* eb = reinterpret_cast<float*>(lds) + w * (MB * LD);
   const int nw = n0 + W * wn;
   float* plane = SPLIT ? part + (long)blockIdx.y * part_plane(a) : nullptr;
+  // vectors: CG lanes along a row, RS rows at a time, BT such in one pass
+  constexpr int CG = W / 4, RS = 64 / CG, IT = MB / RS;
+  constexpr int BT = IT < 4 ? IT : AK == kActOther ? 2 : 4;
+  const int cv = lane % CG * 4, nv = nw + cv;
+  f32x4_t bz, bu;
+  if (!SPLIT && a.vec && nv < a.N) load_bias4<AK>(a, nv, bz, bu);
 #pragma unroll 1
   for (int j = 0; j < NJ; ++j) {
     lds_order();
@@ -281,23 +294,40 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
     lds_order();
     const int mb = m0 + WM * wm + MB * j;
     // column col of the wave: its gate (or only) sum's place in the row
-    auto place = [&](int col) { return GATED ? col / MB * 2 * MB + col % MB : col; };
+    const auto place = [&](int col) { return GATED ? col / MB * 2 * MB + col % MB : col; };
     if (a.vec) {
+      // a lane keeps its columns; what BT rows need is read before any is written
 #pragma unroll 1
-      for (int c = lane; c < MB * W / 4; c += 64) {
-        const int r = c / (W / 4), col = c % (W / 4) * 4;
-        const int m = mb + r, n = nw + col;
-        if (m >= a.M || n >= a.N) continue;
-        const float* row = eb + r * LD + place(col);
-        const f32x4_t z = *reinterpret_cast<const f32x4_t*>(row);
-        f32x4_t u = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (GATED) u = *reinterpret_cast<const f32x4_t*>(row + MB);
-        if constexpr (SPLIT) {
-          float* pr = plane + (long)m * a.N * (GATED ? 2 : 1) + n;
-          *reinterpret_cast<f32x4_t*>(pr) = z;
-          if constexpr (GATED) *reinterpret_cast<f32x4_t*>(pr + a.N) = u;
-        } else {
-          finish4<AK>(a, m, n, z, u);
+      for (int it = 0; it < IT && nv < a.N; it += BT) {
+        f32x4_t z[BT], u[BT];
+        Row4 x[BT];
+        const int r = it * RS + lane / CG, m = mb + r;
+#pragma unroll
+        for (int b = 0; b < BT; ++b) {
+          const float* row = eb + (r + b * RS) * LD + place(cv);
+          z[b] = *reinterpret_cast<const f32x4_t*>(row);
+          u[b] = z[b];
+          if constexpr (GATED) u[b] = *reinterpret_cast<const f32x4_t*>(row + MB);
+          if constexpr (!SPLIT) x[b] = load_row4(a, min(m + b * RS, a.M - 1), nv);
+        }
+        if constexpr (!SPLIT) {
+#pragma unroll
+          for (int b = 0; b < BT; ++b) {
+            z[b] += bz;
+            u[b] += bu;
+          }
+          act_all<AK>(a, z, u);
+        }
+#pragma unroll
+        for (int b = 0; b < BT; ++b) {
+          if (m + b * RS >= a.M) break;
+          if constexpr (SPLIT) {
+            float* pr = plane + (long)(m + b * RS) * a.N * (GATED ? 2 : 1) + nv;
+            *reinterpret_cast<f32x4_t*>(pr) = z[b];
+            if constexpr (GATED) *reinterpret_cast<f32x4_t*>(pr + a.N) = u[b];
+          } else {
+            store_row4(a, m + b * RS, nv, z[b], x[b]);
+          }
         }
       }
     } else {
@@ -365,18 +395,18 @@ namespace {
 // The variants: tile, k of a step, workgroups that share a CU, and what they
 // cost on MI355X, in us: t[i] a step, o[i] a round beside its steps, with i + 1
 // workgroups on a CU.  Fitted to products that fill the chip one to three times
-// over at K = 256, 1024 and 4096 (64 x 64: one per CU 4.6 / 8.5 / 22.5, two
-// 6.3 / 11.2 / 30.6, three 8.8 / 16.4 / 51.4; 256 x 256: 22.5 / 41.6 / 127).
+// over at K = 256, 1024 and 4096 (64 x 64: one per CU 4.5 / 8.2 / 21.9, two
+// 6.0 / 10.5 / 29.0; 256 x 256: 23.0 / 39.3 / 117).
 struct TileKind {
   int m, n, k, occ;
   float t[2], o[2];
 };
 constexpr TileKind kTileKinds[] = {
-    {64, 32, 128, 1, {0.42f, 0.42f}, {1.2f, 1.2f}},
-    {64, 64, 64, 2, {0.295f, 0.40f}, {1.2f, 1.9f}},
-    {128, 64, 64, 2, {0.42f, 0.69f}, {3.2f, 3.6f}},
-    {128, 128, 64, 2, {0.78f, 1.12f}, {3.5f, 5.5f}},
-    {256, 256, 64, 1, {1.72f, 1.72f}, {12.0f, 12.0f}},
+    {64, 32, 128, 1, {0.36f, 0.36f}, {1.3f, 1.3f}},
+    {64, 64, 64, 2, {0.285f, 0.385f}, {1.4f, 2.1f}},
+    {128, 64, 64, 2, {0.39f, 0.73f}, {3.5f, 2.0f}},
+    {128, 128, 64, 2, {0.79f, 1.03f}, {2.3f, 4.3f}},
+    {256, 256, 64, 1, {1.53f, 1.53f}, {11.0f, 11.0f}},
 };
 constexpr float kLaunch = 2.3f;
 constexpr int kCus = 256;
@@ -419,8 +449,8 @@ hipError_t launch_tile_kind(int kind, const LinearArgs& a, int split, float* par
     case 0: return launch_tile<64, 32, 16, 32, 16, 128, 4, false, 1>(a, split, part, stream);
     case 1: return launch_tile<64, 64, 16, 32, 16, 64, 4, false, 4>(a, split, part, stream);
     case 2: return launch_tile<128, 64, 64, 32, 16, 64, 3, false, 2>(a, split, part, stream);
-    case 3: return launch_tile<128, 128, 32, 64, 32, 64, 2, true, 4>(a, split, part, stream);
-    case 4: return launch_tile<256, 256, 128, 64, 32, 64, 2, true, 2>(a, split, part, stream);
+    case 3: return launch_tile<128, 128, 32, 64, 16, 64, 2, true, 4>(a, split, part, stream);
+    case 4: return launch_tile<256, 256, 128, 64, 16, 64, 2, true, 2>(a, split, part, stream);
   }
   return hipErrorInvalidValue;
 }
