@@ -210,6 +210,30 @@ def test_equal_scores_go_to_the_lowest_index(sigmoid):
         assert bool((wts - 1 / 6).abs().max() < 1e-6)
 
 
+@pytest.mark.parametrize("fmt", sorted(FMTS))
+@pytest.mark.parametrize("layer", [LAYERS[0], LAYERS[2], LAYERS[7]])
+def test_few_tokens_keep_unrounded_rows(fmt, layer):
+    """Up to eight tokens of these layers keep activation rows in two bf16
+    parts (2^-18 of a value): with fp32 output nothing of 2^-9 is left.  The
+    fp32 sums of at most 4096 terms leave some 2^-23 sqrt(4096) = 2^-17 of
+    them; rows rounded to bf16 alone would leave 2^-9.2 of the norm."""
+    blk, dense, sg, kw = _block(fmt, layer)
+    W, K = blk.W, blk.top_k
+    for T in (1, 3, 8):
+        x = _x(T, layer[3], 40 + T)
+        out, wts, ids = blk(x, return_routing=True, out_dtype=F32)
+        xd, y = x.double(), torch.zeros((T, W.H), dtype=torch.float64, device=DEV)
+        for t in range(T):
+            pairs = [(int(ids[t, k]), wts[t, k].double()) for k in range(K)]
+            pairs += [(W.E + s, 1.0 if sg is None else torch.sigmoid(xd[t] @ sg[s].double()))
+                      for s in range(W.n_shared)]
+            for e, w in pairs:
+                d13, d2 = dense(e)
+                z = d13 @ xd[t]
+                y[t] += w * (d2 @ (torch.nn.functional.silu(z[:W.I]) * z[W.I:]))
+        assert float((out.double() - y).norm() / y.norm()) < 2.0 ** -13
+
+
 def test_no_tokens_and_given_output():
     blk, dense, sg, kw = _block("fp8", LAYERS[5])
     out, wts, ids = blk(_x(0, 512, 0), return_routing=True)

@@ -25,7 +25,7 @@ Layout layout_of(const Plan& p, int T, int E, int K, int NS, int H, int I) {
   l.ctl_words = kPanels + H / 16;
   l.logits = 0;
   l.act = up256((size_t)T * l.ldl * 4);
-  l.part = l.act + up256((size_t)T * (K + NS) * I * 2);
+  l.part = l.act + up256((size_t)p.parts * T * (K + NS) * I * 2);
   l.ctl = l.part + (p.chunks > 1 ? up256((size_t)p.chunks * T * H * 4) : 0);
   l.total = l.ctl + up256((size_t)l.ctl_words * 4);
   return l;
@@ -110,6 +110,7 @@ hipError_t xtu_few_block(const xtu_few_args* args, hipStream_t stream) {
   f.epl = tiny::wave_epl(t.mode, t.E, f.n_group, t.renormalize, f.logits, f.bias);
   f.chunk_units = p.chunk_units;
   f.chunks = p.chunks;
+  f.parts = p.parts;
   f.stage_bytes = p.stage;
   switch (t.fmt) {
     case kMXFP4: return run_mxfp4(f, p, stream);

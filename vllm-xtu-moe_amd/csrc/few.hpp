@@ -40,6 +40,17 @@
 // adds them in chunk order, so results do not depend on timing.
 // (They do depend on the batch, in the last bits: a token's experts are added in
 // the order in which the batch's tokens bring them up.)
+//
+// Up to eight tokens leave half of the down projection's 16 MFMA rows unused:
+// there every activation row is kept in two bf16 parts, the rounded value and the
+// rest, and row t + 8 multiplies the rest.  That takes the rows' rounding (2^-9 of
+// each value, as much as the output's own) out of the result, and matters most
+// where a few large values make up an output (one token: up to 1.6 times the
+// error of fp32 rows).  It costs the second part's place in LDS, so it is done
+// where the rows fit with no other split into chunks (E = 512, H = 2048, I = 512,
+// one token: 26 us either way; in more chunks, E = 256, H = 7168, I = 2048, two
+// tokens: 101 us, 84 with one part).  Otherwise the rows are rounded to bf16, as
+// everywhere else in this library.
 #pragma once
 #include "decode.hpp"
 
@@ -62,7 +73,7 @@ struct FewArgs {
   float limit, alpha, beta;
   float* logits;            // [T][ldl]: E router logits, then the shared gates'
   int ldl;
-  uint16_t* act;            // [T K + NS T][I]: row t K + k, then T K + s T + t
+  uint16_t* act;            // [parts][T K + NS T][I]: row t K + k, then T K + s T + t
   float* part;              // [chunks][T][H] (chunks > 1)
   unsigned* ctl;
   int ctl_words;
@@ -73,6 +84,7 @@ struct FewArgs {
   int rp, n_sh;             // launch 1: router rows per panel; its shared gate/up items
   int epl;                  // experts per lane of the wave router (0: any E)
   int chunk_units, chunks;  // launch 2: 128-k units of a chunk of the down projection
+  int parts;                // bf16 parts of an activation row
   size_t stage_bytes;
 };
 
@@ -80,7 +92,7 @@ struct FewArgs {
 // and all activation rows fit half its LDS; otherwise one takes what it needs.
 struct Plan {
   size_t stage, lds;
-  int nper, chunk_units, chunks, occ;
+  int nper, chunk_units, chunks, occ, parts;
 };
 
 namespace {
@@ -96,6 +108,20 @@ constexpr int kGroups = 8, kMaxChunks = 8;
 constexpr int kTicket = 0, kDone = kGroups * kLine, kFlag = 2 * kGroups * kLine,
               kTicket3 = kFlag + kLine, kPanels = kTicket3 + kMaxChunks * kGroups * kLine;
 constexpr int kSpin = 1 << 20;
+
+// Column col of activation row `row`, in its parts; read by other workgroups in
+// the same launch.
+__device__ __forceinline__ void store_act(const FewArgs& f, int row, int col, float v) {
+  uint16_t* p = f.act + (long)row * f.I + col;
+  const uint16_t hi = f32_to_bf16(v);
+  __hip_atomic_store(p, hi, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (f.parts == 2) {
+    const float rest = v - bf16_to_f32(hi);   // (no number where v is none: hi says so)
+    __hip_atomic_store(p + (long)f.T * (f.K + f.NS) * f.I,
+                       f32_to_bf16(fabsf(rest) < INFINITY ? rest : 0.f), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+  }
+}
 
 
 // The x rows to LDS, 16 bytes of padding each; a thread's loads go out eight
@@ -119,6 +145,28 @@ __device__ __forceinline__ void stage_x(const FewArgs& f, uint16_t* xs) {
   }
 }
 
+// SwiGLU of a gate/up panel from the K splits' sums, added in their order:
+// thread tid < 256 takes token tid / 16, column tid % 16 (row < 0: none).
+template <int FMT>
+__device__ __forceinline__ void finish_act(const FewArgs& f, const f32x4_t (*red)[kWave], int e,
+                                           int row, int sub, int tid) {
+  if (tid >= 256 || row < 0) return;
+  const int t = tid / 16, n = tid % 16, l = (t / 4) * 16 + n, i = t % 4;
+  float gv = 0.f, uv = 0.f;
+#pragma unroll
+  for (int k = 0; k < kKS; ++k) {
+    gv += red[k][l][i];
+    uv += red[kKS + k][l][i];
+  }
+  if constexpr (FMT == kNVFP4) {
+    if (f.gs13) {
+      gv *= f.gs13[2 * e];
+      uv *= f.gs13[2 * e + 1];
+    }
+  }
+  store_act(f, row, 16 * sub + n, silu_gate(gv, uv, f.limit, f.alpha, f.beta));
+}
+
 // ---------------------------------------------------------------- launch 1
 template <int FMT, int NU>
 __global__ __launch_bounds__(kThreads, 2) void few_router_kernel(FewArgs f) {
@@ -140,16 +188,8 @@ __global__ __launch_bounds__(kThreads, 2) void few_router_kernel(FewArgs f) {
     DecodeArgs a{};
     a.w = f.w13;
     a.s = f.s13;
-    a.gs = f.gs13;
-    a.out = f.act;
-    a.H = f.H;
-    a.I = f.I;
     a.w_estride = f.w13_es;
     a.s_estride = f.s13_es;
-    a.limit = f.limit;
-    a.alpha = f.alpha;
-    a.beta = f.beta;
-    a.ksplit = kKS;
     const int half = w / kKS, ks = w % kKS, nunits = f.H / 128;
     const int u0 = ks * nunits / kKS, u1 = (ks + 1) * nunits / kKS;
     const Stream<FMT> st = make_stream<FMT>(a, ws, half ? npan + sub : sub, f.H);
@@ -164,7 +204,9 @@ __global__ __launch_bounds__(kThreads, 2) void few_router_kernel(FewArgs f) {
       consume_round<FMT, NU, true>(r, acc, u0, u1, xa, nullptr);
       if (u0 + NU < u1) acc = more_rounds<FMT, NU, true>(acc, st, u0 + NU, u1, lane, xa, nullptr);
     }
-    gate_up_epilogue<FMT>(a, red, acc, w, lane, f.T * f.K + sh * f.T, f.T, ws, sub);
+    red[w][lane] = acc;
+    __syncthreads();
+    finish_act<FMT>(f, red, ws, tid / 16 < f.T ? f.T * f.K + sh * f.T + tid / 16 : -1, sub, tid);
     return;
   }
 
@@ -649,33 +691,14 @@ __global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs 
           roll_round<FMT, NU>(r, acc, ub, u1, xa, st, last ? u0 : ub + NU, u1, lane);
         }
         if (tid == 0) g.ticket[it & 1] = t_new;
-        // the K splits in their order; the rows of the tokens that use the
-        // expert, bf16, read by other workgroups in this launch
+        // the rows of the tokens that use the expert
         f32x4_t(*rd_)[kWave] = red[it & 1];
         rd_[w][lane] = acc;
         __syncthreads();
-        if (tid < 256) {
-          const int t = tid / 16, n = tid % 16;
-          if (t < T && wof[slot * kMaxT + t] != 0.f) {
-            const int l = (t / 4) * 16 + n, i = t % 4;
-            float gv = 0.f, uv = 0.f;
-#pragma unroll
-            for (int k = 0; k < kKS; ++k) {
-              gv += rd_[k][l][i];
-              uv += rd_[kKS + k][l][i];
-            }
-            if constexpr (FMT == kNVFP4) {
-              if (f.gs13) {
-                const int e = g.slot_e[slot];
-                gv *= f.gs13[2 * e];
-                uv *= f.gs13[2 * e + 1];
-              }
-            }
-            __hip_atomic_store(f.act + (long)rowof[slot * kMaxT + t] * I + 16 * sub + n,
-                               f32_to_bf16(silu_gate(gv, uv, f.limit, f.alpha, f.beta)),
-                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          }
-        }
+        const int t = tid / 16 % kMaxT;
+        finish_act<FMT>(f, rd_, g.slot_e[slot],
+                        t < T && wof[slot * kMaxT + t] != 0.f ? rowof[slot * kMaxT + t] : -1, sub,
+                        tid);
         ++count;
         cur = nxt;
         nxt = __builtin_amdgcn_readfirstlane(g.ticket[it & 1]);
@@ -698,7 +721,10 @@ __global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs 
 
   // ---- output panels
   const int nu = I / 128, n_slots = n_routed + f.NS, cun = f.chunk_units;
-  const int rows = T * f.K + f.NS * T, lda = cun * 128 + 8;
+  const int parts = f.parts, lda = cun * 128 + 8;
+  const int rows = parts * T * (f.K + f.NS);
+  // MFMA row m: token m & tmask, of part m / 8 if there are two
+  const int tmask = parts == 2 ? 7 : 15, part_row = parts == 2 && m >= 8 ? rows / 2 : 0;
   const __amdgpu_buffer_rsrc_t ract = __builtin_amdgcn_make_buffer_rsrc(
       (void*)f.act, 0, rows * I * 2, kRawBufferFlags);
   Seg<FMT, NPER> ring[D];
@@ -782,12 +808,13 @@ __global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs 
         const int fl = w + kWaves * i;
         if (fl < total) {
           const int j = fl / nseg, u0 = (fl - j * nseg) * NPER;   // within the chunk
-          const uint16_t* xa = stage + (int)rowof[j * kMaxT + m] * lda + q * F::kCK;
+          const int row = (int)rowof[j * kMaxT + (m & tmask)] + part_row;
+          const uint16_t* xa = stage + row * lda + q * F::kCK;
           f32x4_t pe = use_seg<FMT, NPER>(ring[d], u0, units, xa);
           if constexpr (FMT == kNVFP4) {
             if (f.gs2) pe = pe * f.gs2[__builtin_amdgcn_readfirstlane(g.slot_e[j])];
           }
-          const f32x4_t wv = *reinterpret_cast<const f32x4_t*>(wof + j * kMaxT + 4 * q);
+          const f32x4_t wv = *reinterpret_cast<const f32x4_t*>(wof + j * kMaxT + (4 * q & tmask));
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             tacc[k] = wv[k] != 0.f ? __builtin_fmaf(wv[k], pe[k], tacc[k]) : tacc[k];
@@ -815,6 +842,12 @@ __global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs 
           float v = 0.f;
 #pragma unroll
           for (int i = 0; i < kWaves; ++i) v += rd_[i][l][k];
+          if (parts == 2) {
+            float rest = 0.f;
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) rest += rd_[i][l + 32][k];
+            v += rest;
+          }
           const long o = (long)tok * H + 16 * p + n;
           if (f.chunks > 1)
             __hip_atomic_store(f.part + (long)chunk * T * H + o, v, __ATOMIC_RELAXED,
@@ -864,12 +897,13 @@ __global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs 
 // items: where there are fewer panels than CUs, or their last round leaves CUs
 // idle.  Times in us: a CU streams about 25 GB/s, an item costs 0.7 beside its
 // stream, the joining of chunks 2.
-__host__ inline bool make_plan(int T, int E, int K, int NS, int H, int I, float bits, Plan& p) {
+__host__ inline bool plan_parts(int T, int E, int K, int NS, int H, int I, float bits, int parts,
+                                Plan& p) {
   if (T < 1 || T > kMaxT || K < 1 || K > 16 || K > E || E > kMaxE || T * K > kMaxPairs ||
       NS < 0 || NS > kMaxShared || H < 256 || H % 256 || H > 16384 || I < 128 || I % 128 ||
       I > 16384)
     return false;
-  const int slots = std::min(E, T * K) + NS, R = T * (K + NS), nu = I / 128;
+  const int slots = std::min(E, T * K) + NS, R = parts * T * (K + NS), nu = I / 128;
   const size_t fixed = (size_t)2 * kWaves * kWave * 16 + sel_bytes() + table_bytes(slots) + 256;
   const size_t half = 80 * 1024, full = 160 * 1024;
   // x rows, and behind them select_any's keys
@@ -898,6 +932,16 @@ __host__ inline bool make_plan(int T, int E, int K, int NS, int H, int I, float 
   // with more, half as many workgroups end closer together
   p.occ = fixed + p.stage <= half && (active - NS) * (I / 16) <= 2.0 * cus ? 2 : 1;
   p.lds = p.stage + sel_bytes() + table_bytes(slots);
+  p.parts = parts;
+  return true;
+}
+
+__host__ inline bool make_plan(int T, int E, int K, int NS, int H, int I, float bits, Plan& p) {
+  if (!plan_parts(T, E, K, NS, H, I, bits, 1, p)) return false;
+  Plan two;
+  if (T <= 8 && plan_parts(T, E, K, NS, H, I, bits, 2, two) && two.chunks == p.chunks &&
+      two.nper == p.nper && two.occ == p.occ)
+    p = two;
   return true;
 }
 
