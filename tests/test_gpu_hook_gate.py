@@ -149,6 +149,20 @@ def test_without_a_gate_refused():
         hook.apply(x, None, None)
 
 
+def test_gate_of_another_size_refused():
+    hook, gate, kw = _hook("bf16", 8, 256, 128, 2, False, 9)
+    lay, x = hook._layer_ref, _x(2, 256, 2)
+    em = torch.arange(8, dtype=torch.int32)
+    for w, m in ((gate[:6].clone(), None), (torch.cat([gate, gate]), None), (gate, em[:7]),
+                 (torch.cat([gate, gate]), em)):
+        lay.gate.weight = w
+        with pytest.raises(ValueError, match="rows do not fit"):
+            hook.apply(x, None, None, expert_map=m)
+    lay.gate.weight, lay.gate.bias = gate, torch.zeros(7, device=DEV)
+    with pytest.raises(ValueError, match="rows do not fit"):
+        hook.apply(x, None, None)
+
+
 class _Net:
     """Two MoE layers with unquantised shared experts, as a model runs them:
     h += routed(h) + sigmoid(h . v) * down(swiglu(gate/up(h)))."""

@@ -101,12 +101,13 @@ constexpr int kMaxT = 16, kMaxPairs = 256, kMaxShared = 4, kMaxE = 1024, kMaxGro
 constexpr int kThreads = 512, kWaves = 8, kKS = 4;   // waves along K per gate/up half
 constexpr int kLine = 64;                            // words of a counter's own 256 bytes
 
-// Counters (words): per group the gate/up items drawn and those done; a flag set
-// if a wait ever ran out; per chunk and group the output panels drawn; then the
-// chunks done per output panel.
+// Counters (words): per group the gate/up items drawn and those done; per chunk
+// and group the output panels drawn; then the chunks done per output panel.
 constexpr int kGroups = 8, kMaxChunks = 8;
-constexpr int kTicket = 0, kDone = kGroups * kLine, kFlag = 2 * kGroups * kLine,
-              kTicket3 = kFlag + kLine, kPanels = kTicket3 + kMaxChunks * kGroups * kLine;
+constexpr int kTicket = 0, kDone = kGroups * kLine, kTicket3 = 2 * kGroups * kLine,
+              kPanels = kTicket3 + kMaxChunks * kGroups * kLine;
+// Looks at the counters before a wait is given up (about 0.2 s; it ends by itself
+// as long as the workgroups that run make progress).
 constexpr int kSpin = 1 << 20;
 
 // Column col of activation row `row`, in its parts; read by other workgroups in
@@ -368,6 +369,7 @@ struct Sel {
   int slot_e[kMaxPairs + kMaxShared];
   int ticket[2];
   int last;
+  int late;        // the wait for the gate/up items ran out
 };
 
 // One thread of a workgroup draws an item of group g: which = kTicket (gate/up),
@@ -398,6 +400,7 @@ __device__ __forceinline__ int build_selection(const FewArgs& f, Sel& g, uint16_
     wof[i] = 0.f;
   }
   if (tid < kMaxPairs && tid >= A) g.ids[tid] = -1;
+  if (tid == 0) g.late = 0;
   for (int t = wv; t < T; t += kWaves) {
     const float* l = f.logits + (long)t * f.ldl;
     int* ids = g.ids + t * K;
@@ -765,8 +768,7 @@ __global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs 
           v += __shfl_xor(v, 4, kWave);
           if (__builtin_amdgcn_readfirstlane(v) == (unsigned)n2) break;
           if (n == kSpin) {
-            if (lane == 0)
-              __hip_atomic_store(f.ctl + kFlag, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (lane == 0) g.late = 1;
             break;
           }
           __builtin_amdgcn_s_sleep(2);
@@ -848,6 +850,7 @@ __global__ __launch_bounds__(kThreads, 2 * OCC) void few_experts_kernel(FewArgs 
             for (int i = 0; i < kWaves; ++i) rest += rd_[i][l + 32][k];
             v += rest;
           }
+          if (g.late) v = NAN;   // rows may be missing: no answer that looks like one
           const long o = (long)tok * H + 16 * p + n;
           if (f.chunks > 1)
             __hip_atomic_store(f.part + (long)chunk * T * H + o, v, __ATOMIC_RELAXED,

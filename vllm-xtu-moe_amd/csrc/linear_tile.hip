@@ -274,8 +274,13 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
   constexpr int CG = W / 4, RS = 64 / CG, IT = MB / RS;
   constexpr int BT = IT < 4 ? IT : AK == kActOther ? 2 : 4;
   const int cv = lane % CG * 4, nv = nw + cv;
-  f32x4_t bz, bu;
+  const int n1 = nw + lane % W;   // a lane's single column
+  f32x4_t bz = {0.f, 0.f, 0.f, 0.f}, bu = bz;
   if (!SPLIT && a.vec && nv < a.N) load_bias4<AK>(a, nv, bz, bu);
+  if (!SPLIT && !a.vec && a.bias && n1 < a.N) {
+    bz[0] = load_bias(a, n1);
+    if constexpr (GATED) bu[0] = load_bias(a, a.N + n1);
+  }
 #pragma unroll 1
   for (int j = 0; j < NJ; ++j) {
     lds_order();
@@ -331,19 +336,44 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
         }
       }
     } else {
+      // the same by single columns, four rows in one pass
+      constexpr int RS1 = 64 / W;
+      static_assert(MB / RS1 % 4 == 0, "four rows a pass");
 #pragma unroll 1
-      for (int c = lane; c < MB * W; c += 64) {
-        const int r = c / W, col = c % W;
-        const int m = mb + r, n = nw + col;
-        if (m >= a.M || n >= a.N) continue;
-        const float* row = eb + r * LD + place(col);
-        const float z = row[0], u = GATED ? row[MB] : 0.f;
-        if constexpr (SPLIT) {
-          float* pr = plane + (long)m * a.N * (GATED ? 2 : 1) + n;
-          pr[0] = z;
-          if constexpr (GATED) pr[a.N] = u;
-        } else {
-          finish_one<AK>(a, m, n, z, u);
+      for (int it = 0; it < MB / RS1 && n1 < a.N; it += 4) {
+        f32x4_t z[1], u[1], res = {0.f, 0.f, 0.f, 0.f}, sc = {1.f, 1.f, 1.f, 1.f};
+        const int r = it * RS1 + lane / W, m = mb + r;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const float* row = eb + (r + b * RS1) * LD + place(lane % W);
+          z[0][b] = row[0];
+          u[0][b] = GATED ? row[MB] : 0.f;
+          const long mm = min(m + b * RS1, a.M - 1);
+          if (!SPLIT && a.res)
+            res[b] = a.res_bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(a.res)[mm * a.ldr + n1])
+                                : reinterpret_cast<const float*>(a.res)[mm * a.ldr + n1];
+          if (!SPLIT && a.scale) sc[b] = a.scale[mm * a.sstride];
+        }
+        if constexpr (!SPLIT) {
+          z[0] += bz[0];
+          u[0] += bu[0];
+          act_all<AK>(a, z, u);
+          if (a.scale) z[0] *= sc;
+          if (a.res) z[0] += res;
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const long mm = m + b * RS1;
+          if (mm >= a.M) break;
+          if constexpr (SPLIT) {
+            float* pr = plane + mm * a.N * (GATED ? 2 : 1) + n1;
+            pr[0] = z[0][b];
+            if constexpr (GATED) pr[a.N] = u[0][b];
+          } else if (a.out_bf16) {
+            reinterpret_cast<uint16_t*>(a.out)[mm * a.ldo + n1] = f32_to_bf16(z[0][b]);
+          } else {
+            reinterpret_cast<float*>(a.out)[mm * a.ldo + n1] = z[0][b];
+          }
         }
       }
     }

@@ -232,7 +232,7 @@ class XiaotuExperts:
         routed = topk_weights is not None and topk_ids is not None
         gate, gate_bias = None, None
         if not routed and router_logits is None and self.custom_routing_function is None:
-            gate, gate_bias = self._gate(x)
+            gate, gate_bias = self._gate(x, expert_map)
         if gate is not None and (gate_bias is not None or gate.data_ptr() % 16 or expert_map is not None
                                  or not self._monolithic or self._weights is None or self._int8(T)):
             router_logits = linear(x, gate, bias=gate_bias, out_dtype=torch.float32)
@@ -293,7 +293,7 @@ class XiaotuExperts:
             return out
         return res.to(kw.get("out_dtype", torch.float32))
 
-    def _gate(self, x):
+    def _gate(self, x, expert_map=None):
         """(rows [experts, H], logit bias or None) of the layer's router, or
         (None, None) without bf16 rows for x.  A gate's bias that is the
         selection's e_score_correction_bias is no term of the logits."""
@@ -302,6 +302,11 @@ class XiaotuExperts:
         if not isinstance(w, torch.Tensor) or w.dtype != torch.bfloat16 or w.dim() != 2 \
                 or w.shape[1] != x.shape[1] or w.device != x.device or not w.is_contiguous():
             return None, None
+        E = self._weights.E if self._weights is not None else self._host_layer.E
+        if w.shape[0] != (E if expert_map is None else expert_map.numel()) or \
+                (isinstance(b, torch.Tensor) and b.numel() != w.shape[0]):
+            raise ValueError(f"the gate's {w.shape[0]} rows do not fit {E} experts or the "
+                             "expert_map, or its bias does not fit the rows")
         if not isinstance(b, torch.Tensor) or (b is self.e_score_correction_bias
                                                and str(self.scoring_func) == "sigmoid"):
             return w.detach(), None
