@@ -425,18 +425,20 @@ namespace {
 // The variants: tile, k of a step, workgroups that share a CU, and what they
 // cost on MI355X, in us: t[i] a step, o[i] a round beside its steps, with i + 1
 // workgroups on a CU.  Fitted to products that fill the chip one to three times
-// over at K = 256, 1024 and 4096 (64 x 64: one per CU 4.5 / 8.2 / 21.9, two
-// 6.0 / 10.5 / 29.0; 256 x 256: 23.0 / 39.3 / 117).
+// over at K = 256, 1024 and 4096 (64 x 64: one per CU 4.7 / 8.0 / 19.5, two
+// 6.5 / 10.9 / 29.8; 128 x 128 in two stages, two per CU 13.1 / 23.8 / 73.0, in
+// four stages, alone on its CU 9.3 / 15.1 / 42.5; 256 x 256: 23.9 / 40.5 / 117).
 struct TileKind {
   int m, n, k, occ;
   float t[2], o[2];
 };
 constexpr TileKind kTileKinds[] = {
     {64, 32, 128, 1, {0.36f, 0.36f}, {1.3f, 1.3f}},
-    {64, 64, 64, 2, {0.285f, 0.385f}, {1.4f, 2.1f}},
-    {128, 64, 64, 2, {0.39f, 0.73f}, {3.5f, 2.0f}},
-    {128, 128, 64, 2, {0.79f, 1.03f}, {2.3f, 4.3f}},
-    {256, 256, 64, 1, {1.53f, 1.53f}, {11.0f, 11.0f}},
+    {64, 64, 64, 2, {0.24f, 0.39f}, {1.9f, 2.3f}},
+    {128, 64, 64, 2, {0.32f, 0.73f}, {3.1f, 1.8f}},
+    {128, 128, 64, 2, {0.77f, 1.03f}, {2.6f, 5.0f}},
+    {128, 128, 64, 1, {0.56f, 0.56f}, {3.7f, 3.7f}},
+    {256, 256, 64, 1, {1.55f, 1.55f}, {11.0f, 11.0f}},
 };
 constexpr float kLaunch = 2.3f;
 constexpr int kCus = 256;
@@ -477,10 +479,11 @@ hipError_t launch_tile_kind(int kind, const LinearArgs& a, int split, float* par
                             hipStream_t stream) {
   switch (kind) {
     case 0: return launch_tile<64, 32, 16, 32, 16, 128, 4, false, 1>(a, split, part, stream);
-    case 1: return launch_tile<64, 64, 16, 32, 16, 64, 4, false, 4>(a, split, part, stream);
-    case 2: return launch_tile<128, 64, 64, 32, 16, 64, 3, false, 2>(a, split, part, stream);
+    case 1: return launch_tile<64, 64, 16, 32, 16, 64, 4, true, 4>(a, split, part, stream);
+    case 2: return launch_tile<128, 64, 32, 32, 16, 64, 3, true, 4>(a, split, part, stream);
     case 3: return launch_tile<128, 128, 32, 64, 16, 64, 2, true, 4>(a, split, part, stream);
-    case 4: return launch_tile<256, 256, 128, 64, 16, 64, 2, true, 2>(a, split, part, stream);
+    case 4: return launch_tile<128, 128, 64, 32, 16, 64, 4, true, 2>(a, split, part, stream);
+    case 5: return launch_tile<256, 256, 128, 64, 16, 64, 2, true, 2>(a, split, part, stream);
   }
   return hipErrorInvalidValue;
 }
