@@ -112,6 +112,22 @@ def test_large_tiles(M, N, K, act):
                residual=r)
 
 
+@pytest.mark.parametrize("act", ["none", "swiglu", "gelu"])
+@pytest.mark.parametrize("M,N,K", [   # each tile, whole and with K split
+    (446, 1157, 72), (446, 1156, 71), (518, 295, 3176), (2980, 674, 66), (1844, 134, 5344),
+    (1544, 3800, 200), (1543, 3801, 198), (2497, 774, 4096), (3602, 517, 752), (3600, 520, 751),
+    (2907, 322, 4144), (3431, 3585, 130), (3431, 3584, 136), (2830, 1412, 3568)])
+def test_each_tile(M, N, K, act):
+    if act == "swiglu":
+        N = (N + 7) // 8 * 4
+    rows = 2 * N if act == "swiglu" else N
+    x, w = _rand((M, K), 70), _rand((rows, K), 71, 0.05)
+    b, s = _rand((rows,), 72, 0.5, F32), _rand((M,), 73, 1.0, F32)
+    for odt, r in ((BF, _rand((M, N), 74)), (F32, None)):
+        out = linear(x, w, bias=b, activation=act, row_scale=s, residual=r, out_dtype=odt)
+        _check(out, x, w, act, b, s, r, what=f"{act} {odt}")
+
+
 @pytest.mark.parametrize("act", sorted(ACTIVATIONS))
 @pytest.mark.parametrize("M,N,K", [(4, 96, 256), (70, 200, 136), (300, 512, 1024)])
 @pytest.mark.parametrize("bias_dtype,res_dtype,scale", [(BF, F32, True), (F32, BF, False),

@@ -140,7 +140,9 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
   auto issue_one = [&](int s, int st, int j) {
     const uint32_t o = kof[j] < kend - BK * s ? off[j] : 0x80000000u;
     const uint8_t* to = lds + st * STAGE + (WAVES * j + w) * 1024;
-    const uint32_t k = (uint32_t)s * (uint32_t)LROW;
+    // (past the end the last step's, which stays inside the buffer: the range
+    // check is of o against what is left of it)
+    const uint32_t k = (uint32_t)min(s, s1 - 1) * (uint32_t)LROW;
     if (RPJ * j < BM) buf_to_lds(xr, o, k, to);
     else if (GATED && RPJ == MB) buf_to_lds((RPJ * j - BM) / MB % 2 ? ur : wr, o, k, to);
     else buf_to_lds(wave_wr, o, k, to);
