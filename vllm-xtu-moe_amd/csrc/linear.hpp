@@ -89,31 +89,57 @@ __device__ __forceinline__ void finish_one(const LinearArgs& a, int m, int n, fl
   else reinterpret_cast<float*>(a.out)[o] = y;
 }
 
-__device__ __forceinline__ f32x4_t load4(const void* p, long o, int is_bf16) {
-  if (!is_bf16) return *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(p) + o);
+// What an epilogue reads ahead stays as it is in memory until it is used: to
+// convert it is to wait for it.
+__device__ __forceinline__ u32x4_t load_raw4(const void* p, long o, int is_bf16) {
+  if (!is_bf16) return *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const float*>(p) + o);
   const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + o);
-  return f32x4_t{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u),
-                 __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
+  return u32x4_t{v.x, v.y, 0u, 0u};
+}
+
+__device__ __forceinline__ f32x4_t of_raw4(u32x4_t v, int is_bf16) {
+  if (!is_bf16) return __builtin_bit_cast(f32x4_t, v);
+  return f32x4_t{__uint_as_float(v[0] << 16), __uint_as_float(v[0] & 0xffff0000u),
+                 __uint_as_float(v[1] << 16), __uint_as_float(v[1] & 0xffff0000u)};
+}
+
+__device__ __forceinline__ uint32_t load_raw1(const void* p, long o, int is_bf16) {
+  return is_bf16 ? reinterpret_cast<const uint16_t*>(p)[o] : reinterpret_cast<const uint32_t*>(p)[o];
+}
+
+__device__ __forceinline__ float of_raw1(uint32_t v, int is_bf16) {
+  return __uint_as_float(is_bf16 ? v << 16 : v);
 }
 
 // Four columns' bias: of z, and for swiglu of u.
 template <int AK>
-__device__ __forceinline__ void load_bias4(const LinearArgs& a, int n, f32x4_t& bz, f32x4_t& bu) {
-  bz = bu = f32x4_t{0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ void load_bias4(const LinearArgs& a, int n, u32x4_t& bz, u32x4_t& bu) {
+  bz = bu = u32x4_t{0u, 0u, 0u, 0u};   // zero in both types
   if (!a.bias) return;
-  bz = load4(a.bias, n, a.bias_bf16);
-  if constexpr (AK == kActSwiglu) bu = load4(a.bias, a.N + n, a.bias_bf16);
+  bz = load_raw4(a.bias, n, a.bias_bf16);
+  if constexpr (AK == kActSwiglu) bu = load_raw4(a.bias, a.N + n, a.bias_bf16);
 }
 
-// What the epilogue of four columns of a row reads.
+// What the epilogue of four columns of a row reads, and of a single one.
 struct Row4 {
-  f32x4_t res;
+  u32x4_t res;
+  float scale;
+};
+struct Row1 {
+  uint32_t res;
   float scale;
 };
 
 __device__ __forceinline__ Row4 load_row4(const LinearArgs& a, int m, int n) {
-  Row4 r = {{0.f, 0.f, 0.f, 0.f}, 1.f};
-  if (a.res) r.res = load4(a.res, (long)m * a.ldr + n, a.res_bf16);
+  Row4 r = {{0u, 0u, 0u, 0u}, 1.f};
+  if (a.res) r.res = load_raw4(a.res, (long)m * a.ldr + n, a.res_bf16);
+  if (a.scale) r.scale = a.scale[(long)m * a.sstride];
+  return r;
+}
+
+__device__ __forceinline__ Row1 load_row1(const LinearArgs& a, int m, int n) {
+  Row1 r = {0u, 1.f};
+  if (a.res) r.res = load_raw1(a.res, (long)m * a.ldr + n, a.res_bf16);
   if (a.scale) r.scale = a.scale[(long)m * a.sstride];
   return r;
 }
@@ -143,7 +169,7 @@ __device__ __forceinline__ void act_all(const LinearArgs& a, f32x4_t (&z)[C], f3
 __device__ __forceinline__ void store_row4(const LinearArgs& a, int m, int n, f32x4_t y,
                                            const Row4& r) {
   if (a.scale) y *= r.scale;
-  if (a.res) y += r.res;
+  if (a.res) y += of_raw4(r.res, a.res_bf16);
   const long o = (long)m * a.ldo + n;
   if (a.out_bf16) {
     uint2 v;
@@ -158,10 +184,10 @@ __device__ __forceinline__ void store_row4(const LinearArgs& a, int m, int n, f3
 // Columns n .. n + 3 of row m, all of them there (a.vec: N % 4 == 0).
 template <int AK>
 __device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, f32x4_t z, f32x4_t u) {
-  f32x4_t bz, bu;
+  u32x4_t bz, bu;
   load_bias4<AK>(a, n, bz, bu);
   const Row4 r = load_row4(a, m, n);
-  f32x4_t zz[1] = {z + bz}, uu[1] = {u + bu};
+  f32x4_t zz[1] = {z + of_raw4(bz, a.bias_bf16)}, uu[1] = {u + of_raw4(bu, a.bias_bf16)};
   act_all<AK>(a, zz, uu);
   store_row4(a, m, n, zz[0], r);
 }

@@ -152,6 +152,38 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
     for (int j = 0; j < LOADS; ++j) issue_one(s, st, j);
   };
 
+  // The epilogue's part of the wave.  Vectors: CG lanes along a row, RS rows at a
+  // time, BT such in one pass; single columns: RS1 rows, BT1 such.  A wave of one
+  // row block reads what it needs beside the sums here, ahead of the operands.
+  constexpr int W = GATED ? WN / 2 : WN;   // output columns of the wave
+  constexpr int CG = W / 4, RS = 64 / CG, IT = MB / RS, RS1 = 64 / W, IT1 = MB / RS1;
+  constexpr int BT = IT < 4 ? IT : AK == kActOther ? 2 : 4, BT1 = 4;
+  constexpr bool PRE = NJ == 1 && !SPLIT;
+  static_assert(IT1 % BT1 == 0 && (!PRE || IT == BT), "whole passes");
+  const int nw = n0 + W * wn, mw = m0 + WM * wm;
+  const int cv = lane % CG * 4, nv = nw + cv;   // a lane's four columns
+  const int c1 = lane % W, n1 = nw + c1;        // or its single one
+  u32x4_t bz = {0u, 0u, 0u, 0u}, bu = bz;
+  Row4 pre[PRE ? IT : 1];
+  Row1 pre1[PRE ? IT1 : 1];
+  if (!SPLIT && a.vec && nv < a.N) {
+    load_bias4<AK>(a, nv, bz, bu);
+    if constexpr (PRE)
+#pragma unroll
+      for (int b = 0; b < IT; ++b)
+        pre[b] = load_row4(a, min(mw + b * RS + lane / CG, a.M - 1), nv);
+  }
+  if (!SPLIT && !a.vec && n1 < a.N) {
+    if (a.bias) {
+      bz[0] = load_raw1(a.bias, n1, a.bias_bf16);
+      if constexpr (GATED) bu[0] = load_raw1(a.bias, (long)a.N + n1, a.bias_bf16);
+    }
+    if constexpr (PRE)
+#pragma unroll
+      for (int b = 0; b < IT1; ++b)
+        pre1[b] = load_row1(a, min(mw + b * RS1 + lane / W, a.M - 1), n1);
+  }
+
   acc_t acc[NI][NJ];
 #pragma unroll
   for (int i = 0; i < NI; ++i)
@@ -267,22 +299,9 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
   // its own part of LDS, then takes them with consecutive lanes along a row
   // (whole lines to memory).  The loops stay rolled (ActKind).
   constexpr int LD = epi_ld<WN>();
-  constexpr int W = GATED ? WN / 2 : WN;   // output columns of the wave
   __syncthreads();   // every wave is done with the stages
   float* eb = reinterpret_cast<float*>(lds) + w * (MB * LD);
-  const int nw = n0 + W * wn;
   float* plane = SPLIT ? part + (long)blockIdx.y * part_plane(a) : nullptr;
-  // vectors: CG lanes along a row, RS rows at a time, BT such in one pass
-  constexpr int CG = W / 4, RS = 64 / CG, IT = MB / RS;
-  constexpr int BT = IT < 4 ? IT : AK == kActOther ? 2 : 4;
-  const int cv = lane % CG * 4, nv = nw + cv;
-  const int n1 = nw + lane % W;   // a lane's single column
-  f32x4_t bz = {0.f, 0.f, 0.f, 0.f}, bu = bz;
-  if (!SPLIT && a.vec && nv < a.N) load_bias4<AK>(a, nv, bz, bu);
-  if (!SPLIT && !a.vec && a.bias && n1 < a.N) {
-    bz[0] = load_bias(a, n1);
-    if constexpr (GATED) bu[0] = load_bias(a, a.N + n1);
-  }
 #pragma unroll 1
   for (int j = 0; j < NJ; ++j) {
     lds_order();
@@ -299,11 +318,11 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
         }
     }
     lds_order();
-    const int mb = m0 + WM * wm + MB * j;
+    const int mb = mw + MB * j;
     // column col of the wave: its gate (or only) sum's place in the row
     const auto place = [&](int col) { return GATED ? col / MB * 2 * MB + col % MB : col; };
     if (a.vec) {
-      // a lane keeps its columns; what BT rows need is read before any is written
+      // what BT rows need is read before any is written
 #pragma unroll 1
       for (int it = 0; it < IT && nv < a.N; it += BT) {
         f32x4_t z[BT], u[BT];
@@ -315,13 +334,14 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
           z[b] = *reinterpret_cast<const f32x4_t*>(row);
           u[b] = z[b];
           if constexpr (GATED) u[b] = *reinterpret_cast<const f32x4_t*>(row + MB);
-          if constexpr (!SPLIT) x[b] = load_row4(a, min(m + b * RS, a.M - 1), nv);
+          if constexpr (PRE) x[b] = pre[b];
+          else if constexpr (!SPLIT) x[b] = load_row4(a, min(m + b * RS, a.M - 1), nv);
         }
         if constexpr (!SPLIT) {
 #pragma unroll
           for (int b = 0; b < BT; ++b) {
-            z[b] += bz;
-            u[b] += bu;
+            z[b] += of_raw4(bz, a.bias_bf16);
+            u[b] += of_raw4(bu, a.bias_bf16);
           }
           act_all<AK>(a, z, u);
         }
@@ -338,33 +358,33 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, OCC) void linear_tile_ker
         }
       }
     } else {
-      // the same by single columns, four rows in one pass
-      constexpr int RS1 = 64 / W;
-      static_assert(MB / RS1 % 4 == 0, "four rows a pass");
-#pragma unroll 1
-      for (int it = 0; it < MB / RS1 && n1 < a.N; it += 4) {
-        f32x4_t z[1], u[1], res = {0.f, 0.f, 0.f, 0.f}, sc = {1.f, 1.f, 1.f, 1.f};
+      // the same by single columns
+#pragma unroll PRE ? IT1 / BT1 : 1
+      for (int it = 0; it < IT1; it += BT1) {
+        if (n1 >= a.N) break;
+        f32x4_t z[1], u[1];
+        Row1 x[BT1];
         const int r = it * RS1 + lane / W, m = mb + r;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const float* row = eb + (r + b * RS1) * LD + place(lane % W);
+        for (int b = 0; b < BT1; ++b) {
+          const float* row = eb + (r + b * RS1) * LD + place(c1);
           z[0][b] = row[0];
           u[0][b] = GATED ? row[MB] : 0.f;
-          const long mm = min(m + b * RS1, a.M - 1);
-          if (!SPLIT && a.res)
-            res[b] = a.res_bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(a.res)[mm * a.ldr + n1])
-                                : reinterpret_cast<const float*>(a.res)[mm * a.ldr + n1];
-          if (!SPLIT && a.scale) sc[b] = a.scale[mm * a.sstride];
+          if constexpr (PRE) x[b] = pre1[it + b];
+          else if constexpr (!SPLIT) x[b] = load_row1(a, min(m + b * RS1, a.M - 1), n1);
         }
         if constexpr (!SPLIT) {
-          z[0] += bz[0];
-          u[0] += bu[0];
+          z[0] += of_raw1(bz[0], a.bias_bf16);
+          u[0] += of_raw1(bu[0], a.bias_bf16);
           act_all<AK>(a, z, u);
-          if (a.scale) z[0] *= sc;
-          if (a.res) z[0] += res;
+#pragma unroll
+          for (int b = 0; b < BT1; ++b) {
+            if (a.scale) z[0][b] *= x[b].scale;
+            if (a.res) z[0][b] += of_raw1(x[b].res, a.res_bf16);
+          }
         }
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < BT1; ++b) {
           const long mm = m + b * RS1;
           if (mm >= a.M) break;
           if constexpr (SPLIT) {
