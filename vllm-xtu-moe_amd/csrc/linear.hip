@@ -120,8 +120,8 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int spli
 }
 
 // x and w as rows of K8 = K rounded up to 8, zeros behind K: what the tile
-// kernels read.  1013 x 1187 by 771 rows of it: the two launches take 14 us where
-// linear_any_kernel takes 24.
+// kernels read.  1013 x 1187 by 771 rows of it: the two launches take 16 us (with bias,
+// gelu and residual) where linear_any_kernel takes 24.
 __global__ __launch_bounds__(256) void linear_pack_kernel(const uint16_t* x, long ldx, int M,
                                                           const uint16_t* w, long ldw, int rows,
                                                           int K, uint16_t* out) {
