@@ -333,3 +333,62 @@ def test_graphs_captured_from_one_stream_replayed_at_once(T):
         for b, x, o in zip(blks, xs, outs):
             for a, r in zip(o, b(x, return_routing=True)):
                 assert torch.equal(a, r)
+
+
+@pytest.mark.parametrize("bias_dtype", [F32, BF])
+def test_storage_replaced_between_calls(bias_dtype):
+    """The router, the shared gates and the bias are read where they lie at the
+    call: other storage under them, or other values in place, and every batch
+    size answers with those."""
+    E, NS, K, H, I = 64, 2, 6, 512, 256
+    W, dense = _layer("mxfp4", E, NS, H, I)
+
+    def fresh(seed):
+        gate, kw = _router(E, H, True, seed)
+        return gate, _x(NS, H, seed) * 0.05, kw["bias"].to(bias_dtype)
+
+    def block(gate, shared, bias):
+        return MoeBlock(gate, W, top_k=K, shared_gate=shared, scoring="sigmoid", bias=bias)
+
+    params = [torch.nn.Parameter(t, requires_grad=False) for t in fresh(30)]
+    blk = block(*params)
+    xs = [_x(T, H, T) for T in (1, 5, 16, 17, 40)]
+    before = [blk(x, return_routing=True) for x in xs]
+    for k in range(3):
+        new = fresh(31 + k)
+        if k < 2:
+            for p, t in zip(params, new):
+                p.data = t.clone()
+        else:
+            for p, t in zip(params, new):
+                p.copy_(t)
+        want = block(*new)
+        for x, old in zip(xs, before):
+            got, ref = blk(x, return_routing=True), want(x, return_routing=True)
+            for a, b in zip(got, ref):
+                assert torch.equal(a, b)
+            assert not torch.equal(got[0], old[0])
+
+
+def test_storage_that_does_not_fit_refused():
+    E, NS, K, H, I = 64, 2, 6, 512, 256
+    W, dense = _layer("mxfp4", E, NS, H, I)
+    gate, kw = _router(E, H, True, 30)
+    shared = _x(NS, H, 30) * 0.05
+    params = [torch.nn.Parameter(t, requires_grad=False) for t in (gate, shared, kw["bias"])]
+    blk = MoeBlock(params[0], W, top_k=K, shared_gate=params[1], scoring="sigmoid", bias=params[2])
+    x = _x(3, H, 3)
+    want = blk(x)
+    off = torch.empty(E * H + 1, dtype=BF, device=DEV)[1:].view(E, H)
+    for p, bad, match in (
+            (params[0], gate[:32].clone(), "gate_weight"), (params[0], gate.float(), "gate_weight"),
+            (params[0], gate.t().contiguous().t(), "gate_weight"), (params[0], gate.cpu(), "is on"),
+            (params[0], off, "16 bytes"), (params[1], shared[:1].clone(), "shared_gate"),
+            (params[1], shared.cpu(), "is on"), (params[2], kw["bias"][:60].clone(), "bias"),
+            (params[2], kw["bias"].cpu(), "is on")):
+        good, p.data = p.data, bad
+        for xx in (x, _x(40, H, 4)):
+            with pytest.raises(ValueError, match=match):
+                blk(xx)
+        p.data = good
+    assert torch.equal(blk(x), want)

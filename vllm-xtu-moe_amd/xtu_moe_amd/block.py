@@ -29,6 +29,12 @@ ARGS = struct.Struct("@14PN12i4f")
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 16, 64   # the routers' limits
 
 
+def _check_rows(name, t, n, H):
+    """bf16 rows [n, H] that the kernels can read, or None."""
+    if t is not None and (t.shape != (n, H) or t.dtype != torch.bfloat16 or not t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous bf16 [{n}, {H}], got {tuple(t.shape)} {t.dtype}")
+
+
 class MoeBlock:
     """One layer's MoE block over resident experts.
 
@@ -37,7 +43,10 @@ class MoeBlock:
     (grouped, selection by score + bias), with the arguments of ``route``.
     shared_gate: bf16 [n_shared, H]; shared expert s is scaled by
     sigmoid(x . shared_gate[s]) (without it by 1).  swiglu_*: the clamped gated
-    SiLU of every expert.
+    SiLU of every expert.  Every call reads the tensors given here as they are
+    then, in the storage that they have then (their owner may write them or put
+    other storage under them, ``param.data = ...``, between calls); ones that no
+    longer fit are refused.
     """
 
     def __init__(self, gate_weight, weights: ExpertWeights, *, top_k, scoring="softmax",
@@ -50,21 +59,13 @@ class MoeBlock:
             raise ValueError("the block needs device-resident expert weights")
         if W.fmt not in (FMT_BF16, FMT_FP8, FMT_MXFP4, FMT_NVFP4) or W.n_slots != W.n_experts:
             raise ValueError("the block needs BF16, FP8, MXFP4 or NVFP4 planes of every expert")
-        _same_device(W.device, gate_weight=gate_weight, bias=bias, shared_gate=shared_gate)
-        self.W, self.gate_weight, self.shared_gate = W, gate_weight, shared_gate
+        self.W, self.gate_weight, self.shared_gate, self.bias = W, gate_weight, shared_gate, bias
         self.top_k, self.scoring, self.renormalize = int(top_k), scoring, bool(renormalize)
-        self.bias = None if bias is None else bias.to(torch.float32).contiguous()
         self.n_group, self.topk_group = int(n_group), int(topk_group)
         self.routed_scaling_factor = float(routed_scaling_factor)
         self.limit = float(swiglu_limit or 0.0)
         self.alpha, self.beta = float(swiglu_alpha), float(swiglu_beta)
-        # what xtu_few_block takes of the layer, in its order
-        ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-        if any(ptr(t) & 15 for t in (gate_weight, shared_gate)):
-            raise ValueError("gate_weight and shared_gate must start on 16 bytes")
-        self._planes = tuple(ptr(t) for t in (gate_weight, shared_gate, self.bias, W.w13, W.s13,
-                                              W.gs13, W.w2, W.s2, W.gs2))
-        self._keep = (W.w13, W.s13, W.gs13, W.w2, W.s2, W.gs2)
+        self._operands()
         self._shape = (W.H, W.I, W.E, W.n_shared, self.top_k, int(scoring == "sigmoid"),
                        self.renormalize, self.n_group, self.topk_group)
         self._floats = (self.routed_scaling_factor, self.limit, self.alpha, self.beta)
@@ -86,12 +87,8 @@ class MoeBlock:
             raise ValueError("gate_weight is missing")
         if shared_gate is not None and W.n_shared == 0:
             raise ValueError("shared_gate without shared experts")
-        for name, t, n in (("gate_weight", gate_weight, W.E),
-                           ("shared_gate", shared_gate, W.n_shared)):
-            if t is not None and (tuple(t.shape) != (n, W.H) or t.dtype != torch.bfloat16
-                                  or not t.is_contiguous()):
-                raise ValueError(f"{name} must be contiguous bf16 [{n}, {W.H}], got "
-                                 f"{tuple(t.shape)} {t.dtype}")
+        _check_rows("gate_weight", gate_weight, W.E, W.H)
+        _check_rows("shared_gate", shared_gate, W.n_shared, W.H)
         if scoring not in ("softmax", "sigmoid"):
             raise ValueError(f"unsupported scoring function {scoring!r}")
         if bias is not None and (tuple(bias.shape) != (W.E,) or scoring != "sigmoid"):
@@ -106,6 +103,21 @@ class MoeBlock:
                                      or top_k > topk_group * (W.E // n_group)):
             raise ValueError(f"{n_group} groups with {topk_group} kept do not fit {W.E} experts, "
                              f"top {top_k}")
+
+    def _operands(self):
+        """(gate_weight, shared_gate, bias fp32 or None) as they are now, checked
+        against the layer: the kernels take their addresses."""
+        W, gate, shared, bias = self.W, self.gate_weight, self.shared_gate, self.bias
+        _check_rows("gate_weight", gate, W.E, W.H)
+        _check_rows("shared_gate", shared, W.n_shared, W.H)
+        if bias is not None and bias.shape != (W.E,):
+            raise ValueError(f"bias must be [{W.E}], got {tuple(bias.shape)}")
+        _same_device(W.device, gate_weight=gate, shared_gate=shared, bias=bias)
+        if gate.data_ptr() & 15 or (shared is not None and shared.data_ptr() & 15):
+            raise ValueError("gate_weight and shared_gate must start on 16 bytes")
+        if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
+            bias = bias.to(torch.float32).contiguous()
+        return gate, shared, bias
 
     def __call__(self, x, *, out=None, out_dtype=None, return_routing=False, stream=None):
         """x bf16 [T, H] -> [T, H] bf16 (or out_dtype fp32, or into out); with
@@ -125,6 +137,7 @@ class MoeBlock:
                 return self(x, out=out, out_dtype=out_dtype, return_routing=return_routing)
         if out is not None and _overlap(out, x):
             raise ValueError("out overlaps x")
+        operands = self._operands()
         if out is None:
             out = torch.empty(x.shape, dtype=odt, device=x.device)
         T = x.shape[0]
@@ -137,40 +150,44 @@ class MoeBlock:
         ids = x.new_empty((T, self.top_k), dtype=torch.int32)
         wts = x.new_empty((T, self.top_k), dtype=torch.float32)
         if need:
-            self._few(x, out, ids, wts, need)
+            self._few(x, out, ids, wts, need, *operands)
         elif T:
             # (eagerly the stream's scratch: calls on it run in order)
             capturing = torch.cuda.is_current_stream_capturing()
             with scratch_per_call() if capturing else contextlib.nullcontext():
-                self._composed(x, out, ids, wts)
+                self._composed(x, out, ids, wts, *operands)
         return (out, wts, ids) if return_routing else out
 
-    def _few(self, x, out, ids, wts, need):
+    def _few(self, x, out, ids, wts, need, gate, shared, bias):
         """A few tokens, in two launches."""
+        W = self.W
+        # what xtu_few_block takes of the layer, in its order
+        planes = [0 if t is None else t.data_ptr()
+                  for t in (gate, shared, bias, W.w13, W.s13, W.gs13, W.w2, W.s2, W.gs2)]
         if x.data_ptr() & 15:
             x = x.clone()
         # per call: calls on other streams, and graphs, have their own
         ws = x.new_empty(need, dtype=torch.uint8)
-        rc = self._entry(ARGS.pack(x.data_ptr(), *self._planes, out.data_ptr(), ids.data_ptr(),
-                                   wts.data_ptr(), ws.data_ptr(), need, self.W.fmt, x.shape[0],
+        rc = self._entry(ARGS.pack(x.data_ptr(), *planes, out.data_ptr(), ids.data_ptr(),
+                                   wts.data_ptr(), ws.data_ptr(), need, W.fmt, x.shape[0],
                                    *self._shape, out.dtype == torch.bfloat16, *self._floats),
                          raw_stream(x.device.index))
         if rc:
             _lib.check("xtu_few_block", rc)
 
-    def _composed(self, x, out, ids, wts):
+    def _composed(self, x, out, ids, wts, gate, shared, bias):
         """Any number of tokens: the products and the layer one after the other."""
-        logits = linear(x, self.gate_weight, out_dtype=torch.float32)
-        kw = dict(scoring=self.scoring, bias=self.bias, n_group=self.n_group,
+        logits = linear(x, gate, out_dtype=torch.float32)
+        kw = dict(scoring=self.scoring, bias=bias, n_group=self.n_group,
                   topk_group=self.topk_group, routed_scaling_factor=self.routed_scaling_factor,
                   renormalize=self.renormalize)
         act = dict(swiglu_limit=self.limit, swiglu_alpha=self.alpha, swiglu_beta=self.beta,
                    out=out)
-        if self.shared_gate is None:
+        if shared is None:
             moe_forward(x, ids, wts, self.W, router=dict(logits=logits, **kw), **act)
             return
         route(logits, top_k=self.top_k, ids_out=ids, wts_out=wts, **kw)
-        gates = linear(x, self.shared_gate, activation="sigmoid", out_dtype=torch.float32)
-        shared = torch.arange(self.W.E, self.W.n_experts, dtype=torch.int32, device=x.device)
-        moe_forward(x, torch.cat([ids, shared.expand(x.shape[0], -1)], 1),
+        gates = linear(x, shared, activation="sigmoid", out_dtype=torch.float32)
+        sids = torch.arange(self.W.E, self.W.n_experts, dtype=torch.int32, device=x.device)
+        moe_forward(x, torch.cat([ids, sids.expand(x.shape[0], -1)], 1),
                     torch.cat([wts, gates], 1), self._W_all, **act)
