@@ -605,7 +605,9 @@ hipError_t xtu_i8_row_fallback(int gate_up, const void* x, const int32_t* sorted
  * and residual may be NULL.  act: 0 none, 1 relu, 2 silu, 3 gelu (erf), 4 gelu
  * (tanh), 5 sigmoid, 6 swiglu: w and bias hold 2N rows, gate rows [0, N) then
  * up rows, act = the experts' clamped gated SiLU (limit, alpha, beta; the
- * others ignore them).  fp32 sums and epilogue, one rounding to out's type.
+ * others ignore them).  fp32 sums and epilogue, one rounding to out's type.  M up
+ * to 2^31 - 512, N and K up to 2^28, and fewer than 2^32 threads a launch (M N
+ * near 2^34 for the smallest tiles).
  * out may be residual itself (same rows), else it overlaps no input.  M = 0
  * returns at once.  workspace (16-byte aligned, may be NULL):
  * xtu_linear_workspace_bytes() lets a product of few tiles split K, and one

@@ -270,3 +270,20 @@ def test_long_offsets():
     _check(linear(w, x), w, x)
     o = torch.zeros(2 * ld + 64, dtype=BF, device=DEV).as_strided((M, 64), (ld, 1))
     _check(linear(x, w, out=o), x, w)
+
+
+@pytest.mark.parametrize("K", [24, 23])
+def test_outputs_past_2_31_elements(K):
+    """Rows whose elements lie past 2^31 in x, in residual and in the output;
+    their copies (K = 23: rows that do not start on 16 bytes) past 2^31 bytes."""
+    M, N = (1 << 27) + 77, 17
+    x, w = torch.empty((M, K), dtype=BF, device=DEV).normal_(), _rand((N, K), 80)
+    r = torch.empty((M, N), dtype=BF, device=DEV).normal_()
+    out = linear(x, w, residual=r)
+    for a in (0, M // 2, M - 1000):
+        b = a + 1000
+        _check(out[a:b], x[a:b], w, residual=r[a:b], what=f"rows {a} ..")
+    # every row, against the same product of a part that starts elsewhere
+    for a in range(0, M, 1 << 25):
+        assert torch.equal(out[a:a + (1 << 25)], linear(x[a:a + (1 << 25)], w,
+                                                        residual=r[a:a + (1 << 25)]))

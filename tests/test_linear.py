@@ -86,3 +86,28 @@ def test_entry_refuses_on_the_host():
                 dict(sst=-1), dict(ws=8), dict(M=2, N=9), dict(N=1 << 29), dict(K=1 << 29),
                 dict(M=1 << 30, N=1 << 20, ldo=1 << 20)):
         assert rc(**bad) == 1, bad
+
+
+def test_sizes_past_the_kernels_indices_refused():
+    """The kernels count rows in 32 bits, up to a tile past the last one."""
+    x, w = _xw(1, 4, 8)
+    for rows in ((1 << 31) - 511, (1 << 31) - 1, 1 << 31, 1 << 33):
+        _refused("rows", x.expand(rows, 8), w)
+    _refused("CUDA", x.expand((1 << 31) - 512, 8), w)
+    for act in ("none", "swiglu"):   # N columns: 2N rows of w for swiglu
+        _refused("columns", x, w[:1].expand((2 if act == "swiglu" else 1) * (1 << 28) + 2, 8),
+                 activation=act)
+        _refused("CUDA", x, w[:1].expand((2 if act == "swiglu" else 1) * (1 << 28), 8),
+                 activation=act)
+    long = torch.empty((1, (1 << 28) + 1), dtype=BF)   # (never touched)
+    _refused("columns", long, long)
+
+
+@pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
+def test_entry_refuses_row_counts_on_the_host():
+    lib = _lib.load()
+    for M in ((1 << 31) - 511, (1 << 31) - 1):
+        assert lib.xtu_linear(ARGS.pack(16, 16, 0, 0, 0, 16, 0, 8, 8, 0, 8, 0, 0, M, 1, 1, 0, 0, 0,
+                                        1, 0.0, 1.0, 0.0), None) == 1
+        assert lib.xtu_linear_workspace_bytes(M, 1, 1, 0, 0) == 0
+    assert lib.xtu_linear_workspace_bytes((1 << 31) - 512, 1, 1, 0, 0) > 0

@@ -127,7 +127,7 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const uint16_t* x, lon
                                                           int K, uint16_t* out) {
   const int per = (K + 7) / 8;
   const long p = (long)blockIdx.x * 256 + threadIdx.x;
-  if (p >= (long)(M + rows) * per) return;
+  if (p >= ((long)M + rows) * per) return;
   const long r = p / per;
   const int k = (int)(p - r * per) * 8;
   const uint16_t* row = r < M ? x + r * ldx : w + (r - M) * ldw;
@@ -138,6 +138,7 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const uint16_t* x, lon
 
 hipError_t launch_join(const LinearArgs& a, int split, const float* part, hipStream_t stream) {
   const long n = (long)a.M * (a.vec ? a.N / 4 : a.N);
+  if (!grid_fits((n + 255) / 256, 256)) return hipErrorInvalidConfiguration;
   void (*k)(LinearArgs, int, const float*);
   if (a.act == kSwiglu) k = a.vec ? linear_join_kernel<kActSwiglu, 4> : linear_join_kernel<kActSwiglu, 1>;
   else if (a.act == kNone) k = a.vec ? linear_join_kernel<kActNone, 4> : linear_join_kernel<kActNone, 1>;
@@ -150,6 +151,7 @@ hipError_t launch_any(const LinearArgs& a, hipStream_t stream) {
   const int nb = a.act == kSwiglu ? kAnyN / 2 : kAnyN;
   const long gm = (a.M + (long)kAnyM - 1) / kAnyM, gn = ((long)a.N + nb - 1) / nb;
   const unsigned grid = (unsigned)(gm * gn);
+  if (!grid_fits(gm * gn, 256)) return hipErrorInvalidConfiguration;
   if (a.act == kSwiglu) linear_any_kernel<true><<<grid, 256, 0, stream>>>(a);
   else linear_any_kernel<false><<<grid, 256, 0, stream>>>(a);
   return hipPeekAtLastError();
@@ -162,6 +164,9 @@ namespace xtu {
 namespace lin {
 namespace {
 
+// Rows past M, up to a tile's 256, are ints too.
+constexpr int kMaxM = 0x7fffffff - 511;
+
 size_t pack_bytes(int M, long rows, int K) { return (size_t)(M + rows) * ((K + 7) / 8) * 16; }
 
 size_t split_bytes(const TilePlan& p, int M, long rows) {
@@ -171,6 +176,7 @@ size_t split_bytes(const TilePlan& p, int M, long rows) {
 hipError_t launch_pack(LinearArgs& a, long rows, void* ws, hipStream_t stream) {
   const long K8 = (a.K + 7) / 8 * 8, pieces = (a.M + rows) * (K8 / 8);
   uint16_t* out = reinterpret_cast<uint16_t*>(ws);
+  if (!grid_fits((pieces + 255) / 256, 256)) return hipErrorInvalidConfiguration;
   linear_pack_kernel<<<(unsigned)((pieces + 255) / 256), 256, 0, stream>>>(
       a.x, a.ldx, a.M, a.w, a.ldw, (int)rows, a.K, out);
   a.x = out;
@@ -190,7 +196,7 @@ using namespace xtu::lin;
 extern "C" {
 
 size_t xtu_linear_workspace_bytes(int M, int N, int K, int act, int aligned) {
-  if (M <= 0 || N <= 0 || K <= 0 || N > (1 << 28) || K > (1 << 28)) return 0;
+  if (M <= 0 || M > kMaxM || N <= 0 || K <= 0 || N > (1 << 28) || K > (1 << 28)) return 0;
   LinearArgs a{};
   a.M = M;
   a.N = N;
@@ -207,7 +213,7 @@ hipError_t xtu_linear(const xtu_linear_args* args, hipStream_t stream) {
   const xtu_linear_args& t = *args;
   const int M = t.M, N = t.N, K = t.K, act = t.act;
   XTU_CHECK_ARG(M >= 0 && N >= 1 && K >= 1 && act >= kNone && act <= kSwiglu);
-  XTU_CHECK_ARG(N <= (1 << 28) && K <= (1 << 28));
+  XTU_CHECK_ARG(M <= kMaxM && N <= (1 << 28) && K <= (1 << 28));
   if (M == 0) return hipSuccess;
   XTU_CHECK_ARG(t.x && t.w && t.out && t.ldx >= 0 && t.ldw >= 0 && t.ldr >= 0 &&
                 t.scale_stride >= 0);

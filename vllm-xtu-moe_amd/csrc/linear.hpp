@@ -249,6 +249,11 @@ __device__ __forceinline__ u32x4_t load8(const uint16_t* row, int k, int K) {
   return v;
 }
 
+// A launch has fewer than 2^32 threads along x.
+__host__ inline bool grid_fits(long blocks, int threads) {
+  return blocks * threads < (1L << 32);
+}
+
 struct TilePlan {
   int kind, split;
 };

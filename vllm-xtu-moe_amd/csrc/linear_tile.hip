@@ -415,6 +415,7 @@ hipError_t launch_tile(const LinearArgs& a, int split, float* part, hipStream_t 
   constexpr size_t kEpi = (size_t)WAVES * MB * epi_ld<WN>() * 4;
   constexpr size_t lds = kStages > kEpi ? kStages : kEpi;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
+  if (!grid_fits(gm * gn, NT)) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)(gm * gn), (unsigned)split);
   void (*k)(LinearArgs, int, float*) = nullptr;
   if (split > 1)

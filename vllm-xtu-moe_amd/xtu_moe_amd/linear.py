@@ -26,6 +26,8 @@ ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "sigm
 ARGS = struct.Struct("@7P5lN7i3f")
 # workspace bytes per (M, N, K, swiglu, aligned)
 _WS_BYTES: dict = {}
+# what the kernels' 32-bit indices reach (xtu_linear refuses the same)
+MAX_ROWS, MAX_COLS = (1 << 31) - 512, 1 << 28
 _TYPES = (torch.bfloat16, torch.float32)
 _OPERAND = (torch.bfloat16,)
 _ENTRY = None
@@ -91,7 +93,8 @@ def linear(x, w, *, bias=None, activation="none", row_scale=None, residual=None,
            out_dtype=None, swiglu_limit=0.0, swiglu_alpha=1.0, swiglu_beta=0.0, stream=None):
     """residual + row_scale * act(x @ w.T + bias); returns [M, N].
 
-    x [M, K] and w [N, K] bf16, rows contiguous at any row stride; M may be 0.
+    x [M, K] and w [N, K] bf16, rows contiguous at any row stride; M may be 0
+    (at most 2^31 - 512 rows, 2^28 columns of x and of the output).
     activation: "none", "relu", "silu", "gelu" (erf), "gelu_tanh", "sigmoid",
     or "swiglu" (w and bias hold 2N rows, gate rows then up rows; the clamped
     gated SiLU of the experts with swiglu_*).  bias [N] (swiglu [2N]) and
@@ -111,6 +114,10 @@ def linear(x, w, *, bias=None, activation="none", row_scale=None, residual=None,
         raise ValueError(f"w of shape {tuple(w.shape)} does not fit activation {activation!r} "
                          "(at least one row and column; an even number of rows for swiglu)")
     N = rows // 2 if act == 6 else rows
+    if M > MAX_ROWS:
+        raise ValueError(f"x has {M} rows, at most {MAX_ROWS}")
+    if N > MAX_COLS or K > MAX_COLS:
+        raise ValueError(f"{N} output columns of {K} values, at most {MAX_COLS} columns of each")
     dev = x.device
     same = w.device == dev
     bp = sp = rp = sst = ldr = 0
