@@ -630,6 +630,9 @@ typedef struct xtu_linear_args {
 } xtu_linear_args;
 hipError_t xtu_linear(const xtu_linear_args* args, hipStream_t stream);
 size_t xtu_linear_workspace_bytes(int M, int N, int K, int act, int aligned);
+/* Which kernel a product with all of that workspace takes: 0 the stream of few
+ * rows, else 256 * (K splits) + 1 + its tile (an index of kTileKinds), -1 none. */
+int xtu_linear_plan(int M, int N, int K, int act);
 
 /* ------------------------------------------------ MoE block of a few tokens
  * From hidden states x bf16 [T][H] to the layer's output, in two launches:

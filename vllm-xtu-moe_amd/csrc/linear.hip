@@ -208,6 +208,17 @@ size_t xtu_linear_workspace_bytes(int M, int N, int K, int act, int aligned) {
   return pack + split_bytes(plan_tile(M, N, K, act == kSwiglu, true), M, rows);
 }
 
+int xtu_linear_plan(int M, int N, int K, int act) {
+  if (M <= 0 || M > kMaxM || N <= 0 || K <= 0 || N > (1 << 28) || K > (1 << 28)) return -1;
+  LinearArgs a{};
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  if (skinny_fits(a)) return 0;
+  const TilePlan p = plan_tile(M, N, K, act == kSwiglu, true);
+  return 256 * p.split + 1 + p.kind;
+}
+
 hipError_t xtu_linear(const xtu_linear_args* args, hipStream_t stream) {
   XTU_CHECK_ARG(args);
   const xtu_linear_args& t = *args;
