@@ -99,12 +99,14 @@ __device__ __forceinline__ float xtu_sigmoid(float x) {
 }
 
 // Clamped gated SiLU of the expert MLP: gate clamped above only, up on both
-// sides (limit <= 0 disables), act = g * sigmoid(alpha*g) * (u + beta).
+// sides (limit <= 0 disables), act = g * sigmoid(alpha*g) * (u + beta).  NaN stays
+// NaN: minimum and maximum (v_minimum3, v_maximum3) return it, fminf and fmaxf
+// would return the limit.
 __device__ __forceinline__ float silu_gate(float g, float u, float limit, float alpha,
                                            float beta) {
   if (limit > 0.f) {
-    g = fminf(g, limit);
-    u = fminf(fmaxf(u, -limit), limit);
+    g = __builtin_elementwise_minimum(g, limit);
+    u = __builtin_elementwise_minimum(__builtin_elementwise_maximum(u, -limit), limit);
   }
   return (g / (1.f + __expf(-alpha * g))) * (u + beta);
 }
