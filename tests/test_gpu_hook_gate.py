@@ -206,3 +206,40 @@ def test_layers_run_together(T):
         x.copy_(_x(T, 512, 50 + k))
         g.replay()
         _same_bits(out, net(x))
+
+
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("how", ["none given", "data", "copy", "passed", "replaced"])
+def test_sigmoid_gate_bias_selects_once(how, T):
+    """A sigmoid gate's bias is the selection's: the block with it is the
+    answer, however the layer holds it."""
+    E, H, K = 32, 512, 4
+    cls, scale = HOOKS["mxfp4"]
+    d = make_dense_layer(F.FMT_MXFP4, E, H, 256, seed=11)
+    gate, kw = _router(E, H, True, 11)
+    kw["bias"] *= 10                       # enough to change the choice
+    first = kw["bias"].flip(0).contiguous() if how == "replaced" else kw["bias"]
+    bias = torch.nn.Parameter(first.clone())
+    lay = types.SimpleNamespace(layer_name="model.layers.1.mlp.experts", w13_weight=d["w13"],
+                                w2_weight=d["w2"], top_k=K, renormalize=True, swiglu_limit=7.0,
+                                scoring_func="sigmoid", routed_scaling_factor=2.5,
+                                gate=types.SimpleNamespace(weight=gate, bias=bias))
+    lay.w13_weight_scale, lay.w2_weight_scale = d["s13"], d["s2"]
+    if how == "data":
+        lay.e_score_correction_bias = bias.data
+    elif how == "copy":
+        lay.e_score_correction_bias = bias.detach().clone()
+    hook = cls()
+    hook.process_weights_after_loading(lay)
+    if how == "replaced":
+        lay.gate.bias = torch.nn.Parameter(kw["bias"].clone())
+    more = dict(e_score_correction_bias=bias.detach().clone()) if how == "passed" else {}
+    x = _x(T, H, 12)
+    blk = MoeBlock(gate, hook._weights, top_k=K, swiglu_limit=7.0, **kw)
+    out = hook.apply(x, None, None, **more)
+    _same_bits(out, blk(x))
+    logits = linear(x, gate, out_dtype=F32)
+    if T > 16:
+        _same_bits(hook.apply(x, None, None, router_logits=logits), out)
+    twice = route(logits + kw["bias"], top_k=K, **kw)[1]
+    assert not torch.equal(twice, blk(x, return_routing=True)[2])

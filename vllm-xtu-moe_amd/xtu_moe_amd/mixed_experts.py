@@ -48,6 +48,19 @@ except Exception:  # noqa: BLE001
         SWIGLUOAI_UNINTERLEAVE = "swigluoai_uninterleave"
 
 
+def _same_storage(a, b) -> bool:
+    return (isinstance(a, torch.Tensor) and isinstance(b, torch.Tensor) and a.dtype == b.dtype
+            and a.device == b.device and a.numel() == b.numel() and a.data_ptr() == b.data_ptr())
+
+
+def _same_values(a, b) -> bool:
+    """Whether one is a copy of the other, rounded to its type or not."""
+    if not isinstance(b, torch.Tensor) or a.shape != b.shape:
+        return False
+    a, b = a.detach().cpu(), b.detach().cpu()
+    return torch.equal(a.to(b.dtype), b) or torch.equal(a, b.to(a.dtype))
+
+
 class XiaotuExperts:
     """Base hook: subclasses set the format, scale attributes and groups."""
 
@@ -69,6 +82,8 @@ class XiaotuExperts:
         self.num_expert_group = None
         self.topk_group = None
         self.e_score_correction_bias = None
+        self._bias_of_gate = None    # the layer's gate.bias, where loading took that for it
+        self._gate_bias_role = None  # of gate.bias, with sigmoid scoring: "selection", "logits"
         self.routed_scaling_factor = 1.0
         self.swiglu_limit = None
         self.swiglu_alpha = None
@@ -139,17 +154,47 @@ class XiaotuExperts:
 
     def _read_layer_attrs(self, layer) -> None:
         self._layer_ref = layer
+        if self._from_gate():   # loaded before: taken anew
+            self.e_score_correction_bias = None
+        self._bias_of_gate = None
         for name in _ROUTING_ATTRS + _SWIGLU_ATTRS + ("top_k",):
             if hasattr(layer, name):
                 setattr(self, name, getattr(layer, name))
+        gate = getattr(layer, "gate", None)
         if self.e_score_correction_bias is None:
-            gate = getattr(layer, "gate", None)
             for owner, attr in ((gate, "e_score_correction_bias"), (gate, "bias"),
                                 (getattr(layer, "router", None), "e_score_correction_bias")):
                 b = getattr(owner, attr, None) if owner is not None else None
                 if isinstance(b, torch.Tensor):
                     self.e_score_correction_bias = b
+                    self._bias_of_gate = b if attr == "bias" else None
                     break
+        # whether the gate's bias is the selection's (itself, or a copy in any
+        # type) or a term of the logits is settled here, where values can be read
+        b, c = getattr(gate, "bias", None), self.e_score_correction_bias
+        self._gate_bias_role = None
+        if isinstance(b, torch.Tensor):
+            same = self._from_gate() or _same_storage(b, c) or _same_values(b, c)
+            self._gate_bias_role = "selection" if same else "logits"
+
+    def _from_gate(self) -> bool:
+        return (self._bias_of_gate is not None
+                and self.e_score_correction_bias is self._bias_of_gate)
+
+    def _take_selection_bias(self, bias) -> None:
+        """A selection bias given with a call (None: as before)."""
+        if bias is not None and not (self._from_gate()
+                                     and _same_storage(bias, self._selection_bias())):
+            self.e_score_correction_bias = bias
+
+    def _selection_bias(self):
+        """The selection's bias; where loading found it as the layer's
+        gate.bias, the one that the gate holds now."""
+        if self._from_gate():
+            b = getattr(getattr(self._layer_ref, "gate", None), "bias", None)
+            if isinstance(b, torch.Tensor):
+                return b.detach()
+        return self.e_score_correction_bias
 
     @staticmethod
     def _find(layer, name):
@@ -174,7 +219,7 @@ class XiaotuExperts:
             raise ValueError("no topk_ids / topk_weights and no router_logits (and no gate in the "
                              "layer with bf16 rows for these hidden states)")
         if self.use_grouped_topk or str(self.scoring_func) == "sigmoid":
-            bias = self.e_score_correction_bias
+            bias = self._selection_bias()
             if bias is not None:
                 bias = bias.to(router_logits.device)
             return route(router_logits, top_k=int(self.top_k), scoring=str(self.scoring_func),
@@ -212,8 +257,7 @@ class XiaotuExperts:
             self.num_expert_group = num_expert_group
         if topk_group is not None:
             self.topk_group = topk_group
-        if e_score_correction_bias is not None:
-            self.e_score_correction_bias = e_score_correction_bias
+        self._take_selection_bias(e_score_correction_bias)
         if routed_scaling_factor is not None:
             self.routed_scaling_factor = routed_scaling_factor
         T = hidden_states.shape[0]
@@ -295,8 +339,8 @@ class XiaotuExperts:
 
     def _gate(self, x, expert_map=None):
         """(rows [experts, H], logit bias or None) of the layer's router, or
-        (None, None) without bf16 rows for x.  A gate's bias that is the
-        selection's e_score_correction_bias is no term of the logits."""
+        (None, None) without bf16 rows for x.  With sigmoid scoring a gate's
+        bias may be the selection's, and is then no term of the logits."""
         gate = getattr(self._layer_ref, "gate", None)
         w, b = getattr(gate, "weight", None), getattr(gate, "bias", None)
         if not isinstance(w, torch.Tensor) or w.dtype != torch.bfloat16 or w.dim() != 2 \
@@ -307,14 +351,20 @@ class XiaotuExperts:
                 (isinstance(b, torch.Tensor) and b.numel() != w.shape[0]):
             raise ValueError(f"the gate's {w.shape[0]} rows do not fit {E} experts or the "
                              "expert_map, or its bias does not fit the rows")
-        if not isinstance(b, torch.Tensor) or (b is self.e_score_correction_bias
-                                               and str(self.scoring_func) == "sigmoid"):
+        if not isinstance(b, torch.Tensor):
             return w.detach(), None
+        if str(self.scoring_func) == "sigmoid":
+            role = self._gate_bias_role
+            if role == "selection" or _same_storage(b, self._selection_bias()):
+                return w.detach(), None
+            if role is None:
+                raise ValueError("the gate's bias came after loading: with sigmoid scoring it may be "
+                                 "the selection's or a term of the logits (pass router_logits)")
         return w.detach(), b.detach().to(device=x.device, dtype=torch.float32).contiguous()
 
     def _selection_args(self, dev) -> dict:
         if self.use_grouped_topk or str(self.scoring_func) == "sigmoid":
-            bias = self.e_score_correction_bias
+            bias = self._selection_bias()
             if bias is not None:
                 bias = bias.to(device=dev, dtype=torch.float32).contiguous()
             return dict(scoring=str(self.scoring_func), bias=bias,
