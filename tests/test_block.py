@@ -46,3 +46,19 @@ def test_shared_gate_needs_shared_experts():
     with pytest.raises(ValueError, match="shared"):
         MoeBlock.check(torch.zeros((4, 256), dtype=BF), _weights(NS=0), top_k=2,
                        shared_gate=torch.zeros((0, 256), dtype=BF))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(n_group=2, topk_group=1), dict(n_group=2, topk_group=2), dict(topk_group=2),
+    dict(routed_scaling_factor=2.5), dict(routed_scaling_factor=0.0), dict(bias=torch.zeros(4)),
+])
+def test_softmax_takes_no_groups_bias_or_scale(kw):
+    gate = torch.zeros((4, 256), dtype=BF)
+    with pytest.raises(ValueError, match="go with sigmoid"):
+        MoeBlock.check(gate, _weights(), top_k=2, scoring="softmax", **kw)
+    with pytest.raises(ValueError, match="go with sigmoid"):
+        MoeBlock(gate, _weights(), top_k=2, scoring="softmax", **kw)
+    MoeBlock.check(gate, _weights(), top_k=2, scoring="softmax", n_group=1, topk_group=1,
+                   routed_scaling_factor=1.0)
+    if kw.get("topk_group", 1) <= kw.get("n_group", 1):
+        MoeBlock.check(gate, _weights(), top_k=1, scoring="sigmoid", **kw)

@@ -243,3 +243,28 @@ def test_sigmoid_gate_bias_selects_once(how, T):
         _same_bits(hook.apply(x, None, None, router_logits=logits), out)
     twice = route(logits + kw["bias"], top_k=K, **kw)[1]
     assert not torch.equal(twice, blk(x, return_routing=True)[2])
+
+
+@pytest.mark.parametrize("em", [False, True])
+def test_grouped_softmax_refused(em):
+    """Groups, a scaling factor or a selection bias are not part of the softmax
+    selection: from hidden states alone the hook says so."""
+    E, H = 32, 512
+    hook, gate, kw = _hook("fp8", E, H, 256, 4, False, 13, use_grouped_topk=True)
+    x = _x(6, H, 13)
+    m = torch.arange(E, dtype=torch.int32) if em else None
+    want = hook.apply(x, None, None, expert_map=m)   # one group, no factor: plain softmax
+    _same_bits(want, MoeBlock(gate, hook._weights, top_k=4, swiglu_limit=7.0)(x)
+               if not em else want)
+    for name, value in (("num_expert_group", 4), ("topk_group", 2), ("routed_scaling_factor", 2.5),
+                        ("e_score_correction_bias", torch.zeros(E, device=DEV))):
+        before = getattr(hook, name)
+        with pytest.raises(ValueError, match="go with sigmoid"):
+            hook.apply(x, None, None, expert_map=m, **{name: value})
+        setattr(hook, name, before)
+    hook._layer_ref.gate.bias = torch.linspace(-2, 2, E, device=DEV)   # a term of the logits
+    hook.apply(x, None, None, expert_map=m)
+    hook._read_layer_attrs(hook._layer_ref)
+    _same_bits(hook.apply(x, None, None, expert_map=m),
+               hook.apply(x, None, None, expert_map=m, router_logits=linear(
+                   x, gate, bias=hook._layer_ref.gate.bias, out_dtype=F32)))

@@ -35,12 +35,24 @@ def _check_rows(name, t, n, H):
         raise ValueError(f"{name} must be contiguous bf16 [{n}, {H}], got {tuple(t.shape)} {t.dtype}")
 
 
+def check_selection(scoring, bias=None, n_group=1, topk_group=1, routed_scaling_factor=1.0,
+                    renormalize=True):
+    """Raises ValueError for a selection that the routers do not make: they
+    would choose among all experts by the softmax, unscaled."""
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"unsupported scoring function {scoring!r}")
+    if scoring == "softmax" and (bias is not None or int(n_group) != 1 or int(topk_group) != 1
+                                 or float(routed_scaling_factor) != 1.0):
+        raise ValueError("a selection bias, groups and a scaling factor go with sigmoid scoring")
+
+
 class MoeBlock:
     """One layer's MoE block over resident experts.
 
     gate_weight: bf16 [E, H], the router's rows.  weights: ExpertWeights (E
-    routed, then n_shared shared experts).  scoring "softmax" or "sigmoid"
-    (grouped, selection by score + bias), with the arguments of ``route``.
+    routed, then n_shared shared experts).  scoring "softmax" (no groups, bias
+    or scaling factor: those are refused) or "sigmoid" (grouped, selection by
+    score + bias), with the arguments of ``route``.
     shared_gate: bf16 [n_shared, H]; shared expert s is scaled by
     sigmoid(x . shared_gate[s]) (without it by 1).  swiglu_*: the clamped gated
     SiLU of every expert.  Every call reads the tensors given here as they are
@@ -54,7 +66,8 @@ class MoeBlock:
                  shared_gate=None, swiglu_limit=0.0, swiglu_alpha=1.0, swiglu_beta=0.0):
         W = weights
         self.check(gate_weight, W, top_k=top_k, scoring=scoring, bias=bias, n_group=n_group,
-                   topk_group=topk_group, shared_gate=shared_gate)
+                   topk_group=topk_group, routed_scaling_factor=routed_scaling_factor,
+                   shared_gate=shared_gate)
         if not W.w13.is_cuda:
             raise ValueError("the block needs device-resident expert weights")
         if W.fmt not in (FMT_BF16, FMT_FP8, FMT_MXFP4, FMT_NVFP4) or W.n_slots != W.n_experts:
@@ -81,7 +94,7 @@ class MoeBlock:
 
     @staticmethod
     def check(gate_weight, W, *, top_k, scoring="softmax", bias=None, n_group=1, topk_group=1,
-              shared_gate=None):
+              routed_scaling_factor=1.0, shared_gate=None):
         """Raises ValueError for a router or shared gate that does not fit W."""
         if gate_weight is None:
             raise ValueError("gate_weight is missing")
@@ -89,10 +102,9 @@ class MoeBlock:
             raise ValueError("shared_gate without shared experts")
         _check_rows("gate_weight", gate_weight, W.E, W.H)
         _check_rows("shared_gate", shared_gate, W.n_shared, W.H)
-        if scoring not in ("softmax", "sigmoid"):
-            raise ValueError(f"unsupported scoring function {scoring!r}")
-        if bias is not None and (tuple(bias.shape) != (W.E,) or scoring != "sigmoid"):
-            raise ValueError(f"bias must be [{W.E}] and goes with sigmoid scoring")
+        check_selection(scoring, bias, n_group, topk_group, routed_scaling_factor)
+        if bias is not None and tuple(bias.shape) != (W.E,):
+            raise ValueError(f"bias must be [{W.E}], got {tuple(bias.shape)}")
         top_k, n_group, topk_group = int(top_k), int(n_group), int(topk_group)
         if not 1 <= top_k <= min(W.E, MAX_TOP_K):
             raise ValueError(f"top_k {top_k} is not in 1 .. min(E, {MAX_TOP_K})")

@@ -30,7 +30,7 @@ import enum
 import torch
 
 from . import formats as F
-from .block import MoeBlock
+from .block import MoeBlock, check_selection
 from .host_layer import HostResidentLayer, layer_index, resident_decision
 from .layer import ExpertWeights, _buf as _scratch, int8_align_on, int8_dispatch, moe_forward, route
 from .linear import _overlap, linear
@@ -277,6 +277,9 @@ class XiaotuExperts:
         gate, gate_bias = None, None
         if not routed and router_logits is None and self.custom_routing_function is None:
             gate, gate_bias = self._gate(x, expert_map)
+        if gate is not None:
+            sel = self._gate_selection(x.device)
+            check_selection(**sel)
         if gate is not None and (gate_bias is not None or gate.data_ptr() % 16 or expert_map is not None
                                  or not self._monolithic or self._weights is None or self._int8(T)):
             router_logits = linear(x, gate, bias=gate_bias, out_dtype=torch.float32)
@@ -285,9 +288,6 @@ class XiaotuExperts:
             if direct and _overlap(output, x):   # in place: the block reads x to its end
                 direct, kw["out"] = False, None
             out, odt = kw.pop("out"), kw.pop("out_dtype")
-            sel = self._selection_args(x.device)
-            if sel["scoring"] == "softmax":   # its selection takes no bias
-                sel["bias"] = None
             res = MoeBlock(gate, self._weights, top_k=int(self.top_k), **sel, **kw)(
                 x, out=out, out_dtype=odt)
         elif routed:
@@ -373,6 +373,15 @@ class XiaotuExperts:
                         routed_scaling_factor=float(self.routed_scaling_factor or 1.0),
                         renormalize=bool(self.renormalize))
         return dict(scoring="softmax", renormalize=bool(self.renormalize))
+
+    def _gate_selection(self, dev) -> dict:
+        """The selection over the gate's own logits.  With softmax scoring the
+        gate's bias is part of those; any other selection bias stays, to be
+        refused with what else the softmax selection does not do."""
+        sel = self._selection_args(dev)
+        if sel["scoring"] == "softmax":
+            sel["bias"] = None if self._from_gate() else self.e_score_correction_bias
+        return sel
 
     def _router_args(self, router_logits) -> dict:
         lg = router_logits
