@@ -29,10 +29,16 @@ ARGS = struct.Struct("@14PN12i4f")
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 16, 64   # the routers' limits
 
 
-def _check_rows(name, t, n, H):
-    """bf16 rows [n, H] that the kernels can read, or None."""
-    if t is not None and (t.shape != (n, H) or t.dtype != torch.bfloat16 or not t.is_contiguous()):
+def _check_rows(name, t, n, H, dev=None):
+    """Raises ValueError where t is not bf16 rows [n, H] (on dev, starting on 16
+    bytes) that the kernels can read."""
+    if t.shape != (n, H) or t.dtype is not torch.bfloat16 or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous bf16 [{n}, {H}], got {tuple(t.shape)} {t.dtype}")
+    if dev is not None:
+        if t.get_device() != dev.index:
+            _same_device(dev, **{name: t})
+        if t.data_ptr() & 15:
+            raise ValueError(f"{name} must start on 16 bytes")
 
 
 def check_selection(scoring, bias=None, n_group=1, topk_group=1, routed_scaling_factor=1.0,
@@ -73,12 +79,18 @@ class MoeBlock:
         if W.fmt not in (FMT_BF16, FMT_FP8, FMT_MXFP4, FMT_NVFP4) or W.n_slots != W.n_experts:
             raise ValueError("the block needs BF16, FP8, MXFP4 or NVFP4 planes of every expert")
         self.W, self.gate_weight, self.shared_gate, self.bias = W, gate_weight, shared_gate, bias
+        self._dev = W.device
         self.top_k, self.scoring, self.renormalize = int(top_k), scoring, bool(renormalize)
         self.n_group, self.topk_group = int(n_group), int(topk_group)
         self.routed_scaling_factor = float(routed_scaling_factor)
         self.limit = float(swiglu_limit or 0.0)
         self.alpha, self.beta = float(swiglu_alpha), float(swiglu_beta)
         self._operands()
+        # the packed planes stay where they are (held here as they lie)
+        ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+        self._held = tuple(None if t is None else t.detach()
+                           for t in (W.w13, W.s13, W.gs13, W.w2, W.s2, W.gs2))
+        self._planes = tuple(ptr(t) for t in self._held)
         self._shape = (W.H, W.I, W.E, W.n_shared, self.top_k, int(scoring == "sigmoid"),
                        self.renormalize, self.n_group, self.topk_group)
         self._floats = (self.routed_scaling_factor, self.limit, self.alpha, self.beta)
@@ -101,7 +113,8 @@ class MoeBlock:
         if shared_gate is not None and W.n_shared == 0:
             raise ValueError("shared_gate without shared experts")
         _check_rows("gate_weight", gate_weight, W.E, W.H)
-        _check_rows("shared_gate", shared_gate, W.n_shared, W.H)
+        if shared_gate is not None:
+            _check_rows("shared_gate", shared_gate, W.n_shared, W.H)
         check_selection(scoring, bias, n_group, topk_group, routed_scaling_factor)
         if bias is not None and tuple(bias.shape) != (W.E,):
             raise ValueError(f"bias must be [{W.E}], got {tuple(bias.shape)}")
@@ -120,15 +133,16 @@ class MoeBlock:
         """(gate_weight, shared_gate, bias fp32 or None) as they are now, checked
         against the layer: the kernels take their addresses."""
         W, gate, shared, bias = self.W, self.gate_weight, self.shared_gate, self.bias
-        _check_rows("gate_weight", gate, W.E, W.H)
-        _check_rows("shared_gate", shared, W.n_shared, W.H)
-        if bias is not None and bias.shape != (W.E,):
-            raise ValueError(f"bias must be [{W.E}], got {tuple(bias.shape)}")
-        _same_device(W.device, gate_weight=gate, shared_gate=shared, bias=bias)
-        if gate.data_ptr() & 15 or (shared is not None and shared.data_ptr() & 15):
-            raise ValueError("gate_weight and shared_gate must start on 16 bytes")
-        if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
-            bias = bias.to(torch.float32).contiguous()
+        _check_rows("gate_weight", gate, W.E, W.H, self._dev)
+        if shared is not None:
+            _check_rows("shared_gate", shared, W.n_shared, W.H, self._dev)
+        if bias is not None:
+            if bias.shape != (W.E,):
+                raise ValueError(f"bias must be [{W.E}], got {tuple(bias.shape)}")
+            if bias.get_device() != self._dev.index:
+                _same_device(self._dev, bias=bias)
+            if bias.dtype is not torch.float32 or not bias.is_contiguous():
+                bias = bias.to(torch.float32).contiguous()
         return gate, shared, bias
 
     def __call__(self, x, *, out=None, out_dtype=None, return_routing=False, stream=None):
@@ -143,9 +157,9 @@ class MoeBlock:
             raise ValueError(f"output type {odt} (out_dtype {out_dtype}): bf16 or fp32")
         if out is not None and (tuple(out.shape) != tuple(x.shape) or not out.is_contiguous()):
             raise ValueError(f"out must be contiguous {tuple(x.shape)}, got {tuple(out.shape)}")
-        _same_device(W.device, x=x, out=out)
-        if stream is not None or W.device.index != _current_device():
-            with on_stream(stream, W.device):
+        _same_device(self._dev, x=x, out=out)
+        if stream is not None or self._dev.index != _current_device():
+            with on_stream(stream, self._dev):
                 return self(x, out=out, out_dtype=out_dtype, return_routing=return_routing)
         if out is not None and _overlap(out, x):
             raise ValueError("out overlaps x")
@@ -172,17 +186,16 @@ class MoeBlock:
 
     def _few(self, x, out, ids, wts, need, gate, shared, bias):
         """A few tokens, in two launches."""
-        W = self.W
-        # what xtu_few_block takes of the layer, in its order
-        planes = [0 if t is None else t.data_ptr()
-                  for t in (gate, shared, bias, W.w13, W.s13, W.gs13, W.w2, W.s2, W.gs2)]
         if x.data_ptr() & 15:
             x = x.clone()
         # per call: calls on other streams, and graphs, have their own
         ws = x.new_empty(need, dtype=torch.uint8)
-        rc = self._entry(ARGS.pack(x.data_ptr(), *planes, out.data_ptr(), ids.data_ptr(),
-                                   wts.data_ptr(), ws.data_ptr(), need, W.fmt, x.shape[0],
-                                   *self._shape, out.dtype == torch.bfloat16, *self._floats),
+        rc = self._entry(ARGS.pack(x.data_ptr(), gate.data_ptr(),
+                                   0 if shared is None else shared.data_ptr(),
+                                   0 if bias is None else bias.data_ptr(), *self._planes,
+                                   out.data_ptr(), ids.data_ptr(), wts.data_ptr(), ws.data_ptr(),
+                                   need, self.W.fmt, x.shape[0], *self._shape,
+                                   out.dtype == torch.bfloat16, *self._floats),
                          raw_stream(x.device.index))
         if rc:
             _lib.check("xtu_few_block", rc)
