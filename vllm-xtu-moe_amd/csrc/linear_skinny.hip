@@ -10,9 +10,11 @@
 //
 // Few columns: a CU takes in about 25 GB/s whatever its waves ask for, so a
 // product of 256 columns by 7168 k in panels of 16 waits 14 us for 16 CUs; panels
-// of as few columns as give each CU one (the MFMA's other rows repeat the
-// panel's last row, at no further traffic) take 6.6 us.  512 gated columns by
-// 2048 k 7.8 -> 5.1 us.  Cached loads of w beat non-temporal ones here (28672
+// of fewer columns, down to two (the MFMA's other rows repeat the panel's last row,
+// at no further traffic), for about one a CU take 6.6 us: 128 panels here, half the
+// CUs.  512 gated columns by 2048 k 7.8 -> 5.1 us.  What such products wait for
+// besides is x: every workgroup brings all of it to LDS before its first MFMA (4
+// rows of 7168: 57 KB beside 28 KB of w).  Cached loads of w beat non-temporal ones here (28672
 // columns by 7168 k 73 us = 5.65 TB/s against 91).
 #include "linear.hpp"
 
