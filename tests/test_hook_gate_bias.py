@@ -139,3 +139,14 @@ def test_bias_set_on_the_hook():
     hook.e_score_correction_bias = _param(16).detach()
     logit, sel = _terms(hook)
     assert logit is None and torch.equal(sel, _param(16).detach())
+
+
+def test_biases_of_zeros_say_nothing():
+    """Two tensors of zeros may be a bias and its copy or two biases that are
+    filled later: refused with sigmoid scoring, unless they share storage."""
+    b = torch.nn.Parameter(torch.zeros(E))
+    with pytest.raises(ValueError, match="gate's bias"):
+        _terms(_hook(_layer(b, e_score_correction_bias=torch.zeros(E))))
+    for c in (b, b.data):
+        assert _terms(_hook(_layer(b, e_score_correction_bias=c)))[0] is None
+    assert _terms(_hook(_layer(b)))[0] is None

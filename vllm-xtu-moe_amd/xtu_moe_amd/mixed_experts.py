@@ -83,7 +83,7 @@ class XiaotuExperts:
         self.topk_group = None
         self.e_score_correction_bias = None
         self._bias_of_gate = None    # the layer's gate.bias, where loading took that for it
-        self._gate_bias_role = None  # of gate.bias, with sigmoid scoring: "selection", "logits"
+        self._gate_bias_role = None  # of gate.bias with sigmoid scoring, where loading could tell
         self.routed_scaling_factor = 1.0
         self.swiglu_limit = None
         self.swiglu_alpha = None
@@ -174,8 +174,12 @@ class XiaotuExperts:
         b, c = getattr(gate, "bias", None), self.e_score_correction_bias
         self._gate_bias_role = None
         if isinstance(b, torch.Tensor):
-            same = self._from_gate() or _same_storage(b, c) or _same_values(b, c)
-            self._gate_bias_role = "selection" if same else "logits"
+            if self._from_gate() or _same_storage(b, c):
+                self._gate_bias_role = "selection"
+            elif not _same_values(b, c):
+                self._gate_bias_role = "logits"
+            elif bool(b.detach().any()):   # (zeros may both be filled later)
+                self._gate_bias_role = "selection"
 
     def _from_gate(self) -> bool:
         return (self._bias_of_gate is not None
@@ -358,8 +362,9 @@ class XiaotuExperts:
             if role == "selection" or _same_storage(b, self._selection_bias()):
                 return w.detach(), None
             if role is None:
-                raise ValueError("the gate's bias came after loading: with sigmoid scoring it may be "
-                                 "the selection's or a term of the logits (pass router_logits)")
+                raise ValueError("the gate's bias came after loading, or was zeros as the "
+                                 "selection's: with sigmoid scoring it may be the selection's or a "
+                                 "term of the logits (pass router_logits)")
         return w.detach(), b.detach().to(device=x.device, dtype=torch.float32).contiguous()
 
     def _selection_args(self, dev) -> dict:
