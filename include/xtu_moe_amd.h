@@ -634,6 +634,49 @@ size_t xtu_linear_workspace_bytes(int M, int N, int K, int act, int aligned);
  * rows, else 256 * (K splits) + 1 + its tile (an index of kTileKinds), -1 none. */
 int xtu_linear_plan(int M, int N, int K, int act);
 
+/* ------------------------------------------------ router, training step
+ * What a training step takes from router logits [T][E] (fp32, or bf16 with
+ * logits_bf16; rows ld elements apart) and the selected ids int32 [T][K] (an id
+ * outside 0 .. E - 1: no expert): per sequence q, rows starts[q] .. starts[q + 1]
+ * (int32 [S + 1], ascending, clamped to 0 .. T; other rows belong to none; NULL
+ * with S = 1: all rows), the
+ * counts int32 [S][E] of selections and the mean probabilities fp32 [S][E]; the
+ * balance loss, mean over non-empty sequences of E / (K n) sum_e count P; for
+ * mode 0 (softmax) z, the mean of logsumexp^2 over the sequences' rows (mode 1,
+ * sigmoid scores over their sum: z is NULL); weights fp32 [T][K] of the selected
+ * experts: their probabilities (mode 1: sigmoid scores), over their sum with
+ * renormalize, times scale; 0 for no expert.  stat fp32 [T][2] and norm fp32 [2]
+ * are for xtu_router_grad, which writes the logits' gradient [T][E] (their type,
+ * contiguous, 16-byte aligned) from those of weights [T][K], balance and z (fp32 on the
+ * device; each may be NULL: 0).  E <= 1024, K <= 16.  A row of -inf has
+ * probability 0 everywhere and no gradient.  The workspace
+ * (xtu_router_workspace_bytes, 16-byte aligned) carries nothing from call to
+ * call; calls that may overlap each need their own.  The same call gives the same
+ * bits.  The reference trains nothing (its router: vllm_xiaotu_moe/
+ * hybrid_model.py:1877). */
+typedef struct xtu_router_args {
+  const void* logits;
+  const int32_t* ids;
+  const int32_t* starts;
+  float* weights;
+  float* stat;
+  int32_t* counts;
+  float* probs;
+  float* balance;
+  float* z;
+  float* norm;
+  void* workspace;
+  long ld;
+  size_t workspace_bytes;
+  int T, E, K, S, mode, renormalize, logits_bf16;
+  float scale;
+} xtu_router_args;
+size_t xtu_router_workspace_bytes(int T, int E, int S);
+hipError_t xtu_router_losses(const xtu_router_args* args, hipStream_t stream);
+hipError_t xtu_router_grad(const xtu_router_args* args, const float* g_weights,
+                           const float* g_balance, const float* g_z, void* dlogits,
+                           hipStream_t stream);
+
 /* ------------------------------------------------ MoE block of a few tokens
  * From hidden states x bf16 [T][H] to the layer's output, in two launches:
  * router product with gate bf16 [E][H], selection (mode 0 softmax, 1 grouped

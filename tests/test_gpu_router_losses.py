@@ -1,0 +1,344 @@
+"""The router's losses, counts, weights and their gradient against float64.
+
+Tolerances, derived before the first run.  u = 2^-24 is fp32's rounding.  An
+exponential's argument l - m is off by |l - m| u and the exponential by a few u
+itself, a row's sum of non-negative terms by at most 26 u (16 in a lane, six
+joins, the rest for the division), so a probability or score is off by
+R = (|l - m| + 40) u relative, with |l - m| up to D, the largest spread of a row.
+A mean of p over rows adds at most (rows of a lane + 64) u <= 2^-17 relative
+(the rest is in fp64), so P and the balance loss are off by R + 2^-17 relative (all terms
+are non-negative).  lse is off by (|m| + log E + 40) u, z by 2 |lse| of that, plus its
+sums.  A gradient's terms p (h_j - sum p h + z' - c) and w (g_k - sum w g) are
+each off by 2 R + 16 u of the sum of their terms' magnitudes; 1 - s <= 1
+multiplies them.  bf16 outputs: 2^-8 more.
+"""
+import pytest
+import torch
+
+from xtu_moe_amd.layer import route
+from xtu_moe_amd.router import router_losses
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+U = 2.0 ** -24
+
+
+def _inputs(T, E, K, seed=0, dtype=F32, std=1.5, drop=0.0):
+    g = torch.Generator().manual_seed(seed)
+    lg = (torch.randn((T, E), generator=g) * std).to(dtype)
+    ids = torch.rand((T, E), generator=g).argsort(1)[:, :K].to(torch.int32)
+    if drop:
+        ids = torch.where(torch.rand((T, K), generator=g) < drop, -1, ids)
+    gw = torch.randn((T, K), generator=g)
+    return lg.to(DEV), ids.contiguous().to(DEV), gw.to(DEV)
+
+
+def _formula(lg, ids, starts, scoring, renorm, f, gw, gb, gz):
+    """Everything in 64 bits, the gradient written out; with the magnitudes that
+    its terms have."""
+    lg, ids = lg.double(), ids.long()
+    T, E = lg.shape
+    K = ids.shape[1]
+    soft = scoring == "softmax"
+    m = lg.amax(1, keepdim=True) if T else lg[:, :1]
+    m = torch.where(m == -float("inf"), torch.zeros_like(m), m)
+    if soft:
+        s = torch.exp(lg - m)
+        rest = torch.ones_like(s)
+    else:
+        s, rest = torch.sigmoid(lg), torch.sigmoid(-lg)
+    tot = s.sum(1, keepdim=True)
+    p = torch.where(tot > 0, s / tot, torch.zeros_like(s))
+    lse = torch.where(tot > 0, m + torch.log(tot), torch.zeros_like(m))[:, 0]
+    ok = (ids >= 0) & (ids < E)
+    at = torch.where(ok, ids, torch.zeros_like(ids))
+    sel = (p if soft else s).gather(1, at) * ok
+    u = sel
+    if renorm:
+        n = sel.sum(1, keepdim=True)
+        u = torch.where(n > 0, sel / n, torch.zeros_like(sel))
+    w = f * u
+    S = len(starts) - 1
+    counts = torch.zeros((S, E), dtype=torch.int32, device=lg.device)
+    P = torch.zeros((S, E), dtype=F64, device=lg.device)
+    h = torch.zeros_like(lg)
+    used = torch.zeros(T, dtype=torch.bool, device=lg.device)
+    losses = []
+    Q = sum(b > a for a, b in zip(starts[:-1], starts[1:]))
+    for q, (a, b) in enumerate(zip(starts[:-1], starts[1:])):
+        if b == a:
+            continue
+        x = ids[a:b][ok[a:b]]
+        counts[q] = torch.bincount(x, minlength=E).int()
+        P[q] = p[a:b].sum(0) / (b - a)
+        losses.append((counts[q].double() * P[q]).sum() * E / (K * (b - a)))
+        h[a:b] = gb * E * counts[q].double() / (K * (b - a) ** 2 * Q)
+        used[a:b] = True
+    balance = torch.stack(losses).mean() if losses else torch.zeros((), dtype=F64, device=lg.device)
+    n = max(int(used.sum()), 1)
+    z = (lse[used] ** 2).sum() / n
+    zt = torch.where(used, 2 * gz * lse / n, torch.zeros_like(lse))[:, None] if soft \
+        else torch.zeros((T, 1), dtype=F64, device=lg.device)
+    hp = (p * h).sum(1, keepdim=True)
+    gw = gw.double() * ok
+    wg, wga = (w * gw).sum(1, keepdim=True), (w * gw.abs()).sum(1, keepdim=True)
+    c = wg if soft and not renorm else torch.zeros_like(wg)
+    ca = wga if soft and not renorm else torch.zeros_like(wg)
+    term = w * (gw - (wg / f if renorm else 0))
+    terma = w * (gw.abs() + (wga / f if renorm else 0))
+    d = p * (h - hp + zt - c)
+    da = p * (h.abs() + hp.abs() + zt.abs() + ca)
+    d = rest * d.scatter_add(1, at, term * ok)
+    da = da.scatter_add(1, at, terma * ok)
+    return dict(weights=w, balance=balance, z=z, counts=counts, probs=P, d=d, da=da, lse=lse,
+                used=used)
+
+
+def _check(lg, ids, gw, starts=None, scoring="softmax", renorm=True, f=1.0, gb=0.7, gz=0.3,
+           what=""):
+    T, E = lg.shape
+    lg = lg.detach().requires_grad_(True)
+    dev = None if starts is None else torch.tensor(starts, dtype=torch.int32, device=DEV)
+    r = router_losses(lg, ids, scoring=scoring, renormalize=renorm, routed_scaling_factor=f,
+                      seq_starts=dev)
+    outs = [r.weights, r.balance] + ([r.z] if r.z is not None else [])
+    gs = [gw, torch.full((), gb, device=DEV), torch.full((), gz, device=DEV)][:len(outs)]
+    d, = torch.autograd.grad(outs, lg, gs)
+    clamped = [min(max(v, 0), T) for v in (starts or [0, T])]
+    e = _formula(lg.detach(), ids, clamped, scoring, renorm, f, gw, gb,
+                 gz if scoring == "softmax" else 0.0)
+    l64 = lg.detach().double()
+    fin = torch.where(torch.isfinite(l64), l64, torch.zeros_like(l64))
+    D = float((fin.amax(1) - fin.amin(1)).max()) if T else 0.0
+    R = (D + 40) * U
+
+    def near(name, got, want, tol):
+        got = got.detach().double()
+        assert got.shape == want.shape, name
+        bad = ~((got - want).abs() <= tol)
+        assert not bool(bad.any()), (what, name, int(bad.sum()),
+                                     float((got - want).abs()[bad].max()))
+
+    assert torch.equal(r.counts, e["counts"]), what
+    assert r.weights.dtype == r.balance.dtype == r.probs.dtype == F32 and d.dtype == lg.dtype
+    near("weights", r.weights, e["weights"], e["weights"] * (2 * R + 4 * U) + 2.0 ** -140)
+    near("probs", r.probs, e["probs"], e["probs"] * (R + 2.0 ** -17) + 2.0 ** -140)
+    near("balance", r.balance, e["balance"], e["balance"] * (R + 2.0 ** -17))
+    if scoring == "softmax":
+        dl = (fin.abs().max() if T else 0.0) + 47.0
+        near("z", r.z, e["z"], 2 * e["lse"][e["used"]].abs().mean() * dl * U + e["z"] * 2.0 ** -17
+             + 2.0 ** -40 if bool(e["used"].any()) else torch.zeros((), dtype=F64, device=DEV))
+    else:
+        assert r.z is None
+    tol = e["da"] * (2 * R + 16 * U) + 2.0 ** -140
+    near("gradient", d, e["d"], tol + (e["d"].abs() + tol) * (2.0 ** -8 if d.dtype == BF else U))
+    return r, d
+
+
+SHAPES = [   # T, E, K
+    (1, 1, 1), (1, 8, 2), (2, 3, 3), (5, 8, 8), (63, 16, 4), (64, 17, 16), (65, 32, 1), (7, 33, 5),
+    (130, 60, 4), (257, 64, 6), (100, 72, 3), (33, 128, 8), (511, 130, 8), (77, 160, 6),
+    (129, 256, 8), (40, 257, 8), (301, 384, 16), (66, 512, 10), (35, 513, 9), (19, 1000, 7),
+    (50, 1024, 16), (2049, 64, 8), (5003, 128, 8),
+]
+
+
+@pytest.mark.parametrize("scoring,renorm,f", [("softmax", True, 1.0), ("softmax", False, 1.0),
+                                              ("sigmoid", True, 2.5), ("sigmoid", False, 0.5)])
+def test_shapes(scoring, renorm, f):
+    for T, E, K in SHAPES:
+        for dtype in (F32, BF):
+            lg, ids, gw = _inputs(T, E, K, seed=T + E, dtype=dtype, drop=0.1 if T % 2 else 0.0)
+            _check(lg, ids, gw, None, scoring, renorm, f, what=(T, E, K, dtype))
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_sequences(scoring):
+    """Empty ones, one row long, behind and before the rows that none holds."""
+    for T, E, K, starts in [
+        (10, 8, 2, [0, 10]), (10, 8, 2, [0, 0, 10, 10]), (10, 8, 2, [0, 0, 0]), (10, 8, 2, [3, 7]),
+        (10, 8, 2, [2, 2, 5, 5, 5, 9]), (300, 64, 4, list(range(0, 301))),
+        (300, 64, 4, list(range(0, 300, 7))), (777, 256, 8, [0, 1, 300, 300, 555, 700]),
+        (2500, 512, 10, [0, 900, 901, 2400]), (1200, 1024, 4, [5, 600, 1100]),
+        (10, 8, 2, [0, 4, 40]), (10, 8, 2, [-3, 4, 9]), (0, 8, 2, [0, 0]),
+        (4096, 16, 2, [0, 1000, 1001, 4000]), (70, 20, 2, [69, 70]),
+    ]:
+        lg, ids, gw = _inputs(T, E, K, seed=T)
+        _check(lg, ids, gw, starts, scoring, what=(T, E, starts[:8]))
+
+
+def test_no_rows():
+    lg, ids, gw = _inputs(0, 64, 4)
+    r, d = _check(lg, ids, gw)
+    assert r.balance.item() == 0.0 and r.z.item() == 0.0 and not r.counts.any() and d.shape == (0, 64)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_masked_experts_and_empty_rows(scoring, renorm):
+    """-inf and the type's lowest value in places, whole rows of -inf, rows without
+    an expert, the same expert twice, far logits."""
+    lowest = torch.finfo(F32).min
+    for E, K in ((8, 2), (60, 4), (256, 8), (700, 12)):
+        lg, ids, gw = _inputs(90, E, K, seed=E)
+        lg[:, E // 2] = -float("inf")
+        lg[3:9] = -float("inf")
+        ids[20:25] = -1
+        ids[25, 0] = E
+        ids[26, -1] = 2 ** 31 - 1
+        ids[27, :] = ids[27, :1]
+        ids[28, -1] = -2 ** 31
+        _check(lg, ids, gw, [0, 40, 90], scoring, renorm, what=E)
+        low = torch.where(lg == -float("inf"), torch.full_like(lg, -80.0), lg)
+        low[40:45] = -80 + 0.25 * torch.arange(E, device=DEV) / E
+        _check(low, ids, gw, [0, 40, 90], scoring, renorm, what=E)
+        low = lg.clone()
+        low[:, E // 2] = lowest
+        low[3:9] = 1.0
+        got = router_losses(low, ids, scoring=scoring, renormalize=renorm)
+        low[low == lowest] = -float("inf")
+        want = router_losses(low, ids, scoring=scoring, renormalize=renorm)
+        assert all(x is None or bool((x == y).all()) for x, y in zip(got, want))
+
+
+def test_nan_stays_in_its_row():
+    for bad in (float("nan"), float("inf")):
+        lg, ids, gw = _inputs(40, 64, 4, seed=5)
+        lg[7, 30] = bad
+        lg.requires_grad_(True)
+        starts = torch.tensor([0, 20, 40], dtype=torch.int32, device=DEV)
+        r = router_losses(lg, ids, seq_starts=starts)
+        d, = torch.autograd.grad([r.weights], lg, [gw])
+        rows = torch.arange(40, device=DEV) != 7
+        assert r.weights[7].isnan().all() and r.weights[rows].isfinite().all()
+        assert d[7].isnan().any() and d[rows].isfinite().all()
+        assert r.balance.isnan() and r.z.isnan()
+        assert r.probs[0].isnan().any() and r.probs[1].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_strides(dtype):
+    """Rows at other strides and addresses, one row repeated, a slice of columns."""
+    for E in (8, 64, 100, 256):
+        big, ids, gw = _inputs(50, 2 * E + 3, 3, seed=E, dtype=dtype)
+        ids = ids % E
+        for view in (big[:, :E], big[:, 1:E + 1], big[:, E:2 * E], big[::2, 2:E + 2]):
+            n = view.shape[0]
+            _check(view, ids[:n].contiguous(), gw[:n].contiguous(), what=(E, view.stride()))
+    one, ids, gw = _inputs(1, 64, 3, dtype=dtype)
+    _check(one.expand(30, 64), ids.expand(30, 3).contiguous(), gw.expand(30, 3).contiguous())
+
+
+def test_weights_are_the_routers():
+    """What ``route`` gives for its own selection, up to the exponential's rounding."""
+    for E, K, kw in ((64, 6, dict()), (512, 10, dict()), (8, 2, dict(renormalize=False)),
+                     (256, 8, dict(scoring="sigmoid", routed_scaling_factor=2.5))):
+        lg, _, _ = _inputs(333, E, K, seed=E)
+        extra = dict(n_group=8, topk_group=4) if E == 256 else {}
+        w, ids = route(lg, top_k=K, **kw, **extra)
+        r = router_losses(lg, ids, **kw)
+        assert float(((r.weights - w).abs() / w).max()) <= 2.0 ** -18
+        assert int(r.counts.sum()) == 333 * K
+
+
+def test_single_gradients():
+    """Each output's gradient alone is its part of the whole."""
+    lg, ids, gw = _inputs(70, 60, 4, seed=2)
+    one = torch.ones((), device=DEV)
+    lg.requires_grad_(True)
+    r = router_losses(lg, ids)
+    parts = [torch.autograd.grad(o, lg, g, retain_graph=True)[0]
+             for o, g in ((r.weights, gw), (r.balance, one), (r.z, one))]
+    whole, = torch.autograd.grad([r.weights, r.balance, r.z], lg, [gw, one, one])
+    scale = sum(p.abs() for p in parts)
+    assert bool(((sum(parts) - whole).abs() <= 16 * U * scale + 2.0 ** -140).all())
+    assert not r.counts.requires_grad and not r.probs.requires_grad
+    with torch.no_grad():
+        assert not router_losses(lg, ids).balance.requires_grad
+
+
+@pytest.mark.parametrize("scoring,renorm", [("softmax", True), ("softmax", False),
+                                            ("sigmoid", True), ("sigmoid", False)])
+def test_gradient_against_differences(scoring, renorm):
+    """Along random directions v of unit length: (F(l + h v) - F(l - h v)) / 2h is off
+    by h^2 / 6 times a third derivative and by F's rounding over h.  F = sum of
+    weights' dots (|gw| <= 1), balance and z here has |F| <= F0 and third
+    derivatives along v below 30 F0 (softmax and sigmoid have them below 6 per
+    factor, z's square included); F's parts are off by 2^-16 F0."""
+    lg, ids, gw = _inputs(24, 16, 3, seed=9)
+    gw = gw.clamp(-1, 1)
+    lg.requires_grad_(True)
+
+    def F(x):
+        r = router_losses(x, ids, scoring=scoring, renormalize=renorm)
+        out = (r.weights.double() * gw.double()).sum() + r.balance.double()
+        return out if r.z is None else out + r.z.double()
+
+    r = router_losses(lg, ids, scoring=scoring, renormalize=renorm)
+    outs = [r.weights, r.balance] + ([] if r.z is None else [r.z])
+    one = torch.ones((), device=DEV)
+    d, = torch.autograd.grad(outs, lg, [gw] + [one] * (len(outs) - 1))
+    F0 = float((r.weights.sum() + r.balance + (0 if r.z is None else r.z)).detach())
+    h = 2.0 ** -4
+    g = torch.Generator().manual_seed(1)
+    with torch.no_grad():
+        for _ in range(8):
+            v = torch.randn(lg.shape, generator=g).to(DEV)
+            v = v / v.norm()
+            diff = float((F(lg + h * v) - F(lg - h * v)) / (2 * h))
+            assert abs(diff - float((d.double() * v.double()).sum())) <= \
+                F0 * (5 * h * h + 2.0 ** -16 / h)
+
+
+def test_same_bits_and_other_streams():
+    lg, ids, gw = _inputs(3000, 256, 8, seed=3)
+    lg.requires_grad_(True)
+    starts = torch.tensor([0, 700, 2900], dtype=torch.int32, device=DEV)
+
+    def step(stream=None):
+        r = router_losses(lg, ids, seq_starts=starts, stream=stream)
+        d, = torch.autograd.grad([r.weights, r.balance, r.z], lg,
+                                 [gw, torch.ones((), device=DEV), torch.ones((), device=DEV)])
+        return (*r, d)
+
+    first = step()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        here, there = step(), step(side)
+        torch.cuda.synchronize()
+        for x, y, z in zip(first, here, there):
+            assert torch.equal(x, y) and torch.equal(x, z)
+
+
+def test_graph():
+    """Captured forward and backward, replayed between eager steps, with new inputs."""
+    lg, ids, gw = _inputs(600, 128, 8, seed=4)
+    one = torch.ones((), device=DEV)
+
+    def step(x):
+        x = x.detach().requires_grad_(True)
+        r = router_losses(x, ids)
+        d, = torch.autograd.grad([r.weights, r.balance, r.z], x, [gw, one, one])
+        return r.weights, r.balance, r.z, r.counts, d
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(lg)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(lg)
+    for seed in range(4):
+        new = _inputs(600, 128, 8, seed=10 + seed)
+        lg.copy_(new[0])
+        ids.copy_(new[1])
+        want = [t.detach().clone() for t in step(lg)]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(out, want):
+            assert torch.equal(x, y)

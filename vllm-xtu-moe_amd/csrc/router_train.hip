@@ -1,0 +1,669 @@
+// The router's losses, counts and weights of a training step, and their
+// gradient in the logits.
+//
+//   softmax: p = softmax(l)                sigmoid: s = sigmoid(l), p = s / sum s
+//   sequence q of n tokens: c_e = #{(t, k): ids = e},  P_e = mean_t p_te,
+//     L_q = E / (K n) sum_e c_e P_e;  balance = mean of L_q over non-empty ones
+//   z = mean over the sequences' tokens of (logsumexp l)^2          (softmax)
+//   w_k = f u_k, u the selected p (sigmoid: s), over their sum if renormalised
+//
+// Forward: one pass over the logits.  A token belongs to L lanes, each with V of
+// its experts in registers (L V >= E), a wave takes 64 / L tokens at a time, and
+// each lane keeps the sums of its experts over the tokens that it sees, so a
+// workgroup writes one row of sums per chunk of tokens and sequence
+// (router_stats_kernel).  A second launch adds the rows in their order
+// (router_finish_kernel): no floating-point atomics, the same bits every time.
+// Backward: one pass, logits and the selected experts' gradients in, the logits'
+// gradient out (router_grad_kernel); a row's maximum and sum come from the forward.
+//
+// A row of -inf has p = 0, no z and no gradient.  NaN and +inf give NaN.
+#include <type_traits>
+
+#include "xtu_common.hpp"
+
+#include "../../include/xtu_moe_amd.h"
+
+namespace xtu {
+namespace rt {
+namespace {
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kMaxE = 1024, kMaxK = 16;
+constexpr int kCols = 16;          // experts of a workgroup of the second launch
+constexpr int kMaxChunks = 512;    // workgroups of the first launch: two a CU
+
+struct Rows {
+  const void* logits;   // [T][E], rows ld apart
+  long ld;
+  int bf16, vec;        // vec: rows start on 4 elements, E % 4 == 0
+  const int32_t* ids;   // [T][K]
+  const int32_t* starts;   // [S + 1], or null: all rows are one sequence
+  int T, E, K, S, sigmoid, renorm;
+  float scale;
+};
+
+// e^x for x <= 0 (or NaN): 2^(x log2 e) with the product's rounding made good,
+// 2^-22 relative; the unit's exp alone is off by |x| 2^-24 more.
+__device__ __forceinline__ float exp_neg(float x) {
+  x = __builtin_elementwise_maximum(x, -150.f);   // -inf: 0 below; NaN stays
+  const float t = x * 1.44269502f;
+  float r = __builtin_fmaf(x, 1.44269502f, -t);
+  r = __builtin_fmaf(x, 1.92596303e-8f, r);
+  const float e = __builtin_amdgcn_exp2f(t);
+  return __builtin_fmaf(e, r * 0.693147182f, e);
+}
+
+// Reductions over the L lanes of a token.
+template <int L>
+__device__ __forceinline__ float sum_over(float v) {
+#pragma unroll
+  for (int d = 1; d < L; d *= 2) v += __shfl_xor(v, d, 64);
+  return v;
+}
+
+template <int L>
+__device__ __forceinline__ float max_over(float v) {
+#pragma unroll
+  for (int d = 1; d < L; d *= 2) v = fmaxf(v, __shfl_xor(v, d, 64));
+  return v;
+}
+
+__device__ __forceinline__ void lds_order() {
+  __builtin_amdgcn_wave_barrier();
+  __asm__ __volatile__("" ::: "memory");
+}
+
+// A lane's V logits of row t: experts 4 (i + L v) .. + 3; -inf past E.
+template <int L, int V>
+struct Raw {
+  u32x4_t r[V / 4];
+};
+
+template <int L, int V>
+__device__ __forceinline__ void load_row(const Rows& a, long t, int i, Raw<L, V>& raw) {
+  if (a.vec) {
+#pragma unroll
+    for (int v = 0; v < V / 4; ++v) {
+      const int c = 4 * (i + L * v);
+      if (c >= a.E) {
+        raw.r[v] = a.bf16 ? u32x4_t{0xff80ff80u, 0xff80ff80u, 0u, 0u}
+                          : u32x4_t{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u};
+      } else if (a.bf16) {
+        const uint2 w = *reinterpret_cast<const uint2*>(
+            reinterpret_cast<const uint16_t*>(a.logits) + t * a.ld + c);
+        raw.r[v] = u32x4_t{w.x, w.y, 0u, 0u};
+      } else {
+        raw.r[v] = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const float*>(a.logits) +
+                                                     t * a.ld + c);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int v = 0; v < V / 4; ++v) {
+    raw.r[v] = u32x4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = 4 * (i + L * v) + e;
+      if (a.bf16) {
+        const uint32_t x = c < a.E ? reinterpret_cast<const uint16_t*>(a.logits)[t * a.ld + c]
+                                   : 0xff80u;
+        raw.r[v][e / 2] |= x << (16 * (e % 2));
+      } else {
+        raw.r[v][e] = c < a.E ? reinterpret_cast<const uint32_t*>(a.logits)[t * a.ld + c]
+                              : 0xff800000u;
+      }
+    }
+  }
+}
+
+template <int L, int V>
+__device__ __forceinline__ void values(const Rows& a, const Raw<L, V>& raw, float (&l)[V]) {
+#pragma unroll
+  for (int v = 0; v < V / 4; ++v)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (a.bf16) {
+        const uint32_t w = raw.r[v][e / 2];
+        l[4 * v + e] = __uint_as_float(e % 2 ? w & 0xffff0000u : w << 16);
+      } else {
+        l[4 * v + e] = __uint_as_float(raw.r[v][e]);
+      }
+    }
+}
+
+// The score of a logit before its row's sum divides it.  softmax: e^(l - m), m the
+// row's maximum.  sigmoid: sigmoid(l) e^-m with m = min(maximum, 0), so that a row
+// of very negative logits keeps its ratios; sigmoid(l) = score e^m.
+template <bool SIG>
+__device__ __forceinline__ float score(float l, float m) {
+  if constexpr (!SIG) return exp_neg(l - m);
+  const float e = exp_neg(-fabsf(l));
+  float num = l >= 0.f ? 1.f : e;
+  if (m < 0.f) num = exp_neg(l - m);
+  return num / (1.f + e);
+}
+
+// 1 - sigmoid(l), without the cancellation.
+__device__ __forceinline__ float one_minus_sigmoid(float l) {
+  const float e = exp_neg(-fabsf(l));
+  return (l >= 0.f ? e : 1.f) / (1.f + e);
+}
+
+__device__ __forceinline__ int start_of(const Rows& a, int q) {
+  return a.starts ? a.starts[q] : q ? a.T : 0;
+}
+
+// First sequence whose end lies behind row t (S: none), over ends clamped to T.
+__device__ __forceinline__ int seq_of(const Rows& a, int t) {
+  int lo = 0, hi = a.S;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (min(start_of(a, mid + 1), a.T) > t) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+// Rows [begin, end) of sequence q, inside [0, T].
+__device__ __forceinline__ void seq_rows(const Rows& a, int q, int& begin, int& end) {
+  begin = min(max(start_of(a, q), 0), a.T);
+  end = min(max(start_of(a, q + 1), begin), a.T);
+}
+
+// Chunk g holds rows [g C, (g + 1) C).  Its part of sequence q writes row g + q
+// of the partial sums: both grow along the rows, so no two parts share one.
+template <int L, int V, bool SIG>
+__global__ __launch_bounds__(kThreads) void router_stats_kernel(
+    Rows a, int C, float* weights, float2* stat, float* part_p, int32_t* part_c, float* part_z,
+    unsigned* ticket) {
+  constexpr int G = 64 / L, NG = kWaves * G, COLS = L * V;
+  __shared__ __attribute__((aligned(16))) float buf[NG][COLS];   // a token's scores; then sums
+  __shared__ int32_t hist[COLS];
+  __shared__ float zs[NG];
+  const int tid = threadIdx.x, lane = tid % 64, w = tid / 64;
+  const int i = lane % L, g = w * G + lane / L;
+  if (blockIdx.x == 0 && tid == 0) *ticket = 0;   // of the next launch
+  const int c0 = blockIdx.x * C, c1 = min(c0 + C, a.T);
+  for (int c = tid; c < COLS; c += kThreads) hist[c] = 0;
+  int q = seq_of(a, c0);
+  int at = c0;   // rows before are done
+  while (at < c1) {
+    // rows [at, end) are sequence q's, or no one's (q == S, or before its start)
+    int end = c1;
+    bool in = false;
+    if (q < a.S) {
+      int b, e;
+      seq_rows(a, q, b, e);
+      in = at >= b;
+      end = min(c1, in ? e : b);
+      if (end <= at) {   // an empty sequence (or starts that do not ascend)
+        ++q;
+        continue;
+      }
+    }
+    __syncthreads();   // hist is zero, buf free
+    float acc[V], z = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = 0.f;
+    Raw<L, V> next;
+    int t = at + g;
+    if (t < end) load_row(a, t, i, next);
+    for (int t0 = at; t0 < end; t0 += NG, t += NG) {   // every lane of a wave takes each turn
+      const bool on = t < end;
+      float l[V];
+      values(a, next, l);
+      if (t + NG < end) load_row(a, t + NG, i, next);
+      float m = l[0];
+#pragma unroll
+      for (int v = 1; v < V; ++v) m = fmaxf(m, l[v]);
+      m = max_over<L>(m);
+      if (m == -INFINITY) m = 0.f;
+      if (SIG) m = fminf(m, 0.f);
+      float s = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        l[v] = score<SIG>(l[v], m);
+        s += l[v];
+      }
+      s = sum_over<L>(s);
+      const float inv = s == 0.f ? 0.f : 1.f / s;
+      lds_order();
+#pragma unroll
+      for (int v = 0; v < V / 4; ++v)
+        *reinterpret_cast<f32x4_t*>(&buf[g][4 * (i + L * v)]) =
+            f32x4_t{l[4 * v], l[4 * v + 1], l[4 * v + 2], l[4 * v + 3]};
+      lds_order();
+      if (on) {
+        if (in) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) acc[v] = __builtin_fmaf(l[v], inv, acc[v]);
+          if (!SIG && s != 0.f) {
+            const float lse = m + logf(s);
+            z = __builtin_fmaf(lse, lse, z);
+          }
+        }
+        if (i == 0) stat[t] = make_float2(m, inv);
+      }
+      // the selected experts: lanes 0 .. K - 1 of the token, L at a time
+      float total = 0.f;
+      if (a.renorm) {
+        for (int k = i; k < a.K; k += L) {
+          const int e = on ? a.ids[(long)t * a.K + k] : -1;
+          if ((unsigned)e < (unsigned)a.E) total += buf[g][e];
+        }
+        total = sum_over<L>(total);
+      }
+      float f = a.renorm ? (total == 0.f ? 0.f : a.scale / total)
+                         : a.scale * (SIG ? exp_neg(m) : inv);
+      if (!SIG && s != s) f = s;   // a probability of such a row is NaN, whoever is selected
+      for (int k = i; k < a.K; k += L) {
+        if (!on) continue;
+        const long o = (long)t * a.K + k;
+        const int e = a.ids[o];
+        const bool there = (unsigned)e < (unsigned)a.E;
+        weights[o] = there ? buf[g][e] * f : 0.f;
+        if (there && in) atomicAdd(&hist[e], 1);
+      }
+    }
+    if (in) {
+      __syncthreads();   // the scores are read, hist is whole
+#pragma unroll
+      for (int v = 0; v < V / 4; ++v)
+        *reinterpret_cast<f32x4_t*>(&buf[g][4 * (i + L * v)]) =
+            f32x4_t{acc[4 * v], acc[4 * v + 1], acc[4 * v + 2], acc[4 * v + 3]};
+      if (i == 0) zs[g] = z;
+      __syncthreads();
+      const long slot = (long)blockIdx.x + q;
+      for (int c = tid; c < a.E; c += kThreads) {
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < NG; ++k) s += buf[k][c];
+        part_p[slot * a.E + c] = s;
+        part_c[slot * a.E + c] = hist[c];
+        hist[c] = 0;
+      }
+      if (tid == 0) {
+        float s = 0.f;
+        for (int k = 0; k < NG; ++k) s += zs[k];
+        part_z[slot] = s;
+      }
+    }
+    at = end;
+  }
+}
+
+struct Sums {
+  const float* part_p;
+  const int32_t* part_c;
+  const float* part_z;
+  double* loss;        // [S][ceil(E / 16)]
+  double* zsum;        // [S]
+  unsigned* ticket;
+  int32_t* counts;     // [S][E]
+  float* probs;        // [S][E]
+  float* balance;
+  float* z;
+  float* norm;         // [2]: non-empty sequences, their tokens
+};
+
+// A block's 256 values added to one, in a fixed order.
+__device__ __forceinline__ double block_sum(double v, double* red) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  red[tid] = v;
+  for (int d = kThreads / 2; d > 0; d /= 2) {
+    __syncthreads();
+    if (tid < d) red[tid] += red[tid + d];
+  }
+  __syncthreads();
+  return red[0];
+}
+
+// Sixteen experts of a sequence per workgroup: thread (r, c) adds every 16th
+// partial row of expert c.  The workgroup that ends last adds the losses.
+__global__ __launch_bounds__(kThreads) void router_finish_kernel(Rows a, int C, Sums o) {
+  __shared__ double red[kThreads];
+  __shared__ int32_t cnt[kThreads];
+  __shared__ bool last;
+  const int tid = threadIdx.x, nb = (a.E + kCols - 1) / kCols;
+  const int q = blockIdx.x / nb, b = blockIdx.x % nb;
+  const int e = b * kCols + tid % kCols, r = tid / kCols;
+  constexpr int R = kThreads / kCols;
+  int begin, end;
+  seq_rows(a, q, begin, end);
+  const int n = end - begin;
+  const int g0 = begin / C, g1 = n > 0 ? (end - 1) / C + 1 : g0;
+  double p = 0., z = 0.;
+  int32_t c = 0;
+  if (e < a.E) {
+#pragma unroll 4
+    for (int g = g0 + r; g < g1; g += R) {
+      const long at = ((long)g + q) * a.E + e;
+      p += o.part_p[at];
+      c += o.part_c[at];
+    }
+  }
+  if (b == 0)
+    for (int g = g0 + tid; g < g1; g += kThreads) z += o.part_z[(long)g + q];
+  red[tid] = p;
+  cnt[tid] = c;
+  __syncthreads();
+  double loss = 0.;
+  if (tid < kCols && e < a.E) {
+    for (int k = 1; k < R; ++k) {
+      p += red[k * kCols + tid];
+      c += cnt[k * kCols + tid];
+    }
+    p = n > 0 ? p / n : 0.;
+    o.probs[(long)q * a.E + e] = (float)p;
+    o.counts[(long)q * a.E + e] = c;
+    loss = n > 0 ? p * c * a.E / ((double)a.K * n) : 0.;
+  }
+  loss = block_sum(loss, red);
+  if (b == 0) z = block_sum(z, red);
+  if (tid == 0) {
+    o.loss[blockIdx.x] = loss;
+    if (b == 0) o.zsum[q] = z;
+    __threadfence();
+    last = atomicAdd(o.ticket, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();   // the others' sums, not what a cache held of them
+  double sum = 0., zz = 0., rows = 0., seqs = 0.;
+  for (long k = tid; k < (long)a.S * nb; k += kThreads) sum += __hip_atomic_load(
+      &o.loss[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int k = tid; k < a.S; k += kThreads) {
+    int x, y;
+    seq_rows(a, k, x, y);
+    zz += __hip_atomic_load(&o.zsum[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    rows += y - x;
+    seqs += y > x;
+  }
+  sum = block_sum(sum, red);
+  zz = block_sum(zz, red);
+  rows = block_sum(rows, red);
+  seqs = block_sum(seqs, red);
+  if (tid == 0) {
+    *o.balance = seqs > 0. ? (float)(sum / seqs) : 0.f;
+    if (o.z) *o.z = rows > 0. ? (float)(zz / rows) : 0.f;
+    o.norm[0] = (float)seqs;
+    o.norm[1] = (float)rows;
+  }
+}
+
+struct Grads {
+  const float2* stat;
+  const float* weights;
+  const int32_t* counts;
+  const float* norm;
+  const float* g_weights;   // [T][K] or null
+  const float* g_balance;   // one value or null
+  const float* g_z;
+  void* out;                // [T][E], the logits' type
+};
+
+// One token per L lanes again.  The selected experts' parts meet the row's
+// through LDS: lanes 0 .. K - 1 add them where their experts' owners read.
+//   softmax: d_j = p_j (h_j - sum p h + z' - sum_k g_k w_k [not renormalised]) + sel_j
+//   sigmoid: d_j = (1 - s_j) (p_j (h_j - sum p h) + sel_j)
+template <int L, int V, bool SIG>
+__global__ __launch_bounds__(kThreads) void router_grad_kernel(Rows a, int C, Grads o) {
+  constexpr int G = 64 / L, NG = kWaves * G, COLS = L * V;
+  __shared__ __attribute__((aligned(16))) float buf[NG][COLS];
+  const int tid = threadIdx.x, lane = tid % 64, w = tid / 64;
+  const int i = lane % L, g = w * G + lane / L;
+  const int c0 = blockIdx.x * C, c1 = min(c0 + C, a.T);
+#pragma unroll
+  for (int v = 0; v < V / 4; ++v)
+    *reinterpret_cast<f32x4_t*>(&buf[g][4 * (i + L * v)]) = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const float gb = o.g_balance ? *o.g_balance : 0.f;
+  const float seqs = o.norm[0], rows = o.norm[1];
+  const float gz = o.g_z && rows > 0.f ? 2.f * *o.g_z / rows : 0.f;
+  float h[V];
+  int q = -1, qb = 0, qe = 0;   // the sequence whose h is in registers, and its rows
+  Raw<L, V> next;
+  int t = c0 + g;
+  if (t < c1) load_row(a, t, i, next);
+  for (int t0 = c0; t0 < c1; t0 += NG, t += NG) {
+    const bool on = t < c1;
+    float l[V];
+    values(a, next, l);
+    if (t + NG < c1) load_row(a, t + NG, i, next);
+    if (on && (q < 0 || (t >= qe && q < a.S) )) {
+      q = seq_of(a, t);
+      if (q < a.S) seq_rows(a, q, qb, qe);
+      const bool some = q < a.S && qe > qb && gb != 0.f;
+      const float n = (float)(qe - qb);
+      const float f = some ? gb * (float)a.E / ((float)a.K * n * n * seqs) : 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int c = 4 * (i + L * (v / 4)) + v % 4;
+        h[v] = some && c < a.E ? f * (float)o.counts[(long)q * a.E + c] : 0.f;
+      }
+    }
+    const bool in = on && q < a.S && t >= qb && t < qe;
+    const float2 st = on ? o.stat[t] : make_float2(0.f, 0.f);
+    float rest[V], dot = 0.f;   // 1 - s
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (SIG) rest[v] = one_minus_sigmoid(l[v]);
+      l[v] = score<SIG>(l[v], st.x) * st.y;   // p
+      dot = __builtin_fmaf(l[v], h[v], dot);
+    }
+    dot = sum_over<L>(dot);
+    // sum_k w_k g_k
+    float wg = 0.f;
+    if (o.g_weights) {
+      for (int k = i; k < a.K; k += L) {
+        const long at = (long)t * a.K + k;
+        if (on && (unsigned)a.ids[at] < (unsigned)a.E)
+          wg = __builtin_fmaf(o.weights[at], o.g_weights[at], wg);
+      }
+      wg = sum_over<L>(wg);
+      const float mean = a.renorm ? wg / a.scale : 0.f;
+      for (int k = i; k < a.K; k += L) {
+        const long at = (long)t * a.K + k;
+        const int e = on ? a.ids[at] : -1;
+        if ((unsigned)e < (unsigned)a.E) atomicAdd(&buf[g][e], o.weights[at] * (o.g_weights[at] - mean));
+      }
+    }
+    const float lse = !SIG && in && st.y != 0.f ? st.x - logf(st.y) : 0.f;
+    const float base = (in ? -dot : 0.f) + (gz != 0.f ? gz * lse : 0.f) -
+                       (!SIG && !a.renorm ? wg : 0.f);
+    lds_order();
+#pragma unroll
+    for (int v = 0; v < V / 4; ++v) {
+      const f32x4_t sel = *reinterpret_cast<const f32x4_t*>(&buf[g][4 * (i + L * v)]);
+      f32x4_t d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int k = 4 * v + e;
+        d[e] = __builtin_fmaf(l[k], (in ? h[k] : 0.f) + base, sel[e]);
+        if (SIG) d[e] *= rest[k];
+      }
+      const int c = 4 * (i + L * v);
+      if (!on || c >= a.E) continue;
+      const long at = (long)t * a.E + c;
+      if (a.bf16) {
+        uint16_t* p = reinterpret_cast<uint16_t*>(o.out) + at;
+        if (a.E % 4 == 0) {
+          uint2 x;
+          x.x = f32_to_bf16(d[0]) | (uint32_t)f32_to_bf16(d[1]) << 16;
+          x.y = f32_to_bf16(d[2]) | (uint32_t)f32_to_bf16(d[3]) << 16;
+          *reinterpret_cast<uint2*>(p) = x;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + e < a.E) p[e] = f32_to_bf16(d[e]);
+        }
+      } else {
+        float* p = reinterpret_cast<float*>(o.out) + at;
+        if (a.E % 4 == 0) {
+          *reinterpret_cast<f32x4_t*>(p) = d;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + e < a.E) p[e] = d[e];
+        }
+      }
+    }
+    lds_order();
+    if (o.g_weights && on)
+      for (int k = i; k < a.K; k += L) {
+        const int e = a.ids[(long)t * a.K + k];
+        if ((unsigned)e < (unsigned)a.E) buf[g][e] = 0.f;
+      }
+    lds_order();
+  }
+}
+
+// Lanes of a token and its experts a lane, by E.
+struct Layout {
+  int lanes, vals;
+};
+Layout layout_of(int E) {
+  if (E <= 16) return {4, 4};
+  if (E <= 32) return {8, 4};
+  if (E <= 64) return {16, 4};
+  if (E <= 128) return {32, 4};
+  if (E <= 256) return {64, 4};
+  if (E <= 512) return {64, 8};
+  return {64, 16};
+}
+
+// Rows of a chunk: whole turns of a workgroup, about kMaxChunks chunks.
+int chunk_rows(int T, int E) {
+  const int ng = kWaves * 64 / layout_of(E).lanes;
+  const int c = T > 0 ? (int)(((long)T + kMaxChunks - 1) / kMaxChunks) : 1;
+  return (c + ng - 1) / ng * ng;
+}
+
+// The workspace: partial rows, losses, ticket.
+struct Space {
+  size_t p, c, z, loss, zsum, ticket, bytes;
+};
+Space space_of(int T, int E, int S) {
+  const int C = chunk_rows(T, E);
+  const size_t slots = ((size_t)T + C - 1) / C + S, nb = (E + kCols - 1) / kCols;
+  const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  Space s;
+  s.p = 0;
+  s.c = s.p + up(slots * E * 4);
+  s.z = s.c + up(slots * E * 4);
+  s.loss = s.z + up(slots * 4);
+  s.zsum = s.loss + up((size_t)S * nb * 8);
+  s.ticket = s.zsum + up((size_t)S * 8);
+  s.bytes = s.ticket + 256;
+  return s;
+}
+
+template <bool SIG, class F>
+hipError_t by_layout(int E, F f) {
+  switch (layout_of(E).lanes * 100 + layout_of(E).vals) {
+    case 404: return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+    case 804: return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
+    case 1604: return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
+    case 3204: return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
+    case 6404: return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+    case 6408: return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
+    default: return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 16>{});
+  }
+}
+
+bool rows_of(const xtu_router_args& t, Rows& a) {
+  if (t.T < 0 || t.T > (1 << 30) || t.E < 1 || t.E > kMaxE || t.K < 1 || t.K > kMaxK ||
+      t.S < 1 || t.S > (1 << 24) || t.mode < 0 || t.mode > 1 || !(t.scale > 0.f) ||
+      !(t.scale < INFINITY))
+    return false;
+  if ((long)t.S * ((t.E + kCols - 1) / kCols) * kThreads >= (1L << 32)) return false;   // the grid
+  if (t.T > 0 && (!t.logits || !t.ids || t.ld < 0)) return false;
+  if (!t.starts && t.S != 1) return false;
+  const size_t size = t.logits_bf16 ? 2 : 4;
+  a = Rows{t.logits, t.ld, t.logits_bf16, 0, t.ids, t.starts, t.T, t.E, t.K, t.S, t.mode,
+           t.renormalize, t.scale};
+  if (reinterpret_cast<uintptr_t>(t.logits) % size || reinterpret_cast<uintptr_t>(t.ids) % 4 ||
+      reinterpret_cast<uintptr_t>(t.starts) % 4)
+    return false;
+  a.vec = t.E % 4 == 0 && (t.T <= 1 || t.ld % 4 == 0) &&
+          reinterpret_cast<uintptr_t>(t.logits) % (4 * size) == 0;
+  return true;
+}
+
+}  // namespace
+}  // namespace rt
+}  // namespace xtu
+
+using namespace xtu;
+using namespace xtu::rt;
+
+extern "C" {
+
+size_t xtu_router_workspace_bytes(int T, int E, int S) {
+  if (T < 0 || T > (1 << 30) || E < 1 || E > kMaxE || S < 1 || S > (1 << 24)) return 0;
+  return space_of(T, E, S).bytes;
+}
+
+hipError_t xtu_router_losses(const xtu_router_args* args, hipStream_t stream) {
+  XTU_CHECK_ARG(args);
+  const xtu_router_args& t = *args;
+  Rows a;
+  XTU_CHECK_ARG(rows_of(t, a));
+  XTU_CHECK_ARG(t.counts && t.probs && t.balance && t.norm && t.workspace);
+  XTU_CHECK_ARG(t.T == 0 || (t.weights && t.stat));
+  XTU_CHECK_ARG((t.mode == 0) == (t.z != nullptr));
+  const Space s = space_of(t.T, t.E, t.S);
+  XTU_CHECK_ARG(t.workspace_bytes >= s.bytes && reinterpret_cast<uintptr_t>(t.workspace) % 16 == 0);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(t.workspace);
+  float* pp = reinterpret_cast<float*>(ws + s.p);
+  int32_t* pc = reinterpret_cast<int32_t*>(ws + s.c);
+  float* pz = reinterpret_cast<float*>(ws + s.z);
+  unsigned* ticket = reinterpret_cast<unsigned*>(ws + s.ticket);
+  const int C = chunk_rows(t.T, t.E);
+  const int chunks = t.T ? (int)(((long)t.T + C - 1) / C) : 1;   // (one writes the ticket)
+  (void)hipGetLastError();
+  const auto go = [&](auto sig) {
+    return by_layout<decltype(sig)::value>(t.E, [&](auto l, auto v) {
+      router_stats_kernel<decltype(l)::value, decltype(v)::value, decltype(sig)::value>
+          <<<chunks, kThreads, 0, stream>>>(a, C, t.weights, reinterpret_cast<float2*>(t.stat), pp,
+                                            pc, pz, ticket);
+      return hipPeekAtLastError();
+    });
+  };
+  hipError_t e = t.mode ? go(std::true_type{}) : go(std::false_type{});
+  if (e != hipSuccess) return e;
+  const int nb = (t.E + kCols - 1) / kCols;
+  const Sums o{pp, pc, pz, reinterpret_cast<double*>(ws + s.loss),
+               reinterpret_cast<double*>(ws + s.zsum), ticket, t.counts, t.probs, t.balance, t.z,
+               t.norm};
+  router_finish_kernel<<<(unsigned)t.S * nb, kThreads, 0, stream>>>(a, C, o);
+  return hipPeekAtLastError();
+}
+
+hipError_t xtu_router_grad(const xtu_router_args* args, const float* g_weights,
+                           const float* g_balance, const float* g_z, void* dlogits,
+                           hipStream_t stream) {
+  XTU_CHECK_ARG(args);
+  const xtu_router_args& t = *args;
+  Rows a;
+  XTU_CHECK_ARG(rows_of(t, a));
+  if (t.T == 0) return hipSuccess;
+  XTU_CHECK_ARG(t.counts && t.norm && t.weights && t.stat && dlogits);
+  XTU_CHECK_ARG(t.mode == 0 || !g_z);
+  XTU_CHECK_ARG(reinterpret_cast<uintptr_t>(dlogits) % 16 == 0);
+  const int C = chunk_rows(t.T, t.E), chunks = (int)(((long)t.T + C - 1) / C);
+  const Grads o{reinterpret_cast<const float2*>(t.stat), t.weights, t.counts, t.norm, g_weights,
+                g_balance, g_z, dlogits};
+  (void)hipGetLastError();
+  const auto go = [&](auto sig) {
+    return by_layout<decltype(sig)::value>(t.E, [&](auto l, auto v) {
+      router_grad_kernel<decltype(l)::value, decltype(v)::value, decltype(sig)::value>
+          <<<chunks, kThreads, 0, stream>>>(a, C, o);
+      return hipPeekAtLastError();
+    });
+  };
+  return t.mode ? go(std::true_type{}) : go(std::false_type{});
+}
+
+}  // extern "C"

@@ -112,6 +112,9 @@ SIGNATURES = {
     "xtu_linear": (_i, [_vp, _vp]),
     "xtu_linear_plan": (_i, [_i, _i, _i, _i]),
     "xtu_linear_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "xtu_router_workspace_bytes": (_sz, [_i, _i, _i]),
+    "xtu_router_losses": (_i, [_vp, _vp]),
+    "xtu_router_grad": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),
     "xtu_copy_experts": (_i, [_i, _vp, _vp, _l, _vp, _l, _l, _vp]),
     "xtu_copy_2d": (_i, [_vp, _sz, _vp, _sz, _sz, _sz, _vp]),
     "xtu_i8_weight_bytes": (_sz, [_i, _i]),
@@ -158,7 +161,8 @@ _NOT_STATUS = {"xtu_version", "xtu_error_string", "xtu_segment_workspace_bytes",
                "xtu_decode_route_gate_up_ok", "xtu_decode_layer_ok",
                "xtu_decode_layer_barrier_words",
                "xtu_i8_weight_bytes", "xtu_few_workspace_bytes",
-               "xtu_linear_workspace_bytes", "xtu_linear_plan"}
+               "xtu_linear_workspace_bytes", "xtu_linear_plan",
+               "xtu_router_workspace_bytes"}
 
 _LIB = None
 

@@ -1,0 +1,165 @@
+"""The router's training step: losses, per-expert counts and the selected
+experts' weights, with their gradient in the logits.
+
+    ids = layer.route(logits, top_k=K)[1]
+    r = router_losses(logits, ids)
+    (task_loss(r.weights) + 0.01 * r.balance + 0.001 * r.z).backward()
+
+``layer.route`` selects; this gives what a training step differentiates, and the
+counts that say how evenly the experts are used (also to pick a pool's).  The
+reference serves only: its router (vllm_xiaotu_moe/hybrid_model.py:1877) has no
+losses and no gradient.
+"""
+from __future__ import annotations
+
+import struct
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from .block import MAX_EXPERTS, MAX_TOP_K
+from .layer import _same_device
+from .linear import _current_device, on_stream, raw_stream
+
+# xtu_router_args: logits, ids, starts, weights, stat, counts, probs, balance, z,
+# norm, workspace; ld; its bytes; T, E, K, S, mode, renormalize, logits_bf16; scale
+ARGS = struct.Struct("@11PlN7if")
+MAX_ROWS, MAX_SEQUENCES = 1 << 30, 1 << 24
+_WS_BYTES: dict = {}
+
+
+class RouterLosses(NamedTuple):
+    """weights fp32 [T, K]; balance and z fp32 scalars (z None with sigmoid
+    scoring); counts int32 and probs fp32 [S, E], without gradient."""
+    weights: torch.Tensor
+    balance: torch.Tensor
+    z: Optional[torch.Tensor]
+    counts: torch.Tensor
+    probs: torch.Tensor
+
+
+def router_losses(logits, ids, *, scoring="softmax", renormalize=True, routed_scaling_factor=1.0,
+                  seq_starts=None, stream=None) -> RouterLosses:
+    """Losses, counts and weights of a selection; differentiable in logits.
+
+    logits [T, E] fp32 or bf16, rows contiguous at any row stride; ids int32
+    [T, K], the selected experts (an id outside 0 .. E - 1 is no expert: weight
+    0, not counted).  scoring: "softmax" (p = softmax(logits)) or "sigmoid"
+    (scores s = sigmoid(logits), p = s / sum s).  seq_starts int32 [S + 1] on
+    the device: sequence q is rows seq_starts[q] .. seq_starts[q + 1]
+    (ascending; values are clamped to 0 .. T); rows outside them get weights and
+    take part in no loss and no count.  Without it all rows are one sequence.
+
+    weights: the selected experts' p (sigmoid: s), divided by their sum with
+    renormalize, times routed_scaling_factor (sigmoid only), as ``route`` gives
+    them.  balance: mean over non-empty sequences of E / (K n) sum_e counts_e
+    P_e with n rows and P their mean p: 1 for even use.  z: mean over the
+    sequences' rows of logsumexp(logits)^2.  A row of -inf has p = 0 and no
+    gradient; NaN and +inf give NaN.  fp32 arithmetic, sums over rows fp32 and fp64;
+    the same call gives the same bits.  Once differentiable.  Capturable into
+    a HIP graph.
+    """
+    T, E, K, S = _check(logits, ids, scoring, routed_scaling_factor, seq_starts)
+    dev = logits.device
+    if stream is not None or dev.index != _current_device():
+        with on_stream(stream, dev):
+            return router_losses(logits, ids, scoring=scoring, renormalize=renormalize,
+                                 routed_scaling_factor=routed_scaling_factor,
+                                 seq_starts=seq_starts)
+    shape = (T, E, K, S, int(scoring == "sigmoid"), bool(renormalize),
+             logits.dtype == torch.bfloat16, float(routed_scaling_factor))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return RouterLosses(*_Losses.apply(logits, ids, seq_starts, shape))
+    return RouterLosses(*_forward(logits, ids, seq_starts, shape)[:5])
+
+
+def _check(logits, ids, scoring, scale, seq_starts):
+    """(T, E, K, S); raises ValueError for what the kernels do not take."""
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"unsupported scoring function {scoring!r}")
+    if scoring == "softmax" and float(scale) != 1.0:
+        raise ValueError("a scaling factor goes with sigmoid scoring")
+    if not 0.0 < float(scale) < float("inf"):
+        raise ValueError(f"routed_scaling_factor {scale} is not a positive number")
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"logits must be a 2-D fp32 or bf16 tensor, got {tuple(logits.shape)} "
+                         f"{logits.dtype}")
+    T, E = logits.shape
+    if not 1 <= E <= MAX_EXPERTS or T > MAX_ROWS:
+        raise ValueError(f"logits of {T} rows of {E} experts: 1 .. {MAX_EXPERTS} experts, at most "
+                         f"{MAX_ROWS} rows")
+    if logits.stride(1) != 1 and E > 1:
+        raise ValueError(f"logits' rows must be contiguous (column stride {logits.stride(1)})")
+    if ids.dim() != 2 or ids.dtype != torch.int32 or ids.shape[0] != T or not ids.is_contiguous():
+        raise ValueError(f"ids must be contiguous int32 [{T}, K], got {tuple(ids.shape)} {ids.dtype}")
+    K = ids.shape[1]
+    if not 1 <= K <= MAX_TOP_K:
+        raise ValueError(f"ids of {K} experts a row, 1 .. {MAX_TOP_K}")
+    S = 1
+    if seq_starts is not None:
+        if seq_starts.dim() != 1 or seq_starts.dtype != torch.int32 \
+                or not seq_starts.is_contiguous() or not 2 <= seq_starts.numel() <= MAX_SEQUENCES:
+            raise ValueError(f"seq_starts must be contiguous int32 [S + 1], got "
+                             f"{tuple(seq_starts.shape)} {seq_starts.dtype}")
+        S = seq_starts.numel() - 1
+    if not logits.is_cuda:
+        raise ValueError("logits must be a CUDA tensor")
+    _same_device(logits.device, ids=ids, seq_starts=seq_starts)
+    return T, E, K, S
+
+
+def _pack(logits, ids, starts, weights, stat, counts, probs, balance, z, norm, ws, nws, shape):
+    T, E, K, S, mode, renorm, bf16, scale = shape
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    return ARGS.pack(logits.data_ptr(), ids.data_ptr(), ptr(starts), weights.data_ptr(),
+                     stat.data_ptr(), counts.data_ptr(), ptr(probs), ptr(balance), ptr(z),
+                     norm.data_ptr(), ptr(ws), logits.stride(0), nws, T, E, K, S, mode, renorm,
+                     bf16, scale)
+
+
+def _forward(logits, ids, starts, shape):
+    """(weights, balance, z, counts, probs, stat, norm)."""
+    T, E, K, S, mode = shape[:5]
+    new = lambda *size: logits.new_empty(size, dtype=torch.float32)  # noqa: E731
+    weights, stat, norm, probs, balance = new(T, K), new(T, 2), new(2), new(S, E), new()
+    z = None if mode else new()
+    counts = logits.new_empty((S, E), dtype=torch.int32)
+    nws = _WS_BYTES.get((T, E, S))
+    if nws is None:
+        nws = int(_lib.call("xtu_router_workspace_bytes", T, E, S))
+        if len(_WS_BYTES) >= 4096:
+            _WS_BYTES.clear()
+        _WS_BYTES[T, E, S] = nws
+    # per call: calls on other streams, and graphs, have their own
+    ws = logits.new_empty(nws, dtype=torch.uint8)
+    _lib.call("xtu_router_losses",
+              _pack(logits, ids, starts, weights, stat, counts, probs, balance, z, norm, ws, nws,
+                    shape), raw_stream(logits.device.index))
+    return weights, balance, z, counts, probs, stat, norm
+
+
+class _Losses(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, starts, shape):
+        weights, balance, z, counts, probs, stat, norm = _forward(logits, ids, starts, shape)
+        ctx.save_for_backward(logits, ids, starts, weights, stat, counts, norm)
+        ctx.shape = shape
+        ctx.mark_non_differentiable(counts, probs)
+        ctx.set_materialize_grads(False)
+        return weights, balance, z, counts, probs
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_weights, g_balance, g_z, _counts, _probs):
+        if g_weights is None and g_balance is None and g_z is None:
+            return None, None, None, None
+        logits, ids, starts, weights, stat, counts, norm = ctx.saved_tensors
+        T, E = ctx.shape[:2]
+        out = logits.new_empty((T, E))
+        grads = [None if g is None else g.contiguous() for g in (g_weights, g_balance, g_z)]
+        _lib.call("xtu_router_grad",
+                  _pack(logits, ids, starts, weights, stat, counts, None, None, None, norm, None, 0,
+                        ctx.shape), *(0 if g is None else g.data_ptr() for g in grads),
+                  out.data_ptr(), raw_stream(logits.device.index))
+        return out, None, None, None
