@@ -196,6 +196,7 @@ def prepare(case, seed):
         return st
     st = dict(case=case, **_router_inputs(case, seed))
     if own:   # what a training step differentiates
+        _path()
         st["logits"].requires_grad_(True)
     return st
 
@@ -230,7 +231,6 @@ def _run_own(case, st):
         return linear4(st["x"], st["weight"], bias=st["bias"], activation=case["act"],
                        row_scale=st["row_scale"], residual=st["residual"],
                        out_dtype=torch.float32 if case["out"] == "f32" else torch.bfloat16)
-    _path()
     from xtu_moe_amd.router import router_losses
     r = router_losses(st["logits"], st["ids"], scoring=case["scoring"],
                       renormalize=case["renormalize"], routed_scaling_factor=case["scale"],
