@@ -634,6 +634,39 @@ size_t xtu_linear_workspace_bytes(int M, int N, int K, int act, int aligned);
  * rows, else 256 * (K splits) + 1 + its tile (an index of kTileKinds), -1 none. */
 int xtu_linear_plan(int M, int N, int K, int act);
 
+/* ------------------------------------------------ dense product, 4-bit weights
+ * As xtu_linear with w [N][K] (act 6: [2N][K]) in 4 bits: fmt 2 MXFP4 (e2m1, e8m0
+ * per group of 32 k), 3 NVFP4 (e2m1, e4m3 per 16, times the second-level scale gs:
+ * fp32 [1], act 6 [2] = gate, up, on the device; NULL for the others), 4 INT4 (code
+ * - 8, fp32 per group of 32, 64 or 128).  K a multiple of the group, any N.  w: the
+ * records of formats.pack_linear4 (xtu_linear4_weight_bytes of them, 16-byte aligned):
+ * per panel of 16 rows (act 6: gate and up panels in turn) and block of 128 k 1024
+ * bytes of codes [4 q][16 row][16], then the scales.  MXFP4, NVFP4: a 16-byte chunk
+ * holds k = 32 q .. + 31 (low nibble = even k), scales [4 q][16 row][1 or 2].  INT4:
+ * dword j of a chunk holds k = 32 j + 8 q .. + 7 as code ^ 8, scales fp32
+ * [128 / group][16 row], times 16.  Rows and k past the matrix: codes 0, e8m0 127 or
+ * scale 0.  The products are exact in the fp32 sums' operands (INT4: the scale
+ * multiplies each group's fp32 sum).  workspace: as xtu_linear's, for K splits.  The
+ * reference leaves these products to its host (vllm_xiaotu_moe/hybrid_model.py:1752). */
+typedef struct xtu_linear4_args {
+  const void* x;
+  const void* w;
+  const float* gs;
+  const void* bias;
+  const float* row_scale;
+  const void* residual;
+  void* out;
+  void* workspace;
+  long ldx, ldr, ldo, scale_stride;
+  size_t workspace_bytes;
+  int M, N, K, act, fmt, group;
+  int bias_bf16, residual_bf16, out_bf16;
+  float limit, alpha, beta;
+} xtu_linear4_args;
+hipError_t xtu_linear4(const xtu_linear4_args* args, hipStream_t stream);
+size_t xtu_linear4_weight_bytes(int N, int K, int act, int fmt, int group);
+size_t xtu_linear4_workspace_bytes(int M, int N, int K, int act, int fmt, int group);
+
 /* ------------------------------------------------ router, training step
  * What a training step takes from router logits [T][E] (fp32, or bf16 with
  * logits_bf16; rows ld elements apart) and the selected ids int32 [T][K] (an id

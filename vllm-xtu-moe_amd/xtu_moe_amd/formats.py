@@ -273,6 +273,44 @@ def unpack_scales(fmt: int, p, N: int, K: int):
     return d.contiguous().reshape(E, N, K // 16)
 
 
+# ------------------------------------------------- 4-bit weights of linear4
+# records: per panel of 16 rows and block of 128 k, 1024 bytes of codes
+# [4 q][16 row][16 B], then the scales
+def linear4_group(fmt: int, s, K: int) -> int:
+    """The k per scale of a matrix's scales [N, K / group]."""
+    if s.dim() != 2 or s.shape[1] == 0 or K % s.shape[1]:
+        raise ValueError(f"scales {tuple(s.shape)} do not split K={K} into groups")
+    g = K // s.shape[1]
+    groups = {FMT_MXFP4: (32,), FMT_NVFP4: (16,), FMT_INT4: INT4_GROUPS}[fmt]
+    if g not in groups:
+        raise ValueError(f"{FMT_NAMES[fmt]} scales per {g} k are not supported (groups: {groups})")
+    return g
+
+
+def pack_linear4(fmt: int, codes, s, group: int):
+    """codes u8 [n, N, K/2] (low nibble = even k) and scales [n, N, K/group] of n
+    halves (1; 2: gate, up) -> records u8 [panels, blocks, record], the halves'
+    panels in turn.  Rows and k past the matrix are zero codes; INT4 codes
+    become two's complement, their scales are times 16 (the kernels read a code as
+    a fraction of 16)."""
+    n, N, K = codes.shape[0], codes.shape[1], codes.shape[2] * 2
+    P, B = (N + 15) // 16, (K + 127) // 128
+    pad = torch.nn.functional.pad
+    c = codes ^ 0x88 if fmt == FMT_INT4 else codes
+    c = pad(c, (0, B * 64 - K // 2, 0, P * 16 - N))
+    if fmt == FMT_INT4:   # [n][panel][row][block][j][q][4 B] -> [panel][n][block][q][row][j][4 B]
+        c = c.view(n, P, 16, B, 4, 4, 4).permute(1, 0, 3, 5, 2, 4, 6)
+        s = pad(s.float() * 16.0, (0, B * (128 // group) - K // group, 0, P * 16 - N))
+        s = s.view(n, P, 16, B, 128 // group).permute(1, 0, 3, 4, 2).contiguous().view(torch.uint8)
+    else:                 # [n][panel][row][block][q][16 B] -> [panel][n][block][q][row][16 B]
+        c = c.view(n, P, 16, B, 4, 16).permute(1, 0, 3, 4, 2, 5)
+        per = 32 // group
+        s = pad(s.view(torch.uint8), (0, B * 4 * per - K // group, 0, P * 16 - N),
+                value=127 if fmt == FMT_MXFP4 else 0)
+        s = s.view(n, P, 16, B, 4, per).permute(1, 0, 3, 4, 2, 5)
+    return torch.cat([c.reshape(P * n, B, 1024), s.reshape(P * n, B, -1)], 2)
+
+
 def algorithmic_bytes(fmt: int, N: int, K: int) -> int:
     """Bytes a weight stream of one [N, K] matrix must read: codes plus one
     scale per scaling block (no layout padding)."""
