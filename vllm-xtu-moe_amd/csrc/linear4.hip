@@ -39,6 +39,10 @@ size_t xtu_linear4_weight_bytes(int N, int K, int act, int fmt, int group) {
 size_t xtu_linear4_workspace_bytes(int M, int N, int K, int act, int fmt, int group) {
   if (!sizes_ok(M, N, K, act, fmt, group) || M == 0) return 0;
   const bool gated = act == lin::kSwiglu;
+  LinearArgs e{};
+  e.M = M;
+  e.K = K;
+  if (skinny4_fits(e)) return 0;
   return split_bytes(plan4_tile(M, N, K, gated, true), M, N, gated);
 }
 
@@ -72,6 +76,7 @@ hipError_t xtu_linear4(const xtu_linear4_args* args, hipStream_t stream) {
   a.group = t.group;
   a.xvec = al(t.x, 16) && K % 8 == 0 && (M == 1 || t.ldx % 8 == 0);
   (void)hipGetLastError();
+  if (skinny4_fits(a.e)) return launch4_skinny(a, stream);
   Plan4 p = plan4_tile(M, N, K, gated, true);
   if (split_bytes(p, M, N, gated) > (t.workspace ? t.workspace_bytes : 0))
     p = plan4_tile(M, N, K, gated, false);

@@ -169,6 +169,11 @@ __device__ __forceinline__ u32x4_t load_x8(const Linear4Args& a, const uint16_t*
   return lin::load8(row, k, a.e.K);
 }
 
+// At most 16 rows of x, all of x in LDS.
+constexpr size_t kSkinny4Lds = 120 * 1024;
+bool skinny4_fits(const LinearArgs& e);
+hipError_t launch4_skinny(const Linear4Args& a, hipStream_t stream);
+
 struct Plan4 {
   int kind, split;   // kind: blocks of 16 rows of a tile
 };

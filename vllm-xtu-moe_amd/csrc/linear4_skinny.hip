@@ -1,0 +1,129 @@
+// The product with 4-bit weights for at most 16 rows of x (linear4.hpp has the
+// formula and the layout): a stream of w.  All of x sits in LDS.  A unit is up to 16
+// output columns (swiglu: of gate and up both); the waves of a workgroup deal its
+// blocks of 128 k among them, their sums are added through LDS in a fixed order, and
+// the workgroup takes further units in steps of the grid.  A wave has U blocks in
+// flight, over unit ends too.
+#include "linear4.hpp"
+
+namespace xtu {
+namespace l4 {
+namespace {
+
+constexpr int kRowPad = 16;    // bf16 behind a row of x in LDS: rows 32 bytes apart in the banks
+
+template <int FMT, int G, bool GATED, int WV, int U>
+__global__ __launch_bounds__(64 * WV) void linear4_skinny_kernel(Linear4Args a, int rp) {
+  constexpr int H = GATED ? 2 : 1, REC = record_bytes(FMT, G);
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ f32x4_t red[H][WV][64];
+  const LinearArgs& e = a.e;
+  const int tid = threadIdx.x, lane = tid % 64;
+  const int w = __builtin_amdgcn_readfirstlane(tid / 64);
+  const int q = lane / 16, c = lane % 16;
+  const int nb = blocks_of(e.K), per = 16 / rp;   // units of a panel
+  const int units = panels_of(e.N) * per;
+  const int steps = (nb + WV - 1) / WV;           // of a wave and unit
+  Raw<FMT, G> raw[U][H];
+  // block w + WV i of a unit (past the end the last one again, not used)
+  auto load = [&](int unit, int i, Raw<FMT, G> (&r)[H]) {
+    const int row = unit % per * rp;
+    const uint8_t* rec = a.w + ((long)(unit / per) * H * nb + min(w + WV * i, nb - 1)) * REC;
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+      r[h] = load_raw<FMT, G>(rec + (long)h * nb * REC, q, row + min(c, rp - 1),
+                              min(row + 4 * q, 12));
+  };
+  int unit = blockIdx.x;
+#pragma unroll
+  for (int i = 0; i < U; ++i) load(unit, min(i, steps - 1), raw[i]);
+  __builtin_amdgcn_sched_barrier(0);   // x after the first loads of w
+  // x to LDS, zeros behind K
+  const int ldx = nb * 128 + kRowPad, pieces = nb * 16;
+  uint16_t* xs = reinterpret_cast<uint16_t*>(lds);
+  for (int p = tid; p < e.M * pieces; p += 64 * WV) {
+    const int r = p / pieces, k8 = p - r * pieces;
+    *reinterpret_cast<u32x4_t*>(xs + r * ldx + (k8 / 16 * 16 + place_of<FMT>(k8 % 16)) * 8) =
+        load_x8(a, e.x + (long)r * e.ldx, 8 * k8);
+  }
+  __syncthreads();
+  const uint16_t* xl = xs + min(c, e.M - 1) * ldx + 8 * q;
+  const float g0 = a.gs ? a.gs[0] : 1.f, g1 = a.gs && GATED ? a.gs[1] : g0;
+
+  for (; unit < units; unit += gridDim.x) {
+    const int next = min(unit + (int)gridDim.x, units - 1);
+    f32x4_t acc[H][1];
+#pragma unroll
+    for (int h = 0; h < H; ++h) acc[h][0] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < steps; i0 += U) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int s = w + WV * (i0 + i);
+        if (s < nb) {
+          const uint16_t* xb = xl + 128 * s;
+          multiply<FMT, G, H, 1>(raw[i], acc, [&](int j, int) {
+            return *reinterpret_cast<const u32x4_t*>(xb + 32 * j);
+          });
+        }
+        // what comes U steps later, or the next unit's step of this slot
+        const bool more = i0 + U < steps;
+        load(more ? unit : next, min(more ? i0 + U + i : i, steps - 1), raw[i]);
+      }
+    }
+    __syncthreads();   // the sums of the unit before are read
+#pragma unroll
+    for (int h = 0; h < H; ++h) red[h][w][lane] = acc[h][0];
+    __syncthreads();
+    if (tid < 256) {
+      const int t = tid / 64, nl = 4 * q + t, n = unit / per * 16 + unit % per * rp + nl;
+      float z = 0.f, u = 0.f;
+      if (c < e.M && nl < rp && n < e.N) {
+#pragma unroll
+        for (int k = 0; k < WV; ++k) {
+          z += red[0][k][lane][t];
+          if constexpr (GATED) u += red[H - 1][k][lane][t];
+        }
+        lin::finish_one<GATED ? lin::kActSwiglu : lin::kActOther>(e, c, n, z * g0, u * g1);
+      }
+    }
+  }
+}
+
+size_t skinny_lds(const LinearArgs& e) {
+  return (size_t)e.M * (blocks_of(e.K) * 128 + kRowPad) * 2;
+}
+
+template <int WV>
+hipError_t launch(const Linear4Args& a, hipStream_t stream) {
+  const LinearArgs& e = a.e;
+  int rp = 4;   // columns of a unit: about one unit per CU, 16 at most
+  while (rp < 16 && (long)panels_of(e.N) * (16 / rp) > 256) rp *= 2;
+  const long units = (long)panels_of(e.N) * (16 / rp);
+  const size_t lds = skinny_lds(e);
+  const size_t all = lds + (size_t)(e.act == lin::kSwiglu ? 2 : 1) * WV * 1024;
+  const int fit = (int)(160 * 1024 / all), most = 32 / WV;
+  const long grid = 256L * (fit < most ? fit : most);
+  const bool one = blocks_of(e.K) <= WV;   // a block per wave and unit
+  return by_format(a, [&](auto fmt, auto group, auto g) {
+    constexpr int F = decltype(fmt)::value, G = decltype(group)::value;
+    constexpr bool GATED = decltype(g)::value;
+    auto k = one ? linear4_skinny_kernel<F, G, GATED, WV, 1>
+                 : linear4_skinny_kernel<F, G, GATED, WV, 2>;
+    k<<<(unsigned)(units < grid ? units : grid), 64 * WV, lds, stream>>>(a, rp);
+    return hipPeekAtLastError();
+  });
+}
+
+}  // namespace
+
+bool skinny4_fits(const LinearArgs& e) { return e.M <= 16 && skinny_lds(e) <= kSkinny4Lds; }
+
+hipError_t launch4_skinny(const Linear4Args& a, hipStream_t stream) {
+  const int nb = blocks_of(a.e.K);
+  if (nb > 8) return launch<16>(a, stream);
+  if (nb > 4) return launch<8>(a, stream);
+  return launch<4>(a, stream);
+}
+
+}  // namespace l4
+}  // namespace xtu
