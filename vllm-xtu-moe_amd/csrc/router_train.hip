@@ -27,10 +27,16 @@ namespace xtu {
 namespace rt {
 namespace {
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kMaxE = 1024, kMaxK = 16;
-constexpr int kCols = 16;          // experts of a workgroup of the second launch
-constexpr int kMaxChunks = 512;    // workgroups of the first launch: two a CU
+// Forward: 16 waves a workgroup, so that 32 waves a CU write only two rows of sums.
+constexpr int kWaves = 16, kThreads = 64 * kWaves;
+constexpr int kMaxChunks = 512;    // workgroups: two a CU
+constexpr int kOneTurns = 4;       // turns of a workgroup that does without the second launch
+constexpr int kOneSeqs = 64;       // and the sequences that it writes
+// Second launch: 16 experts a workgroup, 16 partial rows at a time.
+constexpr int kCols = 16, kSumThreads = 256;
+// Backward: nothing is shared between waves.
+constexpr int kGradWaves = 4, kGradThreads = 64 * kGradWaves, kGradChunks = 2048;
 
 struct Rows {
   const void* logits;   // [T][E], rows ld apart
@@ -53,18 +59,57 @@ __device__ __forceinline__ float exp_neg(float x) {
   return __builtin_fmaf(e, r * 0.693147182f, e);
 }
 
-// Reductions over the L lanes of a token.
-template <int L>
-__device__ __forceinline__ float sum_over(float v) {
-#pragma unroll
-  for (int d = 1; d < L; d *= 2) v += __shfl_xor(v, d, 64);
+// v of the lane across: within quads, halves of a row of 16, rows, and rows by
+// row (every lane below that size holds the same value by then).
+template <int D>
+__device__ __forceinline__ float across(float v) {
+  const int x = __float_as_int(v);
+  if constexpr (D == 1) return __int_as_float(__builtin_amdgcn_mov_dpp(x, 0xB1, 0xF, 0xF, false));
+  if constexpr (D == 2) return __int_as_float(__builtin_amdgcn_mov_dpp(x, 0x4E, 0xF, 0xF, false));
+  if constexpr (D == 4) return __int_as_float(__builtin_amdgcn_mov_dpp(x, 0x141, 0xF, 0xF, false));
+  return __int_as_float(__builtin_amdgcn_mov_dpp(x, 0x140, 0xF, 0xF, false));   // 8
+}
+
+// The op of all of the L lanes of a token, in each of them.  Register moves only: by
+// way of LDS (__shfl_xor) the six steps take longer than the rest of a row.
+template <int L, class F>
+__device__ __forceinline__ float reduce_over(float v, F op) {
+  if constexpr (L >= 2) v = op(v, across<1>(v));
+  if constexpr (L >= 4) v = op(v, across<2>(v));
+  if constexpr (L >= 8) v = op(v, across<4>(v));
+  if constexpr (L >= 16) v = op(v, across<8>(v));
+  if constexpr (L >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  if constexpr (L >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
   return v;
 }
 
 template <int L>
+__device__ __forceinline__ float sum_over(float v) {
+  return reduce_over<L>(v, [](float x, float y) { return x + y; });
+}
+
+template <int L>
 __device__ __forceinline__ float max_over(float v) {
+  return reduce_over<L>(v, [](float x, float y) { return fmaxf(x, y); });
+}
+
+// The sum over a block's threads in every thread, in a fixed order; red: a value per
+// wave, not in use.
+template <int WAVES>
+__device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
-  for (int d = 1; d < L; d *= 2) v = fmaxf(v, __shfl_xor(v, d, 64));
+  for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d, 64);
+  if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = v;
+  __syncthreads();
+  v = 0.;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) v += red[w];
   return v;
 }
 
@@ -171,30 +216,79 @@ __device__ __forceinline__ void seq_rows(const Rows& a, int q, int& begin, int& 
   end = min(max(start_of(a, q + 1), begin), a.T);
 }
 
+// Ids of a row that a lane takes: k = i, i + L, ..; -1: none.
+template <int L>
+struct Ids {
+  static constexpr int N = (kMaxK + L - 1) / L;
+  int e[N];
+};
+
+template <int L>
+__device__ __forceinline__ void load_ids(const Rows& a, long t, int i, Ids<L>& ids) {
+#pragma unroll
+  for (int n = 0; n < Ids<L>::N; ++n) {
+    const int k = i + L * n;
+    const int e = k < a.K ? a.ids[t * a.K + k] : -1;
+    ids.e[n] = (unsigned)e < (unsigned)a.E ? e : -1;
+  }
+}
+
+struct Sums {
+  float* part_p;       // [chunks + S][E]
+  int32_t* part_c;
+  float* part_z;       // [chunks + S]
+  double* loss;        // [S][ceil(E / 16)]
+  double* zsum;        // [S]
+  unsigned* ticket;
+  int32_t* counts;     // [S][E]
+  float* probs;        // [S][E]
+  float* balance;
+  float* z;
+  float* norm;         // [2]: non-empty sequences, their rows
+};
+
+__device__ __forceinline__ void write_losses(const Sums& o, double loss, double z, double rows,
+                                             double seqs) {
+  *o.balance = seqs > 0. ? (float)(loss / seqs) : 0.f;
+  if (o.z) *o.z = rows > 0. ? (float)(z / rows) : 0.f;
+  o.norm[0] = (float)seqs;
+  o.norm[1] = (float)rows;
+}
+
 // Chunk g holds rows [g C, (g + 1) C).  Its part of sequence q writes row g + q
-// of the partial sums: both grow along the rows, so no two parts share one.
-template <int L, int V, bool SIG>
-__global__ __launch_bounds__(kThreads) void router_stats_kernel(
-    Rows a, int C, float* weights, float2* stat, float* part_p, int32_t* part_c, float* part_z,
-    unsigned* ticket) {
+// of the partial sums: both grow along the rows, so no two parts share one.  ONE: the
+// only chunk, whose sums are the sequences' own, and which writes the losses too.
+template <int L, int V, bool SIG, bool ONE>
+__global__ __launch_bounds__(kThreads, ONE || V > 8 ? 4 : 8) void router_stats_kernel(Rows a, int C, float* weights,
+                                                                float2* stat, Sums o) {
   constexpr int G = 64 / L, NG = kWaves * G, COLS = L * V;
-  __shared__ __attribute__((aligned(16))) float buf[NG][COLS];   // a token's scores; then sums
+  // a token's scores; then a wave's sums
+  __shared__ __attribute__((aligned(16))) float buf[NG][COLS];
   __shared__ int32_t hist[COLS];
-  __shared__ float zs[NG];
+  __shared__ float zs[kWaves];
+  __shared__ double red[4][kWaves];
   const int tid = threadIdx.x, lane = tid % 64, w = tid / 64;
   const int i = lane % L, g = w * G + lane / L;
-  if (blockIdx.x == 0 && tid == 0) *ticket = 0;   // of the next launch
+  if (!ONE && blockIdx.x == 0 && tid == 0) *o.ticket = 0;   // of the next launch
   const int c0 = blockIdx.x * C, c1 = min(c0 + C, a.T);
   for (int c = tid; c < COLS; c += kThreads) hist[c] = 0;
+  double loss = 0., zsum = 0.;
+  if (ONE) {
+    for (int k = tid; k < a.S * a.E; k += kThreads) {   // empty sequences stay so
+      o.counts[k] = 0;
+      o.probs[k] = 0.f;
+    }
+  }
   int q = seq_of(a, c0);
   int at = c0;   // rows before are done
   while (at < c1) {
     // rows [at, end) are sequence q's, or no one's (q == S, or before its start)
-    int end = c1;
+    int end = c1, n = 0;
     bool in = false;
     if (q < a.S) {
       int b, e;
       seq_rows(a, q, b, e);
+      n = e - b;
       in = at >= b;
       end = min(c1, in ? e : b);
       if (end <= at) {   // an empty sequence (or starts that do not ascend)
@@ -207,13 +301,21 @@ __global__ __launch_bounds__(kThreads) void router_stats_kernel(
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = 0.f;
     Raw<L, V> next;
+    Ids<L> nid;
     int t = at + g;
-    if (t < end) load_row(a, t, i, next);
+    if (t < end) {
+      load_row(a, t, i, next);
+      load_ids(a, t, i, nid);
+    }
     for (int t0 = at; t0 < end; t0 += NG, t += NG) {   // every lane of a wave takes each turn
       const bool on = t < end;
       float l[V];
       values(a, next, l);
-      if (t + NG < end) load_row(a, t + NG, i, next);
+      const Ids<L> id = nid;
+      if (t + NG < end) {
+        load_row(a, t + NG, i, next);
+        load_ids(a, t + NG, i, nid);
+      }
       float m = l[0];
 #pragma unroll
       for (int v = 1; v < V; ++v) m = fmaxf(m, l[v]);
@@ -226,110 +328,117 @@ __global__ __launch_bounds__(kThreads) void router_stats_kernel(
         l[v] = score<SIG>(l[v], m);
         s += l[v];
       }
-      s = sum_over<L>(s);
-      const float inv = s == 0.f ? 0.f : 1.f / s;
       lds_order();
 #pragma unroll
       for (int v = 0; v < V / 4; ++v)
         *reinterpret_cast<f32x4_t*>(&buf[g][4 * (i + L * v)]) =
             f32x4_t{l[4 * v], l[4 * v + 1], l[4 * v + 2], l[4 * v + 3]};
       lds_order();
-      if (on) {
-        if (in) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) acc[v] = __builtin_fmaf(l[v], inv, acc[v]);
-          if (!SIG && s != 0.f) {
-            const float lse = m + logf(s);
-            z = __builtin_fmaf(lse, lse, z);
-          }
-        }
-        if (i == 0) stat[t] = make_float2(m, inv);
-      }
+      s = sum_over<L>(s);
+      const float inv = s == 0.f ? 0.f : 1.f / s;
       // the selected experts: lanes 0 .. K - 1 of the token, L at a time
-      float total = 0.f;
-      if (a.renorm) {
-        for (int k = i; k < a.K; k += L) {
-          const int e = on ? a.ids[(long)t * a.K + k] : -1;
-          if ((unsigned)e < (unsigned)a.E) total += buf[g][e];
-        }
-        total = sum_over<L>(total);
+      float sel[Ids<L>::N], total = 0.f;
+#pragma unroll
+      for (int n = 0; n < Ids<L>::N; ++n) {
+        sel[n] = on && id.e[n] >= 0 ? buf[g][id.e[n]] : 0.f;
+        total += sel[n];
       }
+      if (a.renorm) total = sum_over<L>(total);
       float f = a.renorm ? (total == 0.f ? 0.f : a.scale / total)
                          : a.scale * (SIG ? exp_neg(m) : inv);
       if (!SIG && s != s) f = s;   // a probability of such a row is NaN, whoever is selected
-      for (int k = i; k < a.K; k += L) {
-        if (!on) continue;
-        const long o = (long)t * a.K + k;
-        const int e = a.ids[o];
-        const bool there = (unsigned)e < (unsigned)a.E;
-        weights[o] = there ? buf[g][e] * f : 0.f;
-        if (there && in) atomicAdd(&hist[e], 1);
+      if (!on) continue;
+#pragma unroll
+      for (int n = 0; n < Ids<L>::N; ++n) {
+        const int k = i + L * n;
+        if (k < a.K) weights[(long)t * a.K + k] = id.e[n] >= 0 ? sel[n] * f : 0.f;
+        if (in && id.e[n] >= 0) atomicAdd(&hist[id.e[n]], 1);
+      }
+      if (i == 0) stat[t] = make_float2(m, inv);
+      if (!in) continue;
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = __builtin_fmaf(l[v], inv, acc[v]);
+      if (!SIG && i == 0 && s != 0.f) {
+        const float lse = m + logf(s);
+        z = __builtin_fmaf(lse, lse, z);
       }
     }
     if (in) {
       __syncthreads();   // the scores are read, hist is whole
+      // the wave's tokens' sums, then the waves'
 #pragma unroll
-      for (int v = 0; v < V / 4; ++v)
-        *reinterpret_cast<f32x4_t*>(&buf[g][4 * (i + L * v)]) =
-            f32x4_t{acc[4 * v], acc[4 * v + 1], acc[4 * v + 2], acc[4 * v + 3]};
-      if (i == 0) zs[g] = z;
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int d = L; d < 64; d *= 2) acc[v] += __shfl_xor(acc[v], d, 64);
+      z = sum_over<64>(z);
+      if (lane < L)
+#pragma unroll
+        for (int v = 0; v < V / 4; ++v)
+          *reinterpret_cast<f32x4_t*>(&buf[w * G][4 * (i + L * v)]) =
+              f32x4_t{acc[4 * v], acc[4 * v + 1], acc[4 * v + 2], acc[4 * v + 3]};
+      if (lane == 0) zs[w] = z;
       __syncthreads();
-      const long slot = (long)blockIdx.x + q;
+      const long slot = ONE ? q : (long)blockIdx.x + q;
       for (int c = tid; c < a.E; c += kThreads) {
         float s = 0.f;
 #pragma unroll
-        for (int k = 0; k < NG; ++k) s += buf[k][c];
-        part_p[slot * a.E + c] = s;
-        part_c[slot * a.E + c] = hist[c];
+        for (int k = 0; k < kWaves; ++k) s += buf[k * G][c];
+        const int32_t cnt = hist[c];
         hist[c] = 0;
+        if (ONE) {
+          const double p = (double)s / n;
+          o.probs[slot * a.E + c] = (float)p;
+          o.counts[slot * a.E + c] = cnt;
+          loss += p * cnt * a.E / ((double)a.K * n);
+        } else {
+          o.part_p[slot * a.E + c] = s;
+          o.part_c[slot * a.E + c] = cnt;
+        }
       }
       if (tid == 0) {
         float s = 0.f;
-        for (int k = 0; k < NG; ++k) s += zs[k];
-        part_z[slot] = s;
+        for (int k = 0; k < kWaves; ++k) s += zs[k];
+        if (ONE) zsum += s;
+        else o.part_z[slot] = s;
       }
     }
     at = end;
   }
+  if (ONE) {
+    double rows = 0., seqs = 0.;
+    for (int k = tid; k < a.S; k += kThreads) {
+      int b, e;
+      seq_rows(a, k, b, e);
+      rows += e - b;
+      seqs += e > b;
+    }
+    loss = block_sum<kWaves>(loss, red[0]);
+    zsum = block_sum<kWaves>(zsum, red[1]);
+    rows = block_sum<kWaves>(rows, red[2]);
+    seqs = block_sum<kWaves>(seqs, red[3]);
+    if (tid == 0) write_losses(o, loss, zsum, rows, seqs);
+  }
 }
 
-struct Sums {
-  const float* part_p;
-  const int32_t* part_c;
-  const float* part_z;
-  double* loss;        // [S][ceil(E / 16)]
-  double* zsum;        // [S]
-  unsigned* ticket;
-  int32_t* counts;     // [S][E]
-  float* probs;        // [S][E]
-  float* balance;
-  float* z;
-  float* norm;         // [2]: non-empty sequences, their tokens
-};
-
-// A block's 256 values added to one, in a fixed order.
-__device__ __forceinline__ double block_sum(double v, double* red) {
-  const int tid = threadIdx.x;
-  __syncthreads();
-  red[tid] = v;
-  for (int d = kThreads / 2; d > 0; d /= 2) {
-    __syncthreads();
-    if (tid < d) red[tid] += red[tid + d];
-  }
-  __syncthreads();
-  return red[0];
+// Stores and loads that other XCDs' L2s see without a write-back of this one's.
+__device__ __forceinline__ void store_far(double* p, double v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double load_far(const double* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // Sixteen experts of a sequence per workgroup: thread (r, c) adds every 16th
 // partial row of expert c.  The workgroup that ends last adds the losses.
-__global__ __launch_bounds__(kThreads) void router_finish_kernel(Rows a, int C, Sums o) {
-  __shared__ double red[kThreads];
-  __shared__ int32_t cnt[kThreads];
+__global__ __launch_bounds__(kSumThreads) void router_finish_kernel(Rows a, int C, Sums o) {
+  constexpr int R = kSumThreads / kCols, WAVES = kSumThreads / 64;
+  __shared__ double sp[R][kCols];
+  __shared__ int32_t sc[R][kCols];
+  __shared__ double red[5][WAVES];
   __shared__ bool last;
   const int tid = threadIdx.x, nb = (a.E + kCols - 1) / kCols;
   const int q = blockIdx.x / nb, b = blockIdx.x % nb;
-  const int e = b * kCols + tid % kCols, r = tid / kCols;
-  constexpr int R = kThreads / kCols;
+  const int col = tid % kCols, e = b * kCols + col, r = tid / kCols;
   int begin, end;
   seq_rows(a, q, begin, end);
   const int n = end - begin;
@@ -337,7 +446,7 @@ __global__ __launch_bounds__(kThreads) void router_finish_kernel(Rows a, int C, 
   double p = 0., z = 0.;
   int32_t c = 0;
   if (e < a.E) {
-#pragma unroll 4
+#pragma unroll 8
     for (int g = g0 + r; g < g1; g += R) {
       const long at = ((long)g + q) * a.E + e;
       p += o.part_p[at];
@@ -345,52 +454,51 @@ __global__ __launch_bounds__(kThreads) void router_finish_kernel(Rows a, int C, 
     }
   }
   if (b == 0)
-    for (int g = g0 + tid; g < g1; g += kThreads) z += o.part_z[(long)g + q];
-  red[tid] = p;
-  cnt[tid] = c;
-  __syncthreads();
-  double loss = 0.;
-  if (tid < kCols && e < a.E) {
-    for (int k = 1; k < R; ++k) {
-      p += red[k * kCols + tid];
-      c += cnt[k * kCols + tid];
+    for (int g = g0 + tid; g < g1; g += kSumThreads) z += o.part_z[(long)g + q];
+  sp[r][col] = p;
+  sc[r][col] = c;
+  if (b == 0) z = block_sum<WAVES>(z, red[0]);   // (the same for the whole workgroup)
+  else __syncthreads();
+  if (tid < 64) {
+    double loss = 0.;
+    if (tid < kCols && e < a.E) {
+#pragma unroll
+      for (int k = 1; k < R; ++k) {
+        p += sp[k][tid];
+        c += sc[k][tid];
+      }
+      p = n > 0 ? p / n : 0.;
+      o.probs[(long)q * a.E + e] = (float)p;
+      o.counts[(long)q * a.E + e] = c;
+      loss = n > 0 ? p * c * a.E / ((double)a.K * n) : 0.;
     }
-    p = n > 0 ? p / n : 0.;
-    o.probs[(long)q * a.E + e] = (float)p;
-    o.counts[(long)q * a.E + e] = c;
-    loss = n > 0 ? p * c * a.E / ((double)a.K * n) : 0.;
-  }
-  loss = block_sum(loss, red);
-  if (b == 0) z = block_sum(z, red);
-  if (tid == 0) {
-    o.loss[blockIdx.x] = loss;
-    if (b == 0) o.zsum[q] = z;
-    __threadfence();
-    last = atomicAdd(o.ticket, 1u) == gridDim.x - 1;
+#pragma unroll
+    for (int d = kCols / 2; d > 0; d /= 2) loss += __shfl_xor(loss, d, 64);
+    if (tid == 0) {
+      store_far(&o.loss[blockIdx.x], loss);
+      if (b == 0) store_far(&o.zsum[q], z);
+      __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");   // they are there before the ticket
+      last = __hip_atomic_fetch_add(o.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+             gridDim.x - 1;
+    }
   }
   __syncthreads();
   if (!last) return;
-  __threadfence();   // the others' sums, not what a cache held of them
-  double sum = 0., zz = 0., rows = 0., seqs = 0.;
-  for (long k = tid; k < (long)a.S * nb; k += kThreads) sum += __hip_atomic_load(
-      &o.loss[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  for (int k = tid; k < a.S; k += kThreads) {
+  double sum = 0., rows = 0., seqs = 0.;
+  z = 0.;
+  for (long k = tid; k < (long)a.S * nb; k += kSumThreads) sum += load_far(&o.loss[k]);
+  for (int k = tid; k < a.S; k += kSumThreads) {
     int x, y;
     seq_rows(a, k, x, y);
-    zz += __hip_atomic_load(&o.zsum[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    z += load_far(&o.zsum[k]);
     rows += y - x;
     seqs += y > x;
   }
-  sum = block_sum(sum, red);
-  zz = block_sum(zz, red);
-  rows = block_sum(rows, red);
-  seqs = block_sum(seqs, red);
-  if (tid == 0) {
-    *o.balance = seqs > 0. ? (float)(sum / seqs) : 0.f;
-    if (o.z) *o.z = rows > 0. ? (float)(zz / rows) : 0.f;
-    o.norm[0] = (float)seqs;
-    o.norm[1] = (float)rows;
-  }
+  sum = block_sum<WAVES>(sum, red[1]);
+  z = block_sum<WAVES>(z, red[2]);
+  rows = block_sum<WAVES>(rows, red[3]);
+  seqs = block_sum<WAVES>(seqs, red[4]);
+  if (tid == 0) write_losses(o, sum, z, rows, seqs);
 }
 
 struct Grads {
@@ -404,17 +512,46 @@ struct Grads {
   void* out;                // [T][E], the logits' type
 };
 
+// A lane's selected experts of a row with their weights and gradients.
+template <int L>
+struct Picks {
+  Ids<L> id;
+  float w[Ids<L>::N], g[Ids<L>::N];
+  float2 stat;
+};
+
+template <int L>
+__device__ __forceinline__ void load_picks(const Rows& a, const Grads& o, long t, int i,
+                                           Picks<L>& p) {
+  p.stat = o.stat[t];
+  if (!o.g_weights) return;
+  load_ids(a, t, i, p.id);
+#pragma unroll
+  for (int n = 0; n < Ids<L>::N; ++n) {
+    const int k = i + L * n;
+    p.w[n] = k < a.K ? o.weights[t * a.K + k] : 0.f;
+    p.g[n] = k < a.K ? o.g_weights[t * a.K + k] : 0.f;
+  }
+}
+
 // One token per L lanes again.  The selected experts' parts meet the row's
 // through LDS: lanes 0 .. K - 1 add them where their experts' owners read.
 //   softmax: d_j = p_j (h_j - sum p h + z' - sum_k g_k w_k [not renormalised]) + sel_j
 //   sigmoid: d_j = (1 - s_j) (p_j (h_j - sum p h) + sel_j)
 template <int L, int V, bool SIG>
-__global__ __launch_bounds__(kThreads) void router_grad_kernel(Rows a, int C, Grads o) {
-  constexpr int G = 64 / L, NG = kWaves * G, COLS = L * V;
+__global__ __launch_bounds__(kGradThreads) void router_grad_kernel(Rows a, int C, Grads o) {
+  constexpr int G = 64 / L, NG = kGradWaves * G, COLS = L * V;
   __shared__ __attribute__((aligned(16))) float buf[NG][COLS];
   const int tid = threadIdx.x, lane = tid % 64, w = tid / 64;
   const int i = lane % L, g = w * G + lane / L;
   const int c0 = blockIdx.x * C, c1 = min(c0 + C, a.T);
+  Raw<L, V> next;
+  Picks<L> npick;
+  int t = c0 + g;
+  if (t < c1) {
+    load_row(a, t, i, next);
+    load_picks(a, o, t, i, npick);
+  }
 #pragma unroll
   for (int v = 0; v < V / 4; ++v)
     *reinterpret_cast<f32x4_t*>(&buf[g][4 * (i + L * v)]) = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -423,15 +560,16 @@ __global__ __launch_bounds__(kThreads) void router_grad_kernel(Rows a, int C, Gr
   const float gz = o.g_z && rows > 0.f ? 2.f * *o.g_z / rows : 0.f;
   float h[V];
   int q = -1, qb = 0, qe = 0;   // the sequence whose h is in registers, and its rows
-  Raw<L, V> next;
-  int t = c0 + g;
-  if (t < c1) load_row(a, t, i, next);
   for (int t0 = c0; t0 < c1; t0 += NG, t += NG) {
     const bool on = t < c1;
     float l[V];
     values(a, next, l);
-    if (t + NG < c1) load_row(a, t + NG, i, next);
-    if (on && (q < 0 || (t >= qe && q < a.S) )) {
+    const Picks<L> pick = npick;
+    if (t + NG < c1) {
+      load_row(a, t + NG, i, next);
+      load_picks(a, o, t + NG, i, npick);
+    }
+    if (on && (q < 0 || (t >= qe && q < a.S))) {
       q = seq_of(a, t);
       if (q < a.S) seq_rows(a, q, qb, qe);
       const bool some = q < a.S && qe > qb && gb != 0.f;
@@ -444,7 +582,7 @@ __global__ __launch_bounds__(kThreads) void router_grad_kernel(Rows a, int C, Gr
       }
     }
     const bool in = on && q < a.S && t >= qb && t < qe;
-    const float2 st = on ? o.stat[t] : make_float2(0.f, 0.f);
+    const float2 st = pick.stat;
     float rest[V], dot = 0.f;   // 1 - s
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -456,18 +594,14 @@ __global__ __launch_bounds__(kThreads) void router_grad_kernel(Rows a, int C, Gr
     // sum_k w_k g_k
     float wg = 0.f;
     if (o.g_weights) {
-      for (int k = i; k < a.K; k += L) {
-        const long at = (long)t * a.K + k;
-        if (on && (unsigned)a.ids[at] < (unsigned)a.E)
-          wg = __builtin_fmaf(o.weights[at], o.g_weights[at], wg);
-      }
+#pragma unroll
+      for (int n = 0; n < Ids<L>::N; ++n)
+        if (on && pick.id.e[n] >= 0) wg = __builtin_fmaf(pick.w[n], pick.g[n], wg);
       wg = sum_over<L>(wg);
       const float mean = a.renorm ? wg / a.scale : 0.f;
-      for (int k = i; k < a.K; k += L) {
-        const long at = (long)t * a.K + k;
-        const int e = on ? a.ids[at] : -1;
-        if ((unsigned)e < (unsigned)a.E) atomicAdd(&buf[g][e], o.weights[at] * (o.g_weights[at] - mean));
-      }
+#pragma unroll
+      for (int n = 0; n < Ids<L>::N; ++n)
+        if (on && pick.id.e[n] >= 0) atomicAdd(&buf[g][pick.id.e[n]], pick.w[n] * (pick.g[n] - mean));
     }
     const float lse = !SIG && in && st.y != 0.f ? st.x - logf(st.y) : 0.f;
     const float base = (in ? -dot : 0.f) + (gz != 0.f ? gz * lse : 0.f) -
@@ -510,11 +644,10 @@ __global__ __launch_bounds__(kThreads) void router_grad_kernel(Rows a, int C, Gr
       }
     }
     lds_order();
-    if (o.g_weights && on)
-      for (int k = i; k < a.K; k += L) {
-        const int e = a.ids[(long)t * a.K + k];
-        if ((unsigned)e < (unsigned)a.E) buf[g][e] = 0.f;
-      }
+    if (o.g_weights)
+#pragma unroll
+      for (int n = 0; n < Ids<L>::N; ++n)
+        if (on && pick.id.e[n] >= 0) buf[g][pick.id.e[n]] = 0.f;
     lds_order();
   }
 }
@@ -533,11 +666,17 @@ Layout layout_of(int E) {
   return {64, 16};
 }
 
-// Rows of a chunk: whole turns of a workgroup, about kMaxChunks chunks.
-int chunk_rows(int T, int E) {
-  const int ng = kWaves * 64 / layout_of(E).lanes;
-  const int c = T > 0 ? (int)(((long)T + kMaxChunks - 1) / kMaxChunks) : 1;
+// Rows of a chunk: whole turns of a workgroup, about `chunks` chunks.
+int chunk_rows(int T, int E, int waves, int chunks) {
+  const int ng = waves * 64 / layout_of(E).lanes;
+  const int c = T > 0 ? (int)(((long)T + chunks - 1) / chunks) : 1;
   return (c + ng - 1) / ng * ng;
+}
+int forward_rows(int T, int E) { return chunk_rows(T, E, kWaves, kMaxChunks); }
+
+// Whether one workgroup does it all.
+bool one_fits(int T, int E, int S) {
+  return T <= kOneTurns * kWaves * 64 / layout_of(E).lanes && S <= kOneSeqs;
 }
 
 // The workspace: partial rows, losses, ticket.
@@ -545,7 +684,7 @@ struct Space {
   size_t p, c, z, loss, zsum, ticket, bytes;
 };
 Space space_of(int T, int E, int S) {
-  const int C = chunk_rows(T, E);
+  const int C = forward_rows(T, E);
   const size_t slots = ((size_t)T + C - 1) / C + S, nb = (E + kCols - 1) / kCols;
   const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   Space s;
@@ -577,7 +716,7 @@ bool rows_of(const xtu_router_args& t, Rows& a) {
       t.S < 1 || t.S > (1 << 24) || t.mode < 0 || t.mode > 1 || !(t.scale > 0.f) ||
       !(t.scale < INFINITY))
     return false;
-  if ((long)t.S * ((t.E + kCols - 1) / kCols) * kThreads >= (1L << 32)) return false;   // the grid
+  if ((long)t.S * ((t.E + kCols - 1) / kCols) * kSumThreads >= (1L << 32)) return false;   // the grid
   if (t.T > 0 && (!t.logits || !t.ids || t.ld < 0)) return false;
   if (!t.starts && t.S != 1) return false;
   const size_t size = t.logits_bf16 ? 2 : 4;
@@ -616,28 +755,28 @@ hipError_t xtu_router_losses(const xtu_router_args* args, hipStream_t stream) {
   const Space s = space_of(t.T, t.E, t.S);
   XTU_CHECK_ARG(t.workspace_bytes >= s.bytes && reinterpret_cast<uintptr_t>(t.workspace) % 16 == 0);
   uint8_t* ws = reinterpret_cast<uint8_t*>(t.workspace);
-  float* pp = reinterpret_cast<float*>(ws + s.p);
-  int32_t* pc = reinterpret_cast<int32_t*>(ws + s.c);
-  float* pz = reinterpret_cast<float*>(ws + s.z);
-  unsigned* ticket = reinterpret_cast<unsigned*>(ws + s.ticket);
-  const int C = chunk_rows(t.T, t.E);
-  const int chunks = t.T ? (int)(((long)t.T + C - 1) / C) : 1;   // (one writes the ticket)
+  const Sums o{reinterpret_cast<float*>(ws + s.p), reinterpret_cast<int32_t*>(ws + s.c),
+               reinterpret_cast<float*>(ws + s.z), reinterpret_cast<double*>(ws + s.loss),
+               reinterpret_cast<double*>(ws + s.zsum), reinterpret_cast<unsigned*>(ws + s.ticket),
+               t.counts, t.probs, t.balance, t.z, t.norm};
+  const bool one = one_fits(t.T, t.E, t.S);
+  const int C = one ? (t.T ? t.T : 1) : forward_rows(t.T, t.E);
+  const int chunks = one ? 1 : (int)(((long)t.T + C - 1) / C);
+  const int grid = chunks ? chunks : 1;   // (one writes the ticket)
   (void)hipGetLastError();
   const auto go = [&](auto sig) {
     return by_layout<decltype(sig)::value>(t.E, [&](auto l, auto v) {
-      router_stats_kernel<decltype(l)::value, decltype(v)::value, decltype(sig)::value>
-          <<<chunks, kThreads, 0, stream>>>(a, C, t.weights, reinterpret_cast<float2*>(t.stat), pp,
-                                            pc, pz, ticket);
+      constexpr int L = decltype(l)::value, V = decltype(v)::value;
+      constexpr bool SIG = decltype(sig)::value;
+      const auto k = one ? router_stats_kernel<L, V, SIG, true> : router_stats_kernel<L, V, SIG, false>;
+      k<<<grid, kThreads, 0, stream>>>(a, C, t.weights, reinterpret_cast<float2*>(t.stat), o);
       return hipPeekAtLastError();
     });
   };
-  hipError_t e = t.mode ? go(std::true_type{}) : go(std::false_type{});
-  if (e != hipSuccess) return e;
+  const hipError_t e = t.mode ? go(std::true_type{}) : go(std::false_type{});
+  if (e != hipSuccess || one) return e;
   const int nb = (t.E + kCols - 1) / kCols;
-  const Sums o{pp, pc, pz, reinterpret_cast<double*>(ws + s.loss),
-               reinterpret_cast<double*>(ws + s.zsum), ticket, t.counts, t.probs, t.balance, t.z,
-               t.norm};
-  router_finish_kernel<<<(unsigned)t.S * nb, kThreads, 0, stream>>>(a, C, o);
+  router_finish_kernel<<<(unsigned)t.S * nb, kSumThreads, 0, stream>>>(a, C, o);
   return hipPeekAtLastError();
 }
 
@@ -652,14 +791,15 @@ hipError_t xtu_router_grad(const xtu_router_args* args, const float* g_weights,
   XTU_CHECK_ARG(t.counts && t.norm && t.weights && t.stat && dlogits);
   XTU_CHECK_ARG(t.mode == 0 || !g_z);
   XTU_CHECK_ARG(reinterpret_cast<uintptr_t>(dlogits) % 16 == 0);
-  const int C = chunk_rows(t.T, t.E), chunks = (int)(((long)t.T + C - 1) / C);
+  const int C = chunk_rows(t.T, t.E, kGradWaves, kGradChunks);
+  const int chunks = (int)(((long)t.T + C - 1) / C);
   const Grads o{reinterpret_cast<const float2*>(t.stat), t.weights, t.counts, t.norm, g_weights,
                 g_balance, g_z, dlogits};
   (void)hipGetLastError();
   const auto go = [&](auto sig) {
     return by_layout<decltype(sig)::value>(t.E, [&](auto l, auto v) {
       router_grad_kernel<decltype(l)::value, decltype(v)::value, decltype(sig)::value>
-          <<<chunks, kThreads, 0, stream>>>(a, C, o);
+          <<<chunks, kGradThreads, 0, stream>>>(a, C, o);
       return hipPeekAtLastError();
     });
   };
