@@ -48,15 +48,13 @@ struct Rows {
   float scale;
 };
 
-// e^x for x <= 0 (or NaN): 2^(x log2 e) with the product's rounding made good,
-// 2^-22 relative; the unit's exp alone is off by |x| 2^-24 more.
-__device__ __forceinline__ float exp_neg(float x) {
-  x = __builtin_elementwise_maximum(x, -150.f);   // -inf: 0 below; NaN stays
-  const float t = x * 1.44269502f;
-  float r = __builtin_fmaf(x, 1.44269502f, -t);
-  r = __builtin_fmaf(x, 1.92596303e-8f, r);
-  const float e = __builtin_amdgcn_exp2f(t);
-  return __builtin_fmaf(e, r * 0.693147182f, e);
+constexpr float kLog2e = 1.44269504f;
+
+// e^(l - m) as 2^(l log2 e - m log2 e): the rounding of the second product is the same for
+// all of a row and leaves its probabilities alone, that of the difference is |l - m| 2^-24.
+// Two instructions instead of eight with the difference's rounding made good.
+__device__ __forceinline__ float exp_from(float l, float m) {
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(l, kLog2e, -m * kLog2e));
 }
 
 // v of the lane across: within quads, halves of a row of 16, rows, and rows by
@@ -99,18 +97,50 @@ __device__ __forceinline__ float max_over(float v) {
   return reduce_over<L>(v, [](float x, float y) { return fmaxf(x, y); });
 }
 
-// The sum over a block's threads in every thread, in a fixed order; red: a value per
-// wave, not in use.
-template <int WAVES>
-__device__ __forceinline__ double block_sum(double v, double* red) {
+// The same for two's worth of bits.
+template <int D>
+__device__ __forceinline__ double across2(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  uint32_t lo = (uint32_t)b, hi = (uint32_t)(b >> 32);
+  if constexpr (D == 16) {
+    lo = __builtin_amdgcn_ds_swizzle(lo, 0x401F);   // lanes ^ 16
+    hi = __builtin_amdgcn_ds_swizzle(hi, 0x401F);
+  } else if constexpr (D == 32) {
+    const int other = ((int)__lane_id() ^ 32) * 4;
+    lo = __builtin_amdgcn_ds_bpermute(other, lo);
+    hi = __builtin_amdgcn_ds_bpermute(other, hi);
+  } else {
+    lo = __float_as_uint(across<D>(__uint_as_float(lo)));
+    hi = __float_as_uint(across<D>(__uint_as_float(hi)));
+  }
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+  v += across2<1>(v);
+  v += across2<2>(v);
+  v += across2<4>(v);
+  v += across2<8>(v);
+  v += across2<16>(v);
+  return v + across2<32>(v);
+}
+
+// The sums over a block's threads of N values each, in every thread and a fixed order;
+// red: not in use.
+template <int WAVES, int N>
+__device__ __forceinline__ void block_sums(double (&v)[N], double (*red)[N]) {
 #pragma unroll
-  for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d, 64);
-  if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = v;
+  for (int n = 0; n < N; ++n) {
+    v[n] = wave_sum(v[n]);
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64][n] = v[n];
+  }
   __syncthreads();
-  v = 0.;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) v += red[w];
-  return v;
+  for (int n = 0; n < N; ++n) {
+    v[n] = 0.;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) v[n] += red[w][n];
+  }
 }
 
 __device__ __forceinline__ void lds_order() {
@@ -179,20 +209,19 @@ __device__ __forceinline__ void values(const Rows& a, const Raw<L, V>& raw, floa
 
 // The score of a logit before its row's sum divides it.  softmax: e^(l - m), m the
 // row's maximum.  sigmoid: sigmoid(l) e^-m with m = min(maximum, 0), so that a row
-// of very negative logits keeps its ratios; sigmoid(l) = score e^m.
+// of very negative logits keeps its ratios; sigmoid(l) = score e^m.  rest: 1 -
+// sigmoid(l), without the cancellation.
 template <bool SIG>
-__device__ __forceinline__ float score(float l, float m) {
-  if constexpr (!SIG) return exp_neg(l - m);
-  const float e = exp_neg(-fabsf(l));
-  float num = l >= 0.f ? 1.f : e;
-  if (m < 0.f) num = exp_neg(l - m);
-  return num / (1.f + e);
-}
-
-// 1 - sigmoid(l), without the cancellation.
-__device__ __forceinline__ float one_minus_sigmoid(float l) {
-  const float e = exp_neg(-fabsf(l));
-  return (l >= 0.f ? e : 1.f) / (1.f + e);
+__device__ __forceinline__ float score(float l, float m, float& rest) {
+  if constexpr (!SIG) {
+    rest = 1.f;
+    return exp_from(l, m);
+  }
+  const float e = __builtin_amdgcn_exp2f(-fabsf(l) * kLog2e);
+  const float r = __builtin_amdgcn_rcpf(1.f + e), er = e * r;
+  rest = l >= 0.f ? er : r;
+  if (m < 0.f) return exp_from(l, m) * r;   // (every l < 0)
+  return l >= 0.f ? r : er;
 }
 
 __device__ __forceinline__ int start_of(const Rows& a, int q) {
@@ -266,11 +295,18 @@ __global__ __launch_bounds__(kThreads, ONE || V > 8 ? 4 : 8) void router_stats_k
   __shared__ __attribute__((aligned(16))) float buf[NG][COLS];
   __shared__ int32_t hist[COLS];
   __shared__ float zs[kWaves];
-  __shared__ double red[4][kWaves];
+  __shared__ double red[kWaves][4];
   const int tid = threadIdx.x, lane = tid % 64, w = tid / 64;
   const int i = lane % L, g = w * G + lane / L;
-  if (!ONE && blockIdx.x == 0 && tid == 0) *o.ticket = 0;   // of the next launch
   const int c0 = blockIdx.x * C, c1 = min(c0 + C, a.T);
+  Raw<L, V> next;
+  Ids<L> nid;
+  int t = c0 + g;
+  if (t < c1) {   // ahead of the sequences' bounds
+    load_row(a, t, i, next);
+    load_ids(a, t, i, nid);
+  }
+  if (!ONE && blockIdx.x == 0 && tid == 0) *o.ticket = 0;   // of the next launch
   for (int c = tid; c < COLS; c += kThreads) hist[c] = 0;
   double loss = 0., zsum = 0.;
   if (ONE) {
@@ -300,10 +336,8 @@ __global__ __launch_bounds__(kThreads, ONE || V > 8 ? 4 : 8) void router_stats_k
     float acc[V], z = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = 0.f;
-    Raw<L, V> next;
-    Ids<L> nid;
-    int t = at + g;
-    if (t < end) {
+    t = at + g;
+    if (at != c0 && t < end) {
       load_row(a, t, i, next);
       load_ids(a, t, i, nid);
     }
@@ -322,10 +356,10 @@ __global__ __launch_bounds__(kThreads, ONE || V > 8 ? 4 : 8) void router_stats_k
       m = max_over<L>(m);
       if (m == -INFINITY) m = 0.f;
       if (SIG) m = fminf(m, 0.f);
-      float s = 0.f;
+      float s = 0.f, rest;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        l[v] = score<SIG>(l[v], m);
+        l[v] = score<SIG>(l[v], m, rest);
         s += l[v];
       }
       lds_order();
@@ -345,7 +379,7 @@ __global__ __launch_bounds__(kThreads, ONE || V > 8 ? 4 : 8) void router_stats_k
       }
       if (a.renorm) total = sum_over<L>(total);
       float f = a.renorm ? (total == 0.f ? 0.f : a.scale / total)
-                         : a.scale * (SIG ? exp_neg(m) : inv);
+                         : a.scale * (SIG ? __builtin_amdgcn_exp2f(m * kLog2e) : inv);
       if (!SIG && s != s) f = s;   // a probability of such a row is NaN, whoever is selected
       if (!on) continue;
 #pragma unroll
@@ -412,11 +446,9 @@ __global__ __launch_bounds__(kThreads, ONE || V > 8 ? 4 : 8) void router_stats_k
       rows += e - b;
       seqs += e > b;
     }
-    loss = block_sum<kWaves>(loss, red[0]);
-    zsum = block_sum<kWaves>(zsum, red[1]);
-    rows = block_sum<kWaves>(rows, red[2]);
-    seqs = block_sum<kWaves>(seqs, red[3]);
-    if (tid == 0) write_losses(o, loss, zsum, rows, seqs);
+    double v[4] = {loss, zsum, rows, seqs};
+    block_sums<kWaves>(v, red);
+    if (tid == 0) write_losses(o, v[0], v[1], v[2], v[3]);
   }
 }
 
@@ -434,7 +466,7 @@ __global__ __launch_bounds__(kSumThreads) void router_finish_kernel(Rows a, int 
   constexpr int R = kSumThreads / kCols, WAVES = kSumThreads / 64;
   __shared__ double sp[R][kCols];
   __shared__ int32_t sc[R][kCols];
-  __shared__ double red[5][WAVES];
+  __shared__ double red1[WAVES][1], red4[WAVES][4];
   __shared__ bool last;
   const int tid = threadIdx.x, nb = (a.E + kCols - 1) / kCols;
   const int q = blockIdx.x / nb, b = blockIdx.x % nb;
@@ -443,7 +475,7 @@ __global__ __launch_bounds__(kSumThreads) void router_finish_kernel(Rows a, int 
   seq_rows(a, q, begin, end);
   const int n = end - begin;
   const int g0 = begin / C, g1 = n > 0 ? (end - 1) / C + 1 : g0;
-  double p = 0., z = 0.;
+  double p = 0., zz[1] = {0.};
   int32_t c = 0;
   if (e < a.E) {
 #pragma unroll 8
@@ -454,10 +486,10 @@ __global__ __launch_bounds__(kSumThreads) void router_finish_kernel(Rows a, int 
     }
   }
   if (b == 0)
-    for (int g = g0 + tid; g < g1; g += kSumThreads) z += o.part_z[(long)g + q];
+    for (int g = g0 + tid; g < g1; g += kSumThreads) zz[0] += o.part_z[(long)g + q];
   sp[r][col] = p;
   sc[r][col] = c;
-  if (b == 0) z = block_sum<WAVES>(z, red[0]);   // (the same for the whole workgroup)
+  if (b == 0) block_sums<WAVES>(zz, red1);   // (the same for the whole workgroup)
   else __syncthreads();
   if (tid < 64) {
     double loss = 0.;
@@ -472,11 +504,10 @@ __global__ __launch_bounds__(kSumThreads) void router_finish_kernel(Rows a, int 
       o.counts[(long)q * a.E + e] = c;
       loss = n > 0 ? p * c * a.E / ((double)a.K * n) : 0.;
     }
-#pragma unroll
-    for (int d = kCols / 2; d > 0; d /= 2) loss += __shfl_xor(loss, d, 64);
+    loss = wave_sum(loss);
     if (tid == 0) {
       store_far(&o.loss[blockIdx.x], loss);
-      if (b == 0) store_far(&o.zsum[q], z);
+      if (b == 0) store_far(&o.zsum[q], zz[0]);
       __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");   // they are there before the ticket
       last = __hip_atomic_fetch_add(o.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
              gridDim.x - 1;
@@ -484,21 +515,17 @@ __global__ __launch_bounds__(kSumThreads) void router_finish_kernel(Rows a, int 
   }
   __syncthreads();
   if (!last) return;
-  double sum = 0., rows = 0., seqs = 0.;
-  z = 0.;
-  for (long k = tid; k < (long)a.S * nb; k += kSumThreads) sum += load_far(&o.loss[k]);
+  double v[4] = {0., 0., 0., 0.};   // losses, z, rows, sequences
+  for (long k = tid; k < (long)a.S * nb; k += kSumThreads) v[0] += load_far(&o.loss[k]);
   for (int k = tid; k < a.S; k += kSumThreads) {
     int x, y;
     seq_rows(a, k, x, y);
-    z += load_far(&o.zsum[k]);
-    rows += y - x;
-    seqs += y > x;
+    v[1] += load_far(&o.zsum[k]);
+    v[2] += y - x;
+    v[3] += y > x;
   }
-  sum = block_sum<WAVES>(sum, red[1]);
-  z = block_sum<WAVES>(z, red[2]);
-  rows = block_sum<WAVES>(rows, red[3]);
-  seqs = block_sum<WAVES>(seqs, red[4]);
-  if (tid == 0) write_losses(o, sum, z, rows, seqs);
+  block_sums<WAVES>(v, red4);
+  if (tid == 0) write_losses(o, v[0], v[1], v[2], v[3]);
 }
 
 struct Grads {
@@ -586,8 +613,7 @@ __global__ __launch_bounds__(kGradThreads) void router_grad_kernel(Rows a, int C
     float rest[V], dot = 0.f;   // 1 - s
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      if (SIG) rest[v] = one_minus_sigmoid(l[v]);
-      l[v] = score<SIG>(l[v], st.x) * st.y;   // p
+      l[v] = score<SIG>(l[v], st.x, rest[v]) * st.y;   // p
       dot = __builtin_fmaf(l[v], h[v], dot);
     }
     dot = sum_over<L>(dot);
