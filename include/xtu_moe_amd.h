@@ -641,11 +641,10 @@ int xtu_linear_plan(int M, int N, int K, int act);
  * - 8, fp32 per group of 32, 64 or 128).  K a multiple of the group, any N.  w: the
  * records of formats.pack_linear4 (xtu_linear4_weight_bytes of them, 16-byte aligned):
  * per panel of 16 rows (act 6: gate and up panels in turn) and block of 128 k 1024
- * bytes of codes [4 q][16 row][16], then the scales.  MXFP4, NVFP4: a 16-byte chunk
- * holds k = 32 q .. + 31 (low nibble = even k), scales [4 q][16 row][1 or 2].  INT4:
- * dword j of a chunk holds k = 32 j + 8 q .. + 7 as code ^ 8, scales fp32
- * [128 / group][16 row], times 16.  Rows and k past the matrix: codes 0, e8m0 127 or
- * scale 0.  The products are exact in the fp32 sums' operands (INT4: the scale
+ * bytes of codes [4 q][16 row][4 j][4], dword j holding k = 32 j + 8 q .. + 7 (low
+ * nibble first; INT4: code ^ 8), then the scales: MXFP4 [16 row][4 j] bytes, NVFP4
+ * [2 q / 2][16 row][4 j] bytes, INT4 fp32 [128 / group][16 row], times 16.  Rows and
+ * k past the matrix: codes 0 (INT4 too), e8m0 127 or scale 0.  The products are exact in the fp32 sums' operands (INT4: the scale
  * multiplies each group's fp32 sum).  workspace: as xtu_linear's, for K splits.  The
  * reference leaves these products to its host (vllm_xiaotu_moe/hybrid_model.py:1752). */
 typedef struct xtu_linear4_args {

@@ -190,7 +190,7 @@ def test_scales_over_their_range():
     """e8m0 from 0 to 252, e4m3 from its smallest to 448, INT4's -8 and far scales."""
     x = _rand((3, 64), 1, 0.5)
     codes = torch.full((16, 32), 0x77, dtype=torch.uint8)   # 6
-    for b in (1, 20, 127, 200, 250):
+    for b in (0, 1, 20, 127, 200, 250):
         W = Weight4.from_dense("mxfp4", codes.to(DEV), torch.full((16, 2), b, dtype=torch.uint8,
                                                                   device=DEV))
         w = torch.full((16, 64), 6 * 2.0 ** (b - 127), dtype=torch.float64, device=DEV)

@@ -46,11 +46,8 @@ def test_records(fmt, group, gated):
             assert _lib.load().xtu_linear4_weight_bytes(N, K, 6 if gated else 0, fmt, group) == W.nbytes
         n, k = torch.meshgrid(torch.arange(P * 16), torch.arange(B * 128), indexing="ij")
         b, kk = k // 128, k % 128
-        if fmt == F.FMT_INT4:
-            j, q, i = kk // 32, kk // 8 % 4, kk % 8
-            byte = 4 * j + i // 2
-        else:
-            q, byte = kk // 32, kk % 32 // 2
+        j, q = kk // 32, kk // 8 % 4
+        byte = 4 * j + kk % 8 // 2
         for h in range(halves):
             pan = (n // 16) * halves + h
             got = W.data[pan, b, (q * 16 + n % 16) * 16 + byte] >> (4 * (kk % 2)) & 15
@@ -64,9 +61,10 @@ def test_records(fmt, group, gated):
                 planes = W.data[..., 1024:].contiguous().view(torch.float32)
                 got = planes[pan, b, kk // group * 16 + n % 16]
                 sv = sv * 16
+            elif fmt == F.FMT_MXFP4:
+                got = W.data[pan, b, 1024 + (n % 16) * 4 + j]
             else:
-                per = 32 // group
-                got = W.data[pan, b, 1024 + (q * 16 + n % 16) * per + kk % 32 // group]
+                got = W.data[pan, b, 1024 + q // 2 * 64 + (n % 16) * 4 + j]
             assert torch.equal(got, sv)
 
 

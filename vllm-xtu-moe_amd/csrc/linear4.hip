@@ -42,7 +42,7 @@ size_t xtu_linear4_workspace_bytes(int M, int N, int K, int act, int fmt, int gr
   LinearArgs e{};
   e.M = M;
   e.K = K;
-  if (skinny4_fits(e)) return 0;
+  if (skinny4_fits(e) || rows4_fits(e)) return 0;
   return split_bytes(plan4_tile(M, N, K, gated, true), M, N, gated);
 }
 
@@ -76,7 +76,11 @@ hipError_t xtu_linear4(const xtu_linear4_args* args, hipStream_t stream) {
   a.group = t.group;
   a.xvec = al(t.x, 16) && K % 8 == 0 && (M == 1 || t.ldx % 8 == 0);
   (void)hipGetLastError();
+#ifdef L4_NOSKINNY
+  if (rows4_fits(a.e)) return launch4_rows(a, stream);
+#endif
   if (skinny4_fits(a.e)) return launch4_skinny(a, stream);
+  if (rows4_fits(a.e)) return launch4_rows(a, stream);
   Plan4 p = plan4_tile(M, N, K, gated, true);
   if (split_bytes(p, M, N, gated) > (t.workspace ? t.workspace_bytes : 0))
     p = plan4_tile(M, N, K, gated, false);

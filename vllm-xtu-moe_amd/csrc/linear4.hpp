@@ -13,15 +13,15 @@
 // group's fp32 sum.  The epilogue is linear.hpp's.
 //
 // Layout.  Rows in panels of 16 (swiglu: gate and up panels in turn), K in blocks
-// of 128; a block of a panel is one record: 1024 bytes of codes [4 q][16 row][16 B],
-// lane 16 q + row of a wave takes 16 of them, then its scales.
-//   MXFP4, NVFP4: a lane's 16 bytes hold k = 32 q .. 32 q + 31 in order, so that all of
-//     them share one (NVFP4: two) of the scales [4 q][16 row][1 or 2 B].
-//   INT4: dword j of a lane holds k = 32 j + 8 q .. + 7 (as code ^ 8, two's complement),
-//     so that an MFMA's 32 k are of one group; scales fp32 [128 / G][16 row], times
-//     16 (i4x8_to_bf16).
+// of 128; a block of a panel is one record: 1024 bytes of codes [4 q][16 row][4 j][4 B],
+// lane 16 q + row of a wave takes 16 of them, dword j the codes of k = 32 j + 8 q .. + 7
+// (low nibble first; INT4: as code ^ 8, two's complement), which are an MFMA operand's.
+// So an MFMA's 32 k are consecutive, x is read as it lies, and an INT4 group is whole
+// MFMAs.  Then the record's scales, a dword of four for the lanes that share them:
+//   MXFP4: [16 row][4 j] bytes        NVFP4: [2 q / 2][16 row][4 j] bytes
+//   INT4:  fp32 [128 / G][16 row], times 16 (i4x8_to_bf16)
 // A panel's records are consecutive: a wave walks one stream.  Rows and k past the
-// matrix are zero codes under scale one (INT4: zero).
+// matrix are zero codes under scale one (NVFP4, INT4: zero).
 #pragma once
 #include <type_traits>
 
@@ -86,9 +86,9 @@ __device__ __forceinline__ Raw<FMT, G> load_raw(const uint8_t* rec, int q, int r
   r.c = *reinterpret_cast<const u32x4_t*>(rec + (16 * q + row) * 16);
   const uint8_t* sc = rec + 1024;
   if constexpr (FMT == kMx) {
-    r.s = sc[16 * q + row];
+    r.s = *reinterpret_cast<const uint32_t*>(sc + 4 * row);
   } else if constexpr (FMT == kNv) {
-    r.s = *reinterpret_cast<const uint16_t*>(sc + 2 * (16 * q + row));
+    r.s = *reinterpret_cast<const uint32_t*>(sc + 64 * (q / 2) + 4 * row);
   } else {
 #pragma unroll
     for (int g = 0; g < 128 / G; ++g)
@@ -104,17 +104,12 @@ __device__ __forceinline__ u32x4_t operand(const Raw<FMT, G>& r, int j) {
     return i4x8_to_bf16(r.c[j]);
   } else {
     uint32_t o[4];
-    if constexpr (FMT == kMx) fp4x8_to_bf16(r.c[j], e8m0_to_f32(r.s), o);
-    else fp4x8_to_bf16_mul(r.c[j], e4m3_to_f32(j < 2 ? r.s & 0xffu : r.s >> 8), o);
+    // (the converter takes the exponent bits alone: a byte 0 means 2^-127 to it)
+    if constexpr (FMT == kMx)
+      fp4x8_to_bf16(r.c[j], __uint_as_float((j < 3 ? r.s << (23 - 8 * j) : r.s >> 1) & 0x7f800000u), o);
+    else fp4x8_to_bf16_mul(r.c[j], e4m3_to_f32(r.s >> (8 * j)), o);
     return u32x4_t{o[0], o[1], o[2], o[3]};
   }
-}
-
-// Where the 16 bytes of k = 8 p .. 8 p + 7 of a block of x lie in LDS: the lanes of an
-// MFMA of dword j read places 4 j + q.
-template <int FMT>
-__device__ __forceinline__ int place_of(int p) {
-  return FMT == kI4 ? p : p % 4 * 4 + p / 4;
 }
 
 // One block of NP panels times MT blocks of 16 rows of x; x(j, mt) gives the operand
@@ -173,6 +168,10 @@ __device__ __forceinline__ u32x4_t load_x8(const Linear4Args& a, const uint16_t*
 constexpr size_t kSkinny4Lds = 120 * 1024;
 bool skinny4_fits(const LinearArgs& e);
 hipError_t launch4_skinny(const Linear4Args& a, hipStream_t stream);
+
+// At most 64 rows of x.
+bool rows4_fits(const LinearArgs& e);
+hipError_t launch4_rows(const Linear4Args& a, hipStream_t stream);
 
 struct Plan4 {
   int kind, split;   // kind: blocks of 16 rows of a tile

@@ -43,8 +43,7 @@ __global__ __launch_bounds__(64 * WV) void linear4_skinny_kernel(Linear4Args a, 
   uint16_t* xs = reinterpret_cast<uint16_t*>(lds);
   for (int p = tid; p < e.M * pieces; p += 64 * WV) {
     const int r = p / pieces, k8 = p - r * pieces;
-    *reinterpret_cast<u32x4_t*>(xs + r * ldx + (k8 / 16 * 16 + place_of<FMT>(k8 % 16)) * 8) =
-        load_x8(a, e.x + (long)r * e.ldx, 8 * k8);
+    *reinterpret_cast<u32x4_t*>(xs + r * ldx + 8 * k8) = load_x8(a, e.x + (long)r * e.ldx, 8 * k8);
   }
   __syncthreads();
   const uint16_t* xl = xs + min(c, e.M - 1) * ldx + 8 * q;

@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256) void linear4_tile_kernel(Linear4Args a, int pe
 #pragma unroll
     for (int i = 0; i < MT; ++i)
       *reinterpret_cast<u32x4_t*>(lds + st * STAGE + (16 * i + xr) * 256 +
-                                  slot(place_of<FMT>(xp), xr)) = xv[i];
+                                  slot(xp, xr)) = xv[i];
   };
   f32x4_t acc[NP][MT];
 #pragma unroll

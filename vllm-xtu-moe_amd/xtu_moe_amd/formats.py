@@ -275,7 +275,7 @@ def unpack_scales(fmt: int, p, N: int, K: int):
 
 # ------------------------------------------------- 4-bit weights of linear4
 # records: per panel of 16 rows and block of 128 k, 1024 bytes of codes
-# [4 q][16 row][16 B], then the scales
+# [4 q][16 row][4 j][4 B] (k = 32 j + 8 q .. + 7), then the scales
 def linear4_group(fmt: int, s, K: int) -> int:
     """The k per scale of a matrix's scales [N, K / group]."""
     if s.dim() != 2 or s.shape[1] == 0 or K % s.shape[1]:
@@ -298,16 +298,17 @@ def pack_linear4(fmt: int, codes, s, group: int):
     pad = torch.nn.functional.pad
     c = codes ^ 0x88 if fmt == FMT_INT4 else codes
     c = pad(c, (0, B * 64 - K // 2, 0, P * 16 - N))
-    if fmt == FMT_INT4:   # [n][panel][row][block][j][q][4 B] -> [panel][n][block][q][row][j][4 B]
-        c = c.view(n, P, 16, B, 4, 4, 4).permute(1, 0, 3, 5, 2, 4, 6)
+    # [n][panel][row][block][j][q][4 B] -> [panel][n][block][q][row][j][4 B]
+    c = c.view(n, P, 16, B, 4, 4, 4).permute(1, 0, 3, 5, 2, 4, 6)
+    if fmt == FMT_INT4:
         s = pad(s.float() * 16.0, (0, B * (128 // group) - K // group, 0, P * 16 - N))
         s = s.view(n, P, 16, B, 128 // group).permute(1, 0, 3, 4, 2).contiguous().view(torch.uint8)
-    else:                 # [n][panel][row][block][q][16 B] -> [panel][n][block][q][row][16 B]
-        c = c.view(n, P, 16, B, 4, 16).permute(1, 0, 3, 4, 2, 5)
-        per = 32 // group
-        s = pad(s.view(torch.uint8), (0, B * 4 * per - K // group, 0, P * 16 - N),
-                value=127 if fmt == FMT_MXFP4 else 0)
-        s = s.view(n, P, 16, B, 4, per).permute(1, 0, 3, 4, 2, 5)
+    elif fmt == FMT_MXFP4:   # [n][panel][row][block][j] -> [panel][n][block][row][j]
+        s = pad(s, (0, B * 4 - K // 32, 0, P * 16 - N), value=127)
+        s = s.view(n, P, 16, B, 4).permute(1, 0, 3, 2, 4)
+    else:                    # [n][panel][row][block][j][q / 2] -> [panel][n][block][q / 2][row][j]
+        s = pad(s.view(torch.uint8), (0, B * 8 - K // 16, 0, P * 16 - N))
+        s = s.view(n, P, 16, B, 4, 2).permute(1, 0, 3, 5, 2, 4)
     return torch.cat([c.reshape(P * n, B, 1024), s.reshape(P * n, B, -1)], 2)
 
 
