@@ -642,9 +642,10 @@ int xtu_linear_plan(int M, int N, int K, int act);
  * records of formats.pack_linear4 (xtu_linear4_weight_bytes of them, 16-byte aligned):
  * per panel of 16 rows (act 6: gate and up panels in turn) and block of 128 k 1024
  * bytes of codes [4 q][16 row][4 j][4], dword j holding k = 32 j + 8 q .. + 7 (low
- * nibble first; INT4: code ^ 8), then the scales: MXFP4 [16 row][4 j] bytes, NVFP4
- * [2 q / 2][16 row][4 j] bytes, INT4 fp32 [128 / group][16 row], times 16.  Rows and
- * k past the matrix: codes 0 (INT4 too), e8m0 127 or scale 0.  The products are exact in the fp32 sums' operands (INT4: the scale
+ * nibble first; INT4: byte b holds k = b and 4 + b of them, value v as v, negative
+ * as 7 - v), then the scales: MXFP4 [16 row][4 j] bytes, NVFP4 [2 q / 2][16 row][4 j]
+ * bytes, INT4 fp32 [128 / group][16 row].  Rows and k past the matrix: codes 0, e8m0
+ * 127 or scale 0.  The products are exact in the fp32 sums' operands (INT4: the scale
  * multiplies each group's fp32 sum).  workspace: as xtu_linear's, for K splits.  The
  * reference leaves these products to its host (vllm_xiaotu_moe/hybrid_model.py:1752). */
 typedef struct xtu_linear4_args {
@@ -665,6 +666,11 @@ typedef struct xtu_linear4_args {
 hipError_t xtu_linear4(const xtu_linear4_args* args, hipStream_t stream);
 size_t xtu_linear4_weight_bytes(int N, int K, int act, int fmt, int group);
 size_t xtu_linear4_workspace_bytes(int M, int N, int K, int act, int fmt, int group);
+/* Which kernel a product with all of that workspace takes, 16 * (K splits) + 0 the
+ * stream of w (all of x in LDS), 1 rows (nothing staged), 2 slabs (a range of K of x in
+ * LDS), 3 and 4 tiles of 128 x 128 and 128 x 256, 5 tiles of 64 x 128 for rows of x
+ * that do not start on 16 bytes (aligned 0); -1 none. */
+int xtu_linear4_plan(int M, int N, int K, int act, int fmt, int group, int aligned);
 
 /* ------------------------------------------------ router, training step
  * What a training step takes from router logits [T][E] (fp32, or bf16 with

@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from test_gpu_linear import _act64
-from test_linear4 import GROUPS
+from test_linear4 import GROUPS, forms
 from xtu_moe_amd import formats as F
 from xtu_moe_amd.linear import ACTIVATIONS
 from xtu_moe_amd.linear4 import Weight4, linear4
@@ -105,6 +105,22 @@ def test_sizes(fmt, group, gated):
             for odt in (BF, F32):
                 out = linear4(x, W, activation="swiglu" if gated else "none", out_dtype=odt)
                 _check(out, x, w, "swiglu" if gated else "none", what=(M, N, K, odt))
+
+
+@pytest.mark.parametrize("fmt,group", GROUPS)
+@pytest.mark.parametrize("gated", [False, True])
+def test_every_form(fmt, group, gated):
+    """Each kernel, whole and with K split, with the whole epilogue."""
+    for i, ((kernel, _), M, N, K) in enumerate(forms(fmt, group, gated)):
+        x = _rand((M, K + 8), i)
+        x = x[:, 1:K + 1] if kernel == 5 else x[:, :K]
+        W, w = _weight(fmt, group, N, K, gated, seed=70 + i)
+        b = _rand((w.shape[0],), 2, 0.5, F32)
+        r = _rand((M, N), 4, 1.0, BF if i % 2 else F32)
+        for act in ("swiglu",) if gated else ("none", "gelu"):
+            out = linear4(x, W, bias=b, activation=act, residual=r, out_dtype=F32)
+            _check(out, x, w, act, b, residual=r, what=(kernel, M, N, K, act))
+        _check(linear4(x, W, activation=act), x, w, act, what=(kernel, M, N, K))
 
 
 @pytest.mark.parametrize("act", list(ACTIVATIONS))

@@ -24,6 +24,39 @@ def _dense(fmt, rows, K, group, seed=0):
     return codes, s, 0.25 if fmt == F.FMT_NVFP4 else None
 
 
+# (kernel, K split or not) -> M, N, K of a product that takes it, for every format;
+# gated ones have the same number of rows
+FORMS = {
+    (0, False): [(1, 300, 512), (3, 1000, 1024), (1, 166, 6528)],
+    (1, False): [(1, 6022, 1792), (28, 75, 896), (40, 1503, 256), (54, 3011, 128)],
+    (2, False): [(45, 16911, 256), (63, 18531, 896), (32, 19170, 768)],
+    (2, True): [(14, 2000, 8192), (23, 464, 5760), (47, 29, 7552), (58, 308, 3456)],
+    (3, False): [(65, 16, 128), (137, 1140, 384)],
+    (3, True): [(71, 16, 768), (123, 504, 2816)],
+    (4, False): [(1224, 3405, 256), (1887, 2884, 384)],
+    (4, True): [(263, 3675, 3584)],
+    (5, False): [(70, 16, 128), (353, 490, 384)],
+    (5, True): [(81, 17, 512), (300, 1228, 512)],
+}
+
+
+def forms(fmt, group, gated):
+    """(form, M, N, K) of this format: INT4's finer groups have no kernel 4."""
+    for form, sizes in FORMS.items():
+        if form[0] != 4 or fmt != F.FMT_INT4 or group == 128:
+            for M, N, K in sizes:
+                yield form, M, N // 2 if gated else N, K
+
+
+@pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
+@pytest.mark.parametrize("fmt,group", GROUPS)
+@pytest.mark.parametrize("gated", [False, True])
+def test_forms_are_taken(fmt, group, gated):
+    for (kernel, split), M, N, K in forms(fmt, group, gated):
+        plan = _lib.load().xtu_linear4_plan(M, N, K, 6 if gated else 0, fmt, group, int(kernel != 5))
+        assert (plan % 16, plan >= 32) == (kernel, split), (M, N, K, plan % 16, plan // 16)
+
+
 def _w(fmt="mxfp4", rows=4, K=32, gated=False):
     group = {"mxfp4": 32, "nvfp4": 16, "int4": 32}[fmt]
     c, s, gs = _dense(F.fmt_of(fmt), rows, K, group)
@@ -47,20 +80,20 @@ def test_records(fmt, group, gated):
         n, k = torch.meshgrid(torch.arange(P * 16), torch.arange(B * 128), indexing="ij")
         b, kk = k // 128, k % 128
         j, q = kk // 32, kk // 8 % 4
-        byte = 4 * j + kk % 8 // 2
+        i = kk % 8
+        byte, high = (4 * j + i % 4, i // 4) if fmt == F.FMT_INT4 else (4 * j + i // 2, i % 2)
         for h in range(halves):
             pan = (n // 16) * halves + h
-            got = W.data[pan, b, (q * 16 + n % 16) * 16 + byte] >> (4 * (kk % 2)) & 15
+            got = W.data[pan, b, (q * 16 + n % 16) * 16 + byte] >> (4 * high) & 15
             want = torch.zeros(P * 16, B * 128, dtype=torch.uint8)
             nib = torch.stack([codes & 15, codes >> 4], -1).view(halves, N, K)[h]
-            want[:N, :K] = nib ^ 8 if fmt == F.FMT_INT4 else nib
+            want[:N, :K] = torch.where(nib >= 8, nib - 8, 15 - nib) if fmt == F.FMT_INT4 else nib
             assert torch.equal(got, want)
             sv = torch.full((P * 16, B * 128), 127 if fmt == F.FMT_MXFP4 else 0, dtype=s.dtype)
             sv[:N, :K] = s.view(halves, N, -1)[h].repeat_interleave(group, 1)
             if fmt == F.FMT_INT4:
                 planes = W.data[..., 1024:].contiguous().view(torch.float32)
                 got = planes[pan, b, kk // group * 16 + n % 16]
-                sv = sv * 16
             elif fmt == F.FMT_MXFP4:
                 got = W.data[pan, b, 1024 + (n % 16) * 4 + j]
             else:

@@ -90,6 +90,11 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a) {
   }
 }
 
+template <int V>
+struct PartOf { typedef f32x4_t type; };
+template <>
+struct PartOf<1> { typedef float type; };
+
 // Adds the partial sums of the K splits, in their order, and finishes the
 // elements; one thread per V (4 or 1) columns of a row.
 template <int AK, int V>
@@ -102,21 +107,27 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int spli
   const int m = (int)(t / gn), n = (int)(t % gn) * V;
   const long plane = part_plane(a);
   const float* p = part + (long)m * a.N * (GATED ? 2 : 1) + n;
-  if constexpr (V == 4) {
-    f32x4_t z = {0.f, 0.f, 0.f, 0.f}, u = z;
-    for (int k = 0; k < split; ++k, p += plane) {
-      z += *reinterpret_cast<const f32x4_t*>(p);
-      if constexpr (GATED) u += *reinterpret_cast<const f32x4_t*>(p + a.N);
+  // eight planes at a time are asked for before any is added: one memory latency for
+  // them, not one each
+  constexpr int B = 8;
+  typedef typename PartOf<V>::type part_t;
+  const auto add = [&](const float* at) {
+    part_t s{}, v[B];
+    for (int k0 = 0; k0 < split; k0 += B) {
+#pragma unroll
+      for (int i = 0; i < B; ++i)
+        if (k0 + i < split) v[i] = *reinterpret_cast<const part_t*>(at + (k0 + i) * plane);
+#pragma unroll
+      for (int i = 0; i < B; ++i)
+        if (k0 + i < split) s += v[i];
     }
-    finish4<AK>(a, m, n, z, u);
-  } else {
-    float z = 0.f, u = 0.f;
-    for (int k = 0; k < split; ++k, p += plane) {
-      z += p[0];
-      if constexpr (GATED) u += p[a.N];
-    }
-    finish_one<AK>(a, m, n, z, u);
-  }
+    return s;
+  };
+  const part_t z = add(p);
+  part_t u{};
+  if constexpr (GATED) u = add(p + a.N);
+  if constexpr (V == 4) finish4<AK>(a, m, n, z, u);
+  else finish_one<AK>(a, m, n, z, u);
 }
 
 // x and w as rows of K8 = K rounded up to 8, zeros behind K: what the tile

@@ -1,4 +1,4 @@
-// The product with 4-bit weights: argument checks and dispatch.
+// The product with 4-bit weights: argument checks and the choice of a kernel.
 #include "linear4.hpp"
 
 #include "../../include/xtu_moe_amd.h"
@@ -6,10 +6,13 @@
 using namespace xtu;
 using namespace xtu::l4;
 
+namespace xtu {
+namespace l4 {
 namespace {
 
 // Rows past M, up to a tile's 128, are ints too; columns and k as the dense product.
 constexpr int kMaxM = 0x7fffffff - 511, kMaxN = 1 << 28, kMaxK = 1 << 28;
+constexpr int kCus = 256;
 
 bool format_ok(int fmt, int group) {
   if (fmt == kMx) return group == 32;
@@ -22,11 +25,124 @@ bool sizes_ok(int M, int N, int K, int act, int fmt, int group) {
          act >= lin::kNone && act <= lin::kSwiglu && format_ok(fmt, group) && K % group == 0;
 }
 
-size_t split_bytes(const Plan4& p, int M, int N, bool gated) {
-  return p.split > 1 ? (size_t)p.split * M * N * (gated ? 2 : 1) * 4 : 0;
+long up(long n, long d) { return (n + d - 1) / d; }
+
+// Estimated times in us.  A CU takes in about 25 KB a us of what comes in small pieces (w,
+// and x by fragments) and twice that of rows staged whole; a launch and its latencies
+// are 3 to 5, the launch that adds K splits 3 and its partial sums' way.
+
+float join_time(const Shape4& s, int split) {
+  if (split == 1) return 0.f;
+  return 3.0f + 2.f * split * s.M * (float)s.N * (s.gated ? 2 : 1) * 4.f / 5e6f;
+}
+
+float skinny_time(const Shape4& s) {
+  const SkinnyPlan p = skinny4_plan(s);
+  if (p.grid == 0) return 1e30f;
+  const int nb = blocks_of(s.K);
+  const float x = s.M * (float)s.K * 2e-3f;
+  const float w = up(p.units, p.grid) * (s.gated ? 2 : 1) * (float)nb *
+                  record_bytes(s.fmt, s.group) * p.rows / 16 * 1e-3f;
+  return 3.0f + 0.1f * (nb < 16 ? nb : 16) + up(p.grid, kCus) * (x / 50.f + w / 25.f);
+}
+
+float rows_time(const Shape4& s) {
+  const int nb = blocks_of(s.K);
+  const long steps = up(nb, rows4_waves(s));
+  const float kb = s.M * (float)s.K * 2e-3f + 2.f * nb * record_bytes(s.fmt, s.group) * 1e-3f;
+  return 3.2f + up(up(s.N, s.gated ? 16 : 32), kCus) * kb / 25.f + 0.5f * (steps - 1);
+}
+
+// The split of K with the least time, 0 where no range of K fits LDS.
+int slab_split(const Shape4& s, bool may_split, float& time) {
+  const int nb = blocks_of(s.K);
+  const long gx = up(s.N, (s.gated ? 16 : 32) * kSlabWaves);
+  int best = 0;
+  time = 1e30f;
+  for (int split = 1; split <= nb && split <= (may_split ? 64 : 1); ++split) {
+    const int per = (int)up(nb, split);
+    if (up(nb, per) != split || slab4_lds(s.M, per) > kSlabLds) continue;
+    const float kb =
+        per * (s.M * 256.f + 2.f * kSlabWaves * record_bytes(s.fmt, s.group)) * 1e-3f;
+    const float t = 4.0f + up(gx * split, kCus) * kb / 25.f + join_time(s, split);
+    if (t < time) {
+      time = t;
+      best = split;
+    }
+  }
+  return best;
+}
+
+// Up to 64 rows.  Measured, in us (stream of w / rows / slab, MXFP4): M 1: 7168 x 2048
+// 5.8 / 4.8 / 7.2, 7168 x 7168 9.0 / 10.2 / 11.8, 2048 x 16384 9.1 / 14.4 / 11.2,
+// 16384 gated x 7168 24.6 / 29.7 / 32; M 8: 7168 x 7168 11.9 / 12.3 / 12.6; M 16:
+// 512 gated x 2048 6.7 / 7.5 / 9.1, 7168 x 7168 - / 16.0 / 13.6; M 32: 7168 x 2048
+// - / 10.1 / 11.9, 7168 x 7168 - / 22.2 / 15.8; M 64: 7168 x 2048 - / 17.1 / 15.0,
+// 7168 x 7168 - / 40 / 21.
+Plan4 plan_few(const Shape4& s, bool may_split) {
+  float slab;
+  const int split = slab_split(s, may_split, slab);
+  const float skinny = skinny_time(s), rows = rows_time(s);
+  if (skinny <= rows && skinny <= slab) return {kSkinny4, 1};
+  if (rows <= slab) return {kRows4, 1};
+  return {kSlab4, split};
+}
+
+// Steps of 128 k of a tile of 128 rows and 256 or 128 rows of w, alone on its CU, in us
+// (2048 x 2048 gated x 7168, one round of the larger and two of the smaller: MXFP4 91 /
+// 122, NVFP4 115 / 140, INT4 with groups of 128 121 / 148; 128 x 7168 x 2048 in 28 and
+// 56 tiles: 29 / 20).  INT4's finer groups have no room for the larger one's sums.
+Plan4 plan_many(const Shape4& s, bool may_split) {
+  const bool fine = s.fmt == kI4 && s.group != 128;
+  const float step4 = s.fmt == kMx ? 1.5f : s.fmt == kNv ? 1.95f : 2.1f;
+  const float step2 = s.fmt == kMx ? 1.03f : s.fmt == kNv ? 1.2f : fine ? 1.7f : 1.3f;
+  const int nb = blocks_of(s.K);
+  Plan4 best{kWide2, 1};
+  float time = 1e30f;
+  for (int kind : {kWide4, kWide2}) {
+    if (kind == kWide4 && fine) continue;
+    const long tiles = up(s.M, 128) * up(s.N, (s.gated ? 32 : 64) * (kind == kWide4 ? 4 : 2));
+    for (int split : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      if (split > 1 && (!may_split || nb < 2 * split || tiles >= 2 * kCus)) break;
+      const int per = (int)up(nb, split), real = (int)up(nb, per);
+      const float t = 4.0f + up(tiles * real, kCus) * (per * (kind == kWide4 ? step4 : step2) + 2.f) +
+                      join_time(s, real);
+      if (t < time) {
+        time = t;
+        best = Plan4{kind, real};
+      }
+    }
+  }
+  return best;
+}
+
+// Rows of x that do not start on 16 bytes: tiles of 64 rows, x by way of registers.
+Plan4 plan_any(const Shape4& s, bool may_split) {
+  Plan4 p{kTile4, 1};
+  const long tiles = up(s.M, 64) * up(s.N, s.gated ? 64 : 128);
+  if (may_split)
+    while (p.split < 16 && tiles * p.split * 2 <= 2 * kCus && blocks_of(s.K) >= 4 * p.split)
+      p.split *= 2;
+  p.split = (int)up(blocks_of(s.K), up(blocks_of(s.K), p.split));
+  return p;
+}
+
+Plan4 plan(const Shape4& s, bool aligned, bool may_split) {
+  if (s.M <= 64) return plan_few(s, may_split);
+  return aligned ? plan_many(s, may_split) : plan_any(s, may_split);
+}
+
+size_t split_bytes(const Plan4& p, const Shape4& s) {
+  return p.split > 1 ? (size_t)p.split * s.M * s.N * (s.gated ? 2 : 1) * 4 : 0;
+}
+
+Shape4 shape_of(int M, int N, int K, int act, int fmt, int group) {
+  return Shape4{M, N, K, act == lin::kSwiglu, fmt, group};
 }
 
 }  // namespace
+}  // namespace l4
+}  // namespace xtu
 
 extern "C" {
 
@@ -38,12 +154,15 @@ size_t xtu_linear4_weight_bytes(int N, int K, int act, int fmt, int group) {
 
 size_t xtu_linear4_workspace_bytes(int M, int N, int K, int act, int fmt, int group) {
   if (!sizes_ok(M, N, K, act, fmt, group) || M == 0) return 0;
-  const bool gated = act == lin::kSwiglu;
-  LinearArgs e{};
-  e.M = M;
-  e.K = K;
-  if (skinny4_fits(e) || rows4_fits(e)) return 0;
-  return split_bytes(plan4_tile(M, N, K, gated, true), M, N, gated);
+  const Shape4 s = shape_of(M, N, K, act, fmt, group);
+  const size_t a = split_bytes(plan(s, true, true), s), b = split_bytes(plan(s, false, true), s);
+  return a > b ? a : b;
+}
+
+int xtu_linear4_plan(int M, int N, int K, int act, int fmt, int group, int aligned) {
+  if (!sizes_ok(M, N, K, act, fmt, group) || M == 0) return -1;
+  const Plan4 p = plan(shape_of(M, N, K, act, fmt, group), aligned, true);
+  return 16 * p.split + p.kind;
 }
 
 hipError_t xtu_linear4(const xtu_linear4_args* args, hipStream_t stream) {
@@ -59,7 +178,6 @@ hipError_t xtu_linear4(const xtu_linear4_args* args, hipStream_t stream) {
     return reinterpret_cast<uintptr_t>(p) % bytes == 0;
   };
   XTU_CHECK_ARG(al(t.w, 16) && al(t.workspace, 16) && al(t.x, 2) && al(t.gs, 4));
-  const bool gated = t.act == lin::kSwiglu;
   XTU_CHECK_ARG((long)M * N < (1L << 38));   // grids
   // vectors of four elements in the epilogue
   const int vec = N % 4 == 0 && al(t.out, t.out_bf16 ? 8 : 16) && (M == 1 || t.ldo % 4 == 0) &&
@@ -76,15 +194,17 @@ hipError_t xtu_linear4(const xtu_linear4_args* args, hipStream_t stream) {
   a.group = t.group;
   a.xvec = al(t.x, 16) && K % 8 == 0 && (M == 1 || t.ldx % 8 == 0);
   (void)hipGetLastError();
-#ifdef L4_NOSKINNY
-  if (rows4_fits(a.e)) return launch4_rows(a, stream);
-#endif
-  if (skinny4_fits(a.e)) return launch4_skinny(a, stream);
-  if (rows4_fits(a.e)) return launch4_rows(a, stream);
-  Plan4 p = plan4_tile(M, N, K, gated, true);
-  if (split_bytes(p, M, N, gated) > (t.workspace ? t.workspace_bytes : 0))
-    p = plan4_tile(M, N, K, gated, false);
-  return launch4_tile(p, a, reinterpret_cast<float*>(t.workspace), stream);
+  const Shape4 s = shape_of(M, N, K, t.act, t.fmt, t.group);
+  Plan4 p = plan(s, wide4_fits(a), true);
+  if (split_bytes(p, s) > (t.workspace ? t.workspace_bytes : 0)) p = plan(s, wide4_fits(a), false);
+  float* part = reinterpret_cast<float*>(t.workspace);
+  switch (p.kind) {
+    case kSkinny4: return launch4_skinny(a, stream);
+    case kRows4: return launch4_rows(a, stream);
+    case kSlab4: return launch4_slab(a, p.split, part, stream);
+    case kTile4: return launch4_tile(a, p.split, part, stream);
+    default: return launch4_wide(p, a, part, stream);
+  }
 }
 
 }  // extern "C"

@@ -15,11 +15,11 @@
 // Layout.  Rows in panels of 16 (swiglu: gate and up panels in turn), K in blocks
 // of 128; a block of a panel is one record: 1024 bytes of codes [4 q][16 row][4 j][4 B],
 // lane 16 q + row of a wave takes 16 of them, dword j the codes of k = 32 j + 8 q .. + 7
-// (low nibble first; INT4: as code ^ 8, two's complement), which are an MFMA operand's.
+// (low nibble first; INT4: i4x8_to_bf16), which are an MFMA operand's.
 // So an MFMA's 32 k are consecutive, x is read as it lies, and an INT4 group is whole
 // MFMAs.  Then the record's scales, a dword of four for the lanes that share them:
 //   MXFP4: [16 row][4 j] bytes        NVFP4: [2 q / 2][16 row][4 j] bytes
-//   INT4:  fp32 [128 / G][16 row], times 16 (i4x8_to_bf16)
+//   INT4:  fp32 [128 / G][16 row]
 // A panel's records are consecutive: a wave walks one stream.  Rows and k past the
 // matrix are zero codes under scale one (NVFP4, INT4: zero).
 #pragma once
@@ -53,18 +53,22 @@ __host__ __device__ __forceinline__ int blocks_of(int K) { return (K + 127) / 12
 // 16-row panels of a half (swiglu: of the gate half; else of all rows)
 __host__ __device__ __forceinline__ int panels_of(int N) { return (N + 15) / 16; }
 
-// Eight two's complement nibbles of a dword, low nibble first, as bf16 pairs of v / 16:
-// the converter reads a byte's low four bits as a fraction.
+// Eight INT4 codes of a dword as bf16: k = b in byte b's low nibble, 4 + b in its high
+// one.  Code c >= 8 is stored as c - 8 (v = 0 .. 7), c < 8 as 15 - c (8 + |v| - 1), so
+// that a byte of sign and magnitude, 0 .. 8, takes a mask and two sums for four codes at
+// once; as e4m3 that byte is v 2^-9 (subnormal, and 8 2^-9 the first normal), which the
+// converter scales back.  15 instructions; the converter of single nibbles
+// (v_cvt_off_f32_i4) needs fewer but runs at a quarter of the rate.
 __device__ __forceinline__ u32x4_t i4x8_to_bf16(uint32_t w) {
-  const uint32_t o = w >> 4;
-  u32x4_t r;
-#pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    const float lo = __builtin_amdgcn_cvt_off_f32_i4((int)(w >> (8 * b)));
-    const float hi = __builtin_amdgcn_cvt_off_f32_i4((int)(o >> (8 * b)));
-    r[b] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
-  }
-  return r;
+  const uint32_t h0 = w >> 3 & 0x01010101u, h1 = w >> 7 & 0x01010101u;
+  const uint32_t b0 = (h0 << 7) + ((w & 0x07070707u) + h0);
+  const uint32_t b1 = (h1 << 7) + ((w >> 4 & 0x07070707u) + h1);
+  const auto two = [](uint32_t b, auto hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
+                                            b, 512.f, decltype(hi)::value));
+  };
+  return u32x4_t{two(b0, std::false_type{}), two(b0, std::true_type{}),
+                 two(b1, std::false_type{}), two(b1, std::true_type{})};
 }
 
 // A lane's part of a record as it lies in memory.
@@ -97,6 +101,15 @@ __device__ __forceinline__ Raw<FMT, G> load_raw(const uint8_t* rec, int q, int r
   return r;
 }
 
+__device__ __forceinline__ float e4m3_of(uint32_t s, int j) {
+  switch (j) {
+    case 0: return __builtin_amdgcn_cvt_f32_fp8(s, 0);
+    case 1: return __builtin_amdgcn_cvt_f32_fp8(s, 1);
+    case 2: return __builtin_amdgcn_cvt_f32_fp8(s, 2);
+    default: return __builtin_amdgcn_cvt_f32_fp8(s, 3);
+  }
+}
+
 // The MFMA operand of dword j.
 template <int FMT, int G>
 __device__ __forceinline__ u32x4_t operand(const Raw<FMT, G>& r, int j) {
@@ -107,15 +120,17 @@ __device__ __forceinline__ u32x4_t operand(const Raw<FMT, G>& r, int j) {
     // (the converter takes the exponent bits alone: a byte 0 means 2^-127 to it)
     if constexpr (FMT == kMx)
       fp4x8_to_bf16(r.c[j], __uint_as_float((j < 3 ? r.s << (23 - 8 * j) : r.s >> 1) & 0x7f800000u), o);
-    else fp4x8_to_bf16_mul(r.c[j], e4m3_to_f32(r.s >> (8 * j)), o);
+    else fp4x8_to_bf16_mul(r.c[j], e4m3_of(r.s, j), o);
     return u32x4_t{o[0], o[1], o[2], o[3]};
   }
 }
 
 // One block of NP panels times MT blocks of 16 rows of x; x(j, mt) gives the operand
-// of dword j.  acc[p][mt] += the products.
-template <int FMT, int G, int NP, int MT, class X>
-__device__ __forceinline__ void multiply(const Raw<FMT, G> (&r)[NP], f32x4_t (&acc)[NP][MT], X x) {
+// of dword j.  acc[p][mt] += the products.  after(): called behind the first dword's
+// operands, when every record has been waited for.
+template <int FMT, int G, int NP, int MT, class X, class A>
+__device__ __forceinline__ void multiply(const Raw<FMT, G> (&r)[NP], f32x4_t (&acc)[NP][MT], X x,
+                                         A after) {
   constexpr int GM = FMT == kI4 ? G / 32 : 4;   // MFMAs that share a scale
 #pragma unroll
   for (int g = 0; g < 4 / GM; ++g) {
@@ -141,6 +156,7 @@ __device__ __forceinline__ void multiply(const Raw<FMT, G> (&r)[NP], f32x4_t (&a
           }
         }
       }
+      if (j == 0) after();
     }
     if constexpr (FMT == kI4) {
 #pragma unroll
@@ -154,6 +170,11 @@ __device__ __forceinline__ void multiply(const Raw<FMT, G> (&r)[NP], f32x4_t (&a
   }
 }
 
+template <int FMT, int G, int NP, int MT, class X>
+__device__ __forceinline__ void multiply(const Raw<FMT, G> (&r)[NP], f32x4_t (&acc)[NP][MT], X x) {
+  multiply<FMT, G, NP, MT>(r, acc, x, [] {});
+}
+
 // Eight k of a row of x, zeros past K.
 __device__ __forceinline__ u32x4_t load_x8(const Linear4Args& a, const uint16_t* row, int k) {
   if (a.xvec) {
@@ -164,20 +185,42 @@ __device__ __forceinline__ u32x4_t load_x8(const Linear4Args& a, const uint16_t*
   return lin::load8(row, k, a.e.K);
 }
 
-// At most 16 rows of x, all of x in LDS.
-constexpr size_t kSkinny4Lds = 120 * 1024;
-bool skinny4_fits(const LinearArgs& e);
-hipError_t launch4_skinny(const Linear4Args& a, hipStream_t stream);
-
-// At most 64 rows of x.
-bool rows4_fits(const LinearArgs& e);
-hipError_t launch4_rows(const Linear4Args& a, hipStream_t stream);
-
-struct Plan4 {
-  int kind, split;   // kind: blocks of 16 rows of a tile
+struct Shape4 {
+  int M, N, K;
+  bool gated;
+  int fmt, group;
 };
-Plan4 plan4_tile(int M, int N, int K, bool gated, bool may_split);
-hipError_t launch4_tile(const Plan4& p, const Linear4Args& a, float* part, hipStream_t stream);
+
+// The kernels, and the ranges of K that are summed apart.
+enum Kind4 : int { kSkinny4 = 0, kRows4, kSlab4, kWide2, kWide4, kTile4 };
+struct Plan4 {
+  int kind, split;
+};
+
+// Up to 16 rows of x, all of it in LDS: units of `rows` output columns; grid 0: no.
+struct SkinnyPlan {
+  int rows, waves;
+  long units, grid;
+};
+SkinnyPlan skinny4_plan(const Shape4& s);
+hipError_t launch4_skinny(const Linear4Args& a, hipStream_t stream);
+// Up to 64 rows of x, nothing staged.
+int rows4_waves(const Shape4& s);
+hipError_t launch4_rows(const Linear4Args& a, hipStream_t stream);
+// Up to 64 rows of x, a range of `per` blocks of K of them in LDS.
+constexpr int kSlabWaves = 8, kSlabPad = 32;   // pad: bytes behind a row of x in LDS (banks)
+constexpr size_t kSlabLds = 150 * 1024;
+inline size_t slab4_lds(int M, int per) { return (size_t)M * ((size_t)per * 256 + kSlabPad); }
+hipError_t launch4_slab(const Linear4Args& a, int split, float* part, hipStream_t stream);
+// More rows, which start on 16 bytes: tiles of 128 rows and 64 NP rows of w.
+bool wide4_fits(const Linear4Args& a);
+hipError_t launch4_wide(const Plan4& p, const Linear4Args& a, float* part, hipStream_t stream);
+// Any.
+hipError_t launch4_tile(const Linear4Args& a, int split, float* part, hipStream_t stream);
+
+inline Shape4 shape_of(const Linear4Args& a) {
+  return Shape4{a.e.M, a.e.N, a.e.K, a.e.act == lin::kSwiglu, a.fmt, a.group};
+}
 
 // f(format, group, gated) with the three as constants.
 template <class F>

@@ -137,9 +137,10 @@ hipError_t launch(const Linear4Args& a, hipStream_t stream) {
 
 }  // namespace
 
-bool rows4_fits(const LinearArgs& e) { return e.M <= 64; }
+int rows4_waves(const Shape4& s) { return s.M <= 16 && s.fmt != kI4 ? 16 : 8; }
 
 hipError_t launch4_rows(const Linear4Args& a, hipStream_t stream) {
+  if (a.e.M > 64) return hipErrorInvalidValue;
   if (a.e.M <= 16) return launch<1>(a, stream);
   if (a.e.M <= 32) return launch<2>(a, stream);
   if (a.e.M <= 48) return launch<3>(a, stream);

@@ -10,6 +10,7 @@ namespace xtu {
 namespace l4 {
 namespace {
 
+constexpr size_t kLds = 120 * 1024;
 constexpr int kRowPad = 16;    // bf16 behind a row of x in LDS: rows 32 bytes apart in the banks
 
 template <int FMT, int G, bool GATED, int WV, int U>
@@ -88,40 +89,48 @@ __global__ __launch_bounds__(64 * WV) void linear4_skinny_kernel(Linear4Args a, 
   }
 }
 
-size_t skinny_lds(const LinearArgs& e) {
-  return (size_t)e.M * (blocks_of(e.K) * 128 + kRowPad) * 2;
-}
-
 template <int WV>
-hipError_t launch(const Linear4Args& a, hipStream_t stream) {
-  const LinearArgs& e = a.e;
-  int rp = 4;   // columns of a unit: about one unit per CU, 16 at most
-  while (rp < 16 && (long)panels_of(e.N) * (16 / rp) > 256) rp *= 2;
-  const long units = (long)panels_of(e.N) * (16 / rp);
-  const size_t lds = skinny_lds(e);
-  const size_t all = lds + (size_t)(e.act == lin::kSwiglu ? 2 : 1) * WV * 1024;
-  const int fit = (int)(160 * 1024 / all), most = 32 / WV;
-  const long grid = 256L * (fit < most ? fit : most);
-  const bool one = blocks_of(e.K) <= WV;   // a block per wave and unit
+hipError_t launch(const Linear4Args& a, const SkinnyPlan& p, size_t lds, hipStream_t stream) {
+  const bool one = WV < 16 || blocks_of(a.e.K) <= WV;   // a block per wave and unit
   return by_format(a, [&](auto fmt, auto group, auto g) {
     constexpr int F = decltype(fmt)::value, G = decltype(group)::value;
     constexpr bool GATED = decltype(g)::value;
-    auto k = one ? linear4_skinny_kernel<F, G, GATED, WV, 1>
-                 : linear4_skinny_kernel<F, G, GATED, WV, 2>;
-    k<<<(unsigned)(units < grid ? units : grid), 64 * WV, lds, stream>>>(a, rp);
+    auto k = linear4_skinny_kernel<F, G, GATED, WV, 1>;
+    if constexpr (WV == 16)
+      if (!one) k = linear4_skinny_kernel<F, G, GATED, WV, 2>;
+    k<<<(unsigned)p.grid, 64 * WV, lds, stream>>>(a, p.rows);
     return hipPeekAtLastError();
   });
 }
 
+size_t x_bytes(const Shape4& s) {
+  return (size_t)s.M * ((size_t)blocks_of(s.K) * 128 + kRowPad) * 2;
+}
+
 }  // namespace
 
-bool skinny4_fits(const LinearArgs& e) { return e.M <= 16 && skinny_lds(e) <= kSkinny4Lds; }
+SkinnyPlan skinny4_plan(const Shape4& s) {
+  SkinnyPlan p{4, 0, 0, 0};
+  const size_t x = x_bytes(s);
+  if (s.M > 16 || x > kLds) return p;
+  // columns of a unit: about one unit per CU, 16 at most
+  while (p.rows < 16 && (long)panels_of(s.N) * (16 / p.rows) > 256) p.rows *= 2;
+  p.units = (long)panels_of(s.N) * (16 / p.rows);
+  const int nb = blocks_of(s.K);
+  p.waves = nb > 8 ? 16 : nb > 4 ? 8 : 4;
+  const int fit = (int)(160 * 1024 / (x + (size_t)(s.gated ? 2 : 1) * p.waves * 1024));
+  const long all = 256L * (fit < 32 / p.waves ? fit : 32 / p.waves);   // what is resident
+  p.grid = p.units < all ? p.units : all;
+  return p;
+}
 
 hipError_t launch4_skinny(const Linear4Args& a, hipStream_t stream) {
-  const int nb = blocks_of(a.e.K);
-  if (nb > 8) return launch<16>(a, stream);
-  if (nb > 4) return launch<8>(a, stream);
-  return launch<4>(a, stream);
+  const Shape4 s = shape_of(a);
+  const SkinnyPlan p = skinny4_plan(s);
+  if (p.grid == 0) return hipErrorInvalidValue;
+  if (p.waves == 16) return launch<16>(a, p, x_bytes(s), stream);
+  if (p.waves == 8) return launch<8>(a, p, x_bytes(s), stream);
+  return launch<4>(a, p, x_bytes(s), stream);
 }
 
 }  // namespace l4

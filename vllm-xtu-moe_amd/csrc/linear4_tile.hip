@@ -1,5 +1,5 @@
-// The product with 4-bit weights on tiles (linear4.hpp has the formula and the
-// layout).  Four waves, each with NP panels of w times all of the tile's 16 MT rows
+// The product with 4-bit weights on tiles, for many rows of x at any alignment and row
+// stride (linear4.hpp has the formula and the layout).  Four waves, each with NP panels of w times all of the tile's 16 MT rows
 // of x, K in blocks of 128.  A wave's records go from memory to its registers, two
 // blocks ahead, and are made operands there, so a weight is read and expanded once a
 // tile; x goes through LDS, which all waves read, one block ahead.
@@ -175,25 +175,8 @@ hipError_t launch(const Linear4Args& a, int split, float* part, hipStream_t stre
 
 }  // namespace
 
-Plan4 plan4_tile(int M, int N, int K, bool gated, bool may_split) {
-  Plan4 p;
-  p.kind = M <= 16 ? 1 : M <= 32 ? 2 : M <= 64 ? 4 : 8;
-  const int cols = 4 * (gated ? 8 : 16) * 2;
-  const long tiles = ((long)M + 16 * p.kind - 1) / (16 * p.kind) * (((long)N + cols - 1) / cols);
-  p.split = 1;
-  if (may_split)
-    while (p.split < 16 && tiles * p.split * 2 <= 512 && blocks_of(K) >= 4 * p.split) p.split *= 2;
-  return p;
-}
-
-hipError_t launch4_tile(const Plan4& p, const Linear4Args& a, float* part, hipStream_t stream) {
-  switch (p.kind) {
-    case 1: return launch<1, 2>(a, p.split, part, stream);
-    case 2: return launch<2, 2>(a, p.split, part, stream);
-    case 4: return launch<4, 2>(a, p.split, part, stream);
-    case 8: return launch<8, 2>(a, p.split, part, stream);
-  }
-  return hipErrorInvalidValue;
+hipError_t launch4_tile(const Linear4Args& a, int split, float* part, hipStream_t stream) {
+  return launch<4, 2>(a, split, part, stream);
 }
 
 }  // namespace l4

@@ -24,28 +24,6 @@ namespace xtu {
 namespace lin {
 namespace {
 
-// 16 bytes per lane to LDS at dst + 16 * lane, from the buffer's base + off +
-// soff (zeros out of range).
-__device__ __forceinline__ void buf_to_lds(u32x4_t rsrc, uint32_t off, uint32_t soff,
-                                           const uint8_t* dst) {
-  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
-               :: "v"(off), "s"(rsrc), "s"(soff), "{m0}"((uint32_t)(uintptr_t)dst)
-               : "memory");
-}
-
-// Raw buffer over [base, base + bytes), wave-uniform.
-__device__ __forceinline__ u32x4_t raw_buffer(const void* base, uint32_t bytes) {
-  const uint64_t p = reinterpret_cast<uint64_t>(base);
-  u32x4_t r = {(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, bytes, 0x00020000u};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
-  return r;
-}
-
-// s_waitcnt immediates: vmcnt(n), and vmcnt(n) with lgkmcnt(0)
-constexpr int wait_vm(int n) { return 0x0f70 | (n & 15) | ((n >> 4) << 14); }
-constexpr int wait_vm_lgkm0(int n) { return 0x0070 | (n & 15) | ((n >> 4) << 14); }
-
 // Slot of piece p of row r in an LDS row of PCS pieces, for MB rows a read.
 template <int PCS, int MB>
 __device__ __forceinline__ int slot_of(int p, int r) {

@@ -115,6 +115,7 @@ SIGNATURES = {
     "xtu_linear4": (_i, [_vp, _vp]),
     "xtu_linear4_weight_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "xtu_linear4_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "xtu_linear4_plan": (_i, [_i, _i, _i, _i, _i, _i, _i]),
     "xtu_router_workspace_bytes": (_sz, [_i, _i, _i]),
     "xtu_router_losses": (_i, [_vp, _vp]),
     "xtu_router_grad": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),
@@ -166,7 +167,7 @@ _NOT_STATUS = {"xtu_version", "xtu_error_string", "xtu_segment_workspace_bytes",
                "xtu_i8_weight_bytes", "xtu_few_workspace_bytes",
                "xtu_linear_workspace_bytes", "xtu_linear_plan",
                "xtu_router_workspace_bytes", "xtu_linear4_weight_bytes",
-               "xtu_linear4_workspace_bytes"}
+               "xtu_linear4_workspace_bytes", "xtu_linear4_plan"}
 
 _LIB = None
 

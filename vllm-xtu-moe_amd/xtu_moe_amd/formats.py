@@ -275,7 +275,8 @@ def unpack_scales(fmt: int, p, N: int, K: int):
 
 # ------------------------------------------------- 4-bit weights of linear4
 # records: per panel of 16 rows and block of 128 k, 1024 bytes of codes
-# [4 q][16 row][4 j][4 B] (k = 32 j + 8 q .. + 7), then the scales
+# [4 q][16 row][4 j][4 B] (k = 32 j + 8 q .. + 7; low nibble first, INT4: byte b
+# holds b and 4 + b), then the scales
 def linear4_group(fmt: int, s, K: int) -> int:
     """The k per scale of a matrix's scales [N, K / group]."""
     if s.dim() != 2 or s.shape[1] == 0 or K % s.shape[1]:
@@ -290,18 +291,21 @@ def linear4_group(fmt: int, s, K: int) -> int:
 def pack_linear4(fmt: int, codes, s, group: int):
     """codes u8 [n, N, K/2] (low nibble = even k) and scales [n, N, K/group] of n
     halves (1; 2: gate, up) -> records u8 [panels, blocks, record], the halves'
-    panels in turn.  Rows and k past the matrix are zero codes; INT4 codes
-    become two's complement, their scales are times 16 (the kernels read a code as
-    a fraction of 16)."""
+    panels in turn.  Rows and k past the matrix are zeros; an INT4 code of
+    value v = code - 8 is stored as v, a negative one as 7 - v."""
     n, N, K = codes.shape[0], codes.shape[1], codes.shape[2] * 2
     P, B = (N + 15) // 16, (K + 127) // 128
     pad = torch.nn.functional.pad
-    c = codes ^ 0x88 if fmt == FMT_INT4 else codes
+    c = codes
+    if fmt == FMT_INT4:
+        c = torch.stack([codes & 15, codes >> 4], -1)
+        c = torch.where(c >= 8, c - 8, 15 - c).view(n, N, K // 8, 8)
+        c = (c[..., :4] | c[..., 4:] << 4).reshape(n, N, K // 2)
     c = pad(c, (0, B * 64 - K // 2, 0, P * 16 - N))
     # [n][panel][row][block][j][q][4 B] -> [panel][n][block][q][row][j][4 B]
     c = c.view(n, P, 16, B, 4, 4, 4).permute(1, 0, 3, 5, 2, 4, 6)
     if fmt == FMT_INT4:
-        s = pad(s.float() * 16.0, (0, B * (128 // group) - K // group, 0, P * 16 - N))
+        s = pad(s.float(), (0, B * (128 // group) - K // group, 0, P * 16 - N))
         s = s.view(n, P, 16, B, 128 // group).permute(1, 0, 3, 4, 2).contiguous().view(torch.uint8)
     elif fmt == FMT_MXFP4:   # [n][panel][row][block][j] -> [panel][n][block][row][j]
         s = pad(s, (0, B * 4 - K // 32, 0, P * 16 - N), value=127)
