@@ -258,6 +258,43 @@ def test_single_gradients():
         assert not router_losses(lg, ids).balance.requires_grad
 
 
+def test_once_differentiable():
+    """A gradient of the gradient is refused, not wrong; leaves and their kin are
+    checked for changes in place."""
+    lg, ids, gw = _inputs(20, 16, 2, seed=6)
+    lg.requires_grad_(True)
+    d, = torch.autograd.grad(router_losses(lg, ids).weights, lg, gw, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(d.sum(), lg)
+    plain, = torch.autograd.grad(router_losses(lg, ids).weights, lg, gw)
+    assert torch.equal(d.detach(), plain)
+    r = router_losses(lg, ids)
+    ids.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(r.weights, lg, gw)
+
+
+def test_through_the_products():
+    """From hidden states, as a tuning step runs it: the router product's gradient is
+    the logits' times its operands."""
+    g = torch.Generator().manual_seed(3)
+    x = (torch.randn((300, 96), generator=g)).to(DEV).requires_grad_(True)
+    w = (torch.randn((40, 96), generator=g) * 0.1).to(DEV).requires_grad_(True)
+    logits = x @ w.t()
+    ids = route(logits.detach(), top_k=4)[1]
+    r = router_losses(logits, ids)
+    loss = (r.weights ** 2).sum() + 0.5 * r.balance + 0.1 * r.z
+    d, dw, dx = torch.autograd.grad(loss, [logits, w, x])
+    e = _formula(logits.detach(), ids, [0, 300], "softmax", True, 1.0, 2 * r.weights.detach(), 0.5,
+                 0.1)
+    tol = e["da"] * 2.0 ** -17
+    assert bool(((d.double() - e["d"]).abs() <= tol + e["d"].abs() * U).all())
+    xd, wd = x.detach().double(), w.detach().double()
+    full = tol + e["d"].abs() * 300 * 2.0 ** -23
+    assert bool(((dw.double() - e["d"].t() @ xd).abs() <= full.t() @ xd.abs() + 1e-12).all())
+    assert bool(((dx.double() - e["d"] @ wd).abs() <= full @ wd.abs() + 1e-12).all())
+
+
 @pytest.mark.parametrize("scoring,renorm", [("softmax", True), ("softmax", False),
                                             ("sigmoid", True), ("sigmoid", False)])
 def test_gradient_against_differences(scoring, renorm):

@@ -27,6 +27,7 @@ from .linear import _current_device, on_stream, raw_stream
 ARGS = struct.Struct("@11PlN7if")
 MAX_ROWS, MAX_SEQUENCES = 1 << 30, 1 << 24
 _WS_BYTES: dict = {}
+_ENTRIES = None
 
 
 class RouterLosses(NamedTuple):
@@ -118,48 +119,68 @@ def _pack(logits, ids, starts, weights, stat, counts, probs, balance, z, norm, w
                      bf16, scale)
 
 
+def _entries():
+    global _ENTRIES
+    if _ENTRIES is None:
+        lib = _lib.load()
+        _ENTRIES = lib.xtu_router_losses, lib.xtu_router_grad
+    return _ENTRIES
+
+
 def _forward(logits, ids, starts, shape):
     """(weights, balance, z, counts, probs, stat, norm)."""
     T, E, K, S, mode = shape[:5]
-    new = lambda *size: logits.new_empty(size, dtype=torch.float32)  # noqa: E731
-    weights, stat, norm, probs, balance = new(T, K), new(T, 2), new(2), new(S, E), new()
-    z = None if mode else new()
-    counts = logits.new_empty((S, E), dtype=torch.int32)
+    new, f32 = logits.new_empty, torch.float32
+    weights, stat = new((T, K), dtype=f32), new((T, 2), dtype=f32)
+    norm, probs = new(2, dtype=f32), new((S, E), dtype=f32)
+    balance, z = new((), dtype=f32), None if mode else new((), dtype=f32)
+    counts = new((S, E), dtype=torch.int32)
     nws = _WS_BYTES.get((T, E, S))
     if nws is None:
         nws = int(_lib.call("xtu_router_workspace_bytes", T, E, S))
-        if len(_WS_BYTES) >= 4096:
+        if len(_WS_BYTES) >= 4096:   # a server's batch sizes
             _WS_BYTES.clear()
         _WS_BYTES[T, E, S] = nws
     # per call: calls on other streams, and graphs, have their own
-    ws = logits.new_empty(nws, dtype=torch.uint8)
-    _lib.call("xtu_router_losses",
-              _pack(logits, ids, starts, weights, stat, counts, probs, balance, z, norm, ws, nws,
-                    shape), raw_stream(logits.device.index))
+    ws = new(nws, dtype=torch.uint8)
+    rc = _entries()[0](_pack(logits, ids, starts, weights, stat, counts, probs, balance, z, norm,
+                             ws, nws, shape), raw_stream(logits.device.index))
+    if rc:
+        _lib.check("xtu_router_losses", rc)
     return weights, balance, z, counts, probs, stat, norm
+
+
+def _grad(ctx, g_weights, g_balance, g_z):
+    logits, ids, starts, weights, counts = ctx.saved_tensors
+    out = logits.new_empty(logits.shape)
+    grads = [None if g is None else g.contiguous() for g in (g_weights, g_balance, g_z)]
+    rc = _entries()[1](_pack(logits, ids, starts, weights, ctx.stat, counts, None, None, None,
+                             ctx.norm, None, 0, ctx.shape),
+                       *[0 if g is None else g.data_ptr() for g in grads], out.data_ptr(),
+                       raw_stream(logits.device.index))
+    if rc:
+        _lib.check("xtu_router_grad", rc)
+    return out
+
+
+_grad_once = torch.autograd.function.once_differentiable(_grad)
 
 
 class _Losses(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, starts, shape):
-        weights, balance, z, counts, probs, stat, norm = _forward(logits, ids, starts, shape)
-        ctx.save_for_backward(logits, ids, starts, weights, stat, counts, norm)
+        weights, balance, z, counts, probs, ctx.stat, ctx.norm = _forward(logits, ids, starts,
+                                                                          shape)
+        ctx.save_for_backward(logits, ids, starts, weights, counts)
         ctx.shape = shape
         ctx.mark_non_differentiable(counts, probs)
         ctx.set_materialize_grads(False)
         return weights, balance, z, counts, probs
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_weights, g_balance, g_z, _counts, _probs):
         if g_weights is None and g_balance is None and g_z is None:
             return None, None, None, None
-        logits, ids, starts, weights, stat, counts, norm = ctx.saved_tensors
-        T, E = ctx.shape[:2]
-        out = logits.new_empty((T, E))
-        grads = [None if g is None else g.contiguous() for g in (g_weights, g_balance, g_z)]
-        _lib.call("xtu_router_grad",
-                  _pack(logits, ids, starts, weights, stat, counts, None, None, None, norm, None, 0,
-                        ctx.shape), *(0 if g is None else g.data_ptr() for g in grads),
-                  out.data_ptr(), raw_stream(logits.device.index))
-        return out, None, None, None
+        # (a graph of the gradient is refused where it is used; the wrapper costs 6 us)
+        grad = _grad_once if torch.is_grad_enabled() else _grad
+        return grad(ctx, g_weights, g_balance, g_z), None, None, None
