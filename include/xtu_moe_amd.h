@@ -667,9 +667,10 @@ hipError_t xtu_linear4(const xtu_linear4_args* args, hipStream_t stream);
 size_t xtu_linear4_weight_bytes(int N, int K, int act, int fmt, int group);
 size_t xtu_linear4_workspace_bytes(int M, int N, int K, int act, int fmt, int group);
 /* Which kernel a product with all of that workspace takes, 16 * (K splits) + 0 the
- * stream of w (all of x in LDS), 1 rows (nothing staged), 2 slabs (a range of K of x in
- * LDS), 3 and 4 tiles of 128 x 128 and 128 x 256, 5 tiles of 64 x 128 for rows of x
- * that do not start on 16 bytes (aligned 0); -1 none. */
+ * stream of w (all of x in LDS), 1 blocks (a block of x per wave in LDS), 2 slabs (a
+ * range of K of x in LDS), 3 and 4 tiles of 128 x 128 and 128 x 256; for rows of x that
+ * do not start on 16 bytes (aligned 0) 5 tiles of 64 x 128, 6 rows (nothing staged); -1
+ * none. */
 int xtu_linear4_plan(int M, int N, int K, int act, int fmt, int group, int aligned);
 
 /* ------------------------------------------------ router, training step

@@ -113,7 +113,7 @@ def test_every_form(fmt, group, gated):
     """Each kernel, whole and with K split, with the whole epilogue."""
     for i, ((kernel, _), M, N, K) in enumerate(forms(fmt, group, gated)):
         x = _rand((M, K + 8), i)
-        x = x[:, 1:K + 1] if kernel == 5 else x[:, :K]
+        x = x[:, 1:K + 1] if kernel >= 5 else x[:, :K]
         W, w = _weight(fmt, group, N, K, gated, seed=70 + i)
         b = _rand((w.shape[0],), 2, 0.5, F32)
         r = _rand((M, N), 4, 1.0, BF if i % 2 else F32)

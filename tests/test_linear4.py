@@ -27,16 +27,18 @@ def _dense(fmt, rows, K, group, seed=0):
 # (kernel, K split or not) -> M, N, K of a product that takes it, for every format;
 # gated ones have the same number of rows
 FORMS = {
-    (0, False): [(1, 300, 512), (3, 1000, 1024), (1, 166, 6528)],
-    (1, False): [(1, 6022, 1792), (28, 75, 896), (40, 1503, 256), (54, 3011, 128)],
-    (2, False): [(45, 16911, 256), (63, 18531, 896), (32, 19170, 768)],
-    (2, True): [(14, 2000, 8192), (23, 464, 5760), (47, 29, 7552), (58, 308, 3456)],
+    (0, False): [(1, 300, 512), (5, 296, 128), (2, 12000, 640), (1, 150, 9600)],
+    (1, False): [(1, 16, 1792), (3, 4000, 2176), (7, 182, 1536), (16, 534, 1280), (24, 2037, 768),
+                 (42, 407, 640), (50, 102, 384), (64, 1500, 2176)],
+    (2, False): [(20, 16864, 128), (30, 18111, 512), (44, 21292, 128), (51, 18559, 128)],
+    (2, True): [(10, 16, 7808), (26, 396, 8448), (36, 112, 3712), (64, 148, 9216)],
     (3, False): [(65, 16, 128), (137, 1140, 384)],
-    (3, True): [(71, 16, 768), (123, 504, 2816)],
-    (4, False): [(1224, 3405, 256), (1887, 2884, 384)],
-    (4, True): [(263, 3675, 3584)],
+    (3, True): [(71, 16, 896), (123, 504, 2816)],
+    (4, False): [(1224, 3405, 256), (1838, 2228, 512)],
+    (4, True): [(65, 5888, 5248)],
     (5, False): [(70, 16, 128), (353, 490, 384)],
-    (5, True): [(81, 17, 512), (300, 1228, 512)],
+    (5, True): [(85, 18, 512), (300, 1228, 512)],
+    (6, False): [(1, 16, 128), (14, 357, 1280), (29, 203, 1280), (45, 300, 640), (64, 204, 2176)],
 }
 
 
@@ -53,7 +55,7 @@ def forms(fmt, group, gated):
 @pytest.mark.parametrize("gated", [False, True])
 def test_forms_are_taken(fmt, group, gated):
     for (kernel, split), M, N, K in forms(fmt, group, gated):
-        plan = _lib.load().xtu_linear4_plan(M, N, K, 6 if gated else 0, fmt, group, int(kernel != 5))
+        plan = _lib.load().xtu_linear4_plan(M, N, K, 6 if gated else 0, fmt, group, int(kernel < 5))
         assert (plan % 16, plan >= 32) == (kernel, split), (M, N, K, plan % 16, plan // 16)
 
 

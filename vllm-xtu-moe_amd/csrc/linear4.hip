@@ -27,30 +27,36 @@ bool sizes_ok(int M, int N, int K, int act, int fmt, int group) {
 
 long up(long n, long d) { return (n + d - 1) / d; }
 
-// Estimated times in us.  A CU takes in about 25 KB a us of what comes in small pieces (w,
-// and x by fragments) and twice that of rows staged whole; a launch and its latencies
-// are 3 to 5, the launch that adds K splits 3 and its partial sums' way.
+// Estimated times in us.  All CUs together take in w at 6.2 GB a ms, one of them rows
+// of x that are staged whole at 50 KB a us, and what it loads straight to LDS at 65 to
+// 80; a launch and its latencies are 3 to 6, the launch that adds K splits 3 and its
+// partial sums' way.
 
-float join_time(const Shape4& s, int split) {
+float join_time(const Shape4& s, int split, float rate) {
   if (split == 1) return 0.f;
-  return 3.0f + 2.f * split * s.M * (float)s.N * (s.gated ? 2 : 1) * 4.f / 5e6f;
+  return 3.0f + 2.f * split * s.M * (float)s.N * (s.gated ? 2 : 1) * 4.f / rate;
 }
+
+float larger(float a, float b) { return a > b ? a : b; }
 
 float skinny_time(const Shape4& s) {
   const SkinnyPlan p = skinny4_plan(s);
   if (p.grid == 0) return 1e30f;
   const int nb = blocks_of(s.K);
+  const long rounds = up(p.grid, kCus);
   const float x = s.M * (float)s.K * 2e-3f;
-  const float w = up(p.units, p.grid) * (s.gated ? 2 : 1) * (float)nb *
-                  record_bytes(s.fmt, s.group) * p.rows / 16 * 1e-3f;
-  return 3.0f + 0.1f * (nb < 16 ? nb : 16) + up(p.grid, kCus) * (x / 50.f + w / 25.f);
+  const float w = (s.gated ? 2 : 1) * (float)nb * record_bytes(s.fmt, s.group) * p.rows / 16 * 1e-3f;
+  return 3.0f + 0.1f * (nb < 16 ? nb : 16) + rounds * x / 50.f +
+         larger(p.units * w / 6200.f, rounds * up(p.units, p.grid) * w / 50.f);
 }
 
-float rows_time(const Shape4& s) {
+float block_time(const Shape4& s) {
   const int nb = blocks_of(s.K);
-  const long steps = up(nb, rows4_waves(s));
-  const float kb = s.M * (float)s.K * 2e-3f + 2.f * nb * record_bytes(s.fmt, s.group) * 1e-3f;
-  return 3.2f + up(up(s.N, s.gated ? 16 : 32), kCus) * kb / 25.f + 0.5f * (steps - 1);
+  const long units = up(s.N, s.gated ? 16 : 32), rounds = up(units, kCus);
+  const int rows = s.M <= 4 ? 4 : s.M <= 8 ? 8 : (int)up(s.M, 16) * 16;
+  const float x = rows * 0.256f * nb, w = 2.f * nb * record_bytes(s.fmt, s.group) * 1e-3f;
+  return 3.2f + rounds * x / 80.f + larger(units * w / 6200.f, rounds * w / 75.f) +
+         0.35f * up(nb, block4_waves(s)) + 2.f * (rounds - 1);
 }
 
 // The split of K with the least time, 0 where no range of K fits LDS.
@@ -62,9 +68,11 @@ int slab_split(const Shape4& s, bool may_split, float& time) {
   for (int split = 1; split <= nb && split <= (may_split ? 64 : 1); ++split) {
     const int per = (int)up(nb, split);
     if (up(nb, per) != split || slab4_lds(s.M, per) > kSlabLds) continue;
-    const float kb =
-        per * (s.M * 256.f + 2.f * kSlabWaves * record_bytes(s.fmt, s.group)) * 1e-3f;
-    const float t = 4.0f + up(gx * split, kCus) * kb / 25.f + join_time(s, split);
+    const long rounds = up(gx * split, kCus);
+    const float x = slab4_lds(s.M, per) * 1e-3f;
+    const float w = 2e-3f * kSlabWaves * per * record_bytes(s.fmt, s.group);
+    const float t = 6.0f + rounds * x / 65.f + larger(gx * split * w / 6200.f, rounds * w / 50.f) +
+                    1.f * (rounds - 1) + join_time(s, split, 4e6f);
     if (t < time) {
       time = t;
       best = split;
@@ -73,18 +81,19 @@ int slab_split(const Shape4& s, bool may_split, float& time) {
   return best;
 }
 
-// Up to 64 rows.  Measured, in us (stream of w / rows / slab, MXFP4): M 1: 7168 x 2048
-// 5.8 / 4.8 / 7.2, 7168 x 7168 9.0 / 10.2 / 11.8, 2048 x 16384 9.1 / 14.4 / 11.2,
-// 16384 gated x 7168 24.6 / 29.7 / 32; M 8: 7168 x 7168 11.9 / 12.3 / 12.6; M 16:
-// 512 gated x 2048 6.7 / 7.5 / 9.1, 7168 x 7168 - / 16.0 / 13.6; M 32: 7168 x 2048
-// - / 10.1 / 11.9, 7168 x 7168 - / 22.2 / 15.8; M 64: 7168 x 2048 - / 17.1 / 15.0,
-// 7168 x 7168 - / 40 / 21.
-Plan4 plan_few(const Shape4& s, bool may_split) {
+// Up to 64 rows.  Measured, in us (stream of w / blocks / slabs, MXFP4): M 1: 512 gated x
+// 2048 5.6 / 4.5 / -, 7168 x 7168 9.1 / 8.8 / -, 16384 gated x 7168 25 / 30 / 29; M 4: 7168
+// x 7168 10.5 / 9.3 / 11.2; M 8: 7168 x 2048 6.3 / 5.3 / -, 16384 x 7168 17.8 / 18.7 / 17.1;
+// M 16: 7168 x 7168 - / 12.8 / 12.5, 2048 x 16384 - / 19.5 / 13.1, 16384 gated x 7168 - / 47 /
+// 32; M 24: 16384 x 4096 - / 18.4 / 16.5; M 64: 7168 x 2048 - / 9.4 / 14.5, 7168 x 7168 -
+// / 20.6 / 20.4.  (The estimates' choice is the fastest of three or within 4% of it there.)
+Plan4 plan_few(const Shape4& s, bool aligned, bool may_split) {
+  if (!aligned) return {kRows4, 1};
   float slab;
   const int split = slab_split(s, may_split, slab);
-  const float skinny = skinny_time(s), rows = rows_time(s);
-  if (skinny <= rows && skinny <= slab) return {kSkinny4, 1};
-  if (rows <= slab) return {kRows4, 1};
+  const float skinny = skinny_time(s), block = block_time(s);
+  if (skinny <= block && skinny <= slab) return {kSkinny4, 1};
+  if (block <= slab) return {kBlock4, 1};
   return {kSlab4, split};
 }
 
@@ -106,7 +115,7 @@ Plan4 plan_many(const Shape4& s, bool may_split) {
       if (split > 1 && (!may_split || nb < 2 * split || tiles >= 2 * kCus)) break;
       const int per = (int)up(nb, split), real = (int)up(nb, per);
       const float t = 4.0f + up(tiles * real, kCus) * (per * (kind == kWide4 ? step4 : step2) + 2.f) +
-                      join_time(s, real);
+                      join_time(s, real, 5e6f);
       if (t < time) {
         time = t;
         best = Plan4{kind, real};
@@ -128,7 +137,7 @@ Plan4 plan_any(const Shape4& s, bool may_split) {
 }
 
 Plan4 plan(const Shape4& s, bool aligned, bool may_split) {
-  if (s.M <= 64) return plan_few(s, may_split);
+  if (s.M <= 64) return plan_few(s, aligned, may_split);
   return aligned ? plan_many(s, may_split) : plan_any(s, may_split);
 }
 
@@ -195,11 +204,13 @@ hipError_t xtu_linear4(const xtu_linear4_args* args, hipStream_t stream) {
   a.xvec = al(t.x, 16) && K % 8 == 0 && (M == 1 || t.ldx % 8 == 0);
   (void)hipGetLastError();
   const Shape4 s = shape_of(M, N, K, t.act, t.fmt, t.group);
-  Plan4 p = plan(s, wide4_fits(a), true);
-  if (split_bytes(p, s) > (t.workspace ? t.workspace_bytes : 0)) p = plan(s, wide4_fits(a), false);
+  const bool aligned = M <= 64 ? x_in_reach(a) : wide4_fits(a);
+  Plan4 p = plan(s, aligned, true);
+  if (split_bytes(p, s) > (t.workspace ? t.workspace_bytes : 0)) p = plan(s, aligned, false);
   float* part = reinterpret_cast<float*>(t.workspace);
   switch (p.kind) {
     case kSkinny4: return launch4_skinny(a, stream);
+    case kBlock4: return launch4_block(a, stream);
     case kRows4: return launch4_rows(a, stream);
     case kSlab4: return launch4_slab(a, p.split, part, stream);
     case kTile4: return launch4_tile(a, p.split, part, stream);

@@ -192,7 +192,7 @@ struct Shape4 {
 };
 
 // The kernels, and the ranges of K that are summed apart.
-enum Kind4 : int { kSkinny4 = 0, kRows4, kSlab4, kWide2, kWide4, kTile4 };
+enum Kind4 : int { kSkinny4 = 0, kBlock4, kSlab4, kWide2, kWide4, kTile4, kRows4 };
 struct Plan4 {
   int kind, split;
 };
@@ -204,13 +204,16 @@ struct SkinnyPlan {
 };
 SkinnyPlan skinny4_plan(const Shape4& s);
 hipError_t launch4_skinny(const Linear4Args& a, hipStream_t stream);
-// Up to 64 rows of x, nothing staged.
-int rows4_waves(const Shape4& s);
+// Up to 64 rows of x at any alignment, nothing staged.
 hipError_t launch4_rows(const Linear4Args& a, hipStream_t stream);
-// Up to 64 rows of x, a range of `per` blocks of K of them in LDS.
-constexpr int kSlabWaves = 8, kSlabPad = 32;   // pad: bytes behind a row of x in LDS (banks)
-constexpr size_t kSlabLds = 150 * 1024;
-inline size_t slab4_lds(int M, int per) { return (size_t)M * ((size_t)per * 256 + kSlabPad); }
+// Up to 64 rows of x, which start on 16 bytes, blocks of a wave's own in LDS.
+bool x_in_reach(const Linear4Args& a);   // by 32-bit offsets, for this and the next
+int block4_waves(const Shape4& s);
+hipError_t launch4_block(const Linear4Args& a, hipStream_t stream);
+// Up to 64 rows of x, which start on 16 bytes, a range of `per` blocks of K in LDS.
+constexpr int kSlabWaves = 8;
+constexpr size_t kSlabLds = 160 * 1024;
+inline size_t slab4_lds(int M, int per) { return (size_t)((M + 3) / 4) * 1024 * per; }
 hipError_t launch4_slab(const Linear4Args& a, int split, float* part, hipStream_t stream);
 // More rows, which start on 16 bytes: tiles of 128 rows and 64 NP rows of w.
 bool wide4_fits(const Linear4Args& a);

@@ -18,6 +18,8 @@ template <int FMT, int G, int AK, int MT, int U>
 __global__ __launch_bounds__(64 * kWv) void linear4_slab_kernel(Linear4Args a, int per, float* part) {
   constexpr bool GATED = AK == lin::kActSwiglu;
   constexpr int REC = record_bytes(FMT, G), COLS = GATED ? 16 : 32;
+  constexpr int LW = 2 * (1 + (FMT == kI4 ? 128 / G : 1));   // loads of a block's records
+  static_assert(U * LW <= 63, "vmcnt");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const LinearArgs& e = a.e;
   const int tid = threadIdx.x, lane = tid % 64;
@@ -35,39 +37,49 @@ __global__ __launch_bounds__(64 * kWv) void linear4_slab_kernel(Linear4Args a, i
 #pragma unroll
     for (int p = 0; p < 2; ++p) r[p] = load_raw<FMT, G>(wp[p] + o, q, c, 4 * q);
   };
-#pragma unroll
-  for (int i = 0; i < U; ++i) load(s0 + i, raw[i]);
-  __builtin_amdgcn_sched_barrier(0);   // x after the first loads of w
-  // x to LDS, zeros behind K: a wave takes every eighth row
-  const int ldx = per * 256 + kSlabPad, pieces = (s1 - s0) * 16;
-  for (int r0 = w; r0 < e.M; r0 += kWv * 4) {
-    for (int p = lane; p < pieces; p += 64) {
-      u32x4_t v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[i] = load_x8(a, e.x + (long)min(r0 + kWv * i, e.M - 1) * e.ldx, 128 * s0 + 8 * p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (r0 + kWv * i < e.M)
-          *reinterpret_cast<u32x4_t*>(lds + (r0 + kWv * i) * ldx + 16 * p) = v[i];
+  // x straight to LDS, block by block: a load brings four rows, a piece of 16 bytes a
+  // lane (linear_tile.hip has the slots); the waves take turns
+  const u32x4_t xr = lin::raw_buffer(e.x, (uint32_t)(((long)(e.M - 1) * e.ldx + e.K) * 2));
+  const int quads = (e.M + 3) / 4, size = quads * 1024;   // of a block
+  int r = w % quads, s = s0 + w / quads;
+  const int dr = kWv % quads, ds = kWv / quads;
+#pragma unroll 1
+  while (s < s1) {
+    const int row = 4 * r + lane / 16, k = 8 * (lane % 16 ^ (row & 7) << 1);
+    const uint32_t off = (uint32_t)min(row, e.M - 1) * (uint32_t)(e.ldx * 2) + 2 * k;
+    lin::buf_to_lds(xr, k < e.K - 128 * s ? off : 0x80000000u, (uint32_t)s * 256u,
+                    lds + (s - s0) * size + r * 1024);
+    r += dr;
+    s += ds;
+    if (r >= quads) {
+      r -= quads;
+      ++s;
     }
   }
-  __syncthreads();
-  const uint8_t* xl[MT];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) xl[mt] = lds + min(16 * mt + c, e.M - 1) * ldx + 16 * q;
+  for (int i = 0; i < U; ++i) load(s0 + i, raw[i]);
+  __builtin_amdgcn_s_waitcnt(lin::wait_vm(U * LW));   // x; loads come back in order
+  __syncthreads();
+  const uint8_t* xl[MT];   // (rows past M repeat the last one: not written)
+  int slot[MT];            // of place 4 j + q: j moves bits 2 and 3
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int row = min(16 * mt + c, e.M - 1);
+    xl[mt] = lds + row * 256;
+    slot[mt] = (q ^ (row & 7) << 1) * 16;
+  }
   f32x4_t acc[2][MT];
 #pragma unroll
   for (int p = 0; p < 2; ++p)
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) acc[p][mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int s = s0; s < s1; s += U) {
+  for (s = s0; s < s1; s += U) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       if (s + i >= s1) break;
-      const int o = (s + i - s0) * 256;
+      const int o = (s + i - s0) * size;
       multiply<FMT, G, 2, MT>(raw[i], acc, [&](int j, int mt) {
-        return *reinterpret_cast<const u32x4_t*>(xl[mt] + o + 64 * j);
+        return *reinterpret_cast<const u32x4_t*>(xl[mt] + o + (slot[mt] ^ 64 * j));
       });
       load(s + i + U, raw[i]);
     }
