@@ -144,6 +144,37 @@ def test_weights_refused():
         assert Weight4.from_dense("int4", c, f.to(t)).data.shape == (1, 1, 1024 + 256)
 
 
+def test_weights_in_other_orders():
+    """Checkpoint tensors as views: transposed storage, slices, torch's scale types."""
+    for fmt, group in GROUPS:
+        codes, s, gs = _dense(fmt, 40, 256, group, seed=5)
+        want = Weight4.from_dense(fmt, codes, s, gs, gated=True)
+        wide = torch.zeros((40, 200), dtype=torch.uint8)
+        wide[:, 7:135] = codes
+        for c, z in ((codes.t().contiguous().t(), s.t().contiguous().t()), (wide[:, 7:135], s)):
+            got = Weight4.from_dense(fmt, c, z, gs, gated=True)
+            assert torch.equal(got.data, want.data)
+    codes, s, _ = _dense(F.FMT_MXFP4, 40, 256, 32, seed=5)
+    assert torch.equal(Weight4.from_dense("mxfp4", codes, s.view(torch.float8_e8m0fnu)).data,
+                       Weight4.from_dense("mxfp4", codes, s).data)
+
+
+def test_weights_do_not_change():
+    """The kernels take the records' size from N and K: other records are refused."""
+    import dataclasses
+    w = _w("nvfp4", 36, 160, gated=True)
+    for field in ("data", "gs", "N", "K"):
+        with pytest.raises(dataclasses.FrozenInstanceError):
+            setattr(w, field, getattr(w, field))
+    for kw in (dict(data=w.data[:1]), dict(data=w.data.int()), dict(N=40), dict(K=512),
+               dict(gated=False), dict(data=w.data.flip(0).transpose(0, 1)), dict(gs=None),
+               dict(gs=w.gs[:1]), dict(gs=w.gs.double()), dict(fmt=F.FMT_MXFP4, group=32)):
+        with pytest.raises(ValueError, match="must be"):
+            dataclasses.replace(w, **kw)
+    moved = w.to("cpu")
+    assert torch.equal(moved.data, w.data) and moved.nbytes == w.nbytes
+
+
 def _refused(match, *args, **kw):
     with pytest.raises(ValueError, match=match):
         linear4(*args, **kw)

@@ -60,6 +60,7 @@ float block_time(const Shape4& s) {
 }
 
 // The split of K with the least time, 0 where no range of K fits LDS.
+constexpr float kSlabBase = 6.0f;
 int slab_split(const Shape4& s, bool may_split, float& time) {
   const int nb = blocks_of(s.K);
   const long gx = up(s.N, (s.gated ? 16 : 32) * kSlabWaves);
@@ -71,7 +72,7 @@ int slab_split(const Shape4& s, bool may_split, float& time) {
     const long rounds = up(gx * split, kCus);
     const float x = slab4_lds(s.M, per) * 1e-3f;
     const float w = 2e-3f * kSlabWaves * per * record_bytes(s.fmt, s.group);
-    const float t = 6.0f + rounds * x / 65.f + larger(gx * split * w / 6200.f, rounds * w / 50.f) +
+    const float t = kSlabBase + rounds * x / 65.f + larger(gx * split * w / 6200.f, rounds * w / 50.f) +
                     1.f * (rounds - 1) + join_time(s, split, 4e6f);
     if (t < time) {
       time = t;
@@ -89,9 +90,10 @@ int slab_split(const Shape4& s, bool may_split, float& time) {
 // / 20.6 / 20.4.  (The estimates' choice is the fastest of three or within 4% of it there.)
 Plan4 plan_few(const Shape4& s, bool aligned, bool may_split) {
   if (!aligned) return {kRows4, 1};
-  float slab;
-  const int split = slab_split(s, may_split, slab);
   const float skinny = skinny_time(s), block = block_time(s);
+  float slab = 1e30f;
+  int split = 0;
+  if (skinny > kSlabBase && block > kSlabBase) split = slab_split(s, may_split, slab);
   if (skinny <= block && skinny <= slab) return {kSkinny4, 1};
   if (block <= slab) return {kBlock4, 1};
   return {kSlab4, split};

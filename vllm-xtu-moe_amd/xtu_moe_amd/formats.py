@@ -288,6 +288,11 @@ def linear4_group(fmt: int, s, K: int) -> int:
     return g
 
 
+def linear4_record(fmt: int, group: int) -> int:
+    """Bytes of a record."""
+    return 1024 + {FMT_MXFP4: 64, FMT_NVFP4: 128, FMT_INT4: 8192 // group}[fmt]
+
+
 def pack_linear4(fmt: int, codes, s, group: int):
     """codes u8 [n, N, K/2] (low nibble = even k) and scales [n, N, K/group] of n
     halves (1; 2: gate, up) -> records u8 [panels, blocks, record], the halves'

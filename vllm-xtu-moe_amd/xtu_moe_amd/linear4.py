@@ -12,12 +12,14 @@ engine (xiaotu_moe/csrc/moe/moe_v2.hpp:454-470).
 from __future__ import annotations
 
 import struct
+from dataclasses import dataclass, replace
+from typing import Optional
 
 import torch
 
 from . import _lib
 from .formats import (FMT_INT4, FMT_MXFP4, FMT_NAMES, FMT_NVFP4, fmt_of, linear4_group,
-                      pack_linear4)
+                      linear4_record, pack_linear4)
 from .layer import _same_device
 from .linear import (_OPERAND, _TYPES, ACTIVATIONS, MAX_COLS, MAX_ROWS, _current_device, _overlap,
                      _rows, on_stream, raw_stream)
@@ -31,28 +33,53 @@ _WS_BYTES: dict = {}
 _ENTRY = None
 
 
+@dataclass(frozen=True, eq=False)
 class Weight4:
     """One matrix [N, K] (gated: gate rows [N, K], then up rows [N, K]) in the
-    kernels' layout.  Made by ``from_dense``; moved and freed with ``data``."""
+    kernels' layout: ``data`` u8 records, ``gs`` fp32 [1] or [2] (NVFP4; else
+    None).  Made by ``from_dense``; its fields do not change."""
+    fmt: int
+    N: int
+    K: int
+    group: int
+    gated: bool
+    data: torch.Tensor
+    gs: Optional[torch.Tensor]
 
-    def __init__(self, fmt, N, K, group, gated, data, gs):
-        self.fmt, self.N, self.K, self.group, self.gated = fmt, N, K, group, gated
-        self.data, self.gs = data, gs
-        self.nbytes = data.numel()
+    def __post_init__(self):
+        halves = 2 if self.gated else 1
+        need = (halves * -(-self.N // 16), -(-self.K // 128), linear4_record(self.fmt, self.group))
+        d, gs = self.data, self.gs
+        if d.dtype != torch.uint8 or tuple(d.shape) != need or not d.is_contiguous() \
+                or d.data_ptr() % 16:
+            raise ValueError(f"records must be contiguous u8 {need} on 16 bytes, got "
+                             f"{tuple(d.shape)} {d.dtype}")
+        if (gs is not None) != (self.fmt == FMT_NVFP4) or gs is not None and (
+                gs.dtype != torch.float32 or gs.shape != (halves,) or gs.device != d.device
+                or not gs.is_contiguous()):
+            raise ValueError(f"second-level scales must be fp32 [{halves}] beside NVFP4 records")
 
     @property
     def device(self):
         return self.data.device
+
+    @property
+    def nbytes(self):
+        return self.data.numel()
+
+    def to(self, device):
+        """The same matrix on another device."""
+        return replace(self, data=self.data.to(device),
+                       gs=None if self.gs is None else self.gs.to(device))
 
     @classmethod
     def from_dense(cls, fmt, codes, scales, global_scale=None, *, gated=False, device=None):
         """Packs a checkpoint's tensors.
 
         fmt: "mxfp4", "nvfp4" or "int4" (or its number in ``formats``).  codes
-        u8 [rows, K / 2], low nibble = even k.  scales: MXFP4 e8m0 bytes
-        [rows, K / 32] (at most 252: larger ones leave bf16's range; 255 is
-        NaN); NVFP4 e4m3 (as bytes or as torch.float8_e4m3fn, no NaN)
-        [rows, K / 16]; INT4 finite fp32, fp16 or bf16 [rows, K / 32, 64 or
+        u8 [rows, K / 2], low nibble = even k.  scales, as bytes or as torch's
+        type of them: MXFP4 e8m0 [rows, K / 32] (at most 252: larger ones leave
+        bf16's range; 255 is NaN); NVFP4 e4m3 (no NaN) [rows, K / 16]; INT4 finite fp32, fp16 or bf16 [rows, K / 32, 64 or
         128], for value code - 8.  global_scale: NVFP4's second-level scale, a
         number or a tensor of one (gated: one or two, gate and up).  gated:
         rows are [gate; up], for activation "swiglu".  Reads the scales back
@@ -78,10 +105,10 @@ class Weight4:
             if not bool((scales.abs().float() < 2.0 ** 123).all()):
                 raise ValueError("INT4 scales must be finite (below 2^123)")
         else:
-            types = (torch.uint8, torch.float8_e4m3fn) if fmt == FMT_NVFP4 else (torch.uint8,)
-            if scales.dtype not in types:
+            own = torch.float8_e4m3fn if fmt == FMT_NVFP4 else torch.float8_e8m0fnu
+            if scales.dtype not in (torch.uint8, own):
                 raise ValueError(f"{FMT_NAMES[fmt]} scales must be bytes, got {scales.dtype}")
-            b = scales.view(torch.uint8)
+            b = scales = scales.contiguous().view(torch.uint8)
             if fmt == FMT_MXFP4 and bool((b > MAX_E8M0).any()):
                 raise ValueError(f"e8m0 scales above {MAX_E8M0} leave bf16's range")
             if fmt == FMT_NVFP4 and bool(((b & 0x7f) == 0x7f).any()):
@@ -98,8 +125,8 @@ class Weight4:
             gs = gs.expand(halves).contiguous()
         elif global_scale is not None:
             raise ValueError(f"{FMT_NAMES[fmt]} weights have no second-level scale")
-        data = pack_linear4(fmt, codes.to(dev).reshape(halves, rows // halves, -1),
-                            scales.to(dev).reshape(halves, rows // halves, -1), group)
+        split = lambda t: t.to(dev).contiguous().view(halves, rows // halves, -1)  # noqa: E731
+        data = pack_linear4(fmt, split(codes), split(scales), group)
         return cls(fmt, rows // halves, K, group, bool(gated), data, gs)
 
 

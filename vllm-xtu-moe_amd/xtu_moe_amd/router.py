@@ -32,7 +32,8 @@ _ENTRIES = None
 
 class RouterLosses(NamedTuple):
     """weights fp32 [T, K]; balance and z fp32 scalars (z None with sigmoid
-    scoring); counts int32 and probs fp32 [S, E], without gradient."""
+    scoring); counts int32 and probs fp32 [S, E], without gradient.  The backward
+    reads weights and counts: to change them (an all-reduce), take a clone."""
     weights: torch.Tensor
     balance: torch.Tensor
     z: Optional[torch.Tensor]
