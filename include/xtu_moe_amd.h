@@ -646,7 +646,10 @@ int xtu_linear_plan(int M, int N, int K, int act);
  * as 7 - v), then the scales: MXFP4 [16 row][4 j] bytes, NVFP4 [2 q / 2][16 row][4 j]
  * bytes, INT4 fp32 [128 / group][16 row].  Rows and k past the matrix: codes 0, e8m0
  * 127 or scale 0.  The products are exact in the fp32 sums' operands (INT4: the scale
- * multiplies each group's fp32 sum).  workspace: as xtu_linear's, for K splits.  The
+ * multiplies each group's fp32 sum).  workspace (16-byte aligned, may be NULL):
+ * xtu_linear4_workspace_bytes() lets a product of few tiles split K, and x whose rows do
+ * not start on 16 bytes (aligned 0) be copied first; with less the call takes another
+ * way, slower.  The
  * reference leaves these products to its host (vllm_xiaotu_moe/hybrid_model.py:1752). */
 typedef struct xtu_linear4_args {
   const void* x;
@@ -665,13 +668,11 @@ typedef struct xtu_linear4_args {
 } xtu_linear4_args;
 hipError_t xtu_linear4(const xtu_linear4_args* args, hipStream_t stream);
 size_t xtu_linear4_weight_bytes(int N, int K, int act, int fmt, int group);
-size_t xtu_linear4_workspace_bytes(int M, int N, int K, int act, int fmt, int group);
+size_t xtu_linear4_workspace_bytes(int M, int N, int K, int act, int fmt, int group, int aligned);
 /* Which kernel a product with all of that workspace takes, 16 * (K splits) + 0 the
- * stream of w (all of x in LDS), 1 blocks (a block of x per wave in LDS), 2 slabs (a
- * range of K of x in LDS), 3 and 4 tiles of 128 x 128 and 128 x 256; for rows of x that
- * do not start on 16 bytes (aligned 0) 5 tiles of 64 x 128, 6 rows (nothing staged); -1
- * none. */
-int xtu_linear4_plan(int M, int N, int K, int act, int fmt, int group, int aligned);
+ * stream of w (all of x in LDS), 1 blocks (blocks of x per wave in LDS), 2 slabs (a
+ * range of K of x in LDS), 3 and 4 tiles of 128 x 128 and 128 x 256; -1 none. */
+int xtu_linear4_plan(int M, int N, int K, int act, int fmt, int group);
 
 /* ------------------------------------------------ router, training step
  * What a training step takes from router logits [T][E] (fp32, or bf16 with

@@ -14,9 +14,9 @@ import torch
 
 from test_gpu_linear import _act64
 from test_linear4 import GROUPS, forms
-from xtu_moe_amd import formats as F
+from xtu_moe_amd import _lib, formats as F
 from xtu_moe_amd.linear import ACTIVATIONS
-from xtu_moe_amd.linear4 import Weight4, linear4
+from xtu_moe_amd.linear4 import ARGS, Weight4, linear4
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -110,17 +110,40 @@ def test_sizes(fmt, group, gated):
 @pytest.mark.parametrize("fmt,group", GROUPS)
 @pytest.mark.parametrize("gated", [False, True])
 def test_every_form(fmt, group, gated):
-    """Each kernel, whole and with K split, with the whole epilogue."""
+    """Each kernel, whole and with K split, with the whole epilogue; and x at odd
+    addresses, copied first."""
     for i, ((kernel, _), M, N, K) in enumerate(forms(fmt, group, gated)):
-        x = _rand((M, K + 8), i)
-        x = x[:, 1:K + 1] if kernel >= 5 else x[:, :K]
+        big = _rand((M, K + 8), i)
         W, w = _weight(fmt, group, N, K, gated, seed=70 + i)
         b = _rand((w.shape[0],), 2, 0.5, F32)
         r = _rand((M, N), 4, 1.0, BF if i % 2 else F32)
         for act in ("swiglu",) if gated else ("none", "gelu"):
+            x = big[:, :K]
             out = linear4(x, W, bias=b, activation=act, residual=r, out_dtype=F32)
             _check(out, x, w, act, b, residual=r, what=(kernel, M, N, K, act))
-        _check(linear4(x, W, activation=act), x, w, act, what=(kernel, M, N, K))
+            x = big[:, 1:K + 1]
+            _check(linear4(x, W, activation=act), x, w, act, what=(kernel, M, N, K, "odd"))
+
+
+@pytest.mark.parametrize("fmt,group", GROUPS)
+@pytest.mark.parametrize("gated", [False, True])
+def test_entry_without_a_workspace(fmt, group, gated):
+    """No copy of x and no K split: other kernels, the same results up to rounding."""
+    stream = torch.cuda.current_stream().cuda_stream
+    for M, N, K, first in ((1, 40, 256, 1), (16, 2000, 8192, 0), (64, 260, 8192, 0), (50, 300, 640, 1),
+                           (200, 205, 1280, 1), (130, 260, 4096, 0), (65, 64, 128, 3)):
+        big = _rand((M, K + 8), M)
+        x = big[:, first:first + K]
+        W, w = _weight(fmt, group, N, K, gated, seed=M)
+        for vec in (True, False):
+            hold = torch.full((M, N + 4), 7.0, dtype=F32, device=DEV)
+            out = hold[:, :N] if vec else hold[:, 1:N + 1]
+            args = ARGS.pack(x.data_ptr(), W.data.data_ptr(), 0 if W.gs is None else W.gs.data_ptr(),
+                             0, 0, 0, out.data_ptr(), 0, x.stride(0), 0, out.stride(0), 0, 0, M, N, K,
+                             6 if gated else 3, fmt, group, 0, 0, 0, 0.0, 1.0, 0.0)
+            assert _lib.load().xtu_linear4(args, stream) == 0
+            _check(out, x, w, "swiglu" if gated else "gelu", what=(M, N, K, first))
+            assert int((hold == 7.0).sum()) >= 4 * M
 
 
 @pytest.mark.parametrize("act", list(ACTIVATIONS))

@@ -36,9 +36,6 @@ FORMS = {
     (3, True): [(71, 16, 896), (123, 504, 2816)],
     (4, False): [(1224, 3405, 256), (1838, 2228, 512)],
     (4, True): [(65, 5888, 5248)],
-    (5, False): [(70, 16, 128), (353, 490, 384)],
-    (5, True): [(85, 18, 512), (300, 1228, 512)],
-    (6, False): [(1, 16, 128), (14, 357, 1280), (29, 203, 1280), (45, 300, 640), (64, 204, 2176)],
 }
 
 
@@ -55,7 +52,7 @@ def forms(fmt, group, gated):
 @pytest.mark.parametrize("gated", [False, True])
 def test_forms_are_taken(fmt, group, gated):
     for (kernel, split), M, N, K in forms(fmt, group, gated):
-        plan = _lib.load().xtu_linear4_plan(M, N, K, 6 if gated else 0, fmt, group, int(kernel < 5))
+        plan = _lib.load().xtu_linear4_plan(M, N, K, 6 if gated else 0, fmt, group)
         assert (plan % 16, plan >= 32) == (kernel, split), (M, N, K, plan % 16, plan // 16)
 
 
@@ -253,6 +250,8 @@ def test_entry_refuses_on_the_host():
                 dict(fmt=4, group=64, K=96), dict(M=(1 << 31) - 511),
                 dict(M=1 << 30, N=1 << 20, ldo=1 << 20)):
         assert rc(**bad) == 1, bad
-    assert lib.xtu_linear4_workspace_bytes(0, 1, 32, 0, 2, 32) == 0
-    assert lib.xtu_linear4_workspace_bytes(1, 1, 33, 0, 2, 32) == 0
+    assert lib.xtu_linear4_workspace_bytes(0, 1, 32, 0, 2, 32, 1) == 0
+    assert lib.xtu_linear4_workspace_bytes(1, 1, 33, 0, 2, 32, 1) == 0
+    assert lib.xtu_linear4_workspace_bytes(5, 1, 96, 0, 2, 32, 0) == 5 * 96 * 2   # a copy of x
+    assert lib.xtu_linear4_plan(0, 1, 32, 0, 2, 32) == lib.xtu_linear4_plan(1, 1, 48, 0, 2, 32) == -1
     assert lib.xtu_linear4_weight_bytes(1, 32, 0, 1, 32) == 0

@@ -147,6 +147,15 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const uint16_t* x, lon
 
 }  // namespace
 
+hipError_t launch_pack_x(const uint16_t* x, long ldx, int M, int K, uint16_t* out,
+                         hipStream_t stream) {
+  const long pieces = (long)M * ((K + 7) / 8);
+  if (!grid_fits((pieces + 255) / 256, 256)) return hipErrorInvalidConfiguration;
+  linear_pack_kernel<<<(unsigned)((pieces + 255) / 256), 256, 0, stream>>>(x, ldx, M, nullptr, 0, 0,
+                                                                           K, out);
+  return hipPeekAtLastError();
+}
+
 hipError_t launch_join(const LinearArgs& a, int split, const float* part, hipStream_t stream) {
   const long n = (long)a.M * (a.vec ? a.N / 4 : a.N);
   if (!grid_fits((n + 255) / 256, 256)) return hipErrorInvalidConfiguration;

@@ -297,6 +297,9 @@ bool skinny_fits(const LinearArgs& a);
 hipError_t launch_skinny(const LinearArgs& a, hipStream_t stream);
 hipError_t launch_any(const LinearArgs& a, hipStream_t stream);
 hipError_t launch_join(const LinearArgs& a, int split, const float* part, hipStream_t stream);
+// Rows of x at any alignment as rows of K rounded up to 8, zeros behind K.
+hipError_t launch_pack_x(const uint16_t* x, long ldx, int M, int K, uint16_t* out,
+                         hipStream_t stream);
 
 }  // namespace lin
 }  // namespace xtu

@@ -88,8 +88,7 @@ int slab_split(const Shape4& s, bool may_split, float& time) {
 // M 16: 7168 x 7168 - / 12.8 / 12.5, 2048 x 16384 - / 19.5 / 13.1, 16384 gated x 7168 - / 47 /
 // 32; M 24: 16384 x 4096 - / 18.4 / 16.5; M 64: 7168 x 2048 - / 9.4 / 14.5, 7168 x 7168 -
 // / 20.6 / 20.4.  (The estimates' choice is the fastest of three or within 4% of it there.)
-Plan4 plan_few(const Shape4& s, bool aligned, bool may_split) {
-  if (!aligned) return {kRows4, 1};
+Plan4 plan_few(const Shape4& s, bool may_split) {
   const float skinny = skinny_time(s), block = block_time(s);
   float slab = 1e30f;
   int split = 0;
@@ -127,24 +126,21 @@ Plan4 plan_many(const Shape4& s, bool may_split) {
   return best;
 }
 
-// Rows of x that do not start on 16 bytes: tiles of 64 rows, x by way of registers.
-Plan4 plan_any(const Shape4& s, bool may_split) {
-  Plan4 p{kTile4, 1};
-  const long tiles = up(s.M, 64) * up(s.N, s.gated ? 64 : 128);
-  if (may_split)
-    while (p.split < 16 && tiles * p.split * 2 <= 2 * kCus && blocks_of(s.K) >= 4 * p.split)
-      p.split *= 2;
-  p.split = (int)up(blocks_of(s.K), up(blocks_of(s.K), p.split));
-  return p;
-}
-
-Plan4 plan(const Shape4& s, bool aligned, bool may_split) {
-  if (s.M <= 64) return plan_few(s, aligned, may_split);
-  return aligned ? plan_many(s, may_split) : plan_any(s, may_split);
+Plan4 plan(const Shape4& s, bool may_split) {
+  return s.M <= 64 ? plan_few(s, may_split) : plan_many(s, may_split);
 }
 
 size_t split_bytes(const Plan4& p, const Shape4& s) {
   return p.split > 1 ? (size_t)p.split * s.M * s.N * (s.gated ? 2 : 1) * 4 : 0;
+}
+
+// A copy of x.
+size_t pack_bytes(int M, int K) { return (size_t)M * ((K + 7) / 8) * 16; }
+
+// Rows of x on 16 bytes and, 128 of them, in reach of 32-bit offsets.
+bool x_fits(const LinearArgs& e) {
+  return reinterpret_cast<uintptr_t>(e.x) % 16 == 0 && e.K % 8 == 0 &&
+         (e.M == 1 || e.ldx % 8 == 0) && ((e.M == 1 ? 0 : 128 * e.ldx) + e.K) * 2 < (1L << 31);
 }
 
 Shape4 shape_of(int M, int N, int K, int act, int fmt, int group) {
@@ -163,16 +159,15 @@ size_t xtu_linear4_weight_bytes(int N, int K, int act, int fmt, int group) {
          record_bytes(fmt, group);
 }
 
-size_t xtu_linear4_workspace_bytes(int M, int N, int K, int act, int fmt, int group) {
+size_t xtu_linear4_workspace_bytes(int M, int N, int K, int act, int fmt, int group, int aligned) {
   if (!sizes_ok(M, N, K, act, fmt, group) || M == 0) return 0;
   const Shape4 s = shape_of(M, N, K, act, fmt, group);
-  const size_t a = split_bytes(plan(s, true, true), s), b = split_bytes(plan(s, false, true), s);
-  return a > b ? a : b;
+  return split_bytes(plan(s, true), s) + (aligned ? 0 : pack_bytes(M, K));
 }
 
-int xtu_linear4_plan(int M, int N, int K, int act, int fmt, int group, int aligned) {
+int xtu_linear4_plan(int M, int N, int K, int act, int fmt, int group) {
   if (!sizes_ok(M, N, K, act, fmt, group) || M == 0) return -1;
-  const Plan4 p = plan(shape_of(M, N, K, act, fmt, group), aligned, true);
+  const Plan4 p = plan(shape_of(M, N, K, act, fmt, group), true);
   return 16 * p.split + p.kind;
 }
 
@@ -203,19 +198,29 @@ hipError_t xtu_linear4(const xtu_linear4_args* args, hipStream_t stream) {
   a.gs = t.gs;
   a.fmt = t.fmt;
   a.group = t.group;
-  a.xvec = al(t.x, 16) && K % 8 == 0 && (M == 1 || t.ldx % 8 == 0);
   (void)hipGetLastError();
   const Shape4 s = shape_of(M, N, K, t.act, t.fmt, t.group);
-  const bool aligned = M <= 64 ? x_in_reach(a) : wide4_fits(a);
-  Plan4 p = plan(s, aligned, true);
-  if (split_bytes(p, s) > (t.workspace ? t.workspace_bytes : 0)) p = plan(s, aligned, false);
-  float* part = reinterpret_cast<float*>(t.workspace);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(t.workspace);
+  size_t left = ws ? t.workspace_bytes : 0;
+  if (!x_fits(a.e)) {
+    const size_t need = pack_bytes(M, K);
+    LinearArgs copy = a.e;
+    copy.x = reinterpret_cast<const uint16_t*>(ws);
+    copy.ldx = K;
+    if (left < need || !x_fits(copy)) return launch4_tile(a, stream);
+    const hipError_t e = lin::launch_pack_x(a.e.x, a.e.ldx, M, K, reinterpret_cast<uint16_t*>(ws), stream);
+    if (e != hipSuccess) return e;
+    a.e = copy;
+    ws += need;
+    left -= need;
+  }
+  Plan4 p = plan(s, true);
+  if (split_bytes(p, s) > left) p = plan(s, false);
+  float* part = reinterpret_cast<float*>(ws);
   switch (p.kind) {
     case kSkinny4: return launch4_skinny(a, stream);
     case kBlock4: return launch4_block(a, stream);
-    case kRows4: return launch4_rows(a, stream);
     case kSlab4: return launch4_slab(a, p.split, part, stream);
-    case kTile4: return launch4_tile(a, p.split, part, stream);
     default: return launch4_wide(p, a, part, stream);
   }
 }

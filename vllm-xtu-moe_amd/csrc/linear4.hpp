@@ -40,7 +40,6 @@ struct Linear4Args {
   const uint8_t* w;       // records
   const float* gs;        // NVFP4: [1], swiglu [2] (gate, up); else null
   int fmt, group;
-  int xvec;               // rows of x start on 16 bytes, K % 8 == 0
 };
 
 __host__ __device__ constexpr int scale_bytes(int fmt, int group) {
@@ -175,14 +174,11 @@ __device__ __forceinline__ void multiply(const Raw<FMT, G> (&r)[NP], f32x4_t (&a
   multiply<FMT, G, NP, MT>(r, acc, x, [] {});
 }
 
-// Eight k of a row of x, zeros past K.
+// Eight k of a row of x that starts on 16 bytes, zeros past K.
 __device__ __forceinline__ u32x4_t load_x8(const Linear4Args& a, const uint16_t* row, int k) {
-  if (a.xvec) {
-    u32x4_t v = {0u, 0u, 0u, 0u};
-    if (k < a.e.K) v = *reinterpret_cast<const u32x4_t*>(row + k);
-    return v;
-  }
-  return lin::load8(row, k, a.e.K);
+  u32x4_t v = {0u, 0u, 0u, 0u};
+  if (k < a.e.K) v = *reinterpret_cast<const u32x4_t*>(row + k);
+  return v;
 }
 
 struct Shape4 {
@@ -191,8 +187,9 @@ struct Shape4 {
   int fmt, group;
 };
 
-// The kernels, and the ranges of K that are summed apart.
-enum Kind4 : int { kSkinny4 = 0, kBlock4, kSlab4, kWide2, kWide4, kTile4, kRows4 };
+// The kernels, for rows of x on 16 bytes and in reach of 32-bit offsets, and the ranges
+// of K that are summed apart.
+enum Kind4 : int { kSkinny4 = 0, kBlock4, kSlab4, kWide2, kWide4 };
 struct Plan4 {
   int kind, split;
 };
@@ -204,22 +201,18 @@ struct SkinnyPlan {
 };
 SkinnyPlan skinny4_plan(const Shape4& s);
 hipError_t launch4_skinny(const Linear4Args& a, hipStream_t stream);
-// Up to 64 rows of x at any alignment, nothing staged.
-hipError_t launch4_rows(const Linear4Args& a, hipStream_t stream);
-// Up to 64 rows of x, which start on 16 bytes, blocks of a wave's own in LDS.
-bool x_in_reach(const Linear4Args& a);   // by 32-bit offsets, for this and the next
+// Up to 64 rows of x, blocks of them a wave's own in LDS.
 int block4_waves(const Shape4& s);
 hipError_t launch4_block(const Linear4Args& a, hipStream_t stream);
-// Up to 64 rows of x, which start on 16 bytes, a range of `per` blocks of K in LDS.
+// Up to 64 rows of x, a range of `per` blocks of K in LDS.
 constexpr int kSlabWaves = 8;
 constexpr size_t kSlabLds = 160 * 1024;
 inline size_t slab4_lds(int M, int per) { return (size_t)((M + 3) / 4) * 1024 * per; }
 hipError_t launch4_slab(const Linear4Args& a, int split, float* part, hipStream_t stream);
-// More rows, which start on 16 bytes: tiles of 128 rows and 64 NP rows of w.
-bool wide4_fits(const Linear4Args& a);
+// More rows: tiles of 128 rows and 64 NP rows of w.
 hipError_t launch4_wide(const Plan4& p, const Linear4Args& a, float* part, hipStream_t stream);
-// Any.
-hipError_t launch4_tile(const Linear4Args& a, int split, float* part, hipStream_t stream);
+// Any rows, without a workspace.
+hipError_t launch4_tile(const Linear4Args& a, hipStream_t stream);
 
 inline Shape4 shape_of(const Linear4Args& a) {
   return Shape4{a.e.M, a.e.N, a.e.K, a.e.act == lin::kSwiglu, a.fmt, a.group};

@@ -1,10 +1,13 @@
 // The product with 4-bit weights for up to 64 rows of x (linear4.hpp has the formula
-// and the layout): every wave for itself, as in linear4_rows.hip, with x by way of LDS.
-// A workgroup has one unit, two panels (swiglu: a gate and its up panel) times all
-// rows of x; its waves deal the blocks of 128 k among them.  A wave brings its blocks
-// of x straight to its own part of LDS, NB of them at a time, and waits for those
-// alone: no barrier before the sums are added.  Loads that go to LDS come in at some
-// 40 KB a us and CU, loads to registers at 25.
+// and the layout), every wave for itself.  A workgroup has one unit, two panels
+// (swiglu: a gate and its up panel) times all rows of x; its waves deal the blocks of
+// 128 k among them.  A wave brings its blocks of x straight to its own part of LDS, NB
+// of them at a time, and waits for those alone: no barrier before the sums are added,
+// in a fixed order.  What bounds it is x: all of it comes to every CU.  Loads that go
+// to LDS come in at 40 to 65 KB a us and CU, loads to registers at 25 (the same kernel
+// with x in registers, 47 x 7168 x 2048 NVFP4 14.2 us, 8.4 so; 64 x 7168 x 2048 MXFP4 17.1
+// and 9.4; two panels also share x's operands).  16 x 7168 x 7168 NVFP4 13.3 us, 9.9 with
+// the weights in the caches.
 #include "linear4.hpp"
 
 namespace xtu {
@@ -147,10 +150,6 @@ hipError_t launch(const Linear4Args& a, hipStream_t stream) {
 }
 
 }  // namespace
-
-bool x_in_reach(const Linear4Args& a) {
-  return a.xvec && (64 * a.e.ldx + a.e.K) * 2 < (1L << 31);
-}
 
 int block4_waves(const Shape4& s) {
   return s.M <= 16 && !(s.fmt == kI4 && s.group == 32) ? 16 : 8;

@@ -3,9 +3,11 @@
 // LDS; each wave streams that range of its own two panels (swiglu: a gate and its up
 // panel) to its registers, U blocks ahead, and meets no barrier on the way.
 //
-// What bounds it is what a CU can take in, about 25 GB/s: its share of w, which is
-// fixed, and the workgroup's part of x.  Splitting K makes the latter smaller and costs
-// partial sums, which linear_join_kernel adds (linear4.hip weighs them).
+// What bounds it is what a CU takes in: its share of w, which is fixed, and the
+// workgroup's part of x.  Splitting K makes the latter smaller and costs partial sums,
+// which linear_join_kernel adds (linear4.hip weighs them): 16 x 16384 gated x 7168 MXFP4
+// 32 us in 2 ranges (blocks 47), 24 x 16384 x 4096 16.5 in 2 (18.4), 16 x 2048 x 16384
+// 13.1 in 16 (19.5).  More records ahead change nothing (U = 5, 7).
 #include "linear4.hpp"
 
 namespace xtu {

@@ -1,8 +1,11 @@
-// The product with 4-bit weights on tiles, for many rows of x at any alignment and row
-// stride (linear4.hpp has the formula and the layout).  Four waves, each with NP panels of w times all of the tile's 16 MT rows
-// of x, K in blocks of 128.  A wave's records go from memory to its registers, two
-// blocks ahead, and are made operands there, so a weight is read and expanded once a
-// tile; x goes through LDS, which all waves read, one block ahead.
+// The product with 4-bit weights on tiles of 64 rows of x, at any alignment and row
+// stride (linear4.hpp has the formula and the layout): for rows that do not start on 16
+// bytes where there is no workspace to copy them to, or that are too far apart for
+// 32-bit offsets.  Four waves, each with two panels of w times all of the tile's rows, K
+// in blocks of 128.  A wave's records go from memory to its registers, two blocks ahead,
+// and are made operands there; x goes through registers to LDS, which all waves read, one
+// block ahead.  2048 x 4096 x 7168 MXFP4 at odd 2-byte addresses 265 us (copied first and
+// in linear4_wide.hip 107).
 #include "linear4.hpp"
 
 namespace xtu {
@@ -12,7 +15,7 @@ namespace {
 constexpr int kAhead = 2;   // blocks of w in registers
 
 template <int FMT, int G, bool GATED, int MT, int NP>
-__global__ __launch_bounds__(256) void linear4_tile_kernel(Linear4Args a, int per, float* part) {
+__global__ __launch_bounds__(256) void linear4_tile_kernel(Linear4Args a) {
   constexpr int AK = GATED ? lin::kActSwiglu : lin::kActOther;
   constexpr int BM = 16 * MT, REC = record_bytes(FMT, G);
   constexpr int W = GATED ? 8 * NP : 16 * NP;   // output columns of a wave
@@ -35,7 +38,7 @@ __global__ __launch_bounds__(256) void linear4_tile_kernel(Linear4Args a, int pe
   const int m0 = t % gm * BM, tn = t / gm;
   const int nw = (tn * 4 + w) * W;   // first output column of the wave
   const int nb = blocks_of(e.K);
-  const int s0 = (int)blockIdx.y * per, s1 = min(nb, s0 + per);
+  const int s0 = 0, s1 = nb;
 
   // panels past the last one read it again
   const int np = panels_of(e.N) * (GATED ? 2 : 1);
@@ -103,7 +106,6 @@ __global__ __launch_bounds__(256) void linear4_tile_kernel(Linear4Args a, int pe
   __syncthreads();
   const float g0 = a.gs ? a.gs[0] : 1.f, g1 = a.gs && GATED ? a.gs[1] : g0;
   float* eb = reinterpret_cast<float*>(lds) + w * (16 * LD);
-  float* plane = part ? part + (long)blockIdx.y * lin::part_plane(e) : nullptr;
   constexpr int CG = W / 4, RS = 64 / CG > 16 ? 16 : 64 / CG;
 #pragma unroll 1
   for (int j = 0; j < MT; ++j) {
@@ -129,13 +131,7 @@ __global__ __launch_bounds__(256) void linear4_tile_kernel(Linear4Args a, int pe
         const f32x4_t z = *reinterpret_cast<const f32x4_t*>(eb + r * LD + place(cv));
         f32x4_t u = z;
         if constexpr (GATED) u = *reinterpret_cast<const f32x4_t*>(eb + r * LD + place(cv) + 16);
-        if (plane) {
-          float* pr = plane + (long)m * e.N * (GATED ? 2 : 1) + n;
-          *reinterpret_cast<f32x4_t*>(pr) = z;
-          if constexpr (GATED) *reinterpret_cast<f32x4_t*>(pr + e.N) = u;
-        } else {
-          lin::finish4<AK>(e, m, n, z, u);
-        }
+        lin::finish4<AK>(e, m, n, z, u);
       }
     } else {
 #pragma unroll 1
@@ -143,40 +139,24 @@ __global__ __launch_bounds__(256) void linear4_tile_kernel(Linear4Args a, int pe
         const int r = i / W, col = i % W, m = mb + r, n = nw + col;
         if (n >= e.N || m >= e.M) continue;
         const float z = eb[r * LD + place(col)], u = GATED ? eb[r * LD + place(col) + 16] : 0.f;
-        if (plane) {
-          float* pr = plane + (long)m * e.N * (GATED ? 2 : 1) + n;
-          pr[0] = z;
-          if constexpr (GATED) pr[e.N] = u;
-        } else {
-          lin::finish_one<AK>(e, m, n, z, u);
-        }
+        lin::finish_one<AK>(e, m, n, z, u);
       }
     }
   }
 }
 
-template <int MT, int NP>
-hipError_t launch(const Linear4Args& a, int split, float* part, hipStream_t stream) {
-  const bool gated = a.e.act == lin::kSwiglu;
-  const int cols = 4 * (gated ? 8 : 16) * NP, nb = blocks_of(a.e.K);
-  const int per = (nb + split - 1) / split;
-  split = (nb + per - 1) / per;   // no empty range
-  const long tiles = ((long)a.e.M + 16 * MT - 1) / (16 * MT) * (((long)a.e.N + cols - 1) / cols);
-  if (!lin::grid_fits(tiles, 256)) return hipErrorInvalidConfiguration;
-  const hipError_t r = by_format(a, [&](auto fmt, auto group, auto g) {
-    linear4_tile_kernel<decltype(fmt)::value, decltype(group)::value, decltype(g)::value, MT, NP>
-        <<<dim3((unsigned)tiles, (unsigned)split), 256, 0, stream>>>(a, per,
-                                                                     split > 1 ? part : nullptr);
-    return hipPeekAtLastError();
-  });
-  if (r == hipSuccess && split > 1) return lin::launch_join(a.e, split, part, stream);
-  return r;
-}
-
 }  // namespace
 
-hipError_t launch4_tile(const Linear4Args& a, int split, float* part, hipStream_t stream) {
-  return launch<4, 2>(a, split, part, stream);
+hipError_t launch4_tile(const Linear4Args& a, hipStream_t stream) {
+  constexpr int MT = 4, NP = 2;
+  const int cols = 4 * (a.e.act == lin::kSwiglu ? 8 : 16) * NP;
+  const long tiles = ((long)a.e.M + 16 * MT - 1) / (16 * MT) * (((long)a.e.N + cols - 1) / cols);
+  if (!lin::grid_fits(tiles, 256)) return hipErrorInvalidConfiguration;
+  return by_format(a, [&](auto fmt, auto group, auto g) {
+    linear4_tile_kernel<decltype(fmt)::value, decltype(group)::value, decltype(g)::value, MT, NP>
+        <<<(unsigned)tiles, 256, 0, stream>>>(a);
+    return hipPeekAtLastError();
+  });
 }
 
 }  // namespace l4

@@ -114,8 +114,8 @@ SIGNATURES = {
     "xtu_linear_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "xtu_linear4": (_i, [_vp, _vp]),
     "xtu_linear4_weight_bytes": (_sz, [_i, _i, _i, _i, _i]),
-    "xtu_linear4_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
-    "xtu_linear4_plan": (_i, [_i, _i, _i, _i, _i, _i, _i]),
+    "xtu_linear4_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "xtu_linear4_plan": (_i, [_i, _i, _i, _i, _i, _i]),
     "xtu_router_workspace_bytes": (_sz, [_i, _i, _i]),
     "xtu_router_losses": (_i, [_vp, _vp]),
     "xtu_router_grad": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),

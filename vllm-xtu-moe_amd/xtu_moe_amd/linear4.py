@@ -7,7 +7,7 @@ experts' formats: a shared expert beside the routed ones, a dense layer, a
 projection.  The weights are packed once (``Weight4.from_dense``); the arguments
 and the epilogue are ``linear``'s.  The reference leaves these products to its
 host (vllm_xiaotu_moe/hybrid_model.py:1752 ``_shared_out``), and INT4 to its CPU
-engine (xiaotu_moe/csrc/moe/moe_v2.hpp:454-470).
+engine (xiaotu_moe/csrc/moe/moe_v2_packed4_base.inc:4-16).
 """
 from __future__ import annotations
 
@@ -222,16 +222,19 @@ def linear4(x, w: Weight4, *, bias=None, activation="none", row_scale=None, resi
         out = x.new_empty((M, N), dtype=odt)
     if M == 0:
         return out
-    key = (M, N, K, act == 6, w.fmt, w.group)
+    xp = x.data_ptr()
+    aligned = not (xp & 15 or (M > 1 and ldx & 7))
+    key = (M, N, K, act == 6, w.fmt, w.group, aligned)
     nws = _WS_BYTES.get(key)
     if nws is None:
-        nws = int(_lib.call("xtu_linear4_workspace_bytes", M, N, K, act, w.fmt, w.group))
+        nws = int(_lib.call("xtu_linear4_workspace_bytes", M, N, K, act, w.fmt, w.group,
+                            int(aligned)))
         if len(_WS_BYTES) >= 4096:   # a server's prompt lengths
             _WS_BYTES.clear()
         _WS_BYTES[key] = nws
     # allocated per call: calls on other streams, and graphs, have their own
     ws = x.new_empty(nws, dtype=torch.uint8) if nws else None
-    rc = _entry()(ARGS.pack(x.data_ptr(), w.data.data_ptr(), 0 if w.gs is None else w.gs.data_ptr(),
+    rc = _entry()(ARGS.pack(xp, w.data.data_ptr(), 0 if w.gs is None else w.gs.data_ptr(),
                             bp, sp, rp, out.data_ptr(), ws.data_ptr() if nws else 0, ldx, ldr, ldo,
                             sst, nws, M, N, K, act, w.fmt, w.group, b16, r16,
                             odt == torch.bfloat16, swiglu_limit or 0.0, swiglu_alpha, swiglu_beta),
