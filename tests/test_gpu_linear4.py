@@ -112,7 +112,7 @@ def test_sizes(fmt, group, gated):
 def test_every_form(fmt, group, gated):
     """Each kernel, whole and with K split, with the whole epilogue; and x at odd
     addresses, copied first."""
-    for i, ((kernel, _), M, N, K) in enumerate(forms(fmt, group, gated)):
+    for i, (form, M, N, K) in enumerate(forms(fmt, group, gated)):
         big = _rand((M, K + 8), i)
         W, w = _weight(fmt, group, N, K, gated, seed=70 + i)
         b = _rand((w.shape[0],), 2, 0.5, F32)
@@ -120,9 +120,9 @@ def test_every_form(fmt, group, gated):
         for act in ("swiglu",) if gated else ("none", "gelu"):
             x = big[:, :K]
             out = linear4(x, W, bias=b, activation=act, residual=r, out_dtype=F32)
-            _check(out, x, w, act, b, residual=r, what=(kernel, M, N, K, act))
+            _check(out, x, w, act, b, residual=r, what=(form, M, N, K, act))
             x = big[:, 1:K + 1]
-            _check(linear4(x, W, activation=act), x, w, act, what=(kernel, M, N, K, "odd"))
+            _check(linear4(x, W, activation=act), x, w, act, what=(form, M, N, K, "odd"))
 
 
 @pytest.mark.parametrize("fmt,group", GROUPS)

@@ -29,20 +29,24 @@ def _dense(fmt, rows, K, group, seed=0):
 FORMS = {
     (0, False): [(1, 300, 512), (5, 296, 128), (2, 12000, 640), (1, 150, 9600)],
     (1, False): [(1, 16, 1792), (3, 4000, 2176), (7, 182, 1536), (16, 534, 1280), (24, 2037, 768),
-                 (42, 407, 640), (50, 102, 384), (64, 1500, 2176)],
+                 (42, 407, 640), (50, 102, 384), (64, 1500, 2176), (36, 112, 3712),
+                 (65, 16, 128), (137, 1140, 384), (71, 16, 896), (123, 504, 2816),   # parts of
+                 (300, 1700, 640), (97, 3000, 512), (70, 8000, 256), (5000, 34, 256),   # x
+                 (80, 6500, 512), (128, 2000, 640)],
     (2, False): [(20, 16864, 128), (30, 18111, 512), (44, 21292, 128), (51, 18559, 128)],
-    (2, True): [(10, 16, 7808), (26, 396, 8448), (36, 112, 3712), (64, 148, 9216)],
-    (3, False): [(65, 16, 128), (137, 1140, 384)],
-    (3, True): [(71, 16, 896), (123, 504, 2816)],
+    (2, True): [(10, 16, 7808), (13, 40, 9600), (33, 17986, 2944)],
+    (3, False): [(68, 8420, 128), (579, 4514, 256)],
+    (3, True): [(97, 8196, 2304), (1685, 68, 4736)],
     (4, False): [(1224, 3405, 256), (1838, 2228, 512)],
-    (4, True): [(65, 5888, 5248)],
+    (4, True): [(65, 4186, 7296)],
+    None: [(26, 396, 8448), (64, 148, 9216), (65, 5888, 5248)],   # not the same for all
 }
 
 
 def forms(fmt, group, gated):
     """(form, M, N, K) of this format: INT4's finer groups have no kernel 4."""
     for form, sizes in FORMS.items():
-        if form[0] != 4 or fmt != F.FMT_INT4 or group == 128:
+        if form is None or form[0] != 4 or fmt != F.FMT_INT4 or group == 128:
             for M, N, K in sizes:
                 yield form, M, N // 2 if gated else N, K
 
@@ -51,9 +55,9 @@ def forms(fmt, group, gated):
 @pytest.mark.parametrize("fmt,group", GROUPS)
 @pytest.mark.parametrize("gated", [False, True])
 def test_forms_are_taken(fmt, group, gated):
-    for (kernel, split), M, N, K in forms(fmt, group, gated):
+    for form, M, N, K in forms(fmt, group, gated):
         plan = _lib.load().xtu_linear4_plan(M, N, K, 6 if gated else 0, fmt, group)
-        assert (plan % 16, plan >= 32) == (kernel, split), (M, N, K, plan % 16, plan // 16)
+        assert form in ((plan % 16, plan >= 32), None), (M, N, K, plan % 16, plan // 16)
 
 
 def _w(fmt="mxfp4", rows=4, K=32, gated=False):

@@ -30,7 +30,7 @@ long up(long n, long d) { return (n + d - 1) / d; }
 // Estimated times in us.  All CUs together take in w at 6.2 GB a ms, one of them rows
 // of x that are staged whole at 50 KB a us, and what it loads straight to LDS at 65 to
 // 80; a launch and its latencies are 3 to 6, the launch that adds K splits 3 and its
-// partial sums' way.
+// partial sums' way.  A workgroup of blocks after the first on its CU adds 3.5.
 
 float join_time(const Shape4& s, int split, float rate) {
   if (split == 1) return 0.f;
@@ -50,13 +50,16 @@ float skinny_time(const Shape4& s) {
          larger(p.units * w / 6200.f, rounds * up(p.units, p.grid) * w / 50.f);
 }
 
-float block_time(const Shape4& s) {
+float block_time(const Shape4& s, int rows) {
   const int nb = blocks_of(s.K);
-  const long units = up(s.N, s.gated ? 16 : 32), rounds = up(units, kCus);
-  const int rows = s.M <= 4 ? 4 : s.M <= 8 ? 8 : (int)up(s.M, 16) * 16;
+  const long parts = up(s.M, rows), units = up(s.N, s.gated ? 16 : 32);
+  const long rounds = up(units * parts, kCus);
   const float x = rows * 0.256f * nb, w = 2.f * nb * record_bytes(s.fmt, s.group) * 1e-3f;
-  return 3.2f + rounds * x / 80.f + larger(units * w / 6200.f, rounds * w / 75.f) +
-         0.35f * up(nb, block4_waves(s)) + 2.f * (rounds - 1);
+  // (past 64 rows: all of x comes to every XCD that has a unit)
+  const float far = s.M > 64 ? (units < 8 ? units : 8) * s.M * 0.256f * nb : 0.f;
+  return 3.2f + larger(rounds * x / 80.f, far / 4500.f) +
+         larger(units * w / 6200.f, rounds * w / 75.f) +
+         0.35f * up(nb, block4_waves(s, rows)) + 3.5f * (rounds - 1);
 }
 
 // The split of K with the least time, 0 where no range of K fits LDS.
@@ -89,7 +92,7 @@ int slab_split(const Shape4& s, bool may_split, float& time) {
 // 32; M 24: 16384 x 4096 - / 18.4 / 16.5; M 64: 7168 x 2048 - / 9.4 / 14.5, 7168 x 7168 -
 // / 20.6 / 20.4.  (The estimates' choice is the fastest of three or within 4% of it there.)
 Plan4 plan_few(const Shape4& s, bool may_split) {
-  const float skinny = skinny_time(s), block = block_time(s);
+  const float skinny = skinny_time(s), block = block4_plan(s).time;
   float slab = 1e30f;
   int split = 0;
   if (skinny > kSlabBase && block > kSlabBase) split = slab_split(s, may_split, slab);
@@ -102,13 +105,17 @@ Plan4 plan_few(const Shape4& s, bool may_split) {
 // (2048 x 2048 gated x 7168, one round of the larger and two of the smaller: MXFP4 91 /
 // 122, NVFP4 115 / 140, INT4 with groups of 128 121 / 148; 128 x 7168 x 2048 in 28 and
 // 56 tiles: 29 / 20).  INT4's finer groups have no room for the larger one's sums.
+// Blocks against the better of the two, MXFP4: 128 x 2048 x 7168 11.9 / 20.0, 192 x 4096 x
+// 4096 18.2 / 21.5, 256 x 512 x 7168 10.4 / 16.4, 512 x 1024 x 2048 9.8 / 16.8, 192 x 7168 x
+// 2048 22.4 / 20.2, 512 x 2048 x 7168 30.8 / 26.6; x large: 2048 x 128 x 2048 9.6 / 14.7,
+// 4096 x 128 x 2048 19.5 / 16.9.
 Plan4 plan_many(const Shape4& s, bool may_split) {
   const bool fine = s.fmt == kI4 && s.group != 128;
   const float step4 = s.fmt == kMx ? 1.5f : s.fmt == kNv ? 1.95f : 2.1f;
   const float step2 = s.fmt == kMx ? 1.03f : s.fmt == kNv ? 1.2f : fine ? 1.7f : 1.3f;
   const int nb = blocks_of(s.K);
-  Plan4 best{kWide2, 1};
-  float time = 1e30f;
+  Plan4 best{kBlock4, 1};
+  float time = block4_plan(s).time;
   for (int kind : {kWide4, kWide2}) {
     if (kind == kWide4 && fine) continue;
     const long tiles = up(s.M, 128) * up(s.N, (s.gated ? 32 : 64) * (kind == kWide4 ? 4 : 2));
@@ -148,6 +155,22 @@ Shape4 shape_of(int M, int N, int K, int act, int fmt, int group) {
 }
 
 }  // namespace
+
+// The rows of a part of x with the least time.
+BlockPlan block4_plan(const Shape4& s) {
+  if (s.M > kBlockM) return {0, 1e30f};
+  if (s.M <= 8) {
+    const int rows = s.M <= 4 ? 4 : 8;
+    return {rows, block_time(s, rows)};
+  }
+  BlockPlan best{0, 1e30f};
+  for (int rows = 64; rows >= 16; rows -= 16) {
+    const float time = block_time(s, rows);
+    if (rows < s.M + 16 && time < best.time) best = {rows, time};
+  }
+  return best;
+}
+
 }  // namespace l4
 }  // namespace xtu
 

@@ -201,8 +201,15 @@ struct SkinnyPlan {
 };
 SkinnyPlan skinny4_plan(const Shape4& s);
 hipError_t launch4_skinny(const Linear4Args& a, hipStream_t stream);
-// Up to 64 rows of x, blocks of them a wave's own in LDS.
-int block4_waves(const Shape4& s);
+// Up to kBlockM rows of x, 4, 8, 16, 32, 48 or 64 to a workgroup, blocks of them a wave's
+// own in LDS; `time` in us.
+constexpr int kBlockM = 65536;
+struct BlockPlan {
+  int rows;
+  float time;
+};
+BlockPlan block4_plan(const Shape4& s);
+int block4_waves(const Shape4& s, int rows);
 hipError_t launch4_block(const Linear4Args& a, hipStream_t stream);
 // Up to 64 rows of x, a range of `per` blocks of K in LDS.
 constexpr int kSlabWaves = 8;

@@ -1,13 +1,17 @@
-// The product with 4-bit weights for up to 64 rows of x (linear4.hpp has the formula
-// and the layout), every wave for itself.  A workgroup has one unit, two panels
-// (swiglu: a gate and its up panel) times all rows of x; its waves deal the blocks of
+// The product with 4-bit weights for few rows of x or few units (linear4.hpp has the
+// formula and the layout), every wave for itself.  A workgroup has one unit, two panels
+// (swiglu: a gate and its up panel), times 4 LX rows of x; its waves deal the blocks of
 // 128 k among them.  A wave brings its blocks of x straight to its own part of LDS, NB
 // of them at a time, and waits for those alone: no barrier before the sums are added,
-// in a fixed order.  What bounds it is x: all of it comes to every CU.  Loads that go
-// to LDS come in at 40 to 65 KB a us and CU, loads to registers at 25 (the same kernel
-// with x in registers, 47 x 7168 x 2048 NVFP4 14.2 us, 8.4 so; 64 x 7168 x 2048 MXFP4 17.1
-// and 9.4; two panels also share x's operands).  16 x 7168 x 7168 NVFP4 13.3 us, 9.9 with
-// the weights in the caches.
+// in a fixed order.  What bounds it is x: a unit's rows of it come to every CU.  Loads
+// that go to LDS come in at 40 to 65 KB a us and CU, loads to registers at 25 (the same
+// kernel with x in registers, 47 x 7168 x 2048 NVFP4 14.2 us, 8.4 so; 64 x 7168 x 2048
+// MXFP4 17.1 and 9.4; two panels also share x's operands).  16 x 7168 x 7168 NVFP4 13.3
+// us, 9.9 with the weights in the caches.  Where units are fewer than CUs, x is split
+// instead (block4_plan): w is read again, from the caches, and each CU takes in less.  In
+// parts of 16 / 32 / 48 / 64 rows, MXFP4: 64 x 2048 x 7168 9.5 / 11.0 / 12.4 / 15.3 us,
+// 128 x 2048 x 7168 16.6 / 11.9 / 13.0 / 15.7, 80 x 7168 x 2048 22.7 / 16.5 / 13.5 / 15.5,
+// 128 x 4096 x 4096 24.2 / 15.9 / 16.5 / 12.7.
 #include "linear4.hpp"
 
 namespace xtu {
@@ -26,18 +30,20 @@ __global__ __launch_bounds__(64 * WV) void linear4_block_kernel(Linear4Args a) {
   const int w = __builtin_amdgcn_readfirstlane(tid / 64);
   const int q = lane / 16, c = lane % 16;
   const int nb = blocks_of(e.K), unit = blockIdx.x;
+  const int m0 = 4 * LX * (int)blockIdx.y, rows = min(4 * LX, e.M - m0);
   const int last = panels_of(e.N) * (GATED ? 2 : 1) - 1;   // panel
   const int mine = (nb - w + WV - 1) / WV;                 // blocks w, w + WV, ..
   // x: load r of a block brings rows 4 r and on, a piece of 16 bytes a lane
   // (linear_tile.hip has the slots)
-  const u32x4_t xr = lin::raw_buffer(e.x, (uint32_t)(((long)(e.M - 1) * e.ldx + e.K) * 2));
+  const u32x4_t xr = lin::raw_buffer(e.x + (long)m0 * e.ldx,
+                                     (uint32_t)(((long)(rows - 1) * e.ldx + e.K) * 2));
   uint8_t* xs = lds + w * (NB * SIZE);
   auto load_x = [&](int i) {
     const int s = w + WV * min(i, mine - 1);
 #pragma unroll
     for (int r = 0; r < LX; ++r) {
       const int row = 4 * r + lane / 16, k = 8 * (lane % 16 ^ (row & 7) << 1);
-      const uint32_t off = (uint32_t)min(row, e.M - 1) * (uint32_t)(e.ldx * 2) + 2 * k;
+      const uint32_t off = (uint32_t)min(row, rows - 1) * (uint32_t)(e.ldx * 2) + 2 * k;
       lin::buf_to_lds(xr, k < e.K - 128 * s ? off : 0x80000000u, (uint32_t)s * 256u,
                       xs + i % NB * SIZE + r * 1024);
     }
@@ -55,12 +61,12 @@ __global__ __launch_bounds__(64 * WV) void linear4_block_kernel(Linear4Args a) {
   // (swiglu: rows 16 w)
   const int fp = GATED ? 0 : w % 2, fm = 16 * (GATED ? w : w / 2) + c;
   const int fn = unit * COLS + 16 * fp + 4 * q;
-  const bool fin = (GATED ? w : w / 2) < MT && fm < e.M && fn < e.N;
+  const bool fin = (GATED ? w : w / 2) < MT && fm < rows && fn < e.N;
   u32x4_t bz = {0u, 0u, 0u, 0u}, bu = bz;
   lin::Row4 pre = {{0u, 0u, 0u, 0u}, 1.f};
   if (fin && e.vec) {
     lin::load_bias4<AK>(e, fn, bz, bu);
-    pre = lin::load_row4(e, fm, fn);
+    pre = lin::load_row4(e, m0 + fm, fn);
   }
   const float g0 = a.gs ? a.gs[0] : 1.f, g1 = a.gs && GATED ? a.gs[1] : g0;
 
@@ -117,11 +123,11 @@ __global__ __launch_bounds__(64 * WV) void linear4_block_kernel(Linear4Args a) {
     z[0] += lin::of_raw4(bz, e.bias_bf16);
     if constexpr (GATED) u[0] += lin::of_raw4(bu, e.bias_bf16);
     lin::act_all<AK>(e, z, u);
-    lin::store_row4(e, fm, fn, z[0], pre);
+    lin::store_row4(e, m0 + fm, fn, z[0], pre);
   } else {
 #pragma unroll 1
     for (int t = 0; t < 4; ++t) {
-      if (fn + t < e.N) lin::finish_one<AK>(e, fm, fn + t, z[0][0], u[0][0]);
+      if (fn + t < e.N) lin::finish_one<AK>(e, m0 + fm, fn + t, z[0][0], u[0][0]);
       z[0] = __builtin_shufflevector(z[0], z[0], 1, 2, 3, 0);
       u[0] = __builtin_shufflevector(u[0], u[0], 1, 2, 3, 0);
     }
@@ -132,7 +138,7 @@ template <int LX>
 hipError_t launch(const Linear4Args& a, hipStream_t stream) {
   const LinearArgs& e = a.e;
   const int cols = e.act == lin::kSwiglu ? 16 : 32;
-  const long units = ((long)e.N + cols - 1) / cols;
+  const long units = ((long)e.N + cols - 1) / cols, parts = (e.M + 4 * LX - 1) / (4 * LX);
   return by_format(a, [&](auto fmt, auto group, auto g) {
     constexpr int F = decltype(fmt)::value, G = decltype(group)::value;
     // what LDS and the registers hold
@@ -141,28 +147,28 @@ hipError_t launch(const Linear4Args& a, hipStream_t stream) {
     constexpr size_t kX = (size_t)WV * NB * LX * 1024, kSums = (size_t)WV * MT * 2048;
     constexpr size_t kAll = kX > kSums ? kX : kSums;   // the sums take x's place
     static_assert(kAll <= 160 * 1024, "LDS of a CU");
-    if (!lin::grid_fits(units, 64 * WV)) return hipErrorInvalidConfiguration;
+    if (!lin::grid_fits(units * parts, 64 * WV)) return hipErrorInvalidConfiguration;
     auto k = linear4_block_kernel<F, G, decltype(g)::value ? lin::kActSwiglu : lin::kActOther, LX,
                                   WV, NB>;
-    k<<<(unsigned)units, 64 * WV, kAll, stream>>>(a);
+    k<<<dim3((unsigned)units, (unsigned)parts), 64 * WV, kAll, stream>>>(a);
     return hipPeekAtLastError();
   });
 }
 
 }  // namespace
 
-int block4_waves(const Shape4& s) {
-  return s.M <= 16 && !(s.fmt == kI4 && s.group == 32) ? 16 : 8;
+int block4_waves(const Shape4& s, int rows) {
+  return rows <= 16 && !(s.fmt == kI4 && s.group == 32) ? 16 : 8;
 }
 
 hipError_t launch4_block(const Linear4Args& a, hipStream_t stream) {
-  const int M = a.e.M;
-  if (M > 64) return hipErrorInvalidValue;
-  if (M <= 4) return launch<1>(a, stream);
-  if (M <= 8) return launch<2>(a, stream);
-  if (M <= 16) return launch<4>(a, stream);
-  if (M <= 32) return launch<8>(a, stream);
-  if (M <= 48) return launch<12>(a, stream);
+  if (a.e.M > kBlockM) return hipErrorInvalidValue;
+  const int rows = block4_plan(shape_of(a)).rows;
+  if (rows == 4) return launch<1>(a, stream);
+  if (rows == 8) return launch<2>(a, stream);
+  if (rows == 16) return launch<4>(a, stream);
+  if (rows == 32) return launch<8>(a, stream);
+  if (rows == 48) return launch<12>(a, stream);
   return launch<16>(a, stream);
 }
 
