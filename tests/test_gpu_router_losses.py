@@ -379,3 +379,118 @@ def test_graph():
         torch.cuda.synchronize()
         for x, y in zip(out, want):
             assert torch.equal(x, y)
+
+
+def _in_logs(lg, ids, starts, scoring, renorm, f, gw, gb, gz):
+    """The definition in 64 bits, ratios by way of logarithms so that far logits keep
+    them, and the gradient by autograd; ids are all experts.  Beside it the magnitudes
+    of the gradient's terms."""
+    l = lg.detach().double().requires_grad_(True)
+    ids = ids.long()
+    (T, E), K, soft = l.shape, ids.shape[1], scoring == "softmax"
+    x = l if soft else torch.nn.functional.logsigmoid(l)
+    p, s = torch.softmax(x, 1), x.gather(1, ids)
+    u = torch.softmax(s, 1) if renorm else p.gather(1, ids) if soft else torch.exp(s)
+    m = l.detach().amax(1, keepdim=True)   # (torch.logsumexp's own gradient is exp(l - lse),
+    w, lse = f * u, (m + torch.log(torch.exp(l - m).sum(1, keepdim=True)))[:, 0]   # far off: 1)
+    S = len(starts) - 1
+    counts = torch.zeros((S, E), dtype=torch.int32, device=l.device)
+    P = torch.zeros((S, E), dtype=F64, device=l.device)
+    h, zt = torch.zeros((T, E), dtype=F64, device=l.device), torch.zeros((T, 1), dtype=F64,
+                                                                        device=l.device)
+    spans = [(q, a, b) for q, (a, b) in enumerate(zip(starts[:-1], starts[1:])) if b > a]
+    n = sum(b - a for _, a, b in spans)
+    losses, squares = [], []
+    for q, a, b in spans:
+        counts[q] = torch.bincount(ids[a:b].reshape(-1), minlength=E).int()
+        mean = p[a:b].mean(0)
+        P[q] = mean.detach()
+        losses.append((counts[q].double() * mean).sum() * E / (K * (b - a)))
+        squares.append((lse[a:b] ** 2).sum())
+        h[a:b] = abs(gb) * E * counts[q].double() / (K * (b - a) ** 2 * len(spans))
+        zt[a:b] = 2 * abs(gz) * lse[a:b, None].detach().abs() / n
+    balance, z = torch.stack(losses).mean(), torch.stack(squares).sum() / n
+    total = (w * gw.double()).sum() + gb * balance + (gz * z if soft else 0.0)
+    d, = torch.autograd.grad(total, l)
+    p, w = p.detach(), w.detach()
+    wg = (w * gw.double().abs()).sum(1, keepdim=True)
+    da = p * (h + (p * h).sum(1, keepdim=True) + (zt + (0 if renorm else wg) if soft else 0))
+    da = da.scatter_add(1, ids, w * (gw.double().abs() + (wg / f if renorm else 0)))
+    return dict(weights=w, balance=balance.detach(), z=z.detach(), counts=counts, probs=P, d=d,
+                da=da, total=total.detach())
+
+
+MODES = [("softmax", True, 1.0), ("softmax", False, 1.0), ("sigmoid", True, 2.5),
+         ("sigmoid", False, 0.5)]
+
+
+@pytest.mark.parametrize("scoring,renorm,f", MODES)
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_far_logits(scoring, renorm, f, dtype):
+    """Rows wholly or in part at far finite values, the type's lowest and highest among
+    them, in sequences and behind the last one.  Near a far maximum an exponential's
+    argument is the exact difference times log2 e, off by 1.22 |l - m| u, where e^(l - m)
+    is above 2^-126 (|l - m| < 88: R as for a spread of 88); below it vanishes."""
+    top = torch.finfo(dtype).max
+    far = [-1e9, -1e10, -1e30, -top, 1e9, 1e10, 1e30, top, -300.0, 300.0, -5000.25, 5000.25]
+    R = (88 + 40) * U
+    for E, K in ((8, 2), (60, 4), (256, 8), (700, 12)):
+        g = torch.Generator().manual_seed(E)
+        rows = []
+        for v in far:
+            r = torch.randn((4, E), generator=g) * 1.5
+            r[0] = v                                          # all of a row
+            r[1, ::2] = v                                     # half of it
+            r[2] = (r[2].double() + v).clamp(-top, top)       # beside v, as far as the type goes
+            r[3, E // 2] = v                                  # one
+            rows.append(r)
+        rows = torch.cat(rows).to(dtype)
+        lg = torch.cat([rows, torch.randn((12, E), generator=g).to(dtype), rows]).to(DEV)
+        T, used = lg.shape[0], rows.shape[0] + 12
+        ids = torch.sort(lg.float(), dim=1, descending=True, stable=True).indices[:, :K]
+        ids = ids.to(torch.int32).contiguous()
+        gw = torch.randn((T, K), generator=g).to(DEV)
+        starts, gb, gz = [0, 0, 23, used], 0.7, 0.3
+        lg.requires_grad_(True)
+        r = router_losses(lg, ids, scoring=scoring, renormalize=renorm, routed_scaling_factor=f,
+                          seq_starts=torch.tensor(starts, dtype=torch.int32, device=DEV))
+        outs = [r.weights, r.balance] + ([r.z] if r.z is not None else [])
+        d, = torch.autograd.grad(outs, lg, [gw] + [torch.full((), v, device=DEV) for v in (gb, gz)]
+                                 [:len(outs) - 1])
+        e = _in_logs(lg, ids, starts, scoring, renorm, f, gw, gb, gz)
+
+        def near(name, got, want, tol):
+            bad = ~((got.detach().double() - want).abs() <= tol)
+            assert not bool(bad.any()), (E, name, bad.nonzero()[:4].tolist(),
+                                         got[bad][:4].tolist(), want[bad][:4].tolist())
+
+        assert torch.equal(r.counts, e["counts"])
+        near("weights", r.weights, e["weights"], e["weights"] * (2 * R + 4 * U) + f * 2.0 ** -120)
+        near("probs", r.probs, e["probs"], e["probs"] * (R + 2.0 ** -17) + 2.0 ** -120)
+        near("balance", r.balance, e["balance"], e["balance"] * (R + 2.0 ** -17))
+        if r.z is not None:   # 1e30 squared and more leaves fp32
+            assert float(e["z"]) > 1e60 and bool(r.z == float("inf"))
+        tol = e["da"] * (2 * R + 16 * U) + 2.0 ** -110
+        near("gradient", d, e["d"], tol + (e["d"].abs() + tol) * (2.0 ** -8 if dtype == BF else U))
+        # rows behind the last sequence: the weights' gradient alone, whatever the rows are
+        alone, = torch.autograd.grad(router_losses(
+            lg, ids, scoring=scoring, renormalize=renorm, routed_scaling_factor=f).weights, lg, gw)
+        assert torch.equal(d[used:], alone[used:])
+        if scoring == "softmax":   # as the router that serves has them, up to E u of its sum
+            w, at = route(lg.detach().float(), top_k=K, renormalize=renorm)
+            assert torch.equal(at.sort(1).values, ids.sort(1).values)
+            have, want = r.weights.sort(1).values, w.sort(1).values
+            assert bool(((have - want).abs() <= want * 2.0 ** -14 + 2.0 ** -120).all())
+
+
+@pytest.mark.parametrize("v", [-1e10, 1e10, 1e18])
+def test_far_logits_z(v):
+    """z and its gradient where the squares stay in range."""
+    lg = torch.full((70, 24), v, device=DEV).requires_grad_(True)
+    ids = torch.arange(140, device=DEV, dtype=torch.int32).view(70, 2) % 24
+    r = router_losses(lg, ids)
+    d, = torch.autograd.grad([r.z], lg, [torch.ones((), device=DEV)])
+    want = lg.detach().double().logsumexp(1)[0]
+    # lse is off by (|m| + 47) u, its square by twice that; 70 terms are added
+    assert abs(float(r.z.detach()) - float(want) ** 2) <= float(want) ** 2 * 80 * U * 4
+    assert bool(((d.double() - 2 * want / 70 / 24).abs() <= abs(float(want)) / 840 * 64 * U).all())

@@ -50,11 +50,15 @@ struct Rows {
 
 constexpr float kLog2e = 1.44269504f;
 
-// e^(l - m) as 2^(l log2 e - m log2 e): the rounding of the second product is the same for
-// all of a row and leaves its probabilities alone, that of the difference is |l - m| 2^-24.
-// Two instructions instead of eight with the difference's rounding made good.
+// e^(l - m) for l <= m.  Near zero as 2^(l log2 e - m log2 e): the rounding of the second
+// product is the same for all of a row and leaves its probabilities alone, that of the
+// difference would be |l - m| 2^-24.  That common factor leaves fp32's range from |m| of
+// 1e9 on, so from 256 on the difference comes first: it is exact wherever e^(l - m) does not
+// vanish (l is then within a factor of two of m), and zero for a row wholly at the lowest
+// value.  Three instructions each instead of eight with the difference's rounding made good.
 __device__ __forceinline__ float exp_from(float l, float m) {
-  return __builtin_amdgcn_exp2f(__builtin_fmaf(l, kLog2e, -m * kLog2e));
+  const float a = fabsf(m) < 256.f ? 0.f : m;
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(l - a, kLog2e, (a - m) * kLog2e));
 }
 
 // v of the lane across: within quads, halves of a row of 16, rows, and rows by
