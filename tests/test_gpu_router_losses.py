@@ -494,3 +494,27 @@ def test_far_logits_z(v):
     # lse is off by (|m| + 47) u, its square by twice that; 70 terms are added
     assert abs(float(r.z.detach()) - float(want) ** 2) <= float(want) ** 2 * 80 * U * 4
     assert bool(((d.double() - 2 * want / 70 / 24).abs() <= abs(float(want)) / 840 * 64 * U).all())
+
+
+def test_weights_into_the_expert_layer():
+    """A selection's weights into the framework's experts: refused while they require a
+    gradient, taken detached or under no_grad."""
+    from xtu_moe_amd import formats as F
+    from xtu_moe_amd.layer import ExpertWeights, moe_forward
+    g = torch.Generator().manual_seed(8)
+    E, K, H, I = 8, 2, 256, 128
+    w13, w2 = torch.randn((E, 2 * I, H), generator=g) * 0.05, torch.randn((E, H, I), generator=g) * 0.05
+    W = ExpertWeights.from_dense(F.FMT_MXFP4, *F.quantize_mxfp4(w13), *F.quantize_mxfp4(w2),
+                                 device=torch.device(DEV))
+    for T in (3, 40):
+        x = torch.randn((T, H), generator=g).to(BF).to(DEV)
+        lg = torch.randn((T, E), generator=g).to(DEV).requires_grad_(True)
+        w, ids = route(lg.detach(), top_k=K)
+        r = router_losses(lg, ids)
+        with pytest.raises(ValueError, match="no backward"):
+            moe_forward(x, ids, r.weights, W)
+        with torch.no_grad():
+            out = moe_forward(x, ids, r.weights, W, out_dtype=F32)
+        assert torch.equal(out, moe_forward(x, ids, r.weights.detach(), W, out_dtype=F32))
+        (0.01 * r.balance + 0.001 * r.z).backward()
+        assert lg.grad.isfinite().all() and bool(lg.grad.any())

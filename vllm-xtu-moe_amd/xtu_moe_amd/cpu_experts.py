@@ -21,6 +21,7 @@ import os
 import torch
 
 from . import _lib
+from .layer import _no_gradient
 
 ISA_AUTO, ISA_PORTABLE, ISA_AVX512 = -1, 0, 2
 
@@ -99,7 +100,9 @@ class CpuExperts:
     # ----------------------------------------------------------------- use
     def forward(self, x, topk_ids, topk_weights, out=None):
         """Host tensors: x bf16 [T, H], ids int32 / weights fp32 [T, K] ->
-        out fp32 [T, H] (pairs with invalid ids or zero weight add nothing)."""
+        out fp32 [T, H] (pairs with invalid ids or zero weight add nothing).  No
+        backward: with gradients enabled, weights that require one are refused."""
+        _no_gradient("the host engine", topk_weights=topk_weights)
         T, K = topk_ids.shape
         x = x.to(torch.bfloat16).contiguous()
         ids = topk_ids.to(torch.int32).contiguous()
@@ -128,6 +131,8 @@ class CpuExperts:
         reference's non-zero codes say)."""
         if int(defer):
             raise NotImplementedError("deferred cpu_decode (defer=1) is not provided")
+        if torch.is_tensor(weights):
+            _no_gradient("the host engine", weights=weights)
         qlen, top_k = int(qlen), int(top_k)
         if qlen <= 0 or top_k <= 0:
             return 0

@@ -19,6 +19,7 @@ import torch
 
 from . import _lib
 from .cpu_experts import CpuExperts
+from .layer import _no_gradient
 
 
 def _p(t) -> int:
@@ -48,7 +49,9 @@ def pin_split(ids, wts, slotmap, n_local: int, hits=None, out=None):
     sl >= n_local (resident in slot sl - n_local):
     cpu_ids = 0 if res or bad else id; cpu_w = 0 if res or bad else w;
     part_ids = sl - n_local if res else -1; part_w = w if res else 0.
-    hits (int64 device scalar, optional) += the number of resident pairs."""
+    hits (int64 device scalar, optional) += the number of resident pairs.
+    No backward: with gradients enabled, wts that require one are refused."""
+    _no_gradient("the split", wts=wts)
     ids = ids.to(torch.int32).contiguous()
     wts = wts.to(torch.float32).contiguous()
     if slotmap.dtype != torch.int32 or slotmap.numel() < int(n_local):
@@ -125,7 +128,9 @@ class PoolSplitLayer:
         """out[T, H] fp32 = the layer over (x, topk_ids, topk_weights):
         pairs of resident experts and the shared experts on the GPU, the
         other pairs through the host engine (``kw`` goes to the resident
-        layer: swiglu_limit, ...).  Inside a graph capture too."""
+        layer: swiglu_limit, ...).  Inside a graph capture too.  No backward, as
+        ``moe_forward``."""
+        _no_gradient("the expert layer", topk_weights=topk_weights)
         T, K = topk_ids.shape
         H = self.pool.H
         h = x.to(torch.bfloat16).contiguous()

@@ -206,7 +206,7 @@ class LayerPool:
     def forward(self, x, topk_ids, topk_weights, **kw):
         """The resident part of the layer: pairs whose expert is resident (and
         the shared experts); pairs of other experts contribute nothing (the
-        caller adds their share: ring stage or CPU)."""
+        caller adds their share: ring stage or CPU).  No backward, as ``moe_forward``."""
         E = self.n_local
         sm = self.slotmap
         id_map = torch.where(sm >= E, torch.arange(E, dtype=torch.int32, device=self.dev),

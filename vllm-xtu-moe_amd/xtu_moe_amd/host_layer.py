@@ -34,7 +34,7 @@ from .cpu_experts import CpuExperts
 from .cpu_split import PoolSplitLayer
 from .expert_pool import LayerPool, build_layer_pool
 from .host_store import HostExpertStore
-from .layer import ExpertWeights, _buf
+from .layer import ExpertWeights, _buf, _no_gradient
 from .ring import _nslots_default, gpu_moe_layer_from_engine_tiled
 
 RESIDENT_LAYERS_ENV = "XIAOTU_MOE_GPU_RESIDENT_LAYERS"
@@ -170,7 +170,8 @@ class HostResidentLayer:
 
     def forward(self, x, ids, wts, *, int8=False):
         """out fp32 [T, H] of the layer for device x (bf16 [T, H]), ids (int32)
-        and weights (fp32) [T, K]."""
+        and weights (fp32) [T, K].  No backward, as ``moe_forward``."""
+        _no_gradient("the expert layer", weights=wts)
         T, K = ids.shape
         capturing = torch.cuda.is_current_stream_capturing()
         gp_min = gpu_prefill_min_tokens()

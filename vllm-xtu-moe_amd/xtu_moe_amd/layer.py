@@ -480,6 +480,15 @@ def _same_device(dev, **tensors):
             raise ValueError(f"{name} is on {t.device}, expected {dev}")
 
 
+def _no_gradient(what, **tensors):
+    """The expert layer has no backward: an input that a gradient is asked of would
+    get none, silently."""
+    for name, t in tensors.items():
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what} has no backward: {name} requires a gradient (detach it, or "
+                             "call under torch.no_grad())")
+
+
 def route(logits, *, top_k, scoring="softmax", renormalize=True, bias=None, n_group=1,
           topk_group=1, routed_scaling_factor=1.0, ids_out=None, wts_out=None, stream=None):
     """Top-k routing on the GPU.  Returns (topk_weights fp32 [T,K], topk_ids int32 [T,K])."""
@@ -1041,7 +1050,9 @@ def moe_forward(x, topk_ids, topk_weights, W: ExpertWeights, *, swiglu_limit=0.0
     logits first, writing topk_ids / topk_weights (int32 / fp32 buffers).
     fp8_scales_ok: for FP8 slot planes, whether their block scales are
     bounded (fp8_block_scales_bounded).
+    No backward: with gradients enabled, topk_weights that require one are refused.
     """
+    _no_gradient("the expert layer", topk_weights=topk_weights)
     if x.dtype != torch.bfloat16 or not x.is_contiguous():
         raise ValueError("x must be contiguous bf16 [T, H]")
     if W.fmt == FMT_INT4:
@@ -1406,7 +1417,9 @@ def expert_pass(x, seg, W: ExpertWeights, b0: int, b1: int, y, *, slot_map=None,
 
 def combine(seg, y, topk_weights, out, *, stream=None):
     """out[t] = sum_k w[t,k] * y[pos(t,k)] (+ shared rows), pairs in the trash
-    bucket or of weight 0 skipped; bf16 or fp32 out."""
+    bucket or of weight 0 skipped; bf16 or fp32 out.  No backward: with gradients
+    enabled, topk_weights that require one are refused."""
+    _no_gradient("combine", topk_weights=topk_weights)
     T, K = seg.T, seg.K
     _lib.call("xtu_combine", _p(y), _p(seg.inv), _p(topk_weights),
               _p(seg.seg_start) + 4 * (seg.E + seg.NS), T, K, seg.NS, out.shape[1], _p(out),

@@ -29,7 +29,7 @@ import torch
 
 from . import formats as F
 from .host_store import HostExpertStore, empty_slots
-from .layer import _buf, _p, _stream, combine, expert_pass, gemm_tile_m, segmentation
+from .layer import _buf, _no_gradient, _p, _stream, combine, expert_pass, gemm_tile_m, segmentation
 
 DEFAULT_TILE_E = 48
 NSLOTS_ENV = "XIAOTU_GPF_STAGE_NSLOTS"
@@ -220,7 +220,9 @@ def gpu_moe_layer_from_engine_tiled(engine, x, topk_ids, topk_weights, H: int, I
     `out`, gpu_prefill.py:3020, gpu_prefill_fp8.py:1478).  None when the
     layer cannot be streamed (no host store, a shape mismatch, more shared
     experts than a tile holds and no pool for them); nothing is queued then.
-    int8: the INT8 ALIGN GEMMs (MXFP4), as the engine's int8_activation."""
+    int8: the INT8 ALIGN GEMMs (MXFP4), as the engine's int8_activation.
+    No backward, as ``moe_forward``."""
+    _no_gradient("the expert layer", topk_weights=topk_weights)
     device = torch.device(device)
     store = _as_store(engine)
     if store is None or store.H != int(H) or store.I != int(I) or store.E != int(E):

@@ -3,10 +3,13 @@ experts' weights, with their gradient in the logits.
 
     ids = layer.route(logits, top_k=K)[1]
     r = router_losses(logits, ids)
-    (task_loss(r.weights) + 0.01 * r.balance + 0.001 * r.z).backward()
+    (0.01 * r.balance + 0.001 * r.z).backward()
 
 ``layer.route`` selects; this gives what a training step differentiates, and the
-counts that say how evenly the experts are used (also to pick a pool's).  The
+counts that say how evenly the experts are used (also to pick a pool's).
+``weights`` carry a task loss's gradient where the caller combines the experts'
+outputs differentiably; ``layer.moe_forward`` has no backward and refuses them
+(``r.weights.detach()`` goes in).  The
 reference serves only: its router (vllm_xiaotu_moe/hybrid_model.py:1877) has no
 losses and no gradient.
 """
