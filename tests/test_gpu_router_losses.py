@@ -518,3 +518,17 @@ def test_weights_into_the_expert_layer():
         assert torch.equal(out, moe_forward(x, ids, r.weights.detach(), W, out_dtype=F32))
         (0.01 * r.balance + 0.001 * r.z).backward()
         assert lg.grad.isfinite().all() and bool(lg.grad.any())
+
+
+def test_gradients_tangents_refused():
+    """A tangent that comes in with an output's gradient would be lost as well."""
+    from torch.autograd import forward_ad
+    lg, ids, gw = _inputs(20, 16, 2, seed=6)
+    lg.requires_grad_(True)
+    r = router_losses(lg, ids)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(gw, torch.ones_like(gw))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(r.weights, lg, dual, retain_graph=True)
+    d, = torch.autograd.grad(r.weights, lg, gw)
+    assert d.isfinite().all()

@@ -259,3 +259,18 @@ def test_entry_refuses_on_the_host():
     assert lib.xtu_linear4_workspace_bytes(5, 1, 96, 0, 2, 32, 0) == 5 * 96 * 2   # a copy of x
     assert lib.xtu_linear4_plan(0, 1, 32, 0, 2, 32) == lib.xtu_linear4_plan(1, 1, 48, 0, 2, 32) == -1
     assert lib.xtu_linear4_weight_bytes(1, 32, 0, 1, 32) == 0
+
+
+def test_tangents_refused():
+    """Nor a forward-mode derivative, which requires_grad does not show."""
+    from torch.autograd import forward_ad
+    w, zeros = _w(), torch.zeros((3, 32), dtype=BF)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                _refused("forward-mode", dual(zeros), w)
+                for kw in (dict(bias=torch.zeros(4)), dict(row_scale=torch.zeros(3)),
+                           dict(residual=torch.zeros((3, 4))), dict(out=torch.zeros((3, 4)))):
+                    _refused("forward-mode", zeros, w, **{k: dual(v) for k, v in kw.items()})
+                    _refused("CUDA", zeros, w, **kw)

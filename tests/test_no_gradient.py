@@ -4,6 +4,7 @@ import types
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from xtu_moe_amd import cpu_split, layer, ring
 from xtu_moe_amd.cpu_experts import CpuExperts
@@ -37,6 +38,16 @@ def test_weights_that_require_a_gradient(name):
     for w in (logits, torch.softmax(logits, 1), torch.nn.Parameter(torch.ones((T, K)))):
         with pytest.raises(ValueError, match="no backward"):
             ENTRIES[name](w)
+
+
+@pytest.mark.parametrize("name", list(ENTRIES))
+def test_weights_with_a_tangent(name):
+    """A forward-mode tangent, under no_grad too (which does not stop it)."""
+    with forward_ad.dual_level():
+        w = forward_ad.make_dual(torch.ones((T, K)), torch.ones((T, K)))
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(ValueError, match="forward-mode"):
+                ENTRIES[name](w)
 
 
 @pytest.mark.parametrize("name", list(ENTRIES))

@@ -70,3 +70,14 @@ def test_entries_refuse_on_the_host():
     for bad in ((-1, 8, 1), ((1 << 30) + 1, 8, 1), (4, 0, 1), (4, 1025, 1), (4, 8, 0)):
         assert lib.xtu_router_workspace_bytes(*bad) == 0
     assert lib.xtu_router_workspace_bytes(0, 8, 1) > 0   # no rows: the sums of none
+
+
+def test_tangents_refused():
+    """No forward-mode derivative: a result without one would lose it silently."""
+    from torch.autograd import forward_ad
+    lg, ids = torch.zeros((3, 8)), torch.zeros((3, 2), dtype=I32)
+    with forward_ad.dual_level():
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                _refused("forward-mode", forward_ad.make_dual(lg, torch.ones_like(lg)), ids)
+                _refused("CUDA", lg, ids)

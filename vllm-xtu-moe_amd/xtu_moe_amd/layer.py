@@ -17,6 +17,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .formats import (FMT_BF16, FMT_FP8, FMT_INT4, FMT_MXFP4, FMT_NVFP4, INT4_GROUPS,
@@ -480,10 +481,19 @@ def _same_device(dev, **tensors):
             raise ValueError(f"{name} is on {t.device}, expected {dev}")
 
 
+def _has_tangent(*tensors):
+    """Whether a forward-mode derivative runs through any of the given tensors (whose
+    requires_grad does not say so, and which no_grad does not stop)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _no_gradient(what, **tensors):
     """The expert layer has no backward: an input that a gradient is asked of would
     get none, silently."""
     for name, t in tensors.items():
+        if _has_tangent(t):
+            raise ValueError(f"{what} has no forward-mode derivative: {name} carries a tangent")
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{what} has no backward: {name} requires a gradient (detach it, or "
                              "call under torch.no_grad())")

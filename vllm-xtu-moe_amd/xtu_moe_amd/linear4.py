@@ -20,7 +20,7 @@ import torch
 from . import _lib
 from .formats import (FMT_INT4, FMT_MXFP4, FMT_NAMES, FMT_NVFP4, fmt_of, linear4_group,
                       linear4_record, pack_linear4)
-from .layer import _same_device
+from .layer import _has_tangent, _same_device
 from .linear import (_OPERAND, _TYPES, ACTIVATIONS, MAX_COLS, MAX_ROWS, _current_device, _overlap,
                      _rows, on_stream, raw_stream)
 
@@ -150,7 +150,8 @@ def linear4(x, w: Weight4, *, bias=None, activation="none", row_scale=None, resi
     or fp32 per out_dtype, or the given tensor, which may be ``residual`` itself
     and otherwise overlaps no input.  Weights enter the fp32 sums exactly;
     the epilogue is fp32, rounded once.  Capturable into a HIP graph.  No
-    backward: inputs that require a gradient are refused.
+    backward: inputs that require a gradient, or carry a forward-mode tangent,
+    are refused.
     """
     act = ACTIVATIONS.get(activation)
     if act is None:
@@ -208,6 +209,8 @@ def linear4(x, w: Weight4, *, bias=None, activation="none", row_scale=None, resi
         same, grad = same and out.device == dev, grad or out.requires_grad
     if grad and torch.is_grad_enabled():
         raise ValueError("linear4 has no backward: an input requires a gradient")
+    if _has_tangent(x, bias, row_scale, residual, out):
+        raise ValueError("linear4 has no forward-mode derivative: an input carries a tangent")
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor")
     if not same:

@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from .block import MAX_EXPERTS, MAX_TOP_K
-from .layer import _same_device
+from .layer import _has_tangent, _same_device
 from .linear import _current_device, on_stream, raw_stream
 
 # xtu_router_args: logits, ids, starts, weights, stat, counts, probs, balance, z,
@@ -62,8 +62,8 @@ def router_losses(logits, ids, *, scoring="softmax", renormalize=True, routed_sc
     P_e with n rows and P their mean p: 1 for even use.  z: mean over the
     sequences' rows of logsumexp(logits)^2.  A row of -inf has p = 0 and no
     gradient; NaN and +inf give NaN.  fp32 arithmetic, sums over rows fp32 and fp64;
-    the same call gives the same bits.  Once differentiable.  Capturable into
-    a HIP graph.
+    the same call gives the same bits.  Once differentiable, backwards only.
+    Capturable into a HIP graph.
     """
     T, E, K, S = _check(logits, ids, scoring, routed_scaling_factor, seq_starts)
     dev = logits.device
@@ -94,6 +94,8 @@ def _check(logits, ids, scoring, scale, seq_starts):
     if not 1 <= E <= MAX_EXPERTS or T > MAX_ROWS:
         raise ValueError(f"logits of {T} rows of {E} experts: 1 .. {MAX_EXPERTS} experts, at most "
                          f"{MAX_ROWS} rows")
+    if _has_tangent(logits):
+        raise ValueError("router_losses has no forward-mode derivative: logits carry a tangent")
     if logits.stride(1) != 1 and E > 1:
         raise ValueError(f"logits' rows must be contiguous (column stride {logits.stride(1)})")
     if ids.dim() != 2 or ids.dtype != torch.int32 or ids.shape[0] != T or not ids.is_contiguous():
@@ -156,6 +158,8 @@ def _forward(logits, ids, starts, shape):
 
 def _grad(ctx, g_weights, g_balance, g_z):
     logits, ids, starts, weights, counts = ctx.saved_tensors
+    if _has_tangent(logits, g_weights, g_balance, g_z):
+        raise RuntimeError("router_losses' gradient has no forward-mode derivative")
     out = logits.new_empty(logits.shape)
     grads = [None if g is None else g.contiguous() for g in (g_weights, g_balance, g_z)]
     rc = _entries()[1](_pack(logits, ids, starts, weights, ctx.stat, counts, None, None, None,
