@@ -532,3 +532,63 @@ def test_gradients_tangents_refused():
             torch.autograd.grad(r.weights, lg, dual, retain_graph=True)
     d, = torch.autograd.grad(r.weights, lg, gw)
     assert d.isfinite().all()
+
+
+@pytest.mark.parametrize("scoring,renorm,f,term", [
+    m + (t,) for m in MODES for t in ("weights", "balance", "z", "all")
+    if t != "z" or m[0] == "softmax"])
+def test_gradient_against_autograd(scoring, renorm, f, term):
+    """Element by element against autograd of the definition in 64 bits, each loss alone
+    too: within R's bounds of that loss's own terms, a thousandth of the gradient at most,
+    so that a missing term or a wrong sign or factor shows."""
+    pick = lambda name, v: v if term in (name, "all") else 0.0  # noqa: E731
+    for T, E, K in ((9, 8, 3), (130, 60, 4), (257, 64, 6), (33, 128, 8), (700, 256, 8), (50, 1024, 16)):
+        for dtype in (F32, BF):
+            lg, ids, gw = _inputs(T, E, K, seed=T + E, dtype=dtype)
+            gw = gw if term in ("weights", "all") else gw * 0
+            gb, gz = pick("balance", 0.7), pick("z", 0.3)
+            starts = [0, T // 3, T // 3, T - T // 5]
+            lg.requires_grad_(True)
+            r = router_losses(lg, ids, scoring=scoring, renormalize=renorm, routed_scaling_factor=f,
+                              seq_starts=torch.tensor(starts, dtype=torch.int32, device=DEV))
+            outs = [r.weights, r.balance] + ([r.z] if r.z is not None else [])
+            d, = torch.autograd.grad(outs, lg, [gw] + [torch.full((), v, device=DEV)
+                                                       for v in (gb, gz)][:len(outs) - 1])
+            e = _in_logs(lg, ids, starts, scoring, renorm, f, gw, gb, gz)
+            l64 = lg.detach().double()
+            R = (float((l64.amax(1) - l64.amin(1)).max()) + 40) * U
+            tol = e["da"] * (2 * R + 16 * U) + 2.0 ** -140
+            assert float(tol.norm()) <= float(e["d"].norm()) / 1000, (T, E)
+            tol = tol + (e["d"].abs() + tol) * (2.0 ** -8 if dtype == BF else U)
+            bad = ~((d.double() - e["d"]).abs() <= tol)
+            assert not bool(bad.any()), (T, E, dtype, int(bad.sum()))
+
+
+@pytest.mark.parametrize("scoring,renorm,f", MODES)
+def test_gradient_against_differences_of_the_definition(scoring, renorm, f):
+    """Along directions v of unit length against (F(l + h v) - F(l - h v)) / 2h of the
+    definition's F in 64 bits: off by h^2 / 6 times a third derivative (at most 30 F0, as
+    above) and by 2^-50 F0 / h, beside the kernel's own error; all of that a hundredth of
+    what is compared."""
+    lg, ids, gw = _inputs(24, 16, 3, seed=9)
+    starts, gb, gz, h = [0, 10, 24], 0.7, 0.3, 2.0 ** -13
+    lg.requires_grad_(True)
+    r = router_losses(lg, ids, scoring=scoring, renormalize=renorm, routed_scaling_factor=f,
+                      seq_starts=torch.tensor(starts, dtype=torch.int32, device=DEV))
+    outs = [r.weights, r.balance] + ([r.z] if r.z is not None else [])
+    d, = torch.autograd.grad(outs, lg, [gw] + [torch.full((), v, device=DEV) for v in (gb, gz)]
+                             [:len(outs) - 1])
+    F = lambda l: _in_logs(l, ids, starts, scoring, renorm, f, gw, gb, gz)  # noqa: E731
+    e, l64 = F(lg), lg.detach().double()
+    F0 = float((e["weights"] * gw.double().abs()).sum() + gb * e["balance"] + gz * e["z"])
+    own = e["da"] * (2 * (float((l64.amax(1) - l64.amin(1)).max()) + 40) + 16) * U + e["d"].abs() * U
+    g = torch.Generator().manual_seed(1)
+    largest = 0.0
+    for _ in range(8):
+        v = torch.randn(lg.shape, generator=g).double().to(DEV)
+        v = v / v.norm()
+        diff = float((F(l64 + h * v)["total"] - F(l64 - h * v)["total"]) / (2 * h))
+        tol = F0 * (5 * h * h + 2.0 ** -50 / h) + float((own * v.abs()).sum())
+        assert abs(diff - float((d.double() * v).sum())) <= tol
+        largest = max(largest, abs(diff) / tol)
+    assert largest > 100   # (no gradient, or one of the other sign, would show)
