@@ -274,3 +274,16 @@ def test_tangents_refused():
                            dict(residual=torch.zeros((3, 4))), dict(out=torch.zeros((3, 4)))):
                     _refused("forward-mode", zeros, w, **{k: dual(v) for k, v in kw.items()})
                     _refused("CUDA", zeros, w, **kw)
+
+
+def test_unaligned_rows_are_not_read_as_aligned():
+    """The kernel for rows of x at any 2-byte address takes them with a load that claims
+    no more: an access through a 16-byte-aligned type would be right by luck only."""
+    import re
+    src = os.path.join(os.path.dirname(_lib.__file__), "..", "csrc", "linear4_tile.hip")
+    text = open(src).read()
+    loads = [line for line in text.splitlines() if "xrow[i]" in line and "xv[i]" in line]
+    assert len(loads) == 1
+    fn = re.search(r"xv\[i\] = (\w+)\(", loads[0]).group(1)
+    body = re.search(r"u32x4_t " + fn + r"\(.*?\n}", text, re.S).group(0)
+    assert "__builtin_memcpy" in body and "reinterpret_cast" not in body

@@ -14,6 +14,14 @@ namespace {
 
 constexpr int kAhead = 2;   // blocks of w in registers
 
+// Eight k of a row of x at any 2-byte address (one load, which the hardware splits where
+// it has to), zeros past K.
+__device__ __forceinline__ u32x4_t load_any8(const Linear4Args& a, const uint16_t* row, int k) {
+  u32x4_t v = {0u, 0u, 0u, 0u};
+  if (k < a.e.K) __builtin_memcpy(&v, row + k, 16);   // (K % 8 == 0)
+  return v;
+}
+
 template <int FMT, int G, bool GATED, int MT, int NP>
 __global__ __launch_bounds__(256) void linear4_tile_kernel(Linear4Args a) {
   constexpr int AK = GATED ? lin::kActSwiglu : lin::kActOther;
@@ -67,7 +75,7 @@ __global__ __launch_bounds__(256) void linear4_tile_kernel(Linear4Args a) {
   u32x4_t xv[MT];
   auto load_x = [&](int s) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) xv[i] = load_x8(a, xrow[i], 128 * s + 8 * xp);
+    for (int i = 0; i < MT; ++i) xv[i] = load_any8(a, xrow[i], 128 * s + 8 * xp);
   };
   // (16 lanes that read a block's rows at one place touch all banks: linear_tile.hip)
   const auto slot = [](int place, int row) { return (place ^ (row & 7) << 1) * 16; };
