@@ -287,3 +287,31 @@ def test_unaligned_rows_are_not_read_as_aligned():
     fn = re.search(r"xv\[i\] = (\w+)\(", loads[0]).group(1)
     body = re.search(r"u32x4_t " + fn + r"\(.*?\n}", text, re.S).group(0)
     assert "__builtin_memcpy" in body and "reinterpret_cast" not in body
+
+
+def test_second_level_scales_are_checked():
+    c, n = torch.zeros((4, 32), dtype=torch.uint8), torch.full((4, 4), 0x38, dtype=torch.uint8)
+    for bad in (float("nan"), float("inf"), -float("inf"), 1e39):
+        _refused_w("finite", "nvfp4", c, n, bad)
+        _refused_w("finite", "nvfp4", c, n, torch.tensor([1.0, bad]), gated=True)
+    for good in (0.0, -2.0, 3e38):
+        assert Weight4.from_dense("nvfp4", c, n, good).gs.tolist() == [torch.tensor(good).item()]
+
+
+def test_weights_are_constants():
+    """Parameters are packed as they are now; records that claim a gradient are refused."""
+    import dataclasses
+    c, n = torch.zeros((4, 32), dtype=torch.uint8), torch.full((4, 4), 0x38, dtype=torch.uint8)
+    p = torch.nn.Parameter(torch.tensor([2.0]))
+    w = Weight4.from_dense("nvfp4", c, n, p)
+    assert not w.gs.requires_grad and w.gs.tolist() == [2.0]
+    with torch.no_grad():
+        p.fill_(5.0)
+    assert w.gs.tolist() == [2.0]
+    w.gs.requires_grad_(False)
+    with pytest.raises(ValueError, match="without a gradient"):
+        dataclasses.replace(w, gs=torch.nn.Parameter(w.gs.clone()))
+    s = torch.nn.Parameter(torch.ones((4, 2)))
+    got = Weight4.from_dense("int4", c, s)
+    assert not got.data.requires_grad
+    assert torch.equal(got.data, Weight4.from_dense("int4", c, s.detach()).data)

@@ -56,8 +56,9 @@ class Weight4:
                              f"{tuple(d.shape)} {d.dtype}")
         if (gs is not None) != (self.fmt == FMT_NVFP4) or gs is not None and (
                 gs.dtype != torch.float32 or gs.shape != (halves,) or gs.device != d.device
-                or not gs.is_contiguous()):
-            raise ValueError(f"second-level scales must be fp32 [{halves}] beside NVFP4 records")
+                or not gs.is_contiguous() or gs.requires_grad):
+            raise ValueError(f"second-level scales must be fp32 [{halves}] beside NVFP4 records, "
+                             "without a gradient")
 
     @property
     def device(self):
@@ -79,11 +80,12 @@ class Weight4:
         fmt: "mxfp4", "nvfp4" or "int4" (or its number in ``formats``).  codes
         u8 [rows, K / 2], low nibble = even k.  scales, as bytes or as torch's
         type of them: MXFP4 e8m0 [rows, K / 32] (at most 252: larger ones leave
-        bf16's range; 255 is NaN); NVFP4 e4m3 (no NaN) [rows, K / 16]; INT4 finite fp32, fp16 or bf16 [rows, K / 32, 64 or
-        128], for value code - 8.  global_scale: NVFP4's second-level scale, a
-        number or a tensor of one (gated: one or two, gate and up).  gated:
-        rows are [gate; up], for activation "swiglu".  Reads the scales back
-        once to check them.
+        bf16's range; 255 is NaN); NVFP4 e4m3 (no NaN) [rows, K / 16]; INT4 finite
+        fp32, fp16 or bf16 [rows, K / 32, 64 or 128], for value code - 8.
+        global_scale: NVFP4's second-level scale, a finite number or a tensor of one
+        (gated: one or two, gate and up).  gated: rows are [gate; up], for
+        activation "swiglu".  Reads the scales back once to check them.  The
+        result is a constant: parameters are packed as they are now, detached.
         """
         fmt = fmt_of(fmt)
         if fmt not in (FMT_MXFP4, FMT_NVFP4, FMT_INT4):
@@ -98,6 +100,7 @@ class Weight4:
             raise ValueError(f"weights of {rows} rows of {K} values, at most {MAX_COLS} of each")
         if scales.dim() != 2 or scales.shape[0] != rows:
             raise ValueError(f"scales must be [{rows}, K / group], got {tuple(scales.shape)}")
+        scales = scales.detach()
         group = linear4_group(fmt, scales, K)
         if fmt == FMT_INT4:
             if scales.dtype not in (torch.float32, torch.float16, torch.bfloat16):
@@ -118,11 +121,13 @@ class Weight4:
         if fmt == FMT_NVFP4:
             if global_scale is None:
                 raise ValueError("NVFP4 weights need their second-level scale")
-            gs = torch.as_tensor(global_scale, dtype=torch.float32).reshape(-1).to(dev)
+            gs = torch.as_tensor(global_scale, dtype=torch.float32).detach().reshape(-1).to(dev)
             if gs.numel() not in (1, halves):
                 raise ValueError(f"second-level scales: {gs.numel()}, expected 1"
                                  + (" or 2 (gate, up)" if gated else ""))
-            gs = gs.expand(halves).contiguous()
+            if not bool(gs.isfinite().all()):
+                raise ValueError("second-level scales must be finite")
+            gs = gs.expand(halves).clone(memory_format=torch.contiguous_format)   # its own
         elif global_scale is not None:
             raise ValueError(f"{FMT_NAMES[fmt]} weights have no second-level scale")
         split = lambda t: t.to(dev).contiguous().view(halves, rows // halves, -1)  # noqa: E731
