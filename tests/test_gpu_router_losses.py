@@ -592,3 +592,20 @@ def test_gradient_against_differences_of_the_definition(scoring, renorm, f):
         assert abs(diff - float((d.double() * v).sum())) <= tol
         largest = max(largest, abs(diff) / tol)
     assert largest > 100   # (no gradient, or one of the other sign, would show)
+
+
+def test_gradient_penalty_refused():
+    """A loss on the gradient, through outputs whose own gradients are constants: refused,
+    where a constant in its place would leave that loss out."""
+    lg, ids, gw = _inputs(20, 16, 2, seed=6)
+    lg.requires_grad_(True)
+    one = torch.ones((), device=DEV)
+    for pick, g in (("weights", gw), ("balance", one), ("z", one)):
+        out = getattr(router_losses(lg, ids), pick)
+        d, = torch.autograd.grad(out, lg, g, create_graph=True)
+        assert d.requires_grad
+        plain, = torch.autograd.grad(getattr(router_losses(lg, ids), pick), lg, g)
+        assert torch.equal(d.detach(), plain)
+        with pytest.raises(RuntimeError, match="once differentiable"):
+            (out.sum() + d.square().sum()).backward()
+        assert lg.grad is None

@@ -171,7 +171,17 @@ def _grad(ctx, g_weights, g_balance, g_z):
     return out
 
 
-_grad_once = torch.autograd.function.once_differentiable(_grad)
+class _Once(torch.autograd.Function):
+    """The gradient as a node of its own, where a graph of it is asked for: a derivative
+    of it is refused whatever it is asked through (it depends on the logits also where
+    the outputs' gradients are constants)."""
+    @staticmethod
+    def forward(ctx, losses, logits, g_weights, g_balance, g_z):
+        return _grad(losses, g_weights, g_balance, g_z)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("router_losses is once differentiable: its gradient has none")
 
 
 class _Losses(torch.autograd.Function):
@@ -189,6 +199,8 @@ class _Losses(torch.autograd.Function):
     def backward(ctx, g_weights, g_balance, g_z, _counts, _probs):
         if g_weights is None and g_balance is None and g_z is None:
             return None, None, None, None
-        # (a graph of the gradient is refused where it is used; the wrapper costs 6 us)
-        grad = _grad_once if torch.is_grad_enabled() else _grad
-        return grad(ctx, g_weights, g_balance, g_z), None, None, None
+        if torch.is_grad_enabled():   # create_graph
+            d = _Once.apply(ctx, ctx.saved_tensors[0], g_weights, g_balance, g_z)
+        else:
+            d = _grad(ctx, g_weights, g_balance, g_z)
+        return d, None, None, None
