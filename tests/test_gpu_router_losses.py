@@ -609,3 +609,26 @@ def test_gradient_penalty_refused():
         with pytest.raises(RuntimeError, match="once differentiable"):
             (out.sum() + d.square().sum()).backward()
         assert lg.grad is None
+
+
+@pytest.mark.parametrize("renorm", [True, False])
+def test_infinity_with_sigmoid(renorm):
+    """sigmoid(inf) is 1: the row stays finite, and has no slope there."""
+    lg, ids, gw = _inputs(40, 64, 4, seed=5)
+    lg[7, 30], ids[7, 0] = float("inf"), 30
+    ids[7, 1:] = torch.tensor([1, 2, 3], device=DEV)
+    lg[8], lg[9, ::2] = float("inf"), float("inf")
+    starts = [0, 20, 40]
+    lg.requires_grad_(True)
+    r = router_losses(lg, ids, scoring="sigmoid", renormalize=renorm,
+                      seq_starts=torch.tensor(starts, dtype=torch.int32, device=DEV))
+    d, = torch.autograd.grad([r.weights, r.balance], lg, [gw, torch.full((), 0.7, device=DEV)])
+    # (100 stands for inf: sigmoid(100) is 1 and its slope 0 within 2^-140)
+    near = lg.detach().clone()
+    near[near == float("inf")] = 100.0
+    e = _formula(near, ids, starts, "sigmoid", renorm, 1.0, gw, 0.7, 0.0)
+    R = (12 + 40) * U
+    assert bool(((r.weights.detach().double() - e["weights"]).abs() <= e["weights"] * (2 * R + 4 * U)).all())
+    assert bool(((r.probs.double() - e["probs"]).abs() <= e["probs"] * (R + 2.0 ** -17)).all())
+    assert bool(((d.double() - e["d"]).abs() <= e["da"] * (2 * R + 17 * U) + 2.0 ** -120).all())
+    assert bool((d[8] == 0).all()) and d[7, 30] == 0

@@ -81,3 +81,24 @@ def test_tangents_refused():
             with mode():
                 _refused("forward-mode", forward_ad.make_dual(lg, torch.ones_like(lg)), ids)
                 _refused("CUDA", lg, ids)
+
+
+def test_limits_refused():
+    """What the entry does not take is a ValueError, not a library error."""
+    lg, ids = torch.zeros((3, 1024)), torch.zeros((3, 2), dtype=I32)
+    for E, most in ((1024, (1 << 18) - 1), (17, (1 << 23) - 1), (16, (1 << 24) - 1)):
+        starts = torch.zeros(most + 2, dtype=I32)
+        _refused("sixteens", lg[:, :E], ids, seq_starts=starts)
+        _refused("CUDA", lg[:, :E], ids, seq_starts=starts[1:])
+    for f in (1e39, 2.0 ** 128, 1e-39, 5e-324):
+        _refused("positive", lg, ids, scoring="sigmoid", routed_scaling_factor=f)
+    for f in (2.0 ** -126, torch.finfo(torch.float32).max):
+        _refused("CUDA", lg, ids, scoring="sigmoid", routed_scaling_factor=f)
+
+
+@pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
+def test_limits_are_the_entrys():
+    lib = _lib.load()
+    for E, most in ((1024, (1 << 18) - 1), (17, (1 << 23) - 1), (16, (1 << 24) - 1)):
+        assert lib.xtu_router_workspace_bytes(4, E, most) > 0
+        assert lib.xtu_router_workspace_bytes(4, E, most + 1) == 0

@@ -16,7 +16,8 @@
 // Backward: one pass, logits and the selected experts' gradients in, the logits'
 // gradient out (router_grad_kernel); a row's maximum and sum come from the forward.
 //
-// A row of -inf has p = 0, no z and no gradient.  NaN and +inf give NaN.
+// A row of -inf has p = 0, no z and no gradient.  NaN gives NaN, +inf with softmax too
+// (sigmoid: its score is 1).
 #include <type_traits>
 
 #include "xtu_common.hpp"
@@ -741,12 +742,15 @@ hipError_t by_layout(int E, F f) {
   }
 }
 
+// The second launch: a workgroup per sequence and kCols experts, below 2^32 threads.
+bool grid_ok(int E, int S) { return (long)S * ((E + kCols - 1) / kCols) * kSumThreads < (1L << 32); }
+
 bool rows_of(const xtu_router_args& t, Rows& a) {
   if (t.T < 0 || t.T > (1 << 30) || t.E < 1 || t.E > kMaxE || t.K < 1 || t.K > kMaxK ||
-      t.S < 1 || t.S > (1 << 24) || t.mode < 0 || t.mode > 1 || !(t.scale > 0.f) ||
+      t.S < 1 || t.mode < 0 || t.mode > 1 || !(t.scale > 0.f) ||
       !(t.scale < INFINITY))
     return false;
-  if ((long)t.S * ((t.E + kCols - 1) / kCols) * kSumThreads >= (1L << 32)) return false;   // the grid
+  if (!grid_ok(t.E, t.S)) return false;
   if (t.T > 0 && (!t.logits || !t.ids || t.ld < 0)) return false;
   if (!t.starts && t.S != 1) return false;
   const size_t size = t.logits_bf16 ? 2 : 4;
@@ -770,7 +774,7 @@ using namespace xtu::rt;
 extern "C" {
 
 size_t xtu_router_workspace_bytes(int T, int E, int S) {
-  if (T < 0 || T > (1 << 30) || E < 1 || E > kMaxE || S < 1 || S > (1 << 24)) return 0;
+  if (T < 0 || T > (1 << 30) || E < 1 || E > kMaxE || S < 1 || !grid_ok(E, S)) return 0;
   return space_of(T, E, S).bytes;
 }
 

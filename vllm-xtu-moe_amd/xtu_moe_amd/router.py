@@ -28,7 +28,9 @@ from .linear import _current_device, on_stream, raw_stream
 # xtu_router_args: logits, ids, starts, weights, stat, counts, probs, balance, z,
 # norm, workspace; ld; its bytes; T, E, K, S, mode, renormalize, logits_bf16; scale
 ARGS = struct.Struct("@11PlN7if")
-MAX_ROWS, MAX_SEQUENCES = 1 << 30, 1 << 24
+MAX_ROWS = 1 << 30
+MAX_PARTS = 1 << 24   # sequences times sixteens of experts, below: the second launch's grid
+MIN_SCALE, MAX_SCALE = 2.0 ** -126, torch.finfo(torch.float32).max   # what the kernels hold
 _WS_BYTES: dict = {}
 _ENTRIES = None
 
@@ -54,14 +56,18 @@ def router_losses(logits, ids, *, scoring="softmax", renormalize=True, routed_sc
     (scores s = sigmoid(logits), p = s / sum s).  seq_starts int32 [S + 1] on
     the device: sequence q is rows seq_starts[q] .. seq_starts[q + 1]
     (ascending; values are clamped to 0 .. T); rows outside them get weights and
-    take part in no loss and no count.  Without it all rows are one sequence.
+    take part in no loss and no count.  Without it all rows are one sequence.  At
+    most 2^30 rows, S ceil(E / 16) < 2^24, and 2^31 - 1 selections of one expert in
+    a sequence (counts are int32).
 
     weights: the selected experts' p (sigmoid: s), divided by their sum with
     renormalize, times routed_scaling_factor (sigmoid only), as ``route`` gives
     them.  balance: mean over non-empty sequences of E / (K n) sum_e counts_e
     P_e with n rows and P their mean p: 1 for even use.  z: mean over the
     sequences' rows of logsumexp(logits)^2.  A row of -inf has p = 0 and no
-    gradient; NaN and +inf give NaN.  fp32 arithmetic, sums over rows fp32 and fp64;
+    gradient; NaN gives NaN, and so does +inf with softmax (sigmoid: its score is
+    1).  Far finite logits keep their ratios, with sigmoid too, where the scores
+    themselves vanish; z is inf where a square leaves fp32.  fp32 arithmetic, sums over rows fp32 and fp64;
     the same call gives the same bits.  Once differentiable, backwards only.
     Capturable into a HIP graph.
     """
@@ -85,8 +91,8 @@ def _check(logits, ids, scoring, scale, seq_starts):
         raise ValueError(f"unsupported scoring function {scoring!r}")
     if scoring == "softmax" and float(scale) != 1.0:
         raise ValueError("a scaling factor goes with sigmoid scoring")
-    if not 0.0 < float(scale) < float("inf"):
-        raise ValueError(f"routed_scaling_factor {scale} is not a positive number")
+    if not MIN_SCALE <= float(scale) <= MAX_SCALE:
+        raise ValueError(f"routed_scaling_factor {scale} is not a positive fp32 number")
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"logits must be a 2-D fp32 or bf16 tensor, got {tuple(logits.shape)} "
                          f"{logits.dtype}")
@@ -106,10 +112,13 @@ def _check(logits, ids, scoring, scale, seq_starts):
     S = 1
     if seq_starts is not None:
         if seq_starts.dim() != 1 or seq_starts.dtype != torch.int32 \
-                or not seq_starts.is_contiguous() or not 2 <= seq_starts.numel() <= MAX_SEQUENCES:
+                or not seq_starts.is_contiguous() or seq_starts.numel() < 2:
             raise ValueError(f"seq_starts must be contiguous int32 [S + 1], got "
                              f"{tuple(seq_starts.shape)} {seq_starts.dtype}")
         S = seq_starts.numel() - 1
+        if S * -(-E // 16) >= MAX_PARTS:
+            raise ValueError(f"{S} sequences of {E} experts: fewer than {MAX_PARTS} divided by the "
+                             "sixteens of experts")
     if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor")
     _same_device(logits.device, ids=ids, seq_starts=seq_starts)
