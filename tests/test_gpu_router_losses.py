@@ -632,3 +632,22 @@ def test_infinity_with_sigmoid(renorm):
     assert bool(((r.probs.double() - e["probs"]).abs() <= e["probs"] * (R + 2.0 ** -17)).all())
     assert bool(((d.double() - e["d"]).abs() <= e["da"] * (2 * R + 17 * U) + 2.0 ** -120).all())
     assert bool((d[8] == 0).all()) and d[7, 30] == 0
+
+
+@pytest.mark.parametrize("E", [8, 300])
+def test_long_sums(E):
+    """Millions of equal rows (one, repeated), whose rounding errors all have one sign: a
+    lane adds at most 256 of them in fp32, 64 more joins behind that, the rest is in fp64.
+    So P, balance and z are off by R + 320 u (z: twice lse's error more)."""
+    T = 1 << 27 if E == 8 else 1 << 24
+    g = torch.Generator().manual_seed(E)
+    row = torch.randn((1, E), generator=g).to(DEV)
+    ids = torch.zeros((T, 1), dtype=torch.int32, device=DEV)
+    r = router_losses(row.expand(T, E), ids)
+    p = torch.softmax(row.double(), 1)
+    tol = (8 + 40 + 320) * U
+    assert float(((r.probs.double() - p).abs() / p).max()) <= tol
+    assert r.counts[0].tolist() == [T] + [0] * (E - 1)
+    assert abs(float(r.balance) / float(p[0, 0] * E) - 1) <= tol
+    lse = torch.logsumexp(row.double(), 1)
+    assert abs(float(r.z) / float(lse ** 2) - 1) <= 2 * (8 + 6 + 40) * U / float(lse) + 320 * U

@@ -11,7 +11,7 @@
 // its experts in registers (L V >= E), a wave takes 64 / L tokens at a time, and
 // each lane keeps the sums of its experts over the tokens that it sees, so a
 // workgroup writes one row of sums per chunk of tokens and sequence
-// (router_stats_kernel).  A second launch adds the rows in their order
+// (router_stats_kernel).  A second launch adds the rows in their order, in fp64
 // (router_finish_kernel): no floating-point atomics, the same bits every time.
 // Backward: one pass, logits and the selected experts' gradients in, the logits'
 // gradient out (router_grad_kernel); a row's maximum and sum come from the forward.
@@ -31,7 +31,8 @@ namespace {
 constexpr int kMaxE = 1024, kMaxK = 16;
 // Forward: 16 waves a workgroup, so that 32 waves a CU write only two rows of sums.
 constexpr int kWaves = 16, kThreads = 64 * kWaves;
-constexpr int kMaxChunks = 512;    // workgroups: two a CU
+constexpr int kMaxChunks = 512;    // workgroups: two a CU, more where
+constexpr int kLaneRows = 256;     // a lane would add more rows than this in fp32 (fp64 from there)
 constexpr int kOneTurns = 4;       // turns of a workgroup that does without the second launch
 constexpr int kOneSeqs = 64;       // and the sequences that it writes
 // Second launch: 16 experts a workgroup, 16 partial rows at a time.
@@ -703,7 +704,11 @@ int chunk_rows(int T, int E, int waves, int chunks) {
   const int c = T > 0 ? (int)(((long)T + chunks - 1) / chunks) : 1;
   return (c + ng - 1) / ng * ng;
 }
-int forward_rows(int T, int E) { return chunk_rows(T, E, kWaves, kMaxChunks); }
+int forward_rows(int T, int E) {
+  const int c = chunk_rows(T, E, kWaves, kMaxChunks);
+  const int most = kLaneRows * (kWaves * 64 / layout_of(E).lanes);
+  return c < most ? c : most;
+}
 
 // Whether one workgroup does it all.
 bool one_fits(int T, int E, int S) {

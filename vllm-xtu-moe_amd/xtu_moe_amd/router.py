@@ -67,8 +67,8 @@ def router_losses(logits, ids, *, scoring="softmax", renormalize=True, routed_sc
     sequences' rows of logsumexp(logits)^2.  A row of -inf has p = 0 and no
     gradient; NaN gives NaN, and so does +inf with softmax (sigmoid: its score is
     1).  Far finite logits keep their ratios, with sigmoid too, where the scores
-    themselves vanish; z is inf where a square leaves fp32.  fp32 arithmetic, sums over rows fp32 and fp64;
-    the same call gives the same bits.  Once differentiable, backwards only.
+    themselves vanish; z is inf where a square leaves fp32.  fp32 arithmetic, sums over rows in fp32 up to
+    a lane's 256 rows and in fp64 from there; the same call gives the same bits.  Once differentiable, backwards only.
     Capturable into a HIP graph.
     """
     T, E, K, S = _check(logits, ids, scoring, routed_scaling_factor, seq_starts)
