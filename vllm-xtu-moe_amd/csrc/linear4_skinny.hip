@@ -4,7 +4,7 @@
 // blocks of 128 k among them, their sums are added through LDS in a fixed order, and
 // the workgroup takes further units in steps of the grid, with the next unit's first
 // blocks already in flight.  Bound by HBM where there is much of w: 1 x 16384 gated x
-// 7168 MXFP4 24 to 25 us (5.2 TB/s), 8 x 16384 x 7168 17.8.  Few columns: units of four or
+// 7168 MXFP4 24 to 27 us (4.7 to 5.2 TB/s), 8 x 16384 x 7168 17.8.  Few columns: units of four or
 // eight (the MFMA's other rows repeat the last one) put more CUs to work: 7 x 1171 x
 // 1184 INT4 5.3 us.
 #include "linear4.hpp"

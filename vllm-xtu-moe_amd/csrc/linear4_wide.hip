@@ -5,8 +5,9 @@
 // they take a quarter of the LDS traffic that bf16 tiles of w would, and a quarter of
 // their bytes from memory, for being expanded by both waves of a column.  x goes
 // straight to LDS, three stages (linear_tile.hip has the slots).  2048 x 2048 gated x
-// 7168 MXFP4, one round of 256 tiles: 91 us, 1.32 PFLOP/s, MFMAs busy 55% of the cycles
-// at 2.0 GHz, other VALU instructions 44% (NVFP4 115 us, INT4 with groups of 128 121).
+// 7168 MXFP4, one round of 256 tiles: 91 us, 1.32 PFLOP/s, MFMAs busy 54% of the cycles,
+// other VALU instructions 44% (NVFP4 115 us, INT4 with groups of 128 121; 98, 125 and 130 on
+// a card whose bf16 product of 8192 cubed reaches 1.34 PFLOP/s, not 1.42).
 // Tiles of 128 x 128 in waves of 128 x 32, x by way of registers: 194.  The next
 // operand expanded by quarters between the MFMAs of this one: 105.
 #include "linear4.hpp"
