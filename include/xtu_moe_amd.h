@@ -689,7 +689,8 @@ int xtu_linear4_plan(int M, int N, int K, int act, int fmt, int group);
  * are for xtu_router_grad, which writes the logits' gradient [T][E] (their type,
  * contiguous, 16-byte aligned) from those of weights [T][K], balance and z (fp32 on the
  * device; each may be NULL: 0).  E <= 1024, K <= 16, T <= 2^30, S ceil(E / 16) < 2^24.  A row
- * of -inf has probability 0 everywhere and no gradient.  The workspace
+ * of -inf (mode 1: all below -708) has probability 0 everywhere and no gradient.  The
+ * workspace
  * (xtu_router_workspace_bytes, 16-byte aligned) carries nothing from call to
  * call; calls that may overlap each need their own.  The same call gives the same
  * bits.  The reference trains nothing (its router: vllm_xiaotu_moe/

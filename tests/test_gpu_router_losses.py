@@ -12,6 +12,8 @@ sums.  A gradient's terms p (h_j - sum p h + z' - c) and w (g_k - sum w g) are
 each off by 2 R + 16 u of the sum of their terms' magnitudes; 1 - s <= 1
 multiplies them.  bf16 outputs: 2^-8 more.
 """
+import math
+
 import pytest
 import torch
 
@@ -381,16 +383,17 @@ def test_graph():
             assert torch.equal(x, y)
 
 
-def _in_logs(lg, ids, starts, scoring, renorm, f, gw, gb, gz):
-    """The definition in 64 bits, ratios by way of logarithms so that far logits keep
-    them, and the gradient by autograd; ids are all experts.  Beside it the magnitudes
-    of the gradient's terms."""
+def _definition(lg, ids, starts, scoring, renorm, f, gw, gb, gz):
+    """The definition in 64 bits (what vanishes there is zero), and the gradient by
+    autograd; ids are all experts.  Beside it the magnitudes of the gradient's terms."""
     l = lg.detach().double().requires_grad_(True)
     ids = ids.long()
     (T, E), K, soft = l.shape, ids.shape[1], scoring == "softmax"
-    x = l if soft else torch.nn.functional.logsigmoid(l)
-    p, s = torch.softmax(x, 1), x.gather(1, ids)
-    u = torch.softmax(s, 1) if renorm else p.gather(1, ids) if soft else torch.exp(s)
+    over = lambda v, n: v / torch.where(n > 0, n, torch.ones_like(n))  # noqa: E731
+    s = torch.softmax(l, 1) if soft else torch.sigmoid(l)
+    p, u = over(s, s.sum(1, keepdim=True)), s.gather(1, ids)
+    if renorm:   # (softmax: of the selected logits, as a ratio leaves 1e-18 beside them)
+        u = torch.softmax(l.gather(1, ids), 1) if soft else over(u, u.sum(1, keepdim=True))
     m = l.detach().amax(1, keepdim=True)   # (torch.logsumexp's own gradient is exp(l - lse),
     w, lse = f * u, (m + torch.log(torch.exp(l - m).sum(1, keepdim=True)))[:, 0]   # far off: 1)
     S = len(starts) - 1
@@ -430,7 +433,8 @@ def test_far_logits(scoring, renorm, f, dtype):
     """Rows wholly or in part at far finite values, the type's lowest and highest among
     them, in sequences and behind the last one.  Near a far maximum an exponential's
     argument is the exact difference times log2 e, off by 1.22 |l - m| u, where e^(l - m)
-    is above 2^-126 (|l - m| < 88: R as for a spread of 88); below it vanishes."""
+    is above 2^-126 (|l - m| < 88: R as for a spread of 88); below it vanishes.  A row
+    whose sigmoids all vanish in 64 bits is one without probabilities."""
     top = torch.finfo(dtype).max
     far = [-1e9, -1e10, -1e30, -top, 1e9, 1e10, 1e30, top, -300.0, 300.0, -5000.25, 5000.25]
     R = (88 + 40) * U
@@ -457,7 +461,7 @@ def test_far_logits(scoring, renorm, f, dtype):
         outs = [r.weights, r.balance] + ([r.z] if r.z is not None else [])
         d, = torch.autograd.grad(outs, lg, [gw] + [torch.full((), v, device=DEV) for v in (gb, gz)]
                                  [:len(outs) - 1])
-        e = _in_logs(lg, ids, starts, scoring, renorm, f, gw, gb, gz)
+        e = _definition(lg, ids, starts, scoring, renorm, f, gw, gb, gz)
 
         def near(name, got, want, tol):
             bad = ~((got.detach().double() - want).abs() <= tol)
@@ -554,7 +558,7 @@ def test_gradient_against_autograd(scoring, renorm, f, term):
             outs = [r.weights, r.balance] + ([r.z] if r.z is not None else [])
             d, = torch.autograd.grad(outs, lg, [gw] + [torch.full((), v, device=DEV)
                                                        for v in (gb, gz)][:len(outs) - 1])
-            e = _in_logs(lg, ids, starts, scoring, renorm, f, gw, gb, gz)
+            e = _definition(lg, ids, starts, scoring, renorm, f, gw, gb, gz)
             l64 = lg.detach().double()
             R = (float((l64.amax(1) - l64.amin(1)).max()) + 40) * U
             tol = e["da"] * (2 * R + 16 * U) + 2.0 ** -140
@@ -578,7 +582,7 @@ def test_gradient_against_differences_of_the_definition(scoring, renorm, f):
     outs = [r.weights, r.balance] + ([r.z] if r.z is not None else [])
     d, = torch.autograd.grad(outs, lg, [gw] + [torch.full((), v, device=DEV) for v in (gb, gz)]
                              [:len(outs) - 1])
-    F = lambda l: _in_logs(l, ids, starts, scoring, renorm, f, gw, gb, gz)  # noqa: E731
+    F = lambda l: _definition(l, ids, starts, scoring, renorm, f, gw, gb, gz)  # noqa: E731
     e, l64 = F(lg), lg.detach().double()
     F0 = float((e["weights"] * gw.double().abs()).sum() + gb * e["balance"] + gz * e["z"])
     own = e["da"] * (2 * (float((l64.amax(1) - l64.amin(1)).max()) + 40) + 16) * U + e["d"].abs() * U
@@ -651,3 +655,33 @@ def test_long_sums(E):
     assert abs(float(r.balance) / float(p[0, 0] * E) - 1) <= tol
     lse = torch.logsumexp(row.double(), 1)
     assert abs(float(r.z) / float(lse ** 2) - 1) <= 2 * (8 + 6 + 40) * U / float(lse) + 320 * U
+
+
+@pytest.mark.parametrize("scoring,f", [("softmax", 1.0), ("sigmoid", 2.5)])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_selection_far_below_the_maximum(scoring, f, dtype):
+    """The best experts dropped, or never selected: renormalised weights keep the ratios of
+    those that are, up to where their scores leave fp32 beside the row's largest: off by
+    2^-126 over their sum, zero when all of them vanish."""
+    for E, K in ((8, 3), (60, 4), (256, 8), (700, 12)):
+        g = torch.Generator().manual_seed(E)
+        T = 150
+        lg = torch.randn((T, E), generator=g).clamp(-4, 4)
+        ids = torch.stack([torch.randperm(E // 2, generator=g)[:K] for _ in range(T)]).int().to(DEV)
+        down = torch.tensor([30.0, 60.0, 150.0, 600.0, 1e30])[torch.arange(T) % 5, None]
+        lg[:, :E // 2] -= down
+        lg = lg.to(dtype).to(DEV)
+        gw = torch.randn((T, K), generator=g).to(DEV)
+        lg.requires_grad_(True)
+        r = router_losses(lg, ids, scoring=scoring, routed_scaling_factor=f)
+        d, = torch.autograd.grad(r.weights, lg, gw)
+        e = _definition(lg, ids, [0, T], scoring, True, f, gw, 0.0, 0.0)
+        kept = (down < 100)[:, 0].to(DEV)
+        R = (72 + 40) * U   # (4 + 60 + 4 and the type's rounding apart at most)
+        beside = 2.0 ** -126 / math.exp(-72)
+        tol = e["weights"] * (2 * R + 4 * U + beside) + f * beside
+        assert bool(((r.weights.detach().double() - e["weights"]).abs() <= tol)[kept].all()), E
+        assert not bool(r.weights[~kept].any()) and not bool(d[~kept].any())
+        tol = e["da"] * (2 * R + 16 * U + 2 * beside) + f * 4 * beside * gw.abs().max()
+        tol = tol + (e["d"].abs() + tol) * (2.0 ** -8 if dtype == BF else U)
+        assert bool(((d.double() - e["d"]).abs() <= tol)[kept].all()), E

@@ -16,8 +16,9 @@
 // Backward: one pass, logits and the selected experts' gradients in, the logits'
 // gradient out (router_grad_kernel); a row's maximum and sum come from the forward.
 //
-// A row of -inf has p = 0, no z and no gradient.  NaN gives NaN, +inf with softmax too
-// (sigmoid: its score is 1).
+// A row of -inf has p = 0, no z and no gradient; so has one whose sigmoids vanish in 64
+// bits.  NaN gives NaN, +inf with softmax too (sigmoid: its score is 1).
+#include <cfloat>
 #include <type_traits>
 
 #include "xtu_common.hpp"
@@ -51,6 +52,9 @@ struct Rows {
 };
 
 constexpr float kLog2e = 1.44269504f;
+// A row whose sigmoids are all below 64 bits' normal numbers (e^-708) has no scores to speak
+// of, as one of -inf: a mask's lowest value is no score.
+constexpr float kNoScore = -708.f;
 
 // e^(l - m) for l <= m.  Near zero as 2^(l log2 e - m log2 e): the rounding of the second
 // product is the same for all of a row and leaves its probabilities alone, that of the
@@ -215,7 +219,7 @@ __device__ __forceinline__ void values(const Rows& a, const Raw<L, V>& raw, floa
 
 // The score of a logit before its row's sum divides it.  softmax: e^(l - m), m the
 // row's maximum.  sigmoid: sigmoid(l) e^-m with m = min(maximum, 0), so that a row
-// of very negative logits keeps its ratios; sigmoid(l) = score e^m.  rest: 1 -
+// of very negative logits keeps its ratios (kNoScore); sigmoid(l) = score e^m.  rest: 1 -
 // sigmoid(l), without the cancellation.
 template <bool SIG>
 __device__ __forceinline__ float score(float l, float m, float& rest) {
@@ -360,7 +364,7 @@ __global__ __launch_bounds__(kThreads, ONE || V > 8 ? 4 : 8) void router_stats_k
 #pragma unroll
       for (int v = 1; v < V; ++v) m = fmaxf(m, l[v]);
       m = max_over<L>(m);
-      if (m == -INFINITY) m = 0.f;
+      if (m < (SIG ? kNoScore : -FLT_MAX)) m = 0.f;   // (the scores are zero then)
       if (SIG) m = fminf(m, 0.f);
       float s = 0.f, rest;
 #pragma unroll

@@ -66,8 +66,11 @@ def router_losses(logits, ids, *, scoring="softmax", renormalize=True, routed_sc
     P_e with n rows and P their mean p: 1 for even use.  z: mean over the
     sequences' rows of logsumexp(logits)^2.  A row of -inf has p = 0 and no
     gradient; NaN gives NaN, and so does +inf with softmax (sigmoid: its score is
-    1).  Far finite logits keep their ratios, with sigmoid too, where the scores
-    themselves vanish; z is inf where a square leaves fp32.  fp32 arithmetic, sums over rows in fp32 up to
+    1).  Rows of far finite logits are as any (sigmoid: one whose largest is below -708,
+    whose scores vanish in 64 bits too, is as a row of -inf); z is inf where a square
+    leaves fp32.  Renormalised weights lose accuracy where every selected logit lies
+    more than 70 below the row's largest, and are 0 from 87 on: their scores leave
+    fp32 beside it.  fp32 arithmetic, sums over rows in fp32 up to
     a lane's 256 rows and in fp64 from there; the same call gives the same bits.  Once differentiable, backwards only.
     Capturable into a HIP graph.
     """
